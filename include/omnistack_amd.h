@@ -424,6 +424,51 @@ int omni_attn_paged_plan_run(const omni_attn_paged_plan *plan, const void *q, co
 void omni_attn_paged_plan_destroy(omni_attn_paged_plan *plan);
 
 /*
+ * Norm of query and key heads with the rotation by position, in one pass (no
+ * counterpart in the reference, which takes q and k as its callers made them).
+ * For every token (b, t) and head, x of head_dim dims, fp32 with one rounding:
+ *   z = x * weight / sqrt(mean(x^2) + eps)      (z = x when the weights are NULL)
+ *   pair i of the first rotary_dim dims turned by positions[pair_axes[i]] * freq_i,
+ * pairs being the halves (i, i + rotary_dim / 2) or, interleaved, neighbours
+ * (2i, 2i + 1); dims behind rotary_dim keep z.  turns[i] (device, rotary_dim / 2)
+ * = round(freq_i / 2 pi * 2^64) mod 2^64, the fraction of a turn per position;
+ * pair_axes[i] (device) names the pair's row of positions.
+ * q, k, q_out, k_out: device pointers with host arrays of element strides
+ * {batch, token, head}; the last dim is contiguous, pointers and strides are
+ * multiples of 16 bytes.  positions: int32, or int64 when positions64, at host
+ * strides {axis, batch, token}.  Weights (head_dim) of w_dtype, 16-byte aligned.
+ * head_dim 32, 64, 128 or 256; rotary_dim a multiple of 16 (f32: 8), may be 0.
+ * q_out may be q and k_out k (with the same strides).
+ */
+int omni_qk_norm_rope(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, int dtype,
+                      int64_t B, int64_t T, int Hq, int Hkv, int head_dim,
+                      const void *positions, int positions64, const int64_t *position_strides,
+                      const uint64_t *turns, const uint8_t *pair_axes, int rotary_dim, int interleaved,
+                      const void *q_weight, const void *k_weight, int w_dtype, float eps,
+                      void *q_out, const int64_t *q_out_strides, void *k_out, const int64_t *k_out_strides,
+                      void *stream);
+
+/*
+ * Its gradient: dq_out, dk_out are the gradients of the outputs; writes dq, dk
+ * and, with weights, dq_weight and dk_weight (head_dim, w_dtype; summed over
+ * tokens and heads in fp32, in the same order on every run).  q and k are the
+ * forward's inputs, read only with weights.  workspace:
+ * omni_qk_norm_rope_backward_workspace_size(head_dim) bytes with weights, none
+ * without.
+ */
+size_t omni_qk_norm_rope_backward_workspace_size(int head_dim);
+int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                               int dtype, int64_t B, int64_t T, int Hq, int Hkv, int head_dim,
+                               const void *positions, int positions64, const int64_t *position_strides,
+                               const uint64_t *turns, const uint8_t *pair_axes, int rotary_dim, int interleaved,
+                               const void *q_weight, const void *k_weight, int w_dtype, float eps,
+                               const void *dq_out, const int64_t *dq_out_strides,
+                               const void *dk_out, const int64_t *dk_out_strides,
+                               void *dq, const int64_t *dq_strides, void *dk, const int64_t *dk_strides,
+                               void *dq_weight, void *dk_weight, void *workspace, size_t workspace_bytes,
+                               void *stream);
+
+/*
  * Measurement helper with no counterpart in the reference: streams `bytes`
  * (a multiple of 16, 16-byte aligned device buffer) once with n_partials
  * blocks and writes one XOR fold per block to partials[0 .. n_partials),

@@ -6,6 +6,7 @@ are not on a HIP device.  There is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -80,6 +81,12 @@ SIGNATURES = {
                                              ctypes.POINTER(_vp)]),
     "omni_attn_paged_plan_run": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "omni_attn_paged_plan_destroy": (None, [_vp]),
+    "omni_qk_norm_rope": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp, _c_int,
+                                   _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _c_int, _c_f32, _vp, _vp, _vp, _vp, _vp]),
+    "omni_qk_norm_rope_backward_workspace_size": (_c_sz, [_c_int]),
+    "omni_qk_norm_rope_backward": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _vp,
+                                            _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _c_int, _c_f32,
+                                            _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
     "omni_hbm_read_probe": (_c_int, [_vp, _c_sz, _vp, _c_int, _vp]),
     "omni_attn_noalloc_scratch_bytes": (_c_sz, []),
     "omni_attn_noalloc": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_int, _vp,
@@ -150,6 +157,45 @@ def stream_of(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is current (a launch takes the current
+    device's code and properties); nothing to do where it already is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(device)
+
+
+_LEAF_STREAM = "omnistack_rs.stream"
+
+
+def hold_leaves(device: torch.device, *tensors: Optional[torch.Tensor]) -> list:
+    """Gradient nodes of the leaves among `tensors`, marked with the stream of
+    their first use; keep the list until the graph that uses them is built.
+    Under graph capture, a leaf whose node another stream made (an eager graph
+    of it is still alive) is refused: the backward pass would make the
+    captured stream wait for that one, which ends the process when the capture
+    closes."""
+    stream = stream_of(device)
+    nodes = []
+    for t in tensors:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        node = torch.autograd.graph.get_gradient_edge(t).node
+        if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("graph capture with gradients: an autograd graph of the same leaves, built on another "
+                               "stream, is still alive; delete its outputs before capturing")
+        nodes.append(node)
+    return nodes
+
+
+def i64_array(*values: int) -> ctypes.Array:
+    """Host int64 array argument (strides)."""
+    return (ctypes.c_int64 * len(values))(*values)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

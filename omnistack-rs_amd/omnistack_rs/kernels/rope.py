@@ -1,0 +1,253 @@
+"""Norm of query and key heads with the rotation by position, on gfx950
+(omni_qk_norm_rope, omni_qk_norm_rope_backward).
+
+No counterpart in the reference, whose caches hold keys as its callers made
+them: this is the step between a model's projections and ``rotate_kv_cache``
+/ ``PagedKVCache.append`` (keys) or ``omni_attn`` / ``prompt_attention``
+(queries).  For every token and head of q and k, in fp32 with one rounding at
+the end:
+
+    z = x * w / sqrt(mean(x^2) + eps)          (z = x without weights)
+    (z_i, z_i') turned by positions[axis_i] * inv_freq_i
+
+over the pairs of the first ``rotary_dim`` dims; dims behind them keep z.
+Positions may be any integers, as far apart as 64 bits go: angles are exact
+fractions of a turn.
+"""
+from __future__ import annotations
+
+from fractions import Fraction
+from typing import Optional, Sequence
+
+import torch
+
+from .. import _lib
+from .hadamard import HEAD_DIM
+
+_HEAD_DIMS = (32, 64, 128, 256)
+_PI = Fraction(31415926535897932384626433832795028841971, 10 ** 40)
+
+
+class RotaryEmbedding:
+    """Frequencies of a position rotation, prepared on the device once.
+
+    ``inv_freq``: the ``rotary_dim / 2`` angles per position (default
+    ``base ** (-2 i / rotary_dim)``).  ``interleaved``: pairs are neighbours
+    (2i, 2i + 1) instead of the halves (i, i + rotary_dim / 2).  Several
+    position axes (time, height, width) share the pairs: ``sections`` gives
+    each axis its number of pairs in turn, ``pair_axes`` names each pair's
+    axis; ``n_axes`` is then the number of position rows.
+    """
+
+    def __init__(self, head_dim: int = HEAD_DIM, base: float = 10000.0, *, rotary_dim: Optional[int] = None,
+                 inv_freq: Optional[Sequence[float]] = None, sections: Optional[Sequence[int]] = None,
+                 pair_axes: Optional[Sequence[int]] = None, interleaved: bool = False, device="cuda"):
+        if head_dim not in _HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {_HEAD_DIMS}, got {head_dim}")
+        R = head_dim if rotary_dim is None else int(rotary_dim)
+        if R < 0 or R > head_dim or R % 8:
+            raise ValueError(f"rotary_dim must be a multiple of 8 up to head_dim {head_dim}, got {R}")
+        n = R // 2
+        if inv_freq is None:
+            if not 0.0 < float(base) < float("inf"):
+                raise ValueError(f"base must be positive and finite, got {base}")
+            inv_freq = [float(base) ** (-i / n) for i in range(n)]
+        freq = [float(f) for f in (inv_freq.tolist() if isinstance(inv_freq, torch.Tensor) else inv_freq)]
+        if len(freq) != n or any(f != f or abs(f) == float("inf") for f in freq):
+            raise ValueError(f"inv_freq must hold {n} finite values")
+        if sections is not None and pair_axes is not None:
+            raise ValueError("give sections or pair_axes, not both")
+        if sections is not None:
+            if any(int(s) < 0 for s in sections) or sum(int(s) for s in sections) != n:
+                raise ValueError(f"sections must be >= 0 and sum to {n} pairs, got {list(sections)}")
+            axes = [a for a, s in enumerate(sections) for _ in range(int(s))]
+            self.n_axes = len(sections)
+        else:
+            axes = [0] * n if pair_axes is None else [int(a) for a in pair_axes]
+            if len(axes) != n:
+                raise ValueError(f"pair_axes must name the axis of {n} pairs, got {len(axes)}")
+            self.n_axes = max(axes, default=0) + 1
+        if any(a < 0 or a > 255 for a in axes) or not 1 <= self.n_axes <= 256:
+            raise ValueError("position axes must lie in [0, 255]")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, R, bool(interleaved)
+        # fractions of a turn per position, 64 bits, as the int64 with the same bits
+        turns = [round(Fraction(f) / (2 * _PI) * (1 << 64)) % (1 << 64) for f in freq]
+        dev = torch.device(device)
+        self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64).to(dev)
+        self.pair_axes = torch.tensor(axes, dtype=torch.uint8).to(dev)
+        self.device = self.turns.device
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """`t` as the kernels read it: the last dim contiguous, 16-byte steps."""
+    step = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+            all(s % step == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    """Element strides (batch, token, head) of (N, H, D) or (B, H, T, D)."""
+    s = [0 if n == 1 else st for n, st in zip(t.shape, t.stride())]
+    b, tok, h = (0, s[0], s[1]) if t.dim() == 3 else (s[0], s[2], s[1])
+    return _lib.i64_array(b, tok, h)
+
+
+def _check(q, k, positions, rotary, q_weight, k_weight, eps):
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise ValueError(f"q and k must be (N, heads, head_dim) or (B, heads, T, head_dim), got {tuple(q.shape)} "
+                         f"and {tuple(k.shape)}")
+    if not isinstance(rotary, RotaryEmbedding):
+        raise TypeError("rotary must be a RotaryEmbedding")
+    D = rotary.head_dim
+    rows = (1, q.shape[0]) if q.dim() == 3 else (q.shape[0], q.shape[2])
+    krows = (1, k.shape[0]) if k.dim() == 3 else (k.shape[0], k.shape[2])
+    if q.shape[-1] != D or k.shape[-1] != D or rows != krows or q.shape[1] < 1 or k.shape[1] < 1:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree but for their heads and have head_dim {D}")
+    if q.dtype != k.dtype:
+        raise ValueError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
+    unit = 8 if _lib.dtype_code(q.dtype) == 0 else 16
+    if rotary.rotary_dim % unit:
+        raise ValueError(f"rotary_dim must be a multiple of {unit} for {q.dtype}, got {rotary.rotary_dim}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight must be given together")
+    for w in (q_weight, k_weight):
+        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q_weight.dtype):
+            raise ValueError(f"q_weight and k_weight must be ({D},) of one dtype, got {w.dtype} {tuple(w.shape)}")
+    if q_weight is not None:
+        _lib.dtype_code(q_weight.dtype)
+        if not float(eps) >= 0.0:
+            raise ValueError(f"eps must be >= 0, got {eps}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    A = rotary.n_axes
+    want = (A, rows[1]) if q.dim() == 3 else (A, *rows)
+    try:
+        pos = positions.expand(want)
+    except RuntimeError:
+        raise ValueError(f"positions must broadcast to {want}, got {tuple(positions.shape)}") from None
+    dev = _lib.require_device(q, k, positions, q_weight, k_weight)
+    if dev != rotary.device:
+        raise ValueError(f"rotary is on {rotary.device}, q on {dev}")
+    return dev, rows, pos if pos.dim() == 3 else pos[:, None]
+
+
+def _common(q, k, pos, rotary, wq, wk, eps, rows):
+    """The arguments that both directions share, behind the tensors."""
+    return (_lib.dtype_code(q.dtype), *rows, q.shape[1], k.shape[1], rotary.head_dim, _lib.ptr(pos),
+            int(pos.dtype == torch.int64), _lib.i64_array(*pos.stride()), _lib.ptr(rotary.turns),
+            _lib.ptr(rotary.pair_axes), rotary.rotary_dim, int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk),
+            0 if wq is None else _lib.dtype_code(wq.dtype), float(eps))
+
+
+def _forward(q, k, pos, rotary, wq, wk, eps, rows, dev, out):
+    qc, kc = _heads(q), _heads(k)
+    wq, wk = (None if w is None else _heads(w) for w in (wq, wk))
+    qo, ko = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().omni_qk_norm_rope(
+            _lib.ptr(qc), _strides(qc), _lib.ptr(kc), _strides(kc),
+            *_common(qc, kc, pos, rotary, wq, wk, eps, rows),
+            _lib.ptr(qo), _strides(qo), _lib.ptr(ko), _strides(ko), _lib.stream_of(dev)))
+    return qo, ko
+
+
+class _QKNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, rotary, wq, wk, eps, rows, dev):
+        # without a norm the gradient needs neither q nor k
+        ctx.save_for_backward(pos, *((q, k, wq, wk) if wq is not None else ()))
+        ctx.rotary, ctx.eps, ctx.rows, ctx.dev = rotary, eps, rows, dev
+        return _forward(q, k, pos, rotary, wq, wk, eps, rows, dev, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        pos, *rest = ctx.saved_tensors
+        q, k, wq, wk = rest if rest else (gq, gk, None, None)
+        dev, norm = ctx.dev, bool(rest)
+        gq, gk = _heads(gq), _heads(gk)
+        q, k = _heads(q), _heads(k)
+        wqc, wkc = (None if w is None else _heads(w) for w in (wq, wk))
+        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
+        dwq, dwk = (torch.empty_like(wqc), torch.empty_like(wkc)) if norm else (None, None)
+        L = _lib.lib()
+        ws_bytes = L.omni_qk_norm_rope_backward_workspace_size(ctx.rotary.head_dim) if norm else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        with _lib.on_device(dev):
+            _lib.check(L.omni_qk_norm_rope_backward(
+                _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k),
+                *_common(q, k, pos, ctx.rotary, wqc, wkc, ctx.eps, ctx.rows),
+                _lib.ptr(gq), _strides(gq), _lib.ptr(gk), _strides(gk), _lib.ptr(dq), _strides(dq), _lib.ptr(dk),
+                _strides(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_of(dev)))
+        return dq, dk, None, None, dwq, dwk, None, None, None
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: RotaryEmbedding,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
+                 out: Optional[tuple] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm (with weights) and position rotation of q and k, one launch.
+
+    q (N, n_heads, head_dim) and k (N, n_kv_heads, head_dim), tokens packed, or
+    (B, heads, T, head_dim), the layout of the cache's encoder; float32, float16
+    or bfloat16, any strides (slices of a fused projection's output are read in
+    place; a last dim that is not contiguous, or rows off 16 bytes, are copied
+    first).  ``positions`` int32 or int64, broadcast to (n_axes, N) or
+    (n_axes, B, T): one row for text, one per axis for images and video, or one
+    for all axes.  ``q_weight`` / ``k_weight`` (head_dim,): the norms' weights;
+    without them heads are rotated only.  Returns (q', k') in the inputs' dtype,
+    contiguous, or ``out`` (two tensors of the inputs' shapes; the inputs
+    themselves turn in place).  Gradients for q, k and the weights; ``out`` is
+    for calls that need none.  Forward and backward can be captured in a HIP
+    graph once no eager autograd graph of the same leaves is alive (refused
+    otherwise)."""
+    dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    if out is not None:
+        if grad:
+            raise ValueError("out= takes no gradient: call it under torch.no_grad()")
+        for o, t in zip(out, (q, k)):
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or _heads(o) is not o:
+                raise ValueError(f"out must hold {t.dtype} tensors of q's and k's shapes on {t.device}, "
+                                 "their last dim contiguous and rows at 16-byte steps")
+        _check_overlap(q, k, out)
+    if grad:
+        held = _lib.hold_leaves(dev, q, k, q_weight, k_weight)  # noqa: F841 (alive until the graph holds them)
+        return _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev)
+    return _forward(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev, out)
+
+
+def _span(t: torch.Tensor):
+    """First byte and the byte behind the last that `t` reaches."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _check_overlap(q, k, out):
+    """In place means exactly in place.  Slices of one buffer interleave (q and
+    k of a fused projection): those pass where their rows keep to their own
+    columns, which equal strides show."""
+    def same(a, b):
+        return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+
+    def apart(a, b):
+        (a0, a1), (b0, b1) = _span(a), _span(b)
+        if a1 <= b0 or b1 <= a0:
+            return True
+        # one token's heads of each lie within a row of the same length, at columns of their own
+        if a.dim() != 3 or b.dim() != 3 or a.stride(0) != b.stride(0) or a.shape[0] != b.shape[0]:
+            return False
+        row = a.stride(0) * a.element_size()
+        la, lb = (_span(t[:1])[1] - _span(t[:1])[0] for t in (a, b))
+        off = b0 - a0
+        return la <= off and off + lb <= row if off >= 0 else lb <= -off and -off + la <= row
+
+    qo, ko = out
+    for o in out:
+        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
+            raise ValueError("out must not be a broadcast view")
+    if not (apart(qo, ko) and apart(qo, k) and apart(ko, q) and (same(qo, q) or apart(qo, q))
+            and (same(ko, k) or apart(ko, k))):
+        raise ValueError("out may be q and k themselves, but must not overlap them otherwise")
