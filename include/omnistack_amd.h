@@ -469,6 +469,43 @@ int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const vo
                                void *stream);
 
 /*
+ * Attention of whole prompts packed one after another (no counterpart in the
+ * reference, whose dense attention takes padded fp32 batches,
+ * attention/reference.py:72-177): sequence b holds tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1] (device int32, B + 1 entries, from 0, not decreasing, at
+ * most N) of q (N, Hq, D), k and v (N, Hkv, D), f16 or bf16, D 32, 64 or 128;
+ *   out_t = softmax_s(scale q_t . k_s) . v_s within the sequence, s <= t when
+ *   causal; kv head = hq / (Hq / Hkv).
+ * Device pointers with host element strides {token, head}; the last dim is
+ * contiguous, pointers and strides are multiples of 16 bytes, a token stride is
+ * below 2^24 elements.  lse (Hq, N) f32 or NULL: log sum_s exp(scale q_t . k_s).
+ * Rows behind the last sequence: zeros (lse -inf) when fill_rest, else left as
+ * they were.  cu_seqlens that break the rules give rows of no meaning, but
+ * nothing outside the tensors is read or written.
+ */
+int omni_prompt_attn(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                     const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv, int head_dim,
+                     const int32_t *cu_seqlens, int64_t B, float scale, int causal, int fill_rest,
+                     void *out, const int64_t *out_strides, float *lse, void *stream);
+
+/*
+ * Its gradient: out and lse are the forward's results for these inputs, dout
+ * the gradient of out; writes dq, dk, dv (dk and dv summed over the group's
+ * query heads), zeros in rows behind the last sequence.  No atomics: the same
+ * bits on every run.  workspace (16-byte aligned):
+ * omni_prompt_attn_backward_workspace_size(N, Hq) bytes.
+ */
+size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq);
+int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                              const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv,
+                              int head_dim, const int32_t *cu_seqlens, int64_t B, float scale, int causal,
+                              const void *out, const int64_t *out_strides, const float *lse,
+                              const void *dout, const int64_t *dout_strides,
+                              void *dq, const int64_t *dq_strides, void *dk, const int64_t *dk_strides,
+                              void *dv, const int64_t *dv_strides, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/*
  * Measurement helper with no counterpart in the reference: streams `bytes`
  * (a multiple of 16, 16-byte aligned device buffer) once with n_partials
  * blocks and writes one XOR fold per block to partials[0 .. n_partials),

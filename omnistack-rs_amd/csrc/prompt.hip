@@ -1,0 +1,916 @@
+// Attention of whole prompts packed one after another, and its gradient (gfx950).
+//
+// Sequence b holds tokens cu[b] .. cu[b+1] of q (N, Hq, D), k and v (N, Hkv, D)
+// in 16 bits; within it, with kv head h / G of query head h,
+//   o_t = sum_s p_ts v_s,   p_ts = exp(scale q_t . k_s - lse_t),
+//   lse_t = log sum_s exp(scale q_t . k_s),      s <= t when causal.
+// The dense counterpart in the reference takes padded fp32 batches and has no
+// kernel (attention/reference.py:72-177).
+#include <math.h>
+
+#include "omni_common.h"
+
+namespace omni {
+
+typedef float pf16_t __attribute__((ext_vector_type(16)));
+typedef short ps4_t __attribute__((ext_vector_type(4)));
+typedef short ps8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 pb8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 ph8_t __attribute__((ext_vector_type(8)));
+#define PT_LDS __attribute__((address_space(3)))
+
+constexpr int kPtWaves = 4;
+constexpr int kPtRows = 32 * kPtWaves;   // query rows of a block
+constexpr int kPtKeys = 64;              // keys of a tile
+constexpr int kPtBufWord3 = 0x00020000;
+// Exponents of two: a row's running maximum follows its tiles only when one is
+// above it by kPtSlack (rescaling costs D / 2 products a lane), and f16
+// probabilities are kept times 2^kPtF16Up, so that they reach 2^15 at most and
+// the smallest subnormal is 2^-31 of the maximum (bf16 has fp32's range).
+constexpr float kPtSlack = 8.0f;
+constexpr float kPtF16Up = 7.0f;
+
+struct PromptHeads {
+    const char *p;
+    int64_t st, sh;                      // byte strides of a token and a head
+};
+
+struct PromptArgs {
+    PromptHeads q, k, v, o;
+    PromptHeads g, dq, dk, dv;           // backward: the output's gradient, and those of q, k and v
+    float *lse;                          // (Hq, N), or NULL
+    float *lse2, *delta;                 // backward, (Hq, N): lse log2 e, and -sum_d g o
+    float *peaks;                        // backward in f16: kPtPeaks largest squared norms of g's rows, then of v's
+    const int32_t *cu;
+    int64_t N;
+    int B, Hq, Hkv, G;
+    int causal, negate, fill;            // fill: rows of no sequence get zeros
+    int peak_rows;
+    float c, scale;                      // |scale| log2(e)
+};
+
+// ── types ───────────────────────────────────────────────────────────────
+
+template <int DT>
+__device__ __forceinline__ pf16_t pt_mfma(ps8_t a, ps8_t b, pf16_t c) {
+    if constexpr (DT == OMNI_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pb8_t, a), __builtin_bit_cast(pb8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8_t, a), __builtin_bit_cast(ph8_t, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pt_pack(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 t = {a, b};
+    if constexpr (DT == OMNI_BF16) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, b2));
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, h2));
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float pt_value(uint32_t h) {     // low 16 bits
+    return DT == OMNI_BF16 ? bf16_to_f32((uint16_t)h) : f16_to_f32((uint16_t)h);
+}
+
+__device__ __forceinline__ float pt_max_halves(float m) {
+    const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
+}
+__device__ __forceinline__ float pt_sum_halves(float m) {
+    const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return __uint_as_float(u[0]) + __uint_as_float(u[1]);
+}
+
+// Barrier that also waits for the wave's own copies into LDS: they have no
+// register result for the compiler to wait for, and the barrier's own fence
+// does not follow them around a loop.
+__device__ __forceinline__ void pt_sync() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// ── tiles in LDS ────────────────────────────────────────────────────────
+//
+// A tile's rows of D 16-bit values lie one after another, the 16-byte chunks
+// of row r in the order chunk ^ pt_swz(r): both the row reads (16 lanes, a
+// chunk of 16 rows each) and the transposed reads (16 lanes, 32 bytes of four
+// rows, two such groups side by side) then meet every bank once.
+
+template <int D>
+__device__ __forceinline__ int pt_swz(int r) {
+    if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (D == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+}
+
+// The copy of a tile: lane's chunk and row of each of the wave's instructions
+// (the copy writes LDS in lane order, so the swizzle is in the address read).
+template <int D, int ROWS>
+struct PtCopy {
+    static constexpr int CH = D / 8, RPI = 64 / CH, N = ROWS * CH / (64 * kPtWaves);
+    static_assert(N >= 1 && ROWS * CH % (64 * kPtWaves) == 0, "whole instructions");
+    int row, off;                        // of instruction 0; instruction u: rows RPI * kPtWaves * u on
+    uint32_t stride;
+
+    __device__ __forceinline__ void init(int64_t st) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+        row = wave * RPI + lane / CH;
+        stride = (uint32_t)st;
+        // rows of one lane's instructions are RPI * kPtWaves = 16, 32 or 64 apart: one swizzle
+        off = ((lane % CH) ^ pt_swz<D>(row)) * 16;
+    }
+    // Rows r0 .. r0 + ROWS - 1 of a head at `base` (its row 0); rows from `len` on repeat the last.
+    __device__ __forceinline__ void issue(const char *base, int64_t st, int r0, int len, char *lds) const {
+        const int left = min(len - r0, ROWS);
+        const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(base + (int64_t)r0 * st), (short)0, (int)((uint32_t)(left - 1) * stride + 2 * D), kPtBufWord3);
+        char *dst = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
+        if (left == ROWS) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)(dst + u * 1024 * kPtWaves), 16,
+                                                         (uint32_t)(row + RPI * kPtWaves * u) * stride + off, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)(dst + u * 1024 * kPtWaves), 16,
+                                                         (uint32_t)min(row + RPI * kPtWaves * u, left - 1) * stride + off, 0, 0, 0);
+        }
+    }
+};
+
+// A operand of rows r0 .. r0 + 31, dims 16 kk .. 16 kk + 15.
+template <int D>
+__device__ __forceinline__ ps8_t pt_rows(const char *tile, int r0, int kk) {
+    const int lane = threadIdx.x & 63, r = r0 + (lane & 31), ch = 2 * kk + (lane >> 5);
+    return *reinterpret_cast<const ps8_t *>(tile + r * (2 * D) + ((ch ^ pt_swz<D>(r)) * 16));
+}
+
+// A operand of the transposed tile: dims 32 dt .. 32 dt + 31 by rows r0 ..
+// r0 + 15, the rows in the order of an MFMA result's registers: slot (half, j)
+// is row 8 (j / 4) + 4 half + j % 4.
+template <int D>
+__device__ __forceinline__ ps8_t pt_cols(const char *tile, int r0, int dt) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const int byte = (32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3)) * 2;
+    ps4_t v[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int r = r0 + 8 * g + 4 * (lane >> 5) + i / 4;
+        v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (PT_LDS ps4_t *)(tile + r * (2 * D) + (((byte >> 4) ^ pt_swz<D>(r)) * 16) + (byte & 15)));
+    }
+    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Row operand of 32 rows straight from memory: lane's row at `p`, dims 8 half on.
+template <int D>
+__device__ __forceinline__ void pt_load_rows(const char *p, uint32_t flip, ps8_t (&f)[D / 16]) {
+    p += 16 * ((threadIdx.x >> 5) & 1);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        uint4 u = *reinterpret_cast<const uint4 *>(p + 32 * kk);
+        u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
+        f[kk] = __builtin_bit_cast(ps8_t, u);
+    }
+}
+
+// x times f, of the lane's row, to `p`: register i of block d is dim
+// 32 d + 8 (i / 4) + 4 half + i % 4; after the swap each half holds eight dims.
+template <int DT, int D>
+__device__ __forceinline__ void pt_store(char *p, const pf16_t (&x)[D / 32], float f, bool mine) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            uint32_t u[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t lo = pt_pack<DT>(x[d][4 * g + 2 * e] * f, x[d][4 * g + 2 * e + 1] * f);
+                const uint32_t hi = pt_pack<DT>(x[d][4 * g + 4 + 2 * e] * f, x[d][4 * g + 4 + 2 * e + 1] * f);
+                const auto t = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+                u[0][e] = t[0];
+                u[1][e] = t[1];
+            }
+            if (mine) *reinterpret_cast<uint4 *>(p + (32 * d + 8 * (g + half)) * 2) = make_uint4(u[0][0], u[0][1], u[1][0], u[1][1]);
+        }
+}
+
+// Zeros to rows row0 .. row0 + R - 1, below len, of a head.
+template <int D, int R>
+__device__ __forceinline__ void pt_zero_rows(const PromptHeads &o, int start, int row0, int len, int h) {
+    constexpr int CH = D / 8;
+    for (int e = threadIdx.x; e < R * CH; e += blockDim.x) {
+        const int t = row0 + e / CH;
+        if (t < len)
+            *reinterpret_cast<uint4 *>(const_cast<char *>(o.p) + (int64_t)(start + t) * o.st + h * o.sh + e % CH * 16) =
+                make_uint4(0, 0, 0, 0);
+    }
+}
+
+// ── which rows a block takes ────────────────────────────────────────────
+//
+// Row tiles of R are dealt to slots: sequence b has the slots from
+// cu[b] / R + b on, one more than its tokens' tiles at most, so no list is
+// made and the grid, N / R + B + 1 slots, needs only the total.  The slots
+// behind the last sequence's are those of the rows of none.  Of a sequence's
+// tiles those with the most work under a causal mask come first: the last query
+// rows, the first keys.
+
+struct PtSlot {
+    int start, len, tile;                // tile < 0: nothing to do
+    bool none;                           // rows of no sequence
+};
+
+template <int R>
+__device__ __forceinline__ PtSlot pt_slot(const int32_t *cu, int B, int64_t N, int64_t slot, bool last_first) {
+    const int lane = threadIdx.x & 63;
+    // the last b in [0, B] with cu[b] / R + b <= slot, 64 ways a step
+    int lo = 0, n = B + 1;
+    while (n > 1) {
+        const int step = (n + 63) / 64, b = lo + lane * step;
+        const bool below = lane * step < n && (int64_t)((uint32_t)cu[b] / R) + b <= slot;
+        const int at = 63 - __builtin_clzll(__ballot(below) | 1ull);
+        lo += at * step;
+        n = min(step, n - at * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    PtSlot s;
+    const int64_t a = cu[lo], e = lo < B ? (int64_t)cu[lo + 1] : N;
+    const int64_t first = (int64_t)((uint32_t)cu[lo] / R) + lo;
+    s.none = lo == B;
+    // whatever cu holds, rows stay within 0 .. N
+    s.start = (int)(a < 0 ? 0 : a > N ? N : a);
+    const int64_t end = e > N ? N : e;
+    s.len = end > s.start ? (int)(end - s.start) : 0;
+    const int64_t tiles = ((int64_t)s.len + R - 1) / R, at = slot - first;
+    s.tile = at < 0 || at >= tiles ? -1 : (int)(last_first ? tiles - 1 - at : at);
+    return s;
+}
+
+// ── forward ─────────────────────────────────────────────────────────────
+//
+// A wave holds 32 query rows as the B operand of S^T = K Q^T, so lane n and
+// n + 32 share query row n: row statistics are register reductions with one
+// exchange, and the probabilities, rounded to the input's 16 bits, are the B
+// operand of O^T += V^T P^T where they are, with V^T read transposed from LDS.
+// P's rounding (half a step of the inputs' type for each term, the row sum
+// taken of the unrounded) is what feeding the matrix units 16 bits costs; all
+// else is fp32.
+
+template <int DT, int D>
+struct PtRow {
+    static constexpr int NT = D / 32;
+    ps8_t q[D / 16];
+    pf16_t o[NT];
+    float m, l;                          // running maximum of scale s log2 e; the lane's share of the sum
+    int t;                               // the row (of the sequence)
+};
+
+template <int DT, int D, bool MASK>
+__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len,
+                                                const uint32_t *bad, char *scratch) {
+    constexpr int NT = PtRow<DT, D>::NT;
+    const int half = (threadIdx.x >> 5) & 1;
+    pf16_t s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        s[b] = pf16_t{};
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(pt_rows<D>(K, 32 * b, kk), R.q[kk], s[b]);
+    }
+    // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
+    const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (MASK) {
+                if (32 * b + 8 * (i / 4) + i % 4 > seen) s[b][i] = -INFINITY;
+            }
+            mt = fmaxf(mt, s[b][i]);
+        }
+    mt = pt_max_halves(mt);
+    if (MASK && mt == -INFINITY) {
+        // no key, or none above -inf: the maximum stays (scale 0 would make it NaN)
+    } else {
+        mt *= a.c;
+    }
+    if (__builtin_amdgcn_ballot_w64(mt > R.m + kPtSlack)) {
+        const float mn = fmaxf(R.m, mt);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R.m - mn);
+        R.l *= f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) R.o[d][i] *= f;
+        R.m = mn;
+    }
+    const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
+    float sum[2];
+    uint32_t p[2][8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.c, -off));
+            if constexpr (MASK) {
+                if (32 * b + 8 * (i / 4) + i % 4 > seen) x[i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[b][i] = pt_pack<DT>(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+        for (int w = 8; w > 0; w /= 2)
+#pragma unroll
+            for (int i = 0; i < w; ++i) x[i] += x[i + w];
+        sum[b] = x[0];
+    }
+    R.l += sum[0] + sum[1];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint4 u = make_uint4(p[b][4 * k], p[b][4 * k + 1], p[b][4 * k + 2], p[b][4 * k + 3]);
+            const ps8_t pb = __builtin_bit_cast(ps8_t, u);
+#pragma unroll
+            for (int d = 0; d < NT; ++d) R.o[d] = pt_mfma<DT>(pt_cols<D>(V, 32 * b + 16 * k, d), pb, R.o[d]);
+        }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(PromptArgs a) {
+    __shared__ __attribute__((aligned(16))) char k0[kPtKeys * 2 * D], k1[kPtKeys * 2 * D];
+    __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
+    constexpr int NT = D / 32;
+    // kv heads vary fastest, so that with eight of them (or a multiple) a kv
+    // head's blocks share an XCD and its L2; then the group's heads
+    const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int hk = (int)(bid % a.Hkv);
+    const int64_t r = bid / a.Hkv;
+    const int h = hk * a.G + (int)(r % a.G);
+    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, r / a.G, true);
+    if (S.tile < 0) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int row0 = S.tile * kPtRows;
+    if (S.none) {
+        if (!a.fill) return;
+        pt_zero_rows<D, kPtRows>(a.o, S.start, row0, S.len, h);
+        for (int e = threadIdx.x; a.lse && e < kPtRows; e += 64 * kPtWaves)
+            if (row0 + e < S.len) a.lse[(int64_t)h * a.N + S.start + row0 + e] = -INFINITY;
+        return;
+    }
+    const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
+    PtCopy<D, kPtKeys> ck, cv;
+    ck.init(a.k.st);
+    cv.init(a.v.st);
+    ck.issue(kb, a.k.st, 0, S.len, k0);
+    cv.issue(vb, a.v.st, 0, S.len, v0);
+
+    PtRow<DT, D> R;
+    const int w0 = row0 + 32 * wave;     // the wave's first row
+    R.t = w0 + (lane & 31);
+    pt_load_rows<D>(a.q.p + (int64_t)(S.start + min(R.t, S.len - 1)) * a.q.st + h * a.q.sh, a.negate ? 0x80008000u : 0u, R.q);
+    R.m = -INFINITY;
+    R.l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
+
+    const int kend = a.causal ? min(S.len, row0 + kPtRows) : S.len;       // keys that the block sees
+    const int wlast = a.causal ? min(w0 + 31, S.len - 1) : S.len - 1;     // and the wave
+    const bool live = w0 < S.len;
+    auto step = [&](const char *K, const char *V, int j0) {
+        if (!live || j0 > wlast) return;
+        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_forward_tile<DT, D, true>(a, R, K, V, j0, S.len, nullptr, nullptr);
+        else pt_forward_tile<DT, D, false>(a, R, K, V, j0, S.len, nullptr, nullptr);
+    };
+    for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
+        pt_sync();                       // this tile is there, the other buffers are read
+        if (j0 + kPtKeys < kend) {
+            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1);
+            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1);
+        }
+        step(k0, v0, j0);
+        if (j0 + kPtKeys >= kend) break;
+        pt_sync();
+        if (j0 + 2 * kPtKeys < kend) {
+            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0);
+            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0);
+        }
+        step(k1, v1, j0 + kPtKeys);
+    }
+    if (!live) return;
+
+    const float l = pt_sum_halves(R.l);
+    const bool mine = R.t < S.len;
+    pt_store<DT, D>(const_cast<char *>(a.o.p) + (int64_t)(S.start + R.t) * a.o.st + h * a.o.sh, R.o, 1.0f / l, mine);
+    if (a.lse && mine && half == 0)
+        a.lse[(int64_t)h * a.N + S.start + R.t] = (R.m - (DT == OMNI_F16 ? kPtF16Up : 0.0f) + __log2f(l)) * 0.69314718f;
+}
+
+// ── backward ────────────────────────────────────────────────────────────
+//
+// delta_t = sum_d g_td o_td;  p_ts = exp(scale q_t . k_s - lse_t);
+//   dv_s = sum_t p_ts g_t,            ds_ts = p_ts (g_t . v_s - delta_t),
+//   dq_t = scale sum_s ds_ts k_s,     dk_s = scale sum_t ds_ts q_t,
+// dk and dv summed over the group's query heads.  Three launches without
+// atomics, so that results repeat bit for bit: delta; dq by blocks of query
+// rows; dk and dv by blocks of keys.  Scores and g . v are formed twice for it,
+// seven products instead of five.
+//
+// p and ds go to the matrix units in the inputs' 16 bits.  In f16, p is scaled
+// by 2^14 (p <= 1) and ds by the power of two that brings its bound, twice the
+// largest |g_t| |v_s|, to 2^15; the sums are scaled back in fp32.
+
+constexpr int kPtPeaks = 512;
+constexpr float kPtF16P = 14.0f;
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
+    constexpr int LPH = D / 8, HPW = 64 / LPH;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, sub = lane % LPH, grp = lane / LPH;
+    auto norm = [&](const uint4 x, const uint4 y) {          // sum over a head's lanes of x . y
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s = fmaf(pt_value<DT>(u[i]), pt_value<DT>(w[i]), s);
+            s = fmaf(pt_value<DT>(u[i] >> 16), pt_value<DT>(w[i] >> 16), s);
+        }
+#pragma unroll
+        for (int m = LPH / 2; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+        return s;
+    };
+    float pg = 0.0f, pv = 0.0f;
+    const int64_t rows = min((int64_t)max(a.cu[a.B], 0), a.N);   // what lies behind the last sequence counts for nothing
+    for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < rows; t += (int64_t)gridDim.x * 4) {
+        for (int h0 = 0; h0 < a.Hq; h0 += HPW) {
+            const int h = min(h0 + grp, a.Hq - 1);
+            const uint4 g = *reinterpret_cast<const uint4 *>(a.g.p + t * a.g.st + h * a.g.sh + sub * 16);
+            const uint4 o = *reinterpret_cast<const uint4 *>(a.o.p + t * a.o.st + h * a.o.sh + sub * 16);
+            const float d = norm(g, o);
+            if (sub == 0 && h0 + grp < a.Hq) {
+                a.delta[(int64_t)h * a.N + t] = -d;
+                a.lse2[(int64_t)h * a.N + t] = a.lse[(int64_t)h * a.N + t] * 1.44269504f;
+            }
+            // an infinity or NaN stays in its peak: the scale is then 1
+            if constexpr (DT == OMNI_F16) { const float n = norm(g, g); pg = n > pg || n != n ? n : pg; }
+        }
+        if constexpr (DT == OMNI_F16)
+            for (int h0 = 0; h0 < a.Hkv; h0 += HPW) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(a.v.p + t * a.v.st + min(h0 + grp, a.Hkv - 1) * a.v.sh + sub * 16);
+                const float n = norm(v, v);
+                pv = n > pv || n != n ? n : pv;
+            }
+    }
+    if constexpr (DT == OMNI_F16) {
+        __shared__ float peak[2][4];
+#pragma unroll
+        for (int m = 32; m >= LPH; m /= 2) {
+            const float x = __shfl_xor(pg, m, 64), y = __shfl_xor(pv, m, 64);
+            pg = x > pg || x != x ? x : pg;
+            pv = y > pv || y != y ? y : pv;
+        }
+        if (lane == 0) {
+            peak[0][wave] = pg;
+            peak[1][wave] = pv;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            float m = 0.0f;
+            for (int w = 0; w < 4; ++w) { const float x = peak[threadIdx.x][w]; m = x > m || x != x ? x : m; }
+            a.peaks[threadIdx.x * kPtPeaks + blockIdx.x] = m;
+        }
+    }
+}
+
+// The power of two for ds in f16 (1 in bf16), the same in every block.
+template <int DT>
+__device__ __forceinline__ float pt_ds_scale(const PromptArgs &a) {
+    if constexpr (DT == OMNI_BF16) return 1.0f;
+    float m[2] = {0.0f, 0.0f};
+    for (int i = threadIdx.x & 63; i < a.peak_rows; i += 64)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float x = a.peaks[e * kPtPeaks + i];
+            m[e] = x > m[e] || x != x ? x : m[e];
+        }
+#pragma unroll
+    for (int w = 32; w > 0; w /= 2)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float x = __shfl_xor(m[e], w, 64);
+            m[e] = x > m[e] || x != x ? x : m[e];
+        }
+    const float bound = 2.0f * sqrtf(m[0]) * sqrtf(m[1]);
+    if (!(bound > 0.0f) || !(bound < 1.0e30f)) return 1.0f;
+    const int e = 14 - ilogbf(bound);                        // bound 2^e in [2^14, 2^15)
+    return ldexpf(1.0f, min(max(e, -100), 100));
+}
+
+template <int DT, int D>
+struct PtGradRow {
+    static constexpr int NT = D / 32;
+    ps8_t q[D / 16], g[D / 16];
+    pf16_t dq[NT];
+    float lse2, delta;
+    int t;
+};
+
+// One tile of 64 keys for the wave's 32 query rows; transposed like the forward.
+template <int DT, int D, bool MASK>
+__device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, PtGradRow<DT, D> &R, const char *K, const char *V, int j0, int len,
+                                           float up) {
+    const int half = (threadIdx.x >> 5) & 1;
+    const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        pf16_t s = {}, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = R.delta;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(pt_rows<D>(K, 32 * b, kk), R.q[kk], s);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(pt_rows<D>(V, 32 * b, kk), R.g[kk], dp);
+        uint32_t x[8];
+        float ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -R.lse2));
+            ds[i] = p * (DT == OMNI_F16 ? dp[i] * up : dp[i]);
+            if constexpr (MASK) {
+                if (32 * b + 8 * (i / 4) + i % 4 > seen) ds[i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = pt_pack<DT>(ds[2 * i], ds[2 * i + 1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const ps8_t xb = __builtin_bit_cast(ps8_t, make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]));
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) R.dq[d] = pt_mfma<DT>(pt_cols<D>(K, 32 * b + 16 * k, d), xb, R.dq[d]);
+        }
+    }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs a) {
+    __shared__ __attribute__((aligned(16))) char k0[kPtKeys * 2 * D], k1[kPtKeys * 2 * D];
+    __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
+    const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int hk = (int)(bid % a.Hkv);
+    const int64_t r = bid / a.Hkv;
+    const int h = hk * a.G + (int)(r % a.G);
+    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, r / a.G, true);
+    if (S.tile < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int row0 = S.tile * kPtRows;
+    if (S.none) {
+        pt_zero_rows<D, kPtRows>(a.dq, S.start, row0, S.len, h);
+        return;
+    }
+    const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
+    PtCopy<D, kPtKeys> ck, cv;
+    ck.init(a.k.st);
+    cv.init(a.v.st);
+    ck.issue(kb, a.k.st, 0, S.len, k0);
+    cv.issue(vb, a.v.st, 0, S.len, v0);
+
+    PtGradRow<DT, D> R;
+    const int w0 = row0 + 32 * wave;
+    R.t = w0 + (lane & 31);
+    const int64_t at = S.start + min(R.t, S.len - 1);
+    pt_load_rows<D>(a.q.p + at * a.q.st + h * a.q.sh, a.negate ? 0x80008000u : 0u, R.q);
+    pt_load_rows<D>(a.g.p + at * a.g.st + h * a.g.sh, 0u, R.g);
+    R.lse2 = a.lse2[(int64_t)h * a.N + at];
+    R.delta = a.delta[(int64_t)h * a.N + at];
+    const float up = pt_ds_scale<DT>(a);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
+
+    const int kend = a.causal ? min(S.len, row0 + kPtRows) : S.len;
+    const int wlast = a.causal ? min(w0 + 31, S.len - 1) : S.len - 1;
+    const bool live = w0 < S.len;
+    auto step = [&](const char *K, const char *V, int j0) {
+        if (!live || j0 > wlast) return;
+        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_dq_tile<DT, D, true>(a, R, K, V, j0, S.len, up);
+        else pt_dq_tile<DT, D, false>(a, R, K, V, j0, S.len, up);
+    };
+    for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
+        pt_sync();
+        if (j0 + kPtKeys < kend) {
+            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1);
+            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1);
+        }
+        step(k0, v0, j0);
+        if (j0 + kPtKeys >= kend) break;
+        pt_sync();
+        if (j0 + 2 * kPtKeys < kend) {
+            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0);
+            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0);
+        }
+        step(k1, v1, j0 + kPtKeys);
+    }
+    if (!live) return;
+    pt_store<DT, D>(const_cast<char *>(a.dq.p) + (int64_t)(S.start + R.t) * a.dq.st + h * a.dq.sh, R.dq, a.scale / up, R.t < S.len);
+}
+
+// dk and dv: a wave holds 32 keys as B operands of S = Q K^T and G V^T, so
+// that p and ds (rows on registers, keys on lanes) are the B operands of
+// dv^T += G^T P and dk^T += Q^T dS; tiles of 64 rows of q and g go through LDS,
+// one query head of the group after another.
+constexpr int kPtKvWaves = 4;
+constexpr int kPtKvKeys = 32 * kPtKvWaves;
+constexpr int kPtQRows = 64;
+
+template <int DT, int D>
+struct PtGradKey {
+    static constexpr int NT = D / 32;
+    ps8_t k[D / 16], v[D / 16];
+    pf16_t dk[NT], dv[NT];
+    int s;
+};
+
+template <int DT, int D, bool MASK>
+__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, PtGradKey<DT, D> &R, const char *Q, const char *G, const float *lse2,
+                                            const float *delta, int j0, int len, float up) {
+    const int half = (threadIdx.x >> 5) & 1;
+    // register i of block b is row j0 + 32 b + 8 (i / 4) + 4 half + i % 4
+    const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        pf16_t s = {}, dp;
+        float l[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 d4 = *reinterpret_cast<const float4 *>(delta + 32 * b + 2 * i + 4 * half);
+            const float4 l4 = *reinterpret_cast<const float4 *>(lse2 + 32 * b + 2 * i + 4 * half);
+            dp[i] = d4.x; dp[i + 1] = d4.y; dp[i + 2] = d4.z; dp[i + 3] = d4.w;
+            l[i] = l4.x; l[i + 1] = l4.y; l[i + 2] = l4.z; l[i + 3] = l4.w;
+        }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(pt_rows<D>(Q, 32 * b, kk), R.k[kk], s);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(pt_rows<D>(G, 32 * b, kk), R.v[kk], dp);
+        uint32_t x[8], y[8];
+        float p[16], ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[i]));
+            if constexpr (MASK) {
+                const int row = 32 * b + 8 * (i / 4) + i % 4;
+                const bool see = row >= first && row < end;
+                p[i] = see ? p[i] : 0.0f;
+                ds[i] = see ? p[i] * (DT == OMNI_F16 ? dp[i] * up : dp[i]) : 0.0f;
+            } else {
+                ds[i] = p[i] * (DT == OMNI_F16 ? dp[i] * up : dp[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = pt_pack<DT>(p[2 * i], p[2 * i + 1]);
+            y[i] = pt_pack<DT>(ds[2 * i], ds[2 * i + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const ps8_t xb = __builtin_bit_cast(ps8_t, make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]));
+            const ps8_t yb = __builtin_bit_cast(ps8_t, make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]));
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                R.dv[d] = pt_mfma<DT>(pt_cols<D>(G, 32 * b + 16 * k, d), xb, R.dv[d]);
+                R.dk[d] = pt_mfma<DT>(pt_cols<D>(Q, 32 * b + 16 * k, d), yb, R.dk[d]);
+            }
+        }
+    }
+}
+
+// 64 floats of a row statistic, from row j0 of the sequence on (rows from len on repeat the last).
+__device__ __forceinline__ void pt_copy_stat(const float *base, int j0, int len, float *lds) {
+    const int left = min(len - j0, kPtQRows);
+    const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc((void *)(base + j0), (short)0, left * 4, kPtBufWord3);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)lds, 4, (uint32_t)min((int)(threadIdx.x & 63), left - 1) * 4u, 0, 0, 0);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_kernel(PromptArgs a) {
+    __shared__ __attribute__((aligned(16))) char q0[kPtQRows * 2 * D], q1[kPtQRows * 2 * D];
+    __shared__ __attribute__((aligned(16))) char g0[kPtQRows * 2 * D], g1[kPtQRows * 2 * D];
+    __shared__ __attribute__((aligned(16))) float l0[kPtQRows], l1[kPtQRows], d0[kPtQRows], d1[kPtQRows];
+    const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int hk = (int)(bid % a.Hkv);
+    // the first keys are seen by the most rows
+    const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, bid / a.Hkv, false);
+    if (S.tile < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int key0 = S.tile * kPtKvKeys;
+    if (S.none) {
+        pt_zero_rows<D, kPtKvKeys>(a.dk, S.start, key0, S.len, hk);
+        pt_zero_rows<D, kPtKvKeys>(a.dv, S.start, key0, S.len, hk);
+        return;
+    }
+    const int first = a.causal ? key0 / kPtQRows : 0, tiles = (S.len + kPtQRows - 1) / kPtQRows - first;
+    const int n = tiles * a.G;
+    PtCopy<D, kPtQRows> cq, cg;
+    cq.init(a.q.st);
+    cg.init(a.g.st);
+    const char *qb = a.q.p + (int64_t)S.start * a.q.st + (int64_t)hk * a.G * a.q.sh;
+    const char *gb = a.g.p + (int64_t)S.start * a.g.st + (int64_t)hk * a.G * a.g.sh;
+    const float *lb = a.lse2 + (int64_t)hk * a.G * a.N + S.start, *db = a.delta + (int64_t)hk * a.G * a.N + S.start;
+    int gi = 0, ji = first;              // head and tile that the next copy takes
+    auto copy = [&](char *Q, char *G, float *L, float *Dl) {
+        cq.issue(qb + gi * a.q.sh, a.q.st, ji * kPtQRows, S.len, Q);
+        cg.issue(gb + gi * a.g.sh, a.g.st, ji * kPtQRows, S.len, G);
+        if (wave == 0) pt_copy_stat(lb + gi * a.N, ji * kPtQRows, S.len, L);
+        else if (wave == 1) pt_copy_stat(db + gi * a.N, ji * kPtQRows, S.len, Dl);
+        if (++ji == first + tiles) {
+            ji = first;
+            ++gi;
+        }
+    };
+    copy(q0, g0, l0, d0);
+
+    PtGradKey<DT, D> R;
+    const int w0 = key0 + 32 * wave;
+    R.s = w0 + (lane & 31);
+    const int64_t at = S.start + min(R.s, S.len - 1);
+    pt_load_rows<D>(a.k.p + at * a.k.st + hk * a.k.sh, a.negate ? 0x80008000u : 0u, R.k);
+    pt_load_rows<D>(a.v.p + at * a.v.st + hk * a.v.sh, 0u, R.v);
+    const float scale = pt_ds_scale<DT>(a), up = DT == OMNI_F16 ? scale * 6.103515625e-5f : 1.0f;   // p is times 2^14
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) R.dk[d] = R.dv[d] = pf16_t{};
+    const bool live = w0 < S.len;
+    int jc = first;                      // tile in hand
+    auto step = [&](const char *Q, const char *G, const float *L, const float *Dl) {
+        const int j0 = jc * kPtQRows;
+        jc = jc + 1 == first + tiles ? first : jc + 1;
+        if (!live || (a.causal && j0 + kPtQRows - 1 < w0)) return;
+        if (j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31)) pt_dkv_tile<DT, D, true>(a, R, Q, G, L, Dl, j0, S.len, up);
+        else pt_dkv_tile<DT, D, false>(a, R, Q, G, L, Dl, j0, S.len, up);
+    };
+    for (int i = 0; i < n; i += 2) {
+        pt_sync();
+        if (i + 1 < n) copy(q1, g1, l1, d1);
+        step(q0, g0, l0, d0);
+        if (i + 1 >= n) break;
+        pt_sync();
+        if (i + 2 < n) copy(q0, g0, l0, d0);
+        step(q1, g1, l1, d1);
+    }
+    if (!live) return;
+    const bool mine = R.s < S.len;
+    pt_store<DT, D>(const_cast<char *>(a.dk.p) + (int64_t)(S.start + R.s) * a.dk.st + hk * a.dk.sh, R.dk, a.scale / scale, mine);
+    pt_store<DT, D>(const_cast<char *>(a.dv.p) + (int64_t)(S.start + R.s) * a.dv.st + hk * a.dv.sh, R.dv,
+                    DT == OMNI_F16 ? 6.103515625e-5f : 1.0f, mine);
+}
+
+// ── host ────────────────────────────────────────────────────────────────
+
+static int prompt_heads(const char *who, const char *what, const void *p, const int64_t *s, PromptHeads &t) {
+    OMNI_CHECK_ARG(p && s, "%s: NULL %s", who, what);
+    OMNI_CHECK_ARG(reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0,
+                   "%s: %s and its strides must be multiples of 16 bytes", who, what);
+    // a tile's 64 rows are addressed with 32-bit offsets
+    OMNI_CHECK_ARG(s[0] >= 0 && s[0] < (int64_t(1) << 24) && s[1] >= 0, "%s: %s: token stride out of range", who, what);
+    t.p = static_cast<const char *>(p);
+    t.st = 2 * s[0];
+    t.sh = 2 * s[1];
+    return OMNI_OK;
+}
+
+static int prompt_args(const char *who, int dtype, int64_t N, int Hq, int Hkv, int D, const int32_t *cu, int64_t B, float scale,
+                       PromptArgs &a) {
+    OMNI_CHECK_ARG(dtype == OMNI_F16 || dtype == OMNI_BF16, "%s: dtype must be f16 or bf16", who);
+    OMNI_CHECK_ARG(D == 32 || D == 64 || D == 128, "%s: head_dim must be 32, 64 or 128, got %d", who, D);
+    OMNI_CHECK_ARG(N >= 0 && B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "%s: bad shape (Hq must be a multiple of Hkv)", who);
+    OMNI_CHECK_ARG(N < (int64_t(1) << 31) - 1024 && B < (int64_t(1) << 30) && Hq <= 65536, "%s: shape too large", who);
+    OMNI_CHECK_ARG(scale == scale && fabsf(scale) <= 3.0e38f, "%s: scale must be finite", who);
+    a.N = N;
+    a.B = (int)B;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.G = Hq / Hkv;
+    a.cu = cu;
+    a.negate = scale < 0.0f;
+    a.scale = scale;
+    a.c = fabsf(scale) * 1.44269504088896f;
+    return OMNI_OK;
+}
+
+// Fewer than 2^32 threads in a dimension.
+static bool prompt_grid(int64_t blocks, dim3 &grid) {
+    const int64_t gx = blocks < (1 << 22) ? blocks : (1 << 22), gy = (blocks + gx - 1) / gx;
+    grid = dim3((unsigned)gx, (unsigned)gy);
+    return gy <= 65535;
+}
+
+}  // namespace omni
+
+using namespace omni;
+
+#define OMNI_TRY(call)                   \
+    do {                                 \
+        const int rc_ = (call);          \
+        if (rc_ != OMNI_OK) return rc_;  \
+    } while (0)
+
+template <int DT>
+static void prompt_launch_forward(const PromptArgs &a, int D, dim3 grid, hipStream_t st) {
+    const dim3 block(64 * kPtWaves);
+    if (D == 32) hipLaunchKernelGGL((prompt_forward_kernel<DT, 32>), grid, block, 0, st, a);
+    else if (D == 64) hipLaunchKernelGGL((prompt_forward_kernel<DT, 64>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((prompt_forward_kernel<DT, 128>), grid, block, 0, st, a);
+}
+
+extern "C" int omni_prompt_attn(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv, int head_dim,
+                                const int32_t *cu_seqlens, int64_t B, float scale, int causal, int fill_rest, void *out,
+                                const int64_t *out_strides, float *lse, void *stream) {
+    const char *who = "omni_prompt_attn";
+    PromptArgs a = {};
+    OMNI_TRY(prompt_args(who, dtype, N, Hq, Hkv, head_dim, cu_seqlens, B, scale, a));
+    if (N == 0) return OMNI_OK;
+    OMNI_TRY(prompt_heads(who, "q", q, q_strides, a.q));
+    OMNI_TRY(prompt_heads(who, "k", k, k_strides, a.k));
+    OMNI_TRY(prompt_heads(who, "v", v, v_strides, a.v));
+    OMNI_TRY(prompt_heads(who, "out", out, out_strides, a.o));
+    OMNI_CHECK_ARG(cu_seqlens, "%s: NULL cu_seqlens", who);
+    a.lse = lse;
+    a.causal = causal != 0;
+    a.fill = fill_rest != 0;
+    dim3 grid;
+    OMNI_CHECK_ARG(prompt_grid((N / kPtRows + B + 1) * Hq, grid), "%s: grid too large", who);
+    if (dtype == OMNI_F16) prompt_launch_forward<OMNI_F16>(a, head_dim, grid, as_stream(stream));
+    else prompt_launch_forward<OMNI_BF16>(a, head_dim, grid, as_stream(stream));
+    OMNI_CHECK_LAUNCH(who);
+    return OMNI_OK;
+}
+
+template <int DT, int D>
+static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
+    const char *who = "omni_prompt_attn_backward";
+    dim3 rows, keys;
+    OMNI_CHECK_ARG(prompt_grid((a.N / kPtRows + a.B + 1) * a.Hq, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv, keys),
+                   "%s: grid too large", who);
+    hipLaunchKernelGGL((prompt_delta_kernel<DT, D>), dim3(a.peak_rows), dim3(256), 0, st, a);
+    OMNI_CHECK_LAUNCH(who);
+    hipLaunchKernelGGL((prompt_dq_kernel<DT, D>), rows, dim3(64 * kPtWaves), 0, st, a);
+    OMNI_CHECK_LAUNCH(who);
+    hipLaunchKernelGGL((prompt_dkv_kernel<DT, D>), keys, dim3(64 * kPtKvWaves), 0, st, a);
+    OMNI_CHECK_LAUNCH(who);
+    return OMNI_OK;
+}
+
+extern "C" size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq) {
+    return N > 0 && Hq > 0 ? (size_t)N * (size_t)Hq * 8 + kPtPeaks * 8 : 0;
+}
+
+extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                                         const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv,
+                                         int head_dim, const int32_t *cu_seqlens, int64_t B, float scale, int causal,
+                                         const void *out, const int64_t *out_strides, const float *lse, const void *dout,
+                                         const int64_t *dout_strides, void *dq, const int64_t *dq_strides, void *dk,
+                                         const int64_t *dk_strides, void *dv, const int64_t *dv_strides, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+    const char *who = "omni_prompt_attn_backward";
+    PromptArgs a = {};
+    OMNI_TRY(prompt_args(who, dtype, N, Hq, Hkv, head_dim, cu_seqlens, B, scale, a));
+    if (N == 0) return OMNI_OK;
+    OMNI_TRY(prompt_heads(who, "q", q, q_strides, a.q));
+    OMNI_TRY(prompt_heads(who, "k", k, k_strides, a.k));
+    OMNI_TRY(prompt_heads(who, "v", v, v_strides, a.v));
+    OMNI_TRY(prompt_heads(who, "out", out, out_strides, a.o));
+    OMNI_TRY(prompt_heads(who, "dout", dout, dout_strides, a.g));
+    OMNI_TRY(prompt_heads(who, "dq", dq, dq_strides, a.dq));
+    OMNI_TRY(prompt_heads(who, "dk", dk, dk_strides, a.dk));
+    OMNI_TRY(prompt_heads(who, "dv", dv, dv_strides, a.dv));
+    OMNI_CHECK_ARG(cu_seqlens && lse, "%s: NULL cu_seqlens or lse", who);
+    const size_t need = omni_prompt_attn_backward_workspace_size(N, Hq);
+    if (!workspace || workspace_bytes < need) {
+        set_error("%s: workspace of %zu bytes needed", who, need);
+        return OMNI_EWORKSPACE;
+    }
+    OMNI_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", who);
+    a.lse = const_cast<float *>(lse);
+    a.peaks = static_cast<float *>(workspace);
+    a.lse2 = a.peaks + 2 * kPtPeaks;
+    a.delta = a.lse2 + (size_t)N * Hq;
+    a.causal = causal != 0;
+    a.peak_rows = (int)(N / 4 + 1 < kPtPeaks ? N / 4 + 1 : kPtPeaks);
+    hipStream_t st = as_stream(stream);
+    if (dtype == OMNI_F16) {
+        if (head_dim == 32) return prompt_launch_backward<OMNI_F16, 32>(a, st);
+        if (head_dim == 64) return prompt_launch_backward<OMNI_F16, 64>(a, st);
+        return prompt_launch_backward<OMNI_F16, 128>(a, st);
+    }
+    if (head_dim == 32) return prompt_launch_backward<OMNI_BF16, 32>(a, st);
+    if (head_dim == 64) return prompt_launch_backward<OMNI_BF16, 64>(a, st);
+    return prompt_launch_backward<OMNI_BF16, 128>(a, st);
+}

@@ -225,29 +225,31 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two (rows, heads, dim) tensors may share memory.  Slices of one
+    buffer interleave (q and k of a fused projection): those are apart where a
+    row's heads of each lie within rows of the same length, at columns of their
+    own."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() != 3 or b.dim() != 3 or a.stride(0) != b.stride(0):
+        return True
+    row = a.stride(0) * a.element_size()
+    la, lb = (_span(t[:1])[1] - _span(t[:1])[0] for t in (a, b))
+    off = (b0 - a0) % row if row else 0
+    return off < la or off + lb > row
+
+
 def _check_overlap(q, k, out):
-    """In place means exactly in place.  Slices of one buffer interleave (q and
-    k of a fused projection): those pass where their rows keep to their own
-    columns, which equal strides show."""
+    """In place means exactly in place."""
     def same(a, b):
         return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
-
-    def apart(a, b):
-        (a0, a1), (b0, b1) = _span(a), _span(b)
-        if a1 <= b0 or b1 <= a0:
-            return True
-        # one token's heads of each lie within a row of the same length, at columns of their own
-        if a.dim() != 3 or b.dim() != 3 or a.stride(0) != b.stride(0) or a.shape[0] != b.shape[0]:
-            return False
-        row = a.stride(0) * a.element_size()
-        la, lb = (_span(t[:1])[1] - _span(t[:1])[0] for t in (a, b))
-        off = b0 - a0
-        return la <= off and off + lb <= row if off >= 0 else lb <= -off and -off + la <= row
 
     qo, ko = out
     for o in out:
         if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
             raise ValueError("out must not be a broadcast view")
-    if not (apart(qo, ko) and apart(qo, k) and apart(ko, q) and (same(qo, q) or apart(qo, q))
-            and (same(ko, k) or apart(ko, k))):
+    if overlap(qo, ko) or overlap(qo, k) or overlap(ko, q) or not (same(qo, q) or not overlap(qo, q)) or \
+            not (same(ko, k) or not overlap(ko, k)):
         raise ValueError("out may be q and k themselves, but must not overlap them otherwise")

@@ -1,0 +1,316 @@
+"""Attention of packed prompts (omni_prompt_attn) and its gradient against the
+definition in 64 bits.
+
+Bars, derived before the first run.  u is half a step of the inputs' type,
+u32 that of fp32.  Scores are fp32 sums of exact products: each is off by at
+most (D + 2) u32 |scale| sum |q||k| <= X, an absolute error in the exponent, so
+a probability is off by a factor within 1 +- (2 X + 2^-20) (its own error, the
+row sum's and the exponential's).  A probability is then rounded to the
+inputs' type, u p, before the product with v (row sums take the unrounded).
+So |o - o'| <= (u + 2 X + 2^-20) sum_s p |v| + u |o|.
+Backward, with e = 2 X + 2^-20 + u for a rounded probability: dv is off by
+e sum p |g| + u |dv|.  dp - delta is an fp32 sum of D products, and delta comes
+from the rounded output: off by Y = (u + D u32) (|g| . |o| + sum_d |g||v|) + |g| . |o - o'|;
+ds = p (dp - delta) by p Y + (e + u) |ds|; dq and dk by |scale| times the sum of
+that with |k| or |q|, and u of themselves.  f16 subnormals: probabilities are
+held times 2^7 at least, ds at least 2^-26 of its bound 2 max|g| max|v|.  bf16 goes
+as far down as fp32, whose exponential gives 0 below the smallest normal, and
+whose products do: 2^-126 a probability and a ds more (at scale 3 a key's
+gradient was 0 for 1.9e-38, all of its terms of that size, before this term was
+in the bar).
+"""
+import math
+
+import pytest
+import torch
+
+from tests import _data
+
+gpu = pytest.mark.gpu
+U32 = 2.0 ** -24
+DT = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _cu(lengths, extra=0):
+    c = [0]
+    for n in lengths:
+        c.append(c[-1] + n)
+    return torch.tensor(c, dtype=torch.int32), c[-1] + extra
+
+
+def _inputs(N, Hq, Hkv, D, dtype, seed, gain=1.0):
+    g = _data.gen(seed)
+    mk = lambda h: torch.randn(N, h, D, generator=g)  # noqa: E731
+    return (mk(Hq) * gain).to(DT[dtype]), mk(Hkv).to(DT[dtype]), mk(Hkv).to(DT[dtype]), mk(Hq).to(DT[dtype])
+
+
+def _visible(x, seen):
+    """0 where not seen, whatever stands there."""
+    return torch.where(seen, x, torch.zeros_like(x))
+
+
+def _want(q, k, v, cu, causal, scale, do=None):
+    """Outputs, gradients and their bars in float64 on the inputs' device, by
+    sequence and head; hidden keys and rows count for nothing, NaN or not."""
+    u, D, G = torch.finfo(q.dtype).eps / 2, q.shape[2], q.shape[1] // k.shape[1]
+    q64, k64, v64 = q.double(), k.double(), v.double()
+    o, ob = torch.zeros_like(q64), torch.zeros_like(q64)
+    lse = torch.full((q.shape[1], q.shape[0]), -math.inf, dtype=torch.float64, device=q.device)
+    r = dict(o=(o, ob), lse=lse)
+    if do is not None:
+        g64 = do.double()
+        for n, t in (("dq", q64), ("dk", k64), ("dv", v64)):
+            r[n] = (torch.zeros_like(t), torch.zeros_like(t))
+        n = int(cu[-1])
+        tiny = 2.0 ** -25 * (g64[:n].norm(dim=-1).max() * v64[:n].norm(dim=-1).max()) if n and q.dtype == torch.float16 else 0.0
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        if a == b:
+            continue
+        see = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device)
+        if causal:
+            see = see.tril()
+        for h in range(q.shape[1]):
+            Q, K, V = q64[a:b, h], k64[a:b, h // G], v64[a:b, h // G]
+            s = torch.where(see, Q @ K.T * scale, -math.inf)
+            p = torch.softmax(s, -1)
+            l = torch.logsumexp(s, -1)
+            X = (D + 2) * U32 * abs(scale) * _visible(Q.abs() @ K.abs().T, see)
+            e = u + 2 * X.amax(-1, keepdim=True) + 2.0 ** -20
+            O = p @ V
+            o[a:b, h], lse[h, a:b] = O, l
+            pmin = 2.0 ** -126 if q.dtype == torch.bfloat16 else 2.0 ** -31
+            ob[a:b, h] = u * O.abs() + e * (p @ V.abs()) + pmin * (see.double() @ V.abs())
+            if do is None:
+                continue
+            g = g64[a:b, h]
+            dp = g @ V.T
+            delta = (g * O).sum(-1, keepdim=True)
+            Y = (u + D * U32) * (g.abs() @ V.abs().T + (g.abs() * O.abs()).sum(-1, keepdim=True)) + \
+                (g.abs() * ob[a:b, h]).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            dsb = p * Y + (e + u) * ds.abs() + (tiny + 2.0 ** -126 * (1 + (dp - delta).abs())) * see.double()
+            r["dq"][0][a:b, h] = ds @ K * scale
+            r["dq"][1][a:b, h] = dsb @ K.abs() * abs(scale) + u * (ds @ K * scale).abs()
+            r["dk"][0][a:b, h // G] += ds.T @ Q * scale
+            r["dk"][1][a:b, h // G] += dsb.T @ Q.abs() * abs(scale)
+            r["dv"][0][a:b, h // G] += p.T @ g
+            pm = 2.0 ** -126 if q.dtype == torch.bfloat16 else 2.0 ** -38
+            r["dv"][1][a:b, h // G] += (p * e).T @ g.abs() + pm * (see.double().T @ g.abs())
+    if do is not None:
+        for n in ("dk", "dv"):
+            r[n][1].add_(u * r[n][0].abs())
+    return r
+
+
+def _close(got, want, bar, tag):
+    dtype, got = got.dtype, got.double()
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0          # an f16 subnormal's half step
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan), f"{tag}: NaN in other places"
+    err = torch.where(nan, 0.0, (got - want).abs())
+    err = torch.where(got == want, 0.0, err)                          # infinities alike
+    bar = torch.where(nan, 1.0, bar + tiny)
+    worst = torch.where(err == 0, 0.0, err / bar).max().item() if err.numel() else 0.0
+    print(f"[prompt] {tag}: worst error / bar {worst:.3f}", flush=True)
+    if not worst <= 1.0:
+        i = torch.where(err == 0, 0.0, err / bar).argmax()
+        raise AssertionError(f"{tag}: {worst} at {int(i)}: {got.reshape(-1)[i].item()} for {want.reshape(-1)[i].item()}, "
+                             f"bar {bar.reshape(-1)[i].item()}")
+
+
+SHAPES = [
+    # lengths, rows behind the last, Hq, Hkv, D, dtype, causal
+    ([1], 0, 1, 1, 128, "bf16", True),
+    ([64], 0, 4, 1, 128, "bf16", True),
+    ([200], 3, 8, 2, 128, "bf16", True),
+    ([50] * 7, 0, 6, 3, 128, "f16", True),
+    ([0, 33, 0, 1, 129, 128, 0], 40, 4, 2, 128, "bf16", True),
+    ([257, 127, 63, 65], 0, 4, 4, 128, "f16", False),
+    ([700], 0, 5, 1, 64, "bf16", True),
+    ([31, 300, 2], 130, 8, 8, 64, "f16", True),
+    ([190, 191], 0, 2, 1, 64, "bf16", False),
+    ([513, 40], 0, 6, 2, 32, "f16", True),
+    ([97] * 5, 7, 16, 4, 32, "bf16", False),
+    ([1] * 200, 0, 2, 1, 32, "bf16", True),
+    ([], 5, 2, 1, 64, "bf16", True),
+    ([1030], 0, 2, 2, 128, "f16", False),
+]
+
+
+@gpu
+@pytest.mark.parametrize("lengths,extra,Hq,Hkv,D,dtype,causal", SHAPES)
+def test_outputs_and_gradients(device, lengths, extra, Hq, Hkv, D, dtype, causal):
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu(lengths, extra)
+    q, k, v, do = (t.to(device) for t in _inputs(N, Hq, Hkv, D, dtype, 900 + N + D))
+    if extra:                                       # what lies behind the last sequence is not looked at
+        for t in (q, k, v, do):
+            t[N - extra:] = float("nan")
+    scale = 1 / math.sqrt(D)
+    want = _want(q, k, v, cu, causal, scale, do)
+    print(f"[prompt] {lengths[:8]} +{extra} {Hq}/{Hkv} D{D} {dtype} causal={causal}", flush=True)
+    plain, plse = prompt_attention(q, k, v, cu.to(device), causal=causal, return_lse=True)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o, lse = prompt_attention(*leaves, cu.to(device), causal=causal, return_lse=True)
+    assert torch.equal(o, plain) and torch.equal(lse, plse)
+    _close(o.detach(), *want["o"], "out")
+    live = torch.isfinite(want["lse"])
+    assert torch.equal(torch.isfinite(lse), live)
+    assert bool(((lse.double() - want["lse"])[live].abs() < 2e-5).all())
+    grads = torch.autograd.grad(o, leaves, do)
+    again = torch.autograd.grad(prompt_attention(*leaves, cu.to(device), causal=causal), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again)), "not the same on a second run"
+    for n, g in zip(("dq", "dk", "dv"), grads):
+        _close(g, *want[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [0.3, -0.2, 0.0, 3.0])
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f16", 32)])
+def test_scales(device, scale, dtype, D):
+    """Negative, zero and sharp scores."""
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([150, 5])
+    q, k, v, do = (t.to(device) for t in _inputs(N, 4, 2, D, dtype, 41))
+    want = _want(q, k, v, cu, True, scale, do)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = prompt_attention(*leaves, cu, scale=scale)
+    _close(o.detach(), *want["o"], f"scale {scale} out")
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)):
+        _close(g, *want[n], f"scale {scale} {n}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("gain", [2.0 ** -12, 2.0 ** 9])
+def test_small_and_large_gradients(device, dtype, gain):
+    """Gradients far from one: f16's range is not left and its subnormals cost nothing."""
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([260, 70])
+    q, k, v, do = (t.to(device) for t in _inputs(N, 4, 1, 64, dtype, 43))
+    do = do * gain
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(prompt_attention(*leaves, cu), leaves, do)
+    want = _want(q.detach(), k.detach(), v.detach(), cu, True, 0.125, do)
+    for n, g in zip(("dq", "dk", "dv"), grads):
+        _close(g, *want[n], f"gain {gain} {n}")
+
+
+@gpu
+def test_growing_scores(device):
+    """Each key's score above the last by a few powers of two: the running
+    maximum moves in every tile, the sums are rescaled, and slack is used."""
+    from omnistack_rs.attention import prompt_attention
+    for step in (0.05, 0.7, -0.5):
+        N, D = 300, 128
+        q = torch.ones(N, 2, D, device=device, dtype=torch.bfloat16)
+        k = (torch.arange(N, device=device)[:, None, None] * step / D).to(torch.bfloat16).expand(N, 1, D).contiguous()
+        _, _, v, do = (t.to(device) for t in _inputs(N, 2, 1, D, "bf16", 44))
+        cu = torch.tensor([0, N])
+        want = _want(q, k, v, cu, True, 1.0, do)
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        o = prompt_attention(*leaves, cu, scale=1.0)
+        _close(o.detach(), *want["o"], f"step {step}")
+        for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)):
+            _close(g, *want[n], f"step {step} {n}")
+
+
+@gpu
+def test_layouts_and_out(device):
+    """Slices of a fused projection, head-major storage, odd starts: the same
+    bits; `out` keeps the rows behind the last sequence."""
+    from omnistack_rs.attention import prompt_attention
+    lengths, Hq, Hkv, D = [130, 70], 4, 2, 64
+    cu, N = _cu(lengths, 9)
+    q, k, v, _ = (t.to(device) for t in _inputs(N, Hq, Hkv, D, "bf16", 45))
+    cu = cu.to(device)
+    want = prompt_attention(q, k, v, cu)
+    assert bool((want[200:] == 0).all())
+    buf = torch.cat([t.reshape(N, -1) for t in (q, k, v)], 1)
+    qs, ks, vs = (t.view(N, -1, D) for t in buf.split([Hq * D, Hkv * D, Hkv * D], 1))
+    assert torch.equal(prompt_attention(qs, ks, vs, cu), want)
+    hm = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert torch.equal(prompt_attention(*hm, cu), want)
+    odd = [torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape) for t in (q, k, v)]
+    assert torch.equal(prompt_attention(*odd, cu), want)
+    assert torch.equal(prompt_attention(q, k, v, [0, 130, 200]), want)
+    out = torch.full((N, Hq, D), 7.0, device=device, dtype=q.dtype)
+    assert prompt_attention(q, k, v, cu, out=out) is out
+    assert torch.equal(out[:200], want[:200]) and bool((out[200:] == 7).all())
+    with pytest.raises(ValueError, match="overlap"):
+        prompt_attention(q, k, v, cu, out=q)
+    with pytest.raises(ValueError, match="gradient"):
+        prompt_attention(q.clone().requires_grad_(), k, v, cu, out=out)
+    with pytest.raises(ValueError, match="rise"):
+        prompt_attention(q, k, v, torch.tensor([0, 5, 4], device=device))
+
+
+@gpu
+def test_capture_and_other_stream(device):
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([90, 1, 200])
+    q, k, v, do = (t.to(device) for t in _inputs(N, 4, 2, 128, "f16", 46))
+    cu = cu.to(device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = prompt_attention(*leaves, cu, validate=False)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    alive = prompt_attention(*leaves, cu, validate=False)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            q.mul_(1.25)
+            do.mul_(-0.5)
+            cu.copy_(torch.tensor([0, 100 + i, 150, 291]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), f"replay {i}"
+
+
+def test_refusals():
+    """Checked before any device work: on CPU tensors the last check is the device's."""
+    from omnistack_rs.attention import prompt_attention
+    q, k = torch.zeros(9, 4, 64, dtype=torch.bfloat16), torch.zeros(9, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="HIP"):
+        prompt_attention(q, k, k, [0, 9])
+    for args, kw in [((q[0], k, k, [0, 9]), {}), ((q, k, k[:8], [0, 9]), {}), ((q[:, :3], k, k, [0, 9]), {}),
+                     ((q[..., :48], k[..., :48], k[..., :48], [0, 9]), {}), ((q.float(), k.float(), k.float(), [0, 9]), {}),
+                     ((q, k.half(), k, [0, 9]), {}), ((q, k, k, [0, 10]), {}), ((q, k, k, [1, 9]), {}), ((q, k, k, [0, 5, 4]), {}),
+                     ((q, k, k, []), {}), ((q, k, k, [0.0, 9.0]), {}), ((q, k, k, [0, 9]), dict(scale=float("nan"))),
+                     ((q, k, k, [0, 9]), dict(scale=float("inf"))), ((q, k, k, [[0, 9]]), {})]:
+        with pytest.raises(ValueError):
+            prompt_attention(*args, **kw)
+
+
+def test_native_refusals():
+    import ctypes
+    from omnistack_rs import _lib
+    L = _lib.lib()
+    s, odd, far = ((ctypes.c_int64 * 2)(*x) for x in ((128, 64), (127, 64), (1 << 24, 64)))
+
+    def call(q=4096, qs=s, dtype=2, N=5, Hq=2, Hkv=1, D=64, cu=4096, B=1, scale=1.0):
+        return L.omni_prompt_attn(q, qs, 4096, s, 4096, s, dtype, N, Hq, Hkv, D, cu, B, scale, 1, 1, 4096, s, None, None)
+    for kw, msg in ((dict(dtype=0), "f16 or bf16"), (dict(D=48), "head_dim"), (dict(Hq=3, Hkv=2), "multiple"), (dict(N=-1), "shape"),
+                    (dict(N=1 << 31), "large"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
+                    (dict(q=None), "NULL"), (dict(q=4104), "16 bytes"), (dict(qs=odd), "16 bytes"), (dict(qs=far), "stride"),
+                    (dict(cu=None), "NULL")):
+        assert call(**kw) == _lib.OMNI_EINVAL and msg in _lib.last_error(), (kw, _lib.last_error())
+    assert call(N=0, q=None) == 0
+    assert L.omni_prompt_attn_backward_workspace_size(10, 4) == 10 * 4 * 8 + 4096
+    a = (4096, s)
+    rc = L.omni_prompt_attn_backward(*a, *a, *a, 2, 5, 2, 1, 64, 4096, 1, 1.0, 1, *a, 4096, *a, *a, *a, *a, 4096, 100, None)
+    assert rc == _lib.OMNI_EWORKSPACE and "workspace" in _lib.last_error()
