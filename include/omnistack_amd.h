@@ -479,6 +479,7 @@ int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const vo
  * Device pointers with host element strides {token, head}; the last dim is
  * contiguous, pointers and strides are multiples of 16 bytes, a token stride is
  * below 2^24 elements.  lse (Hq, N) f32 or NULL: log sum_s exp(scale q_t . k_s).
+ * out_rest (as out) or NULL: what the rounding of out left, for the gradient.
  * Rows behind the last sequence: zeros (lse -inf) when fill_rest, else left as
  * they were.  cu_seqlens that break the rules give rows of no meaning, but
  * nothing outside the tensors is read or written.
@@ -486,11 +487,12 @@ int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const vo
 int omni_prompt_attn(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
                      const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv, int head_dim,
                      const int32_t *cu_seqlens, int64_t B, float scale, int causal, int fill_rest,
-                     void *out, const int64_t *out_strides, float *lse, void *stream);
+                     void *out, const int64_t *out_strides, float *lse,
+                     void *out_rest, const int64_t *out_rest_strides, void *stream);
 
 /*
- * Its gradient: out and lse are the forward's results for these inputs, dout
- * the gradient of out; writes dq, dk, dv (dk and dv summed over the group's
+ * Its gradient: out, out_rest and lse are the forward's results for these
+ * inputs, dout the gradient of out; writes dq, dk, dv (dk and dv summed over the group's
  * query heads), zeros in rows behind the last sequence.  No atomics: the same
  * bits on every run.  workspace (16-byte aligned):
  * omni_prompt_attn_backward_workspace_size(N, Hq) bytes.
@@ -499,7 +501,8 @@ size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq);
 int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
                               const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv,
                               int head_dim, const int32_t *cu_seqlens, int64_t B, float scale, int causal,
-                              const void *out, const int64_t *out_strides, const float *lse,
+                              const void *out, const int64_t *out_strides,
+                              const void *out_rest, const int64_t *out_rest_strides, const float *lse,
                               const void *dout, const int64_t *dout_strides,
                               void *dq, const int64_t *dq_strides, void *dk, const int64_t *dk_strides,
                               void *dv, const int64_t *dv_strides, void *workspace, size_t workspace_bytes,

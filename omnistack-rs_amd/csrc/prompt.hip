@@ -8,6 +8,8 @@
 // kernel (attention/reference.py:72-177).
 #include <math.h>
 
+#include <type_traits>
+
 #include "omni_common.h"
 
 namespace omni {
@@ -36,7 +38,7 @@ struct PromptHeads {
 };
 
 struct PromptArgs {
-    PromptHeads q, k, v, o;
+    PromptHeads q, k, v, o, olo;         // olo: what rounding took from o, for the gradient
     PromptHeads g, dq, dk, dv;           // backward: the output's gradient, and those of q, k and v
     float *lse;                          // (Hq, N), or NULL
     float *lse2, *delta;                 // backward, (Hq, N): lse log2 e, and -sum_d g o
@@ -70,6 +72,22 @@ __device__ __forceinline__ uint32_t pt_pack(float a, float b) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, h2));
     }
+}
+
+// Sum of the two values of a word and c.
+template <int DT>
+__device__ __forceinline__ float pt_add2(uint32_t v, float c) {
+    if constexpr (DT == OMNI_BF16) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v), __builtin_bit_cast(b2, 0x3f803f80u), c, false);
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v), __builtin_bit_cast(h2, 0x3c003c00u), c, false);
+    }
+}
+
+__device__ __forceinline__ ps8_t pt_frag(const uint32_t *p) {
+    return __builtin_bit_cast(ps8_t, make_uint4(p[0], p[1], p[2], p[3]));
 }
 
 template <int DT>
@@ -108,65 +126,80 @@ __device__ __forceinline__ int pt_swz(int r) {
     else return (r >> 2) & 3;
 }
 
-// The copy of a tile: lane's chunk and row of each of the wave's instructions
-// (the copy writes LDS in lane order, so the swizzle is in the address read).
+// The copy of a tile, N instructions a wave, each a KB of LDS in lane order (so
+// the swizzle is in the address read): instruction u takes rows
+// RPI * kPtWaves * u on, 16, 32 or 64 rows apart, which swizzle alike.
 template <int D, int ROWS>
 struct PtCopy {
-    static constexpr int CH = D / 8, RPI = 64 / CH, N = ROWS * CH / (64 * kPtWaves);
-    static_assert(N >= 1 && ROWS * CH % (64 * kPtWaves) == 0, "whole instructions");
-    int row, off;                        // of instruction 0; instruction u: rows RPI * kPtWaves * u on
-    uint32_t stride;
+    static constexpr int CH = D / 8, RPI = 64 / CH, STEP = RPI * kPtWaves, N = ROWS / STEP;
+    static_assert(N >= 1 && ROWS % STEP == 0, "whole instructions");
+    int row, chunk;                      // lane's row and byte in the row, of instruction 0
 
-    __device__ __forceinline__ void init(int64_t st) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-        row = wave * RPI + lane / CH;
-        stride = (uint32_t)st;
-        // rows of one lane's instructions are RPI * kPtWaves = 16, 32 or 64 apart: one swizzle
-        off = ((lane % CH) ^ pt_swz<D>(row)) * 16;
+    __device__ __forceinline__ void init() {
+        const int lane = threadIdx.x & 63;
+        row = threadIdx.x / 64 * RPI + lane / CH;
+        chunk = ((lane % CH) ^ pt_swz<D>(row)) * 16;
     }
-    // Rows r0 .. r0 + ROWS - 1 of a head at `base` (its row 0); rows from `len` on repeat the last.
+    // Rows r0 .. r0 + ROWS - 1 of a head at `base` (its row 0) to `lds`; rows from `len` on repeat the last.
     __device__ __forceinline__ void issue(const char *base, int64_t st, int r0, int len, char *lds) const {
+        const uint32_t stride = (uint32_t)st;
         const int left = min(len - r0, ROWS);
         const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc(
             (void *)(base + (int64_t)r0 * st), (short)0, (int)((uint32_t)(left - 1) * stride + 2 * D), kPtBufWord3);
         char *dst = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
+        int r = row;
+        asm volatile("" : "+v"(r));      // no register for each instruction's offset through the loop
         if (left == ROWS) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)(dst + u * 1024 * kPtWaves), 16,
-                                                         (uint32_t)(row + RPI * kPtWaves * u) * stride + off, 0, 0, 0);
+                                                         (uint32_t)r * stride + chunk, STEP * u * stride, 0, 0);
         } else {
 #pragma unroll
             for (int u = 0; u < N; ++u)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)(dst + u * 1024 * kPtWaves), 16,
-                                                         (uint32_t)min(row + RPI * kPtWaves * u, left - 1) * stride + off, 0, 0, 0);
+                                                         (uint32_t)min(r + STEP * u, left - 1) * stride + chunk, 0, 0, 0);
         }
     }
 };
 
-// A operand of rows r0 .. r0 + 31, dims 16 kk .. 16 kk + 15.
+// A lane's byte offsets in a tile: of its row's chunk in the row reads, and of
+// its part of four rows in the transposed ones.  Every other read of the lane
+// is these with bits flipped and a constant added (the swizzle of rows 16 on is
+// the same; dims and the upper eight rows flip chunk bits).  fresh() hides that
+// they do not change: the compiler would keep each sum of a buffer's address
+// and an offset in a register of its own through the loop, 50 of them, instead
+// of adding it in the read.
 template <int D>
-__device__ __forceinline__ ps8_t pt_rows(const char *tile, int r0, int kk) {
-    const int lane = threadIdx.x & 63, r = r0 + (lane & 31), ch = 2 * kk + (lane >> 5);
-    return *reinterpret_cast<const ps8_t *>(tile + r * (2 * D) + ((ch ^ pt_swz<D>(r)) * 16));
-}
-
-// A operand of the transposed tile: dims 32 dt .. 32 dt + 31 by rows r0 ..
-// r0 + 15, the rows in the order of an MFMA result's registers: slot (half, j)
-// is row 8 (j / 4) + 4 half + j % 4.
-template <int D>
-__device__ __forceinline__ ps8_t pt_cols(const char *tile, int r0, int dt) {
-    const int lane = threadIdx.x & 63, i = lane & 15;
-    const int byte = (32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3)) * 2;
-    ps4_t v[2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const int r = r0 + 8 * g + 4 * (lane >> 5) + i / 4;
-        v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (PT_LDS ps4_t *)(tile + r * (2 * D) + (((byte >> 4) ^ pt_swz<D>(r)) * 16) + (byte & 15)));
+struct PtLane {
+    uint32_t r, c;
+    __device__ __forceinline__ void init() {
+        const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31, i = lane & 15;
+        r = n * (2 * D) + ((half ^ pt_swz<D>(n)) * 16);
+        const int row = 4 * half + i / 4, byte = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) * 2;
+        c = row * (2 * D) + (((byte >> 4) ^ pt_swz<D>(row)) * 16) + (byte & 15);
     }
-    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-}
+    __device__ __forceinline__ PtLane fresh() const {
+        PtLane x = *this;
+        asm volatile("" : "+v"(x.r), "+v"(x.c));
+        return x;
+    }
+    // A operand of rows r0 .. r0 + 31 (a multiple of 32), dims 16 kk .. 16 kk + 15
+    __device__ __forceinline__ ps8_t rows(const char *tile, int r0, int kk) const {
+        return *reinterpret_cast<const ps8_t *>(tile + ((r ^ (uint32_t)(32 * kk)) + (uint32_t)(r0 * 2 * D)));
+    }
+    // A operand of the transposed tile: dims 32 dt .. 32 dt + 31 by rows r0 .. r0 +
+    // 15, the rows in the order of an MFMA result's registers: slot (half, j) is
+    // row 8 (j / 4) + 4 half + j % 4
+    __device__ __forceinline__ ps8_t cols(const char *tile, int r0, int dt) const {
+        ps4_t v[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            v[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (PT_LDS ps4_t *)(tile + ((c ^ (uint32_t)(64 * dt + 32 * g)) + (uint32_t)((r0 + 8 * g) * 2 * D))));
+        return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // Row operand of 32 rows straight from memory: lane's row at `p`, dims 8 half on.
 template <int D>
@@ -182,23 +215,36 @@ __device__ __forceinline__ void pt_load_rows(const char *p, uint32_t flip, ps8_t
 
 // x times f, of the lane's row, to `p`: register i of block d is dim
 // 32 d + 8 (i / 4) + 4 half + i % 4; after the swap each half holds eight dims.
-template <int DT, int D>
-__device__ __forceinline__ void pt_store(char *p, const pf16_t (&x)[D / 32], float f, bool mine) {
+// LO: what the rounding leaves, rounded, to `q`.
+template <int DT, int D, bool LO = false>
+__device__ __forceinline__ void pt_store(char *p, const pf16_t (&x)[D / 32], float f, bool mine, char *q = nullptr) {
     const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
-            uint32_t u[2][2];
+            uint32_t u[2][2], w[2][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t lo = pt_pack<DT>(x[d][4 * g + 2 * e] * f, x[d][4 * g + 2 * e + 1] * f);
-                const uint32_t hi = pt_pack<DT>(x[d][4 * g + 4 + 2 * e] * f, x[d][4 * g + 4 + 2 * e + 1] * f);
+                const float y[4] = {x[d][4 * g + 2 * e] * f, x[d][4 * g + 2 * e + 1] * f, x[d][4 * g + 4 + 2 * e] * f,
+                                    x[d][4 * g + 4 + 2 * e + 1] * f};
+                const uint32_t lo = pt_pack<DT>(y[0], y[1]), hi = pt_pack<DT>(y[2], y[3]);
                 const auto t = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
                 u[0][e] = t[0];
                 u[1][e] = t[1];
+                if constexpr (LO) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(
+                        pt_pack<DT>(y[0] - pt_value<DT>(lo), y[1] - pt_value<DT>(lo >> 16)),
+                        pt_pack<DT>(y[2] - pt_value<DT>(hi), y[3] - pt_value<DT>(hi >> 16)), false, false);
+                    w[0][e] = r[0];
+                    w[1][e] = r[1];
+                }
             }
-            if (mine) *reinterpret_cast<uint4 *>(p + (32 * d + 8 * (g + half)) * 2) = make_uint4(u[0][0], u[0][1], u[1][0], u[1][1]);
+            const int at = (32 * d + 8 * (g + half)) * 2;
+            if (mine) *reinterpret_cast<uint4 *>(p + at) = make_uint4(u[0][0], u[0][1], u[1][0], u[1][1]);
+            if constexpr (LO) {
+                if (mine) *reinterpret_cast<uint4 *>(q + at) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+            }
         }
 }
 
@@ -260,30 +306,41 @@ __device__ __forceinline__ PtSlot pt_slot(const int32_t *cu, int B, int64_t N, i
 // n + 32 share query row n: row statistics are register reductions with one
 // exchange, and the probabilities, rounded to the input's 16 bits, are the B
 // operand of O^T += V^T P^T where they are, with V^T read transposed from LDS.
-// P's rounding (half a step of the inputs' type for each term, the row sum
-// taken of the unrounded) is what feeding the matrix units 16 bits costs; all
-// else is fp32.
+// P's rounding, half a step of the inputs' type for each term, is what feeding
+// the matrix units 16 bits costs; all else is fp32.  The output is divided by
+// the sum of the rounded terms, so that weights sum to one and a row with one
+// large term has no error from it; lse is of the unrounded ones.
+//
+// For a gradient (LO) the output's own rounding is kept as well, and the first
+// tile of keys, which is all that the first rows of a causal sequence and all
+// rows of a short one see, adds the probabilities' rounding errors as a second
+// product: delta_t = sum_d g_td o_td is taken from dp_ts, and where few keys hold
+// the weight the difference is a small one of large terms.  With o in 16 bits
+// alone dq and dk were off by 1.5 to 2.8 times what rounding them costs
+// (sequences of 8 to 1024, scores of deviation 1 to 3), so by 1.4 to 1.5.
 
 template <int DT, int D>
 struct PtRow {
     static constexpr int NT = D / 32;
     ps8_t q[D / 16];
     pf16_t o[NT];
-    float m, l;                          // running maximum of scale s log2 e; the lane's share of the sum
+    float m;                             // running maximum of scale s log2 e
+    float l, l16;                        // the lane's share of the sum of the probabilities, and of the rounded ones
     int t;                               // the row (of the sequence)
 };
 
-template <int DT, int D, bool MASK>
-__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len,
-                                                const uint32_t *bad, char *scratch) {
+// LO: the probabilities' rounding errors, rounded in turn, are added as well.
+template <int DT, int D, bool MASK, bool LO>
+__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len) {
     constexpr int NT = PtRow<DT, D>::NT;
+    const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
     pf16_t s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         s[b] = pf16_t{};
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(pt_rows<D>(K, 32 * b, kk), R.q[kk], s[b]);
+        for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
     // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
     const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -307,6 +364,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, PtRow<DT, D
         const float mn = fmaxf(R.m, mt);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R.m - mn);
         R.l *= f;
+        R.l16 *= f;
 #pragma unroll
         for (int d = 0; d < NT; ++d)
 #pragma unroll
@@ -314,8 +372,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, PtRow<DT, D
         R.m = mn;
     }
     const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
-    float sum[2];
-    uint32_t p[2][8];
+    uint32_t p[2][8], lo[LO ? 2 : 1][8];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         float x[16];
@@ -326,27 +383,41 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, PtRow<DT, D
                 if (32 * b + 8 * (i / 4) + i % 4 > seen) x[i] = 0.0f;
             }
         }
+        float sum16 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[b][i] = pt_pack<DT>(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) {
+            p[b][i] = pt_pack<DT>(x[2 * i], x[2 * i + 1]);
+            if constexpr (LO) {
+                const float e0 = x[2 * i] - pt_value<DT>(p[b][i]), e1 = x[2 * i + 1] - pt_value<DT>(p[b][i] >> 16);
+                lo[b][i] = pt_pack<DT>(e0, e1);
+                sum16 = pt_add2<DT>(lo[b][i], sum16);
+            }
+            sum16 = pt_add2<DT>(p[b][i], sum16);
+        }
+        R.l16 += sum16;
+        if (a.lse) {
 #pragma unroll
-        for (int w = 8; w > 0; w /= 2)
+            for (int w = 8; w > 0; w /= 2)
 #pragma unroll
-            for (int i = 0; i < w; ++i) x[i] += x[i + w];
-        sum[b] = x[0];
+                for (int i = 0; i < w; ++i) x[i] += x[i + w];
+            R.l += x[0];
+        }
     }
-    R.l += sum[0] + sum[1];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const uint4 u = make_uint4(p[b][4 * k], p[b][4 * k + 1], p[b][4 * k + 2], p[b][4 * k + 3]);
-            const ps8_t pb = __builtin_bit_cast(ps8_t, u);
+            const ps8_t pb = pt_frag(p[b] + 4 * k);
 #pragma unroll
-            for (int d = 0; d < NT; ++d) R.o[d] = pt_mfma<DT>(pt_cols<D>(V, 32 * b + 16 * k, d), pb, R.o[d]);
+            for (int d = 0; d < NT; ++d) {
+                const ps8_t v = A.cols(V, 32 * b + 16 * k, d);
+                R.o[d] = pt_mfma<DT>(v, pb, R.o[d]);
+                if constexpr (LO) R.o[d] = pt_mfma<DT>(v, pt_frag(lo[b] + 4 * k), R.o[d]);
+            }
         }
 }
 
-template <int DT, int D>
+template <int DT, int D, bool LO>
 __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(PromptArgs a) {
     __shared__ __attribute__((aligned(16))) char k0[kPtKeys * 2 * D], k1[kPtKeys * 2 * D];
     __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
@@ -370,27 +441,30 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
     PtCopy<D, kPtKeys> ck, cv;
-    ck.init(a.k.st);
-    cv.init(a.v.st);
+    ck.init();
+    cv.init();
     ck.issue(kb, a.k.st, 0, S.len, k0);
     cv.issue(vb, a.v.st, 0, S.len, v0);
 
+    PtLane<D> A;
+    A.init();
     PtRow<DT, D> R;
     const int w0 = row0 + 32 * wave;     // the wave's first row
     R.t = w0 + (lane & 31);
     pt_load_rows<D>(a.q.p + (int64_t)(S.start + min(R.t, S.len - 1)) * a.q.st + h * a.q.sh, a.negate ? 0x80008000u : 0u, R.q);
     R.m = -INFINITY;
-    R.l = 0.0f;
+    R.l = R.l16 = 0.0f;
 #pragma unroll
     for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
 
     const int kend = a.causal ? min(S.len, row0 + kPtRows) : S.len;       // keys that the block sees
     const int wlast = a.causal ? min(w0 + 31, S.len - 1) : S.len - 1;     // and the wave
     const bool live = w0 < S.len;
-    auto step = [&](const char *K, const char *V, int j0) {
+    auto step = [&](const char *K, const char *V, int j0, auto even) {
         if (!live || j0 > wlast) return;
-        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_forward_tile<DT, D, true>(a, R, K, V, j0, S.len, nullptr, nullptr);
-        else pt_forward_tile<DT, D, false>(a, R, K, V, j0, S.len, nullptr, nullptr);
+        if (LO && even && j0 == 0) pt_forward_tile<DT, D, true, LO && decltype(even)::value>(a, A, R, K, V, j0, S.len);
+        else if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_forward_tile<DT, D, true, false>(a, A, R, K, V, j0, S.len);
+        else pt_forward_tile<DT, D, false, false>(a, A, R, K, V, j0, S.len);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();                       // this tile is there, the other buffers are read
@@ -398,20 +472,25 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
             ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1);
             cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1);
         }
-        step(k0, v0, j0);
+        step(k0, v0, j0, std::true_type());
         if (j0 + kPtKeys >= kend) break;
         pt_sync();
         if (j0 + 2 * kPtKeys < kend) {
             ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0);
             cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0);
         }
-        step(k1, v1, j0 + kPtKeys);
+        step(k1, v1, j0 + kPtKeys, std::false_type());
     }
     if (!live) return;
 
-    const float l = pt_sum_halves(R.l);
     const bool mine = R.t < S.len;
-    pt_store<DT, D>(const_cast<char *>(a.o.p) + (int64_t)(S.start + R.t) * a.o.st + h * a.o.sh, R.o, 1.0f / l, mine);
+    const float inv = 1.0f / pt_sum_halves(R.l16), l = pt_sum_halves(R.l);
+    char *op = const_cast<char *>(a.o.p) + (int64_t)(S.start + R.t) * a.o.st + h * a.o.sh;
+    if constexpr (LO) {
+        pt_store<DT, D, true>(op, R.o, inv, mine, const_cast<char *>(a.olo.p) + (int64_t)(S.start + R.t) * a.olo.st + h * a.olo.sh);
+    } else {
+        pt_store<DT, D>(op, R.o, inv, mine);
+    }
     if (a.lse && mine && half == 0)
         a.lse[(int64_t)h * a.N + S.start + R.t] = (R.m - (DT == OMNI_F16 ? kPtF16Up : 0.0f) + __log2f(l)) * 0.69314718f;
 }
@@ -456,7 +535,8 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
             const int h = min(h0 + grp, a.Hq - 1);
             const uint4 g = *reinterpret_cast<const uint4 *>(a.g.p + t * a.g.st + h * a.g.sh + sub * 16);
             const uint4 o = *reinterpret_cast<const uint4 *>(a.o.p + t * a.o.st + h * a.o.sh + sub * 16);
-            const float d = norm(g, o);
+            const uint4 lo = *reinterpret_cast<const uint4 *>(a.olo.p + t * a.olo.st + h * a.olo.sh + sub * 16);
+            const float d = norm(g, o) + norm(g, lo);
             if (sub == 0 && h0 + grp < a.Hq) {
                 a.delta[(int64_t)h * a.N + t] = -d;
                 a.lse2[(int64_t)h * a.N + t] = a.lse[(int64_t)h * a.N + t] * 1.44269504f;
@@ -527,19 +607,22 @@ struct PtGradRow {
 
 // One tile of 64 keys for the wave's 32 query rows; transposed like the forward.
 template <int DT, int D, bool MASK>
-__device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, PtGradRow<DT, D> &R, const char *K, const char *V, int j0, int len,
+__device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradRow<DT, D> &R, const char *K, const char *V, int j0, int len,
                                            float up) {
+    const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
     const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         pf16_t s = {}, dp;
+        float first = R.delta;
+        asm volatile("" : "+v"(first));  // sixteen copies made here, not kept through the loop
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dp[i] = R.delta;
+        for (int i = 0; i < 16; ++i) dp[i] = first;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(pt_rows<D>(K, 32 * b, kk), R.q[kk], s);
+        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(pt_rows<D>(V, 32 * b, kk), R.g[kk], dp);
+        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(A.rows(V, 32 * b, kk), R.g[kk], dp);
         uint32_t x[8];
         float ds[16];
 #pragma unroll
@@ -556,7 +639,7 @@ __device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, PtGradRow<DT, D>
         for (int k = 0; k < 2; ++k) {
             const ps8_t xb = __builtin_bit_cast(ps8_t, make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]));
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) R.dq[d] = pt_mfma<DT>(pt_cols<D>(K, 32 * b + 16 * k, d), xb, R.dq[d]);
+            for (int d = 0; d < D / 32; ++d) R.dq[d] = pt_mfma<DT>(A.cols(K, 32 * b + 16 * k, d), xb, R.dq[d]);
         }
     }
 }
@@ -579,11 +662,13 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
     PtCopy<D, kPtKeys> ck, cv;
-    ck.init(a.k.st);
-    cv.init(a.v.st);
+    ck.init();
+    cv.init();
     ck.issue(kb, a.k.st, 0, S.len, k0);
     cv.issue(vb, a.v.st, 0, S.len, v0);
 
+    PtLane<D> A;
+    A.init();
     PtGradRow<DT, D> R;
     const int w0 = row0 + 32 * wave;
     R.t = w0 + (lane & 31);
@@ -601,8 +686,8 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     const bool live = w0 < S.len;
     auto step = [&](const char *K, const char *V, int j0) {
         if (!live || j0 > wlast) return;
-        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_dq_tile<DT, D, true>(a, R, K, V, j0, S.len, up);
-        else pt_dq_tile<DT, D, false>(a, R, K, V, j0, S.len, up);
+        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_dq_tile<DT, D, true>(a, A, R, K, V, j0, S.len, up);
+        else pt_dq_tile<DT, D, false>(a, A, R, K, V, j0, S.len, up);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();
@@ -640,8 +725,9 @@ struct PtGradKey {
 };
 
 template <int DT, int D, bool MASK>
-__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, PtGradKey<DT, D> &R, const char *Q, const char *G, const float *lse2,
+__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *Q, const char *G, const float *lse2,
                                             const float *delta, int j0, int len, float up) {
+    const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
     // register i of block b is row j0 + 32 b + 8 (i / 4) + 4 half + i % 4
     const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
@@ -657,9 +743,11 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, PtGradKey<DT, D
             l[i] = l4.x; l[i + 1] = l4.y; l[i + 2] = l4.z; l[i + 3] = l4.w;
         }
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(pt_rows<D>(Q, 32 * b, kk), R.k[kk], s);
+        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(A.rows(Q, 32 * b, kk), R.k[kk], s);
+        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(pt_rows<D>(G, 32 * b, kk), R.v[kk], dp);
+        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(A.rows(G, 32 * b, kk), R.v[kk], dp);
+        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
         uint32_t x[8], y[8];
         float p[16], ds[16];
 #pragma unroll
@@ -685,10 +773,11 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, PtGradKey<DT, D
             const ps8_t yb = __builtin_bit_cast(ps8_t, make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]));
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
-                R.dv[d] = pt_mfma<DT>(pt_cols<D>(G, 32 * b + 16 * k, d), xb, R.dv[d]);
-                R.dk[d] = pt_mfma<DT>(pt_cols<D>(Q, 32 * b + 16 * k, d), yb, R.dk[d]);
+                R.dv[d] = pt_mfma<DT>(A.cols(G, 32 * b + 16 * k, d), xb, R.dv[d]);
+                R.dk[d] = pt_mfma<DT>(A.cols(Q, 32 * b + 16 * k, d), yb, R.dk[d]);
             }
         }
+        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -719,8 +808,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
     const int first = a.causal ? key0 / kPtQRows : 0, tiles = (S.len + kPtQRows - 1) / kPtQRows - first;
     const int n = tiles * a.G;
     PtCopy<D, kPtQRows> cq, cg;
-    cq.init(a.q.st);
-    cg.init(a.g.st);
+    cq.init();
+    cg.init();
     const char *qb = a.q.p + (int64_t)S.start * a.q.st + (int64_t)hk * a.G * a.q.sh;
     const char *gb = a.g.p + (int64_t)S.start * a.g.st + (int64_t)hk * a.G * a.g.sh;
     const float *lb = a.lse2 + (int64_t)hk * a.G * a.N + S.start, *db = a.delta + (int64_t)hk * a.G * a.N + S.start;
@@ -737,6 +826,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
     };
     copy(q0, g0, l0, d0);
 
+    PtLane<D> A;
+    A.init();
     PtGradKey<DT, D> R;
     const int w0 = key0 + 32 * wave;
     R.s = w0 + (lane & 31);
@@ -752,8 +843,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
         const int j0 = jc * kPtQRows;
         jc = jc + 1 == first + tiles ? first : jc + 1;
         if (!live || (a.causal && j0 + kPtQRows - 1 < w0)) return;
-        if (j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31)) pt_dkv_tile<DT, D, true>(a, R, Q, G, L, Dl, j0, S.len, up);
-        else pt_dkv_tile<DT, D, false>(a, R, Q, G, L, Dl, j0, S.len, up);
+        if (j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31)) pt_dkv_tile<DT, D, true>(a, A, R, Q, G, L, Dl, j0, S.len, up);
+        else pt_dkv_tile<DT, D, false>(a, A, R, Q, G, L, Dl, j0, S.len, up);
     };
     for (int i = 0; i < n; i += 2) {
         pt_sync();
@@ -821,18 +912,23 @@ using namespace omni;
         if (rc_ != OMNI_OK) return rc_;  \
     } while (0)
 
+template <int DT, int D>
+static void prompt_launch_forward(const PromptArgs &a, dim3 grid, hipStream_t st) {
+    if (a.olo.p) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, true>), grid, dim3(64 * kPtWaves), 0, st, a);
+    else hipLaunchKernelGGL((prompt_forward_kernel<DT, D, false>), grid, dim3(64 * kPtWaves), 0, st, a);
+}
 template <int DT>
 static void prompt_launch_forward(const PromptArgs &a, int D, dim3 grid, hipStream_t st) {
-    const dim3 block(64 * kPtWaves);
-    if (D == 32) hipLaunchKernelGGL((prompt_forward_kernel<DT, 32>), grid, block, 0, st, a);
-    else if (D == 64) hipLaunchKernelGGL((prompt_forward_kernel<DT, 64>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((prompt_forward_kernel<DT, 128>), grid, block, 0, st, a);
+    if (D == 32) prompt_launch_forward<DT, 32>(a, grid, st);
+    else if (D == 64) prompt_launch_forward<DT, 64>(a, grid, st);
+    else prompt_launch_forward<DT, 128>(a, grid, st);
 }
 
 extern "C" int omni_prompt_attn(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
                                 const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv, int head_dim,
                                 const int32_t *cu_seqlens, int64_t B, float scale, int causal, int fill_rest, void *out,
-                                const int64_t *out_strides, float *lse, void *stream) {
+                                const int64_t *out_strides, float *lse, void *out_rest, const int64_t *out_rest_strides,
+                                void *stream) {
     const char *who = "omni_prompt_attn";
     PromptArgs a = {};
     OMNI_TRY(prompt_args(who, dtype, N, Hq, Hkv, head_dim, cu_seqlens, B, scale, a));
@@ -841,6 +937,7 @@ extern "C" int omni_prompt_attn(const void *q, const int64_t *q_strides, const v
     OMNI_TRY(prompt_heads(who, "k", k, k_strides, a.k));
     OMNI_TRY(prompt_heads(who, "v", v, v_strides, a.v));
     OMNI_TRY(prompt_heads(who, "out", out, out_strides, a.o));
+    if (out_rest) OMNI_TRY(prompt_heads(who, "out_rest", out_rest, out_rest_strides, a.olo));
     OMNI_CHECK_ARG(cu_seqlens, "%s: NULL cu_seqlens", who);
     a.lse = lse;
     a.causal = causal != 0;
@@ -875,7 +972,8 @@ extern "C" size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq) {
 extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
                                          const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv,
                                          int head_dim, const int32_t *cu_seqlens, int64_t B, float scale, int causal,
-                                         const void *out, const int64_t *out_strides, const float *lse, const void *dout,
+                                         const void *out, const int64_t *out_strides, const void *out_rest,
+                                         const int64_t *out_rest_strides, const float *lse, const void *dout,
                                          const int64_t *dout_strides, void *dq, const int64_t *dq_strides, void *dk,
                                          const int64_t *dk_strides, void *dv, const int64_t *dv_strides, void *workspace,
                                          size_t workspace_bytes, void *stream) {
@@ -887,6 +985,7 @@ extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides
     OMNI_TRY(prompt_heads(who, "k", k, k_strides, a.k));
     OMNI_TRY(prompt_heads(who, "v", v, v_strides, a.v));
     OMNI_TRY(prompt_heads(who, "out", out, out_strides, a.o));
+    OMNI_TRY(prompt_heads(who, "out_rest", out_rest, out_rest_strides, a.olo));
     OMNI_TRY(prompt_heads(who, "dout", dout, dout_strides, a.g));
     OMNI_TRY(prompt_heads(who, "dq", dq, dq_strides, a.dq));
     OMNI_TRY(prompt_heads(who, "dk", dk, dk_strides, a.dk));

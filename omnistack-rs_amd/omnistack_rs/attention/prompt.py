@@ -61,25 +61,27 @@ def _check(q, k, v, cu_seqlens, scale, validate):
     return dev, cu.to(device=dev, dtype=torch.int32).contiguous(), scale
 
 
-def _forward(q, k, v, cu, scale, causal, out, need_lse, dev):
+def _forward(q, k, v, cu, scale, causal, out, need_lse, dev, need_rest=False):
     N, Hq, D = q.shape
     qc, kc, vc = _rows(q), _rows(k), _rows(v)
     o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
     lse = torch.empty(Hq, N, dtype=torch.float32, device=dev) if need_lse else None
+    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_rest else None
     with _lib.on_device(dev):
         _lib.check(_lib.lib().omni_prompt_attn(
             _lib.ptr(qc), _strides(qc), _lib.ptr(kc), _strides(kc), _lib.ptr(vc), _strides(vc), _lib.dtype_code(q.dtype),
             N, Hq, k.shape[1], D, _lib.ptr(cu), cu.numel() - 1, scale, int(causal), int(out is None),
-            _lib.ptr(o), _strides(o), _lib.ptr(lse), _lib.stream_of(dev)))
-    return o, lse
+            _lib.ptr(o), _strides(o), _lib.ptr(lse), _lib.ptr(rest), _strides(rest) if need_rest else None,
+            _lib.stream_of(dev)))
+    return (o, lse, rest) if need_rest else (o, lse)
 
 
 class _PromptAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, scale, causal, dev):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        o, lse = _forward(q, k, v, cu, scale, causal, None, True, dev)
-        ctx.save_for_backward(q, k, v, o, lse, cu)
+        o, lse, rest = _forward(q, k, v, cu, scale, causal, None, True, dev, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, cu)
         ctx.scale, ctx.causal, ctx.dev = scale, causal, dev
         ctx.mark_non_differentiable(lse)
         return o, lse
@@ -87,7 +89,7 @@ class _PromptAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, _):
-        q, k, v, o, lse, cu = ctx.saved_tensors
+        q, k, v, o, rest, lse, cu = ctx.saved_tensors
         N, Hq, D = q.shape
         do = _rows(do)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=ctx.dev) for t in (q, k, v))
@@ -98,7 +100,7 @@ class _PromptAttention(torch.autograd.Function):
             _lib.check(L.omni_prompt_attn_backward(
                 _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), _lib.dtype_code(q.dtype),
                 N, Hq, k.shape[1], D, _lib.ptr(cu), cu.numel() - 1, ctx.scale, int(ctx.causal),
-                _lib.ptr(o), _strides(o), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq),
+                _lib.ptr(o), _strides(o), _lib.ptr(rest), _strides(rest), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq),
                 _lib.ptr(dk), _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), ws_bytes, _lib.stream_of(ctx.dev)))
         return dq, dk, dv, None, None, None, None
 

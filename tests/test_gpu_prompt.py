@@ -152,7 +152,9 @@ def test_outputs_and_gradients(device, lengths, extra, Hq, Hkv, D, dtype, causal
     plain, plse = prompt_attention(q, k, v, cu.to(device), causal=causal, return_lse=True)
     leaves = [t.requires_grad_() for t in (q, k, v)]
     o, lse = prompt_attention(*leaves, cu.to(device), causal=causal, return_lse=True)
-    assert torch.equal(o, plain) and torch.equal(lse, plse)
+    # the forward of a gradient adds terms below the probabilities' rounding
+    assert torch.equal(lse, plse)
+    _close(plain, *want["o"], "out alone")
     _close(o.detach(), *want["o"], "out")
     live = torch.isfinite(want["lse"])
     assert torch.equal(torch.isfinite(lse), live)
@@ -303,7 +305,7 @@ def test_native_refusals():
     s, odd, far = ((ctypes.c_int64 * 2)(*x) for x in ((128, 64), (127, 64), (1 << 24, 64)))
 
     def call(q=4096, qs=s, dtype=2, N=5, Hq=2, Hkv=1, D=64, cu=4096, B=1, scale=1.0):
-        return L.omni_prompt_attn(q, qs, 4096, s, 4096, s, dtype, N, Hq, Hkv, D, cu, B, scale, 1, 1, 4096, s, None, None)
+        return L.omni_prompt_attn(q, qs, 4096, s, 4096, s, dtype, N, Hq, Hkv, D, cu, B, scale, 1, 1, 4096, s, None, None, None, None)
     for kw, msg in ((dict(dtype=0), "f16 or bf16"), (dict(D=48), "head_dim"), (dict(Hq=3, Hkv=2), "multiple"), (dict(N=-1), "shape"),
                     (dict(N=1 << 31), "large"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
                     (dict(q=None), "NULL"), (dict(q=4104), "16 bytes"), (dict(qs=odd), "16 bytes"), (dict(qs=far), "stride"),
@@ -312,5 +314,5 @@ def test_native_refusals():
     assert call(N=0, q=None) == 0
     assert L.omni_prompt_attn_backward_workspace_size(10, 4) == 10 * 4 * 8 + 4096
     a = (4096, s)
-    rc = L.omni_prompt_attn_backward(*a, *a, *a, 2, 5, 2, 1, 64, 4096, 1, 1.0, 1, *a, 4096, *a, *a, *a, *a, 4096, 100, None)
+    rc = L.omni_prompt_attn_backward(*a, *a, *a, 2, 5, 2, 1, 64, 4096, 1, 1.0, 1, *a, *a, 4096, *a, *a, *a, *a, 4096, 100, None)
     assert rc == _lib.OMNI_EWORKSPACE and "workspace" in _lib.last_error()
