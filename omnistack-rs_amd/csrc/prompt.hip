@@ -48,7 +48,8 @@ struct PromptArgs {
     int B, Hq, Hkv, G;
     int causal, negate, fill;            // fill: rows of no sequence get zeros
     int peak_rows;
-    float c, scale;                      // |scale| log2(e)
+    float c, cs, scale;                  // |scale| log2(e), scale log2(e)
+    float hide;                          // a hidden score: cs times it is -inf
 };
 
 // ── types ───────────────────────────────────────────────────────────────
@@ -203,7 +204,7 @@ struct PtLane {
 
 // Row operand of 32 rows straight from memory: lane's row at `p`, dims 8 half on.
 template <int D>
-__device__ __forceinline__ void pt_load_rows(const char *p, uint32_t flip, ps8_t (&f)[D / 16]) {
+__device__ __forceinline__ void pt_load_rows(const char *p, ps8_t (&f)[D / 16], uint32_t flip = 0) {
     p += 16 * ((threadIdx.x >> 5) & 1);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -330,8 +331,8 @@ struct PtRow {
 };
 
 // LO: the probabilities' rounding errors, rounded in turn, are added as well.
-template <int DT, int D, bool MASK, bool LO>
-__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len) {
+template <int DT, int D, bool LO>
+__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len, bool masked) {
     constexpr int NT = PtRow<DT, D>::NT;
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
@@ -342,24 +343,21 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
-    // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
-    const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
+    if (masked) {
+        // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
+        const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (32 * b + 8 * (i / 4) + i % 4 > seen) s[b][i] = -INFINITY;
+    }
     float mt = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if constexpr (MASK) {
-                if (32 * b + 8 * (i / 4) + i % 4 > seen) s[b][i] = -INFINITY;
-            }
-            mt = fmaxf(mt, s[b][i]);
-        }
-    mt = pt_max_halves(mt);
-    if (MASK && mt == -INFINITY) {
-        // no key, or none above -inf: the maximum stays (scale 0 would make it NaN)
-    } else {
-        mt *= a.c;
-    }
+        for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[b][i]);
+    mt = pt_max_halves(mt) * a.c;
     if (__builtin_amdgcn_ballot_w64(mt > R.m + kPtSlack)) {
         const float mn = fmaxf(R.m, mt);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(R.m - mn);
@@ -379,9 +377,6 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             x[i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.c, -off));
-            if constexpr (MASK) {
-                if (32 * b + 8 * (i / 4) + i % 4 > seen) x[i] = 0.0f;
-            }
         }
         float sum16 = 0.0f;
 #pragma unroll
@@ -451,7 +446,8 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     PtRow<DT, D> R;
     const int w0 = row0 + 32 * wave;     // the wave's first row
     R.t = w0 + (lane & 31);
-    pt_load_rows<D>(a.q.p + (int64_t)(S.start + min(R.t, S.len - 1)) * a.q.st + h * a.q.sh, a.negate ? 0x80008000u : 0u, R.q);
+    pt_load_rows<D>(a.q.p + (int64_t)(S.start + min(R.t, S.len - 1)) * a.q.st + h * a.q.sh, R.q,
+                    a.negate ? 0x80008000u : 0u);
     R.m = -INFINITY;
     R.l = R.l16 = 0.0f;
 #pragma unroll
@@ -462,9 +458,9 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     const bool live = w0 < S.len;
     auto step = [&](const char *K, const char *V, int j0, auto even) {
         if (!live || j0 > wlast) return;
-        if (LO && even && j0 == 0) pt_forward_tile<DT, D, true, LO && decltype(even)::value>(a, A, R, K, V, j0, S.len);
-        else if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_forward_tile<DT, D, true, false>(a, A, R, K, V, j0, S.len);
-        else pt_forward_tile<DT, D, false, false>(a, A, R, K, V, j0, S.len);
+        const bool masked = j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0);
+        if (LO && decltype(even)::value && j0 == 0) pt_forward_tile<DT, D, LO>(a, A, R, K, V, j0, S.len, masked);
+        else pt_forward_tile<DT, D, false>(a, A, R, K, V, j0, S.len, masked);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();                       // this tile is there, the other buffers are read
@@ -606,9 +602,9 @@ struct PtGradRow {
 };
 
 // One tile of 64 keys for the wave's 32 query rows; transposed like the forward.
-template <int DT, int D, bool MASK>
+template <int DT, int D>
 __device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradRow<DT, D> &R, const char *K, const char *V, int j0, int len,
-                                           float up) {
+                                           bool masked, float up) {
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
     const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -623,15 +619,20 @@ __device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, const PtLane<D> 
         for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(A.rows(V, 32 * b, kk), R.g[kk], dp);
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (32 * b + 8 * (i / 4) + i % 4 > seen) {
+                    s[i] = a.hide;
+                    dp[i] = 0.0f;
+                }
+        }
         uint32_t x[8];
         float ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -R.lse2));
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -R.lse2));
             ds[i] = p * (DT == OMNI_F16 ? dp[i] * up : dp[i]);
-            if constexpr (MASK) {
-                if (32 * b + 8 * (i / 4) + i % 4 > seen) ds[i] = 0.0f;
-            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = pt_pack<DT>(ds[2 * i], ds[2 * i + 1]);
@@ -673,8 +674,8 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     const int w0 = row0 + 32 * wave;
     R.t = w0 + (lane & 31);
     const int64_t at = S.start + min(R.t, S.len - 1);
-    pt_load_rows<D>(a.q.p + at * a.q.st + h * a.q.sh, a.negate ? 0x80008000u : 0u, R.q);
-    pt_load_rows<D>(a.g.p + at * a.g.st + h * a.g.sh, 0u, R.g);
+    pt_load_rows<D>(a.q.p + at * a.q.st + h * a.q.sh, R.q);
+    pt_load_rows<D>(a.g.p + at * a.g.st + h * a.g.sh, R.g);
     R.lse2 = a.lse2[(int64_t)h * a.N + at];
     R.delta = a.delta[(int64_t)h * a.N + at];
     const float up = pt_ds_scale<DT>(a);
@@ -686,8 +687,7 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     const bool live = w0 < S.len;
     auto step = [&](const char *K, const char *V, int j0) {
         if (!live || j0 > wlast) return;
-        if (j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0)) pt_dq_tile<DT, D, true>(a, A, R, K, V, j0, S.len, up);
-        else pt_dq_tile<DT, D, false>(a, A, R, K, V, j0, S.len, up);
+        pt_dq_tile<DT, D>(a, A, R, K, V, j0, S.len, j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0), up);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();
@@ -714,63 +714,74 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
 // one query head of the group after another.
 constexpr int kPtKvWaves = 4;
 constexpr int kPtKvKeys = 32 * kPtKvWaves;
-constexpr int kPtQRows = 64;
+
+// At D = 128 the sums of dk and dv take 128 registers a lane.  Two waves a SIMD
+// (256 registers) then leave room for v's operands but not k's, which are read
+// from LDS again for every 32 rows, and for two blocks' tiles of 32 rows in LDS.
+template <int D>
+struct PtKv {
+    static constexpr bool KLDS = D == 128;
+    static constexpr int ROWS = D == 128 ? 32 : 64;
+};
 
 template <int DT, int D>
 struct PtGradKey {
     static constexpr int NT = D / 32;
-    ps8_t k[D / 16], v[D / 16];
+    ps8_t k[PtKv<D>::KLDS ? 1 : D / 16], v[D / 16];
     pf16_t dk[NT], dv[NT];
     int s;
 };
 
-template <int DT, int D, bool MASK>
-__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *Q, const char *G, const float *lse2,
-                                            const float *delta, int j0, int len, float up) {
+template <int DT, int D>
+__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *K, int k0, const char *Q,
+                                            const char *G, const float *lse2, const float *delta, int j0, int len, bool masked, float up) {
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
-    // register i of block b is row j0 + 32 b + 8 (i / 4) + 4 half + i % 4
-    const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < PtKv<D>::ROWS / 32; ++b) {
         pf16_t s = {}, dp;
-        float l[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const float4 d4 = *reinterpret_cast<const float4 *>(delta + 32 * b + 2 * i + 4 * half);
-            const float4 l4 = *reinterpret_cast<const float4 *>(lse2 + 32 * b + 2 * i + 4 * half);
             dp[i] = d4.x; dp[i + 1] = d4.y; dp[i + 2] = d4.z; dp[i + 3] = d4.w;
-            l[i] = l4.x; l[i + 1] = l4.y; l[i + 2] = l4.z; l[i + 3] = l4.w;
         }
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(A.rows(Q, 32 * b, kk), R.k[kk], s);
-        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
+        for (int kk = 0; kk < D / 16; ++kk) {
+            s = pt_mfma<DT>(A.rows(Q, 32 * b, kk), PtKv<D>::KLDS ? A.rows(K, k0, kk) : R.k[PtKv<D>::KLDS ? 0 : kk], s);
+            dp = pt_mfma<DT>(A.rows(G, 32 * b, kk), R.v[kk], dp);
+        }
+        if (masked) {
+            // register i is row j0 + 32 b + 8 (i / 4) + 4 half + i % 4
+            const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) dp = pt_mfma<DT>(A.rows(G, 32 * b, kk), R.v[kk], dp);
-        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
-        uint32_t x[8], y[8];
-        float p[16], ds[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[i]));
-            if constexpr (MASK) {
+            for (int i = 0; i < 16; ++i) {
                 const int row = 32 * b + 8 * (i / 4) + i % 4;
-                const bool see = row >= first && row < end;
-                p[i] = see ? p[i] : 0.0f;
-                ds[i] = see ? p[i] * (DT == OMNI_F16 ? dp[i] * up : dp[i]) : 0.0f;
-            } else {
-                ds[i] = p[i] * (DT == OMNI_F16 ? dp[i] * up : dp[i]);
+                if (row < first || row >= end) {
+                    s[i] = a.hide;
+                    dp[i] = 0.0f;
+                }
+            }
+        }
+        uint32_t x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 l4 = *reinterpret_cast<const float4 *>(lse2 + 32 * b + 2 * i + 4 * half);
+            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+            float p[4], ds[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[e]));
+                ds[e] = p[e] * (DT == OMNI_F16 ? dp[i + e] * up : dp[i + e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                x[i / 2 + e] = pt_pack<DT>(p[2 * e], p[2 * e + 1]);
+                y[i / 2 + e] = pt_pack<DT>(ds[2 * e], ds[2 * e + 1]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = pt_pack<DT>(p[2 * i], p[2 * i + 1]);
-            y[i] = pt_pack<DT>(ds[2 * i], ds[2 * i + 1]);
-        }
-#pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const ps8_t xb = __builtin_bit_cast(ps8_t, make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]));
-            const ps8_t yb = __builtin_bit_cast(ps8_t, make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]));
+            const ps8_t xb = pt_frag(x + 4 * k), yb = pt_frag(y + 4 * k);
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
                 R.dv[d] = pt_mfma<DT>(A.cols(G, 32 * b + 16 * k, d), xb, R.dv[d]);
@@ -781,18 +792,22 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D>
     }
 }
 
-// 64 floats of a row statistic, from row j0 of the sequence on (rows from len on repeat the last).
+// ROWS (64 at most) floats of a row statistic, from row j0 of the sequence on (rows from len on repeat the last).
+template <int ROWS>
 __device__ __forceinline__ void pt_copy_stat(const float *base, int j0, int len, float *lds) {
-    const int left = min(len - j0, kPtQRows);
+    const int left = min(len - j0, ROWS);
     const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc((void *)(base + j0), (short)0, left * 4, kPtBufWord3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)lds, 4, (uint32_t)min((int)(threadIdx.x & 63), left - 1) * 4u, 0, 0, 0);
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptArgs a) {
+    constexpr int kPtQRows = PtKv<D>::ROWS;
+    constexpr bool KLDS = PtKv<D>::KLDS;
     __shared__ __attribute__((aligned(16))) char q0[kPtQRows * 2 * D], q1[kPtQRows * 2 * D];
     __shared__ __attribute__((aligned(16))) char g0[kPtQRows * 2 * D], g1[kPtQRows * 2 * D];
-    __shared__ __attribute__((aligned(16))) float l0[kPtQRows], l1[kPtQRows], d0[kPtQRows], d1[kPtQRows];
+    __shared__ __attribute__((aligned(16))) char kt[KLDS ? kPtKvKeys * 2 * D : 16];
+    __shared__ __attribute__((aligned(16))) float l0[64], l1[64], d0[64], d1[64];
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
     // the first keys are seen by the most rows
@@ -817,13 +832,18 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
     auto copy = [&](char *Q, char *G, float *L, float *Dl) {
         cq.issue(qb + gi * a.q.sh, a.q.st, ji * kPtQRows, S.len, Q);
         cg.issue(gb + gi * a.g.sh, a.g.st, ji * kPtQRows, S.len, G);
-        if (wave == 0) pt_copy_stat(lb + gi * a.N, ji * kPtQRows, S.len, L);
-        else if (wave == 1) pt_copy_stat(db + gi * a.N, ji * kPtQRows, S.len, Dl);
+        if (wave == 0) pt_copy_stat<kPtQRows>(lb + gi * a.N, ji * kPtQRows, S.len, L);
+        else if (wave == 1) pt_copy_stat<kPtQRows>(db + gi * a.N, ji * kPtQRows, S.len, Dl);
         if (++ji == first + tiles) {
             ji = first;
             ++gi;
         }
     };
+    if constexpr (KLDS) {
+        PtCopy<D, kPtKvKeys> ck;
+        ck.init();
+        ck.issue(a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, a.k.st, key0, S.len, kt);
+    }
     copy(q0, g0, l0, d0);
 
     PtLane<D> A;
@@ -832,8 +852,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
     const int w0 = key0 + 32 * wave;
     R.s = w0 + (lane & 31);
     const int64_t at = S.start + min(R.s, S.len - 1);
-    pt_load_rows<D>(a.k.p + at * a.k.st + hk * a.k.sh, a.negate ? 0x80008000u : 0u, R.k);
-    pt_load_rows<D>(a.v.p + at * a.v.st + hk * a.v.sh, 0u, R.v);
+    if constexpr (!KLDS) pt_load_rows<D>(a.k.p + at * a.k.st + hk * a.k.sh, R.k);
+    pt_load_rows<D>(a.v.p + at * a.v.st + hk * a.v.sh, R.v);
     const float scale = pt_ds_scale<DT>(a), up = DT == OMNI_F16 ? scale * 6.103515625e-5f : 1.0f;   // p is times 2^14
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) R.dk[d] = R.dv[d] = pf16_t{};
@@ -843,8 +863,7 @@ __global__ __launch_bounds__(64 * kPtKvWaves, D == 128 ? 1 : 2) void prompt_dkv_
         const int j0 = jc * kPtQRows;
         jc = jc + 1 == first + tiles ? first : jc + 1;
         if (!live || (a.causal && j0 + kPtQRows - 1 < w0)) return;
-        if (j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31)) pt_dkv_tile<DT, D, true>(a, A, R, Q, G, L, Dl, j0, S.len, up);
-        else pt_dkv_tile<DT, D, false>(a, A, R, Q, G, L, Dl, j0, S.len, up);
+        pt_dkv_tile<DT, D>(a, A, R, kt, 32 * wave, Q, G, L, Dl, j0, S.len, j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31), up);
     };
     for (int i = 0; i < n; i += 2) {
         pt_sync();
@@ -891,7 +910,10 @@ static int prompt_args(const char *who, int dtype, int64_t N, int Hq, int Hkv, i
     a.cu = cu;
     a.negate = scale < 0.0f;
     a.scale = scale;
-    a.c = fabsf(scale) * 1.44269504088896f;
+    // a scale of 0 is next to 0 instead, so that hidden scores stay at -inf
+    a.c = fmaxf(fabsf(scale) * 1.44269504088896f, 1.0e-37f);
+    a.cs = scale < 0.0f ? -a.c : a.c;
+    a.hide = scale < 0.0f ? INFINITY : -INFINITY;
     return OMNI_OK;
 }
 
