@@ -136,18 +136,19 @@ struct PtCopy {
     static_assert(N >= 1 && ROWS % STEP == 0, "whole instructions");
     int row, chunk;                      // lane's row and byte in the row, of instruction 0
 
-    __device__ __forceinline__ void init() {
+    // by wave w (uniform) of four
+    __device__ __forceinline__ void init(int w) {
         const int lane = threadIdx.x & 63;
-        row = threadIdx.x / 64 * RPI + lane / CH;
+        row = w * RPI + lane / CH;
         chunk = ((lane % CH) ^ pt_swz<D>(row)) * 16;
     }
     // Rows r0 .. r0 + ROWS - 1 of a head at `base` (its row 0) to `lds`; rows from `len` on repeat the last.
-    __device__ __forceinline__ void issue(const char *base, int64_t st, int r0, int len, char *lds) const {
+    __device__ __forceinline__ void issue(const char *base, int64_t st, int r0, int len, char *lds, int w) const {
         const uint32_t stride = (uint32_t)st;
         const int left = min(len - r0, ROWS);
         const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc(
             (void *)(base + (int64_t)r0 * st), (short)0, (int)((uint32_t)(left - 1) * stride + 2 * D), kPtBufWord3);
-        char *dst = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
+        char *dst = lds + w * 1024;
         int r = row;
         asm volatile("" : "+v"(r));      // no register for each instruction's offset through the loop
         if (left == ROWS) {
@@ -174,11 +175,12 @@ struct PtCopy {
 template <int D>
 struct PtLane {
     uint32_t r, c;
-    __device__ __forceinline__ void init() {
+    // of the tile's rows from row0 (a multiple of 32) on
+    __device__ __forceinline__ void init(int row0 = 0) {
         const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31, i = lane & 15;
-        r = n * (2 * D) + ((half ^ pt_swz<D>(n)) * 16);
+        r = (row0 + n) * (2 * D) + ((half ^ pt_swz<D>(n)) * 16);
         const int row = 4 * half + i / 4, byte = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) * 2;
-        c = row * (2 * D) + (((byte >> 4) ^ pt_swz<D>(row)) * 16) + (byte & 15);
+        c = (row0 + row) * (2 * D) + (((byte >> 4) ^ pt_swz<D>(row)) * 16) + (byte & 15);
     }
     __device__ __forceinline__ PtLane fresh() const {
         PtLane x = *this;
@@ -436,10 +438,10 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
     PtCopy<D, kPtKeys> ck, cv;
-    ck.init();
-    cv.init();
-    ck.issue(kb, a.k.st, 0, S.len, k0);
-    cv.issue(vb, a.v.st, 0, S.len, v0);
+    ck.init(wave);
+    cv.init(wave);
+    ck.issue(kb, a.k.st, 0, S.len, k0, wave);
+    cv.issue(vb, a.v.st, 0, S.len, v0, wave);
 
     PtLane<D> A;
     A.init();
@@ -465,15 +467,15 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();                       // this tile is there, the other buffers are read
         if (j0 + kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1);
-            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1);
+            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1, wave);
+            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1, wave);
         }
         step(k0, v0, j0, std::true_type());
         if (j0 + kPtKeys >= kend) break;
         pt_sync();
         if (j0 + 2 * kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0);
-            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0);
+            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0, wave);
+            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0, wave);
         }
         step(k1, v1, j0 + kPtKeys, std::false_type());
     }
@@ -663,10 +665,10 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
     PtCopy<D, kPtKeys> ck, cv;
-    ck.init();
-    cv.init();
-    ck.issue(kb, a.k.st, 0, S.len, k0);
-    cv.issue(vb, a.v.st, 0, S.len, v0);
+    ck.init(wave);
+    cv.init(wave);
+    ck.issue(kb, a.k.st, 0, S.len, k0, wave);
+    cv.issue(vb, a.v.st, 0, S.len, v0, wave);
 
     PtLane<D> A;
     A.init();
@@ -692,15 +694,15 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();
         if (j0 + kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1);
-            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1);
+            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1, wave);
+            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1, wave);
         }
         step(k0, v0, j0);
         if (j0 + kPtKeys >= kend) break;
         pt_sync();
         if (j0 + 2 * kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0);
-            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0);
+            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0, wave);
+            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0, wave);
         }
         step(k1, v1, j0 + kPtKeys);
     }
@@ -711,109 +713,130 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
 // dk and dv: a wave holds 32 keys as B operands of S = Q K^T and G V^T, so
 // that p and ds (rows on registers, keys on lanes) are the B operands of
 // dv^T += G^T P and dk^T += Q^T dS; tiles of 64 rows of q and g go through LDS,
-// one query head of the group after another.
-constexpr int kPtKvWaves = 4;
-constexpr int kPtKvKeys = 32 * kPtKvWaves;
-
+// one query head of the group after another.  Four waves share 128 keys and the
+// first 32 rows of every tile, four more the same keys and the other rows; the
+// halves are added through LDS at the end.  A wave's own run, every row that
+// sees its keys, times the group, is the longest there is: at 4096 of 8192
+// packed tokens and G = 4 it is longer than a CU's share of all, and with one
+// wave for all rows (two blocks a CU) the launch took 690 us instead of 525 us.
+//
 // At D = 128 the sums of dk and dv take 128 registers a lane.  Two waves a SIMD
 // (256 registers) then leave room for v's operands but not k's, which are read
-// from LDS again for every 32 rows, and for two blocks' tiles of 32 rows in LDS.
-template <int D>
-struct PtKv {
-    static constexpr bool KLDS = D == 128;
-    static constexpr int ROWS = D == 128 ? 32 : 64;
-};
+// from LDS again for every tile.
+constexpr int kPtKvWaves = 8;
+constexpr int kPtKvKeys = 128;
+constexpr int kPtQRows = 64;
 
 template <int DT, int D>
 struct PtGradKey {
     static constexpr int NT = D / 32;
-    ps8_t k[PtKv<D>::KLDS ? 1 : D / 16], v[D / 16];
+    static constexpr bool KLDS = D == 128;
+    ps8_t k[KLDS ? 1 : D / 16], v[D / 16];
     pf16_t dk[NT], dv[NT];
     int s;
 };
 
+// 32 rows from row j0 on.  kr: the lane's offset in K's tile (KLDS).
 template <int DT, int D>
-__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *K, int k0, const char *Q,
-                                            const char *G, const float *lse2, const float *delta, int j0, int len, bool masked, float up) {
-    const PtLane<D> A = lane_at.fresh();
+__device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *K,
+                                            const PtLane<D> &key_at, const char *Q, const char *G, const float *lse2,
+                                            const float *delta, int j0, int len, bool masked, float up) {
+    constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
+    const PtLane<D> A = lane_at.fresh(), AK = KLDS ? key_at.fresh() : A;
     const int half = (threadIdx.x >> 5) & 1;
+    pf16_t s = {}, dp;
 #pragma unroll
-    for (int b = 0; b < PtKv<D>::ROWS / 32; ++b) {
-        pf16_t s = {}, dp;
+    for (int i = 0; i < 16; i += 4) {
+        const float4 d4 = *reinterpret_cast<const float4 *>(delta + 2 * i + 4 * half);
+        dp[i] = d4.x; dp[i + 1] = d4.y; dp[i + 2] = d4.z; dp[i + 3] = d4.w;
+    }
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 d4 = *reinterpret_cast<const float4 *>(delta + 32 * b + 2 * i + 4 * half);
-            dp[i] = d4.x; dp[i + 1] = d4.y; dp[i + 2] = d4.z; dp[i + 3] = d4.w;
-        }
+    for (int kk = 0; kk < D / 16; ++kk) {
+        s = pt_mfma<DT>(A.rows(Q, 0, kk), KLDS ? AK.rows(K, 0, kk) : R.k[KLDS ? 0 : kk], s);
+        dp = pt_mfma<DT>(A.rows(G, 0, kk), R.v[kk], dp);
+    }
+    if (masked) {
+        // register i is row j0 + 8 (i / 4) + 4 half + i % 4
+        const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            s = pt_mfma<DT>(A.rows(Q, 32 * b, kk), PtKv<D>::KLDS ? A.rows(K, k0, kk) : R.k[PtKv<D>::KLDS ? 0 : kk], s);
-            dp = pt_mfma<DT>(A.rows(G, 32 * b, kk), R.v[kk], dp);
-        }
-        if (masked) {
-            // register i is row j0 + 32 b + 8 (i / 4) + 4 half + i % 4
-            const int first = (a.causal ? R.s : 0) - j0 - 4 * half, end = len - j0 - 4 * half;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = 32 * b + 8 * (i / 4) + i % 4;
-                if (row < first || row >= end) {
-                    s[i] = a.hide;
-                    dp[i] = 0.0f;
-                }
+        for (int i = 0; i < 16; ++i) {
+            const int row = 8 * (i / 4) + i % 4;
+            if (row < first || row >= end) {
+                s[i] = a.hide;
+                dp[i] = 0.0f;
             }
         }
-        uint32_t x[8], y[8];
+    }
+    uint32_t x[8], y[8];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 l4 = *reinterpret_cast<const float4 *>(lse2 + 32 * b + 2 * i + 4 * half);
-            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-            float p[4], ds[4];
+    for (int i = 0; i < 16; i += 4) {
+        const float4 l4 = *reinterpret_cast<const float4 *>(lse2 + 2 * i + 4 * half);
+        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+        float p[4], ds[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[e]));
-                ds[e] = p[e] * (DT == OMNI_F16 ? dp[i + e] * up : dp[i + e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                x[i / 2 + e] = pt_pack<DT>(p[2 * e], p[2 * e + 1]);
-                y[i / 2 + e] = pt_pack<DT>(ds[2 * e], ds[2 * e + 1]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[e]));
+            ds[e] = p[e] * (DT == OMNI_F16 ? dp[i + e] * up : dp[i + e]);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const ps8_t xb = pt_frag(x + 4 * k), yb = pt_frag(y + 4 * k);
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                R.dv[d] = pt_mfma<DT>(A.cols(G, 32 * b + 16 * k, d), xb, R.dv[d]);
-                R.dk[d] = pt_mfma<DT>(A.cols(Q, 32 * b + 16 * k, d), yb, R.dk[d]);
-            }
+        for (int e = 0; e < 2; ++e) {
+            x[i / 2 + e] = pt_pack<DT>(p[2 * e], p[2 * e + 1]);
+            y[i / 2 + e] = pt_pack<DT>(ds[2 * e], ds[2 * e + 1]);
         }
-        if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const ps8_t xb = pt_frag(x + 4 * k), yb = pt_frag(y + 4 * k);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+            R.dv[d] = pt_mfma<DT>(A.cols(G, 16 * k, d), xb, R.dv[d]);
+            R.dk[d] = pt_mfma<DT>(A.cols(Q, 16 * k, d), yb, R.dk[d]);
+        }
     }
 }
 
-// ROWS (64 at most) floats of a row statistic, from row j0 of the sequence on (rows from len on repeat the last).
-template <int ROWS>
+// kPtQRows floats of a row statistic, from row j0 of the sequence on (rows from len on repeat the last).
 __device__ __forceinline__ void pt_copy_stat(const float *base, int j0, int len, float *lds) {
-    const int left = min(len - j0, ROWS);
+    const int left = min(len - j0, kPtQRows);
     const __amdgpu_buffer_rsrc_t R = __builtin_amdgcn_make_buffer_rsrc((void *)(base + j0), (short)0, left * 4, kPtBufWord3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)lds, 4, (uint32_t)min((int)(threadIdx.x & 63), left - 1) * 4u, 0, 0, 0);
 }
 
+// The upper half's sums to the lower half: lane's registers in LDS, a KB a register quad and wave.
+template <int NT>
+__device__ __forceinline__ void pt_give(char *lds, const pf16_t (&x)[NT]) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16) =
+                make_float4(x[d][i], x[d][i + 1], x[d][i + 2], x[d][i + 3]);
+}
+template <int NT>
+__device__ __forceinline__ void pt_take(const char *lds, pf16_t (&x)[NT]) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 y = *reinterpret_cast<const float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16);
+            x[d][i] += y.x; x[d][i + 1] += y.y; x[d][i + 2] += y.z; x[d][i + 3] += y.w;
+        }
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptArgs a) {
-    constexpr int kPtQRows = PtKv<D>::ROWS;
-    constexpr bool KLDS = PtKv<D>::KLDS;
+    constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
     __shared__ __attribute__((aligned(16))) char q0[kPtQRows * 2 * D], q1[kPtQRows * 2 * D];
     __shared__ __attribute__((aligned(16))) char g0[kPtQRows * 2 * D], g1[kPtQRows * 2 * D];
     __shared__ __attribute__((aligned(16))) char kt[KLDS ? kPtKvKeys * 2 * D : 16];
-    __shared__ __attribute__((aligned(16))) float l0[64], l1[64], d0[64], d1[64];
+    __shared__ __attribute__((aligned(16))) float l0[kPtQRows], l1[kPtQRows], d0[kPtQRows], d1[kPtQRows];
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
     // the first keys are seen by the most rows
     const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, bid / a.Hkv, false);
     if (S.tile < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kw = wave & 3, upper = wave >> 2;
     const int key0 = S.tile * kPtKvKeys;
     if (S.none) {
         pt_zero_rows<D, kPtKvKeys>(a.dk, S.start, key0, S.len, hk);
@@ -822,34 +845,33 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     }
     const int first = a.causal ? key0 / kPtQRows : 0, tiles = (S.len + kPtQRows - 1) / kPtQRows - first;
     const int n = tiles * a.G;
-    PtCopy<D, kPtQRows> cq, cg;
-    cq.init();
-    cg.init();
-    const char *qb = a.q.p + (int64_t)S.start * a.q.st + (int64_t)hk * a.G * a.q.sh;
-    const char *gb = a.g.p + (int64_t)S.start * a.g.st + (int64_t)hk * a.G * a.g.sh;
-    const float *lb = a.lse2 + (int64_t)hk * a.G * a.N + S.start, *db = a.delta + (int64_t)hk * a.G * a.N + S.start;
+    PtCopy<D, kPtQRows> cp;
+    cp.init(kw);
+    const PromptHeads &src = upper ? a.g : a.q;          // the lower waves copy q, the upper g
+    const char *sb = src.p + (int64_t)S.start * src.st + (int64_t)hk * a.G * src.sh;
+    const float *stat = (upper ? a.delta : a.lse2) + (int64_t)hk * a.G * a.N + S.start;
     int gi = 0, ji = first;              // head and tile that the next copy takes
     auto copy = [&](char *Q, char *G, float *L, float *Dl) {
-        cq.issue(qb + gi * a.q.sh, a.q.st, ji * kPtQRows, S.len, Q);
-        cg.issue(gb + gi * a.g.sh, a.g.st, ji * kPtQRows, S.len, G);
-        if (wave == 0) pt_copy_stat<kPtQRows>(lb + gi * a.N, ji * kPtQRows, S.len, L);
-        else if (wave == 1) pt_copy_stat<kPtQRows>(db + gi * a.N, ji * kPtQRows, S.len, Dl);
+        cp.issue(sb + gi * src.sh, src.st, ji * kPtQRows, S.len, upper ? G : Q, kw);
+        if (kw == 0) pt_copy_stat(stat + gi * a.N, ji * kPtQRows, S.len, upper ? Dl : L);
         if (++ji == first + tiles) {
             ji = first;
             ++gi;
         }
     };
     if constexpr (KLDS) {
-        PtCopy<D, kPtKvKeys> ck;
-        ck.init();
-        ck.issue(a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, a.k.st, key0, S.len, kt);
+        static_assert(kPtKvKeys == 2 * kPtQRows, "a half of the keys by either half of the waves");
+        const int k0 = key0 + kPtQRows * upper;
+        if (k0 < S.len)
+            cp.issue(a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, a.k.st, k0, S.len, kt + kPtQRows * 2 * D * upper, kw);
     }
     copy(q0, g0, l0, d0);
 
-    PtLane<D> A;
-    A.init();
+    PtLane<D> A, AK;
+    A.init(32 * upper);
+    AK.init(32 * kw);
     PtGradKey<DT, D> R;
-    const int w0 = key0 + 32 * wave;
+    const int w0 = key0 + 32 * kw;
     R.s = w0 + (lane & 31);
     const int64_t at = S.start + min(R.s, S.len - 1);
     if constexpr (!KLDS) pt_load_rows<D>(a.k.p + at * a.k.st + hk * a.k.sh, R.k);
@@ -860,10 +882,11 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     const bool live = w0 < S.len;
     int jc = first;                      // tile in hand
     auto step = [&](const char *Q, const char *G, const float *L, const float *Dl) {
-        const int j0 = jc * kPtQRows;
+        const int j0 = jc * kPtQRows + 32 * upper;
         jc = jc + 1 == first + tiles ? first : jc + 1;
-        if (!live || (a.causal && j0 + kPtQRows - 1 < w0)) return;
-        pt_dkv_tile<DT, D>(a, A, R, kt, 32 * wave, Q, G, L, Dl, j0, S.len, j0 + kPtQRows > S.len || (a.causal && j0 < w0 + 31), up);
+        if (!live || j0 >= S.len || (a.causal && j0 + 31 < w0)) return;
+        pt_dkv_tile<DT, D>(a, A, R, kt, AK, Q, G, L + 32 * upper, Dl + 32 * upper, j0, S.len,
+                           j0 + 32 > S.len || (a.causal && j0 < w0 + 31), up);
     };
     for (int i = 0; i < n; i += 2) {
         pt_sync();
@@ -874,7 +897,17 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
         if (i + 2 < n) copy(q0, g0, l0, d0);
         step(q1, g1, l1, d1);
     }
-    if (!live) return;
+    // dk, then dv, of the upper half by way of the tiles' buffers, one a wave
+    char *lds = kw == 0 ? q0 : kw == 1 ? q1 : kw == 2 ? g0 : g1;
+    __syncthreads();
+    if (upper) pt_give(lds, R.dk);
+    __syncthreads();
+    if (!upper) pt_take(lds, R.dk);
+    __syncthreads();
+    if (upper) pt_give(lds, R.dv);
+    __syncthreads();
+    if (upper || !live) return;
+    pt_take(lds, R.dv);
     const bool mine = R.s < S.len;
     pt_store<DT, D>(const_cast<char *>(a.dk.p) + (int64_t)(S.start + R.s) * a.dk.st + hk * a.dk.sh, R.dk, a.scale / scale, mine);
     pt_store<DT, D>(const_cast<char *>(a.dv.p) + (int64_t)(S.start + R.s) * a.dv.st + hk * a.dv.sh, R.dv,
