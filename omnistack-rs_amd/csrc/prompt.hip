@@ -251,40 +251,43 @@ __device__ __forceinline__ void pt_store(char *p, const pf16_t (&x)[D / 32], flo
         }
 }
 
-// Zeros to rows row0 .. row0 + R - 1, below len, of a head.
+// Zeros to rows row0 .. row0 + R - 1 of a slot's: token r / G, head h0 + r % G.
 template <int D, int R>
-__device__ __forceinline__ void pt_zero_rows(const PromptHeads &o, int start, int row0, int len, int h) {
+__device__ __forceinline__ void pt_zero_rows(const PromptHeads &o, int start, int row0, int len, int h0, int G) {
     constexpr int CH = D / 8;
     for (int e = threadIdx.x; e < R * CH; e += blockDim.x) {
-        const int t = row0 + e / CH;
+        const int r = row0 + e / CH, t = r / G;
         if (t < len)
-            *reinterpret_cast<uint4 *>(const_cast<char *>(o.p) + (int64_t)(start + t) * o.st + h * o.sh + e % CH * 16) =
+            *reinterpret_cast<uint4 *>(const_cast<char *>(o.p) + (int64_t)(start + t) * o.st + (h0 + r - t * G) * o.sh + e % CH * 16) =
                 make_uint4(0, 0, 0, 0);
     }
 }
 
 // ── which rows a block takes ────────────────────────────────────────────
 //
-// Row tiles of R are dealt to slots: sequence b has the slots from
-// cu[b] / R + b on, one more than its tokens' tiles at most, so no list is
-// made and the grid, N / R + B + 1 slots, needs only the total.  The slots
-// behind the last sequence's are those of the rows of none.  Of a sequence's
-// tiles those with the most work under a causal mask come first: the last query
-// rows, the first keys.
+// A sequence's rows are its tokens, or its tokens' query heads of one kv head,
+// head by head (row r: token r / G, head r % G of the group), so that a short
+// sequence's heads fill a tile together and share its keys.  Tiles of R rows
+// are dealt to slots: sequence b has the slots from G cu[b] / R + b on, one more
+// than its tiles at most, so no list is made and the grid, G N / R + B + 1
+// slots, needs only the total.  The slots behind the last sequence's are those
+// of the tokens of none.  Of a sequence's tiles those with the most work under a
+// causal mask come first: the last query rows, the first keys.
 
 struct PtSlot {
-    int start, len, tile;                // tile < 0: nothing to do
-    bool none;                           // rows of no sequence
+    int start, len, tile;                // tokens; tile < 0: nothing to do
+    bool none;                           // tokens of no sequence
 };
 
 template <int R>
-__device__ __forceinline__ PtSlot pt_slot(const int32_t *cu, int B, int64_t N, int64_t slot, bool last_first) {
+__device__ __forceinline__ PtSlot pt_slot(const int32_t *cu, int B, int64_t N, int G, int64_t slot, bool last_first) {
     const int lane = threadIdx.x & 63;
-    // the last b in [0, B] with cu[b] / R + b <= slot, 64 ways a step
+    auto base = [&](int b) { return (int64_t)((uint64_t)(uint32_t)cu[b] * (uint32_t)G / R) + b; };
+    // the last b in [0, B] with base(b) <= slot, 64 ways a step
     int lo = 0, n = B + 1;
     while (n > 1) {
         const int step = (n + 63) / 64, b = lo + lane * step;
-        const bool below = lane * step < n && (int64_t)((uint32_t)cu[b] / R) + b <= slot;
+        const bool below = lane * step < n && base(b) <= slot;
         const int at = 63 - __builtin_clzll(__ballot(below) | 1ull);
         lo += at * step;
         n = min(step, n - at * step);
@@ -292,16 +295,31 @@ __device__ __forceinline__ PtSlot pt_slot(const int32_t *cu, int B, int64_t N, i
     lo = __builtin_amdgcn_readfirstlane(lo);
     PtSlot s;
     const int64_t a = cu[lo], e = lo < B ? (int64_t)cu[lo + 1] : N;
-    const int64_t first = (int64_t)((uint32_t)cu[lo] / R) + lo;
     s.none = lo == B;
-    // whatever cu holds, rows stay within 0 .. N
+    // whatever cu holds, tokens stay within 0 .. N
     s.start = (int)(a < 0 ? 0 : a > N ? N : a);
     const int64_t end = e > N ? N : e;
     s.len = end > s.start ? (int)(end - s.start) : 0;
-    const int64_t tiles = ((int64_t)s.len + R - 1) / R, at = slot - first;
+    const int64_t tiles = ((int64_t)s.len * G + R - 1) / R, at = slot - base(lo);
     s.tile = at < 0 || at >= tiles ? -1 : (int)(last_first ? tiles - 1 - at : at);
     return s;
 }
+
+// The wave's 32 query rows from row w0 of the sequence's (kv head hk).
+struct PtQueries {
+    int t, h;                            // the lane's token and head (its row, or the last)
+    int first, last;                     // the wave's tokens
+    bool mine, live;                     // the lane's row is one; the wave's first is
+    __device__ __forceinline__ void init(const PromptArgs &a, const PtSlot &S, int hk, int w0) {
+        const int rows = S.len * a.G, row = w0 + (threadIdx.x & 31), r = min(row, rows - 1);
+        mine = row < rows;
+        live = w0 < rows;
+        t = r / a.G;
+        h = hk * a.G + r - t * a.G;
+        first = w0 / a.G;
+        last = min((w0 + 31) / a.G, S.len - 1);
+    }
+};
 
 // ── forward ─────────────────────────────────────────────────────────────
 //
@@ -338,6 +356,9 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
     constexpr int NT = PtRow<DT, D>::NT;
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
+    // issue order only: of a SIMD's two waves the one feeding the matrix units goes
+    // first (8192 tokens without a mask 1025 -> 978 us; no gain in the gradient's kernels)
+    __builtin_amdgcn_s_setprio(1);
     pf16_t s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -345,6 +366,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (masked) {
         // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
         const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -400,6 +422,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
             R.l += x[0];
         }
     }
+    __builtin_amdgcn_s_setprio(2);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -412,6 +435,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
                 if constexpr (LO) R.o[d] = pt_mfma<DT>(v, pt_frag(lo[b] + 4 * k), R.o[d]);
             }
         }
+    __builtin_amdgcn_s_setprio(0);
 }
 
 template <int DT, int D, bool LO>
@@ -420,20 +444,20 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
     constexpr int NT = D / 32;
     // kv heads vary fastest, so that with eight of them (or a multiple) a kv
-    // head's blocks share an XCD and its L2; then the group's heads
+    // head's blocks share an XCD and its L2
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
-    const int64_t r = bid / a.Hkv;
-    const int h = hk * a.G + (int)(r % a.G);
-    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, r / a.G, true);
+    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, a.G, bid / a.Hkv, true);
     if (S.tile < 0) return;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int row0 = S.tile * kPtRows;
     if (S.none) {
         if (!a.fill) return;
-        pt_zero_rows<D, kPtRows>(a.o, S.start, row0, S.len, h);
-        for (int e = threadIdx.x; a.lse && e < kPtRows; e += 64 * kPtWaves)
-            if (row0 + e < S.len) a.lse[(int64_t)h * a.N + S.start + row0 + e] = -INFINITY;
+        pt_zero_rows<D, kPtRows>(a.o, S.start, row0, S.len, hk * a.G, a.G);
+        for (int e = threadIdx.x; a.lse && e < kPtRows; e += 64 * kPtWaves) {
+            const int r = row0 + e, t = r / a.G;
+            if (t < S.len) a.lse[(int64_t)(hk * a.G + r - t * a.G) * a.N + S.start + t] = -INFINITY;
+        }
         return;
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
@@ -445,22 +469,21 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
 
     PtLane<D> A;
     A.init();
+    PtQueries W;
+    W.init(a, S, hk, row0 + 32 * wave);
     PtRow<DT, D> R;
-    const int w0 = row0 + 32 * wave;     // the wave's first row
-    R.t = w0 + (lane & 31);
-    pt_load_rows<D>(a.q.p + (int64_t)(S.start + min(R.t, S.len - 1)) * a.q.st + h * a.q.sh, R.q,
-                    a.negate ? 0x80008000u : 0u);
+    R.t = W.t;
+    pt_load_rows<D>(a.q.p + (int64_t)(S.start + W.t) * a.q.st + W.h * a.q.sh, R.q, a.negate ? 0x80008000u : 0u);
     R.m = -INFINITY;
     R.l = R.l16 = 0.0f;
 #pragma unroll
     for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
 
-    const int kend = a.causal ? min(S.len, row0 + kPtRows) : S.len;       // keys that the block sees
-    const int wlast = a.causal ? min(w0 + 31, S.len - 1) : S.len - 1;     // and the wave
-    const bool live = w0 < S.len;
+    const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;   // keys that the block sees
+    const int wlast = a.causal ? W.last : S.len - 1;                                  // the last that the wave sees
     auto step = [&](const char *K, const char *V, int j0, auto even) {
-        if (!live || j0 > wlast) return;
-        const bool masked = j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0);
+        if (!W.live || j0 > wlast) return;
+        const bool masked = j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > W.first);
         if (LO && decltype(even)::value && j0 == 0) pt_forward_tile<DT, D, LO>(a, A, R, K, V, j0, S.len, masked);
         else pt_forward_tile<DT, D, false>(a, A, R, K, V, j0, S.len, masked);
     };
@@ -479,18 +502,15 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
         }
         step(k1, v1, j0 + kPtKeys, std::false_type());
     }
-    if (!live) return;
+    if (!W.live) return;
 
-    const bool mine = R.t < S.len;
+    const int64_t at = S.start + W.t;
     const float inv = 1.0f / pt_sum_halves(R.l16), l = pt_sum_halves(R.l);
-    char *op = const_cast<char *>(a.o.p) + (int64_t)(S.start + R.t) * a.o.st + h * a.o.sh;
-    if constexpr (LO) {
-        pt_store<DT, D, true>(op, R.o, inv, mine, const_cast<char *>(a.olo.p) + (int64_t)(S.start + R.t) * a.olo.st + h * a.olo.sh);
-    } else {
-        pt_store<DT, D>(op, R.o, inv, mine);
-    }
-    if (a.lse && mine && half == 0)
-        a.lse[(int64_t)h * a.N + S.start + R.t] = (R.m - (DT == OMNI_F16 ? kPtF16Up : 0.0f) + __log2f(l)) * 0.69314718f;
+    char *op = const_cast<char *>(a.o.p) + at * a.o.st + W.h * a.o.sh;
+    if constexpr (LO) pt_store<DT, D, true>(op, R.o, inv, W.mine, const_cast<char *>(a.olo.p) + at * a.olo.st + W.h * a.olo.sh);
+    else pt_store<DT, D>(op, R.o, inv, W.mine);
+    if (a.lse && W.mine && (threadIdx.x & 32) == 0)
+        a.lse[(int64_t)W.h * a.N + at] = (R.m - (DT == OMNI_F16 ? kPtF16Up : 0.0f) + __log2f(l)) * 0.69314718f;
 }
 
 // ── backward ────────────────────────────────────────────────────────────
@@ -653,14 +673,12 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
-    const int64_t r = bid / a.Hkv;
-    const int h = hk * a.G + (int)(r % a.G);
-    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, r / a.G, true);
+    const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, a.G, bid / a.Hkv, true);
     if (S.tile < 0) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int row0 = S.tile * kPtRows;
     if (S.none) {
-        pt_zero_rows<D, kPtRows>(a.dq, S.start, row0, S.len, h);
+        pt_zero_rows<D, kPtRows>(a.dq, S.start, row0, S.len, hk * a.G, a.G);
         return;
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
@@ -672,24 +690,24 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
 
     PtLane<D> A;
     A.init();
+    PtQueries W;
+    W.init(a, S, hk, row0 + 32 * wave);
     PtGradRow<DT, D> R;
-    const int w0 = row0 + 32 * wave;
-    R.t = w0 + (lane & 31);
-    const int64_t at = S.start + min(R.t, S.len - 1);
-    pt_load_rows<D>(a.q.p + at * a.q.st + h * a.q.sh, R.q);
-    pt_load_rows<D>(a.g.p + at * a.g.st + h * a.g.sh, R.g);
-    R.lse2 = a.lse2[(int64_t)h * a.N + at];
-    R.delta = a.delta[(int64_t)h * a.N + at];
+    R.t = W.t;
+    const int64_t at = S.start + W.t;
+    pt_load_rows<D>(a.q.p + at * a.q.st + W.h * a.q.sh, R.q);
+    pt_load_rows<D>(a.g.p + at * a.g.st + W.h * a.g.sh, R.g);
+    R.lse2 = a.lse2[(int64_t)W.h * a.N + at];
+    R.delta = a.delta[(int64_t)W.h * a.N + at];
     const float up = pt_ds_scale<DT>(a);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
 
-    const int kend = a.causal ? min(S.len, row0 + kPtRows) : S.len;
-    const int wlast = a.causal ? min(w0 + 31, S.len - 1) : S.len - 1;
-    const bool live = w0 < S.len;
+    const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;
+    const int wlast = a.causal ? W.last : S.len - 1;
     auto step = [&](const char *K, const char *V, int j0) {
-        if (!live || j0 > wlast) return;
-        pt_dq_tile<DT, D>(a, A, R, K, V, j0, S.len, j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > w0), up);
+        if (!W.live || j0 > wlast) return;
+        pt_dq_tile<DT, D>(a, A, R, K, V, j0, S.len, j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > W.first), up);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();
@@ -706,8 +724,8 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
         }
         step(k1, v1, j0 + kPtKeys);
     }
-    if (!live) return;
-    pt_store<DT, D>(const_cast<char *>(a.dq.p) + (int64_t)(S.start + R.t) * a.dq.st + h * a.dq.sh, R.dq, a.scale / up, R.t < S.len);
+    if (!W.live) return;
+    pt_store<DT, D>(const_cast<char *>(a.dq.p) + at * a.dq.st + W.h * a.dq.sh, R.dq, a.scale / up, W.mine);
 }
 
 // dk and dv: a wave holds 32 keys as B operands of S = Q K^T and G V^T, so
@@ -833,14 +851,14 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
     // the first keys are seen by the most rows
-    const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, bid / a.Hkv, false);
+    const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, 1, bid / a.Hkv, false);
     if (S.tile < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kw = wave & 3, upper = wave >> 2;
     const int key0 = S.tile * kPtKvKeys;
     if (S.none) {
-        pt_zero_rows<D, kPtKvKeys>(a.dk, S.start, key0, S.len, hk);
-        pt_zero_rows<D, kPtKvKeys>(a.dv, S.start, key0, S.len, hk);
+        pt_zero_rows<D, kPtKvKeys>(a.dk, S.start, key0, S.len, hk, 1);
+        pt_zero_rows<D, kPtKvKeys>(a.dv, S.start, key0, S.len, hk, 1);
         return;
     }
     const int first = a.causal ? key0 / kPtQRows : 0, tiles = (S.len + kPtQRows - 1) / kPtQRows - first;
@@ -933,7 +951,7 @@ static int prompt_args(const char *who, int dtype, int64_t N, int Hq, int Hkv, i
     OMNI_CHECK_ARG(dtype == OMNI_F16 || dtype == OMNI_BF16, "%s: dtype must be f16 or bf16", who);
     OMNI_CHECK_ARG(D == 32 || D == 64 || D == 128, "%s: head_dim must be 32, 64 or 128, got %d", who, D);
     OMNI_CHECK_ARG(N >= 0 && B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "%s: bad shape (Hq must be a multiple of Hkv)", who);
-    OMNI_CHECK_ARG(N < (int64_t(1) << 31) - 1024 && B < (int64_t(1) << 30) && Hq <= 65536, "%s: shape too large", who);
+    OMNI_CHECK_ARG(N < (int64_t(1) << 31) && N * Hq < (int64_t(1) << 31) - 1024 && B < (int64_t(1) << 30), "%s: shape too large", who);
     OMNI_CHECK_ARG(scale == scale && fabsf(scale) <= 3.0e38f, "%s: scale must be finite", who);
     a.N = N;
     a.B = (int)B;
@@ -998,7 +1016,7 @@ extern "C" int omni_prompt_attn(const void *q, const int64_t *q_strides, const v
     a.causal = causal != 0;
     a.fill = fill_rest != 0;
     dim3 grid;
-    OMNI_CHECK_ARG(prompt_grid((N / kPtRows + B + 1) * Hq, grid), "%s: grid too large", who);
+    OMNI_CHECK_ARG(prompt_grid((N * a.G / kPtRows + B + 1) * Hkv, grid), "%s: grid too large", who);
     if (dtype == OMNI_F16) prompt_launch_forward<OMNI_F16>(a, head_dim, grid, as_stream(stream));
     else prompt_launch_forward<OMNI_BF16>(a, head_dim, grid, as_stream(stream));
     OMNI_CHECK_LAUNCH(who);
@@ -1009,7 +1027,7 @@ template <int DT, int D>
 static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
     const char *who = "omni_prompt_attn_backward";
     dim3 rows, keys;
-    OMNI_CHECK_ARG(prompt_grid((a.N / kPtRows + a.B + 1) * a.Hq, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv, keys),
+    OMNI_CHECK_ARG(prompt_grid((a.N * a.G / kPtRows + a.B + 1) * a.Hkv, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv, keys),
                    "%s: grid too large", who);
     hipLaunchKernelGGL((prompt_delta_kernel<DT, D>), dim3(a.peak_rows), dim3(256), 0, st, a);
     OMNI_CHECK_LAUNCH(who);
