@@ -263,6 +263,67 @@ __device__ __forceinline__ void pt_zero_rows(const PromptHeads &o, int start, in
     }
 }
 
+// Hidden keys and rows count for nothing, whatever they hold, but a matrix unit
+// multiplies their weight of 0 with it.  Tiles that hide some are therefore
+// looked through (a tenth of such a tile's time), and a wave that met an
+// infinity or a NaN there computes its result again, term by term and from
+// memory.  Tokens behind the sequence need no look: the copies put its last
+// token in their place, which all that could see them see.
+template <int DT>
+__device__ __forceinline__ bool pt_all_finite(const char *tile, int bytes) {
+    // an exponent of ones carries into the sign's place
+    constexpr uint32_t ONES = DT == OMNI_BF16 ? 0x7f807f80u : 0x7c007c00u, LAST = DT == OMNI_BF16 ? 0x00800080u : 0x04000400u;
+    uint32_t any = 0;
+    for (int at = (threadIdx.x & 63) * 16; at < bytes; at += 1024) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(tile + at);
+        any |= ((u.x & ONES) + LAST) | ((u.y & ONES) + LAST) | ((u.z & ONES) + LAST) | ((u.w & ONES) + LAST);
+    }
+    return __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0) == 0;
+}
+
+// acc += sum over rows r0 .. r0 + 31 of x (its row 0 at `base`) of w times the
+// row, where the lane's column sees it, rows first .. end - 1.  w is laid out as
+// an MFMA result.
+template <int DT, int D>
+__device__ __forceinline__ void pt_add_terms(pf16_t (&acc)[D / 32], pf16_t w, const char *base, int64_t st, int r0, int first, int end) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+        // the weights of the lower half's row and of the upper's; the next ones move up
+        const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(w[0]), __float_as_uint(w[0]), false, false);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+            const float f = __uint_as_float(h ? u[1] : u[0]);
+            const int r = r0 + 8 * (i / 4) + 4 * h + i % 4;
+            if (r < first || r >= end) continue;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(base + (int64_t)r * st + (32 * d + 8 * g + 4 * half) * 2);
+                    const float x[4] = {pt_value<DT>(v.x), pt_value<DT>(v.x >> 16), pt_value<DT>(v.y), pt_value<DT>(v.y >> 16)};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[d][4 * g + e] = fmaf(f, x[e], acc[d][4 * g + e]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 15; ++k) w[k] = w[k + 1];
+    }
+}
+
+// x . y of 32 rows of each: A operand rows r0 .. of x from memory (rows from len
+// on repeat the last), B operand y(kk).
+template <int DT, int D, class Y>
+__device__ __forceinline__ pf16_t pt_product(const char *base, int64_t st, int r0, int len, float init, Y y) {
+    const char *p = base + (int64_t)min(r0 + (int)(threadIdx.x & 31), len - 1) * st + 16 * ((threadIdx.x >> 5) & 1);
+    pf16_t s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = init;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) s = pt_mfma<DT>(*reinterpret_cast<const ps8_t *>(p + 32 * kk), y(kk), s);
+    return s;
+}
+
 // ── which rows a block takes ────────────────────────────────────────────
 //
 // A sequence's rows are its tokens, or its tokens' query heads of one kv head,
@@ -347,7 +408,8 @@ struct PtRow {
     pf16_t o[NT];
     float m;                             // running maximum of scale s log2 e
     float l, l16;                        // the lane's share of the sum of the probabilities, and of the rounded ones
-    int t;                               // the row (of the sequence)
+    int t;                               // the row's token (of the sequence)
+    bool met;                            // an infinity or NaN among hidden values
 };
 
 // LO: the probabilities' rounding errors, rounded in turn, are added as well.
@@ -367,6 +429,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
         for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
     __builtin_amdgcn_s_setprio(0);
+    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(V, kPtKeys * 2 * D));
     if (masked) {
         // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
         const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -476,6 +539,7 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     pt_load_rows<D>(a.q.p + (int64_t)(S.start + W.t) * a.q.st + W.h * a.q.sh, R.q, a.negate ? 0x80008000u : 0u);
     R.m = -INFINITY;
     R.l = R.l16 = 0.0f;
+    R.met = false;
 #pragma unroll
     for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
 
@@ -503,6 +567,25 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
         step(k1, v1, j0 + kPtKeys, std::false_type());
     }
     if (!W.live) return;
+    if (R.met) {
+        // term by term, the maximum being known (of the rounded probabilities' sums alone)
+        const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
+        R.l = R.l16 = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
+#pragma unroll 1
+        for (int j0 = 0; j0 <= wlast; j0 += 32) {
+            pf16_t p = pt_product<DT, D>(kb, a.k.st, j0, S.len, 0.0f, [&](int kk) { return R.q[kk]; });
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -off));
+                if (j0 + 8 * (i / 4) + 4 * (int)((threadIdx.x >> 5) & 1) + i % 4 > R.t) p[i] = 0.0f;
+                R.l += p[i];
+            }
+            pt_add_terms<DT, D>(R.o, p, vb, a.v.st, j0, 0, min(R.t + 1, S.len));
+        }
+        R.l16 = R.l;
+    }
 
     const int64_t at = S.start + W.t;
     const float inv = 1.0f / pt_sum_halves(R.l16), l = pt_sum_halves(R.l);
@@ -559,14 +642,14 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
                 a.delta[(int64_t)h * a.N + t] = -d;
                 a.lse2[(int64_t)h * a.N + t] = a.lse[(int64_t)h * a.N + t] * 1.44269504f;
             }
-            // an infinity or NaN stays in its peak: the scale is then 1
-            if constexpr (DT == OMNI_F16) { const float n = norm(g, g); pg = n > pg || n != n ? n : pg; }
+            // what is not finite has no say: its results are not either
+            if constexpr (DT == OMNI_F16) { const float n = norm(g, g); pg = n > pg && n < INFINITY ? n : pg; }
         }
         if constexpr (DT == OMNI_F16)
             for (int h0 = 0; h0 < a.Hkv; h0 += HPW) {
                 const uint4 v = *reinterpret_cast<const uint4 *>(a.v.p + t * a.v.st + min(h0 + grp, a.Hkv - 1) * a.v.sh + sub * 16);
                 const float n = norm(v, v);
-                pv = n > pv || n != n ? n : pv;
+                pv = n > pv && n < INFINITY ? n : pv;
             }
     }
     if constexpr (DT == OMNI_F16) {
@@ -574,8 +657,8 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
 #pragma unroll
         for (int m = 32; m >= LPH; m /= 2) {
             const float x = __shfl_xor(pg, m, 64), y = __shfl_xor(pv, m, 64);
-            pg = x > pg || x != x ? x : pg;
-            pv = y > pv || y != y ? y : pv;
+            pg = fmaxf(pg, x);
+            pv = fmaxf(pv, y);
         }
         if (lane == 0) {
             peak[0][wave] = pg;
@@ -584,7 +667,7 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
         __syncthreads();
         if (threadIdx.x < 2) {
             float m = 0.0f;
-            for (int w = 0; w < 4; ++w) { const float x = peak[threadIdx.x][w]; m = x > m || x != x ? x : m; }
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, peak[threadIdx.x][w]);
             a.peaks[threadIdx.x * kPtPeaks + blockIdx.x] = m;
         }
     }
@@ -597,19 +680,13 @@ __device__ __forceinline__ float pt_ds_scale(const PromptArgs &a) {
     float m[2] = {0.0f, 0.0f};
     for (int i = threadIdx.x & 63; i < a.peak_rows; i += 64)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float x = a.peaks[e * kPtPeaks + i];
-            m[e] = x > m[e] || x != x ? x : m[e];
-        }
+        for (int e = 0; e < 2; ++e) m[e] = fmaxf(m[e], a.peaks[e * kPtPeaks + i]);
 #pragma unroll
     for (int w = 32; w > 0; w /= 2)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float x = __shfl_xor(m[e], w, 64);
-            m[e] = x > m[e] || x != x ? x : m[e];
-        }
+        for (int e = 0; e < 2; ++e) m[e] = fmaxf(m[e], __shfl_xor(m[e], w, 64));
     const float bound = 2.0f * sqrtf(m[0]) * sqrtf(m[1]);
-    if (!(bound > 0.0f) || !(bound < 1.0e30f)) return 1.0f;
+    if (!(bound > 0.0f)) return 1.0f;
     const int e = 14 - ilogbf(bound);                        // bound 2^e in [2^14, 2^15)
     return ldexpf(1.0f, min(max(e, -100), 100));
 }
@@ -621,6 +698,7 @@ struct PtGradRow {
     pf16_t dq[NT];
     float lse2, delta;
     int t;
+    bool met;                            // an infinity or NaN among hidden keys
 };
 
 // One tile of 64 keys for the wave's 32 query rows; transposed like the forward.
@@ -629,6 +707,7 @@ __device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, const PtLane<D> 
                                            bool masked, float up) {
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
+    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(K, kPtKeys * 2 * D));
     const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -702,6 +781,7 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     const float up = pt_ds_scale<DT>(a);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
+    R.met = false;
 
     const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;
     const int wlast = a.causal ? W.last : S.len - 1;
@@ -725,6 +805,18 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
         step(k1, v1, j0 + kPtKeys);
     }
     if (!W.live) return;
+    if (R.met) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
+#pragma unroll 1
+        for (int j0 = 0; j0 <= wlast; j0 += 32) {
+            const pf16_t s = pt_product<DT, D>(kb, a.k.st, j0, S.len, 0.0f, [&](int kk) { return R.q[kk]; });
+            pf16_t ds = pt_product<DT, D>(vb, a.v.st, j0, S.len, R.delta, [&](int kk) { return R.g[kk]; });
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[i] *= __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -R.lse2)) * up;
+            pt_add_terms<DT, D>(R.dq, ds, kb, a.k.st, j0, 0, min(R.t + 1, S.len));
+        }
+    }
     pt_store<DT, D>(const_cast<char *>(a.dq.p) + at * a.dq.st + W.h * a.dq.sh, R.dq, a.scale / up, W.mine);
 }
 
@@ -752,15 +844,17 @@ struct PtGradKey {
     ps8_t k[KLDS ? 1 : D / 16], v[D / 16];
     pf16_t dk[NT], dv[NT];
     int s;
+    bool met;                            // an infinity or NaN among hidden rows
 };
 
-// 32 rows from row j0 on.  kr: the lane's offset in K's tile (KLDS).
+// 32 rows from row j0 on, in the tiles from row r0 on.
 template <int DT, int D>
 __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtGradKey<DT, D> &R, const char *K,
                                             const PtLane<D> &key_at, const char *Q, const char *G, const float *lse2,
-                                            const float *delta, int j0, int len, bool masked, float up) {
+                                            const float *delta, int j0, int r0, int len, bool masked, float up) {
     constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
     const PtLane<D> A = lane_at.fresh(), AK = KLDS ? key_at.fresh() : A;
+    R.met = R.met || (masked && a.causal && !(pt_all_finite<DT>(Q + r0 * 2 * D, 64 * D) && pt_all_finite<DT>(G + r0 * 2 * D, 64 * D)));
     const int half = (threadIdx.x >> 5) & 1;
     pf16_t s = {}, dp;
 #pragma unroll
@@ -897,13 +991,14 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     const float scale = pt_ds_scale<DT>(a), up = DT == OMNI_F16 ? scale * 6.103515625e-5f : 1.0f;   // p is times 2^14
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) R.dk[d] = R.dv[d] = pf16_t{};
+    R.met = false;
     const bool live = w0 < S.len;
     int jc = first;                      // tile in hand
     auto step = [&](const char *Q, const char *G, const float *L, const float *Dl) {
         const int j0 = jc * kPtQRows + 32 * upper;
         jc = jc + 1 == first + tiles ? first : jc + 1;
         if (!live || j0 >= S.len || (a.causal && j0 + 31 < w0)) return;
-        pt_dkv_tile<DT, D>(a, A, R, kt, AK, Q, G, L + 32 * upper, Dl + 32 * upper, j0, S.len,
+        pt_dkv_tile<DT, D>(a, A, R, kt, AK, Q, G, L + 32 * upper, Dl + 32 * upper, j0, 32 * upper, S.len,
                            j0 + 32 > S.len || (a.causal && j0 < w0 + 31), up);
     };
     for (int i = 0; i < n; i += 2) {
@@ -914,6 +1009,29 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
         pt_sync();
         if (i + 2 < n) copy(q0, g0, l0, d0);
         step(q1, g1, l1, d1);
+    }
+    if (R.met) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) R.dk[d] = R.dv[d] = pf16_t{};
+#pragma unroll 1
+        for (int g = 0; g < a.G; ++g) {
+            const int64_t h = hk * a.G + g;
+            const char *qb = a.q.p + (int64_t)S.start * a.q.st + h * a.q.sh, *gb = a.g.p + (int64_t)S.start * a.g.st + h * a.g.sh;
+#pragma unroll 1
+            for (int j0 = w0 / 64 * 64 + 32 * upper; j0 < S.len; j0 += 64) {       // the rows that this half takes in every tile
+                if (j0 + 31 < w0) continue;
+                pf16_t s = pt_product<DT, D>(qb, a.q.st, j0, S.len, 0.0f, [&](int kk) { return KLDS ? AK.rows(kt, 0, kk) : R.k[KLDS ? 0 : kk]; });
+                pf16_t ds = pt_product<DT, D>(gb, a.g.st, j0, S.len, 0.0f, [&](int kk) { return R.v[kk]; });
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int64_t row = h * a.N + S.start + min(j0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4, S.len - 1);
+                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - a.lse2[row]));
+                    ds[i] = s[i] * ((ds[i] + a.delta[row]) * up);
+                }
+                pt_add_terms<DT, D>(R.dv, s, gb, a.g.st, j0, R.s, S.len);
+                pt_add_terms<DT, D>(R.dk, ds, qb, a.q.st, j0, R.s, S.len);
+            }
+        }
     }
     // dk, then dv, of the upper half by way of the tiles' buffers, one a wave
     char *lds = kw == 0 ? q0 : kw == 1 ? q1 : kw == 2 ? g0 : g1;

@@ -316,3 +316,59 @@ def test_native_refusals():
     a = (4096, s)
     rc = L.omni_prompt_attn_backward(*a, *a, *a, 2, 5, 2, 1, 64, 4096, 1, 1.0, 1, *a, *a, 4096, *a, *a, *a, *a, 4096, 100, None)
     assert rc == _lib.OMNI_EWORKSPACE and "workspace" in _lib.last_error()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("D,dtype,G", [(128, "bf16", 4), (64, "f16", 1), (32, "bf16", 3)])
+def test_infinities_and_nan_stay_with_who_sees_them(device, bad, D, dtype, G):
+    """A token that holds an infinity or a NaN in q, k, v or the output's
+    gradient: what does not see it is as if it held an ordinary number (the
+    bars of two computations of one result), other sequences and heads are the
+    same bits (f16: the scale of ds may be another power of two, within the
+    bars); what sees a NaN is NaN."""
+    from omnistack_rs.attention import prompt_attention
+    lengths, Hkv = [70, 230, 40], 2
+    cu, N = _cu(lengths)
+    base = [t.to(device) for t in _inputs(N, Hkv * G, Hkv, D, dtype, 60)]
+    a, b = 70, 300                                   # the second sequence's tokens
+
+    def run(q, k, v, do):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = prompt_attention(*leaves, cu)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    want = _want(*base[:3], cu, True, 1 / math.sqrt(D), base[3])
+    bars = [2 * want[n][1] for n in ("o", "dq", "dk", "dv")]
+    clean = run(*base)
+    for at in (0, 1, 33, 63, 64, 100, 229):
+        for which in range(4):
+            x = [t.clone() for t in base]
+            x[which][a + at, 0, 5] = bad             # head 0 (of kv head 0, query head 0)
+            got = run(*x)
+            for i, (g, c, bar) in enumerate(zip(got, clean, bars)):
+                name = f"{'q k v do'.split()[which]} at {at}: {'o dq dk dv'.split()[i]}"
+                heads = g.shape[1] // Hkv            # of kv head 0; the other's are untouched
+                if dtype == "bf16" or i == 0:
+                    assert torch.equal(g[:a], c[:a]) and torch.equal(g[b:], c[b:]), name
+                    assert torch.equal(g[a:b, heads:], c[a:b, heads:]), name
+                others = [(g[:a].double() - c[:a].double()).abs() <= bar[:a] + 2.0 ** -24,
+                          (g[b:].double() - c[b:].double()).abs() <= bar[b:] + 2.0 ** -24]
+                assert all(bool(x.all()) for x in others), name
+                rows = torch.ones(b - a, g.shape[1], dtype=torch.bool, device=device)     # who may differ
+                rows[:, heads:] = False
+                if which in (0, 3) and i < 2:        # q, do: query head 0's row alone (do: not the output)
+                    rows[:] = False
+                    rows[at, 0] = not (which == 3 and i == 0)
+                elif which in (0, 3):                # keys that the row sees
+                    rows[at + 1:] = False
+                elif i < 2:                          # k, v: rows that see the key
+                    rows[:at] = False
+                elif which == 2 and i == 3:          # v is not in dv
+                    rows[:] = False
+                same = ~rows
+                err = (g[a:b].double() - c[a:b].double()).abs()[same]
+                ok = bool((err <= bars[i][a:b][same] + 2.0 ** -24).all())     # NaN fails
+                assert ok, f"{name}: {err.max().item()}"
+                if math.isnan(bad) and rows.any() and not (which == 3 and i == 1):
+                    assert bool(torch.isnan(g[a:b][rows]).any(-1).all()), f"{name}: NaN was lost"
