@@ -285,8 +285,11 @@ __device__ __forceinline__ bool pt_all_finite(const char *tile, int bytes) {
 // row, where the lane's column sees it, rows first .. end - 1.  w is laid out as
 // an MFMA result.
 template <int DT, int D>
-__device__ __forceinline__ void pt_add_terms(pf16_t (&acc)[D / 32], pf16_t w, const char *base, int64_t st, int r0, int first, int end) {
+__device__ __forceinline__ void pt_add_terms(float (&acc)[D / 32][16], const pf16_t &weights, const char *base, int64_t st, int r0, int first, int end) {
     const int half = (threadIdx.x >> 5) & 1;
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = weights[i];
 #pragma unroll 1
     for (int i = 0; i < 16; ++i) {
         // the weights of the lower half's row and of the upper's; the next ones move up
@@ -309,6 +312,21 @@ __device__ __forceinline__ void pt_add_terms(pf16_t (&acc)[D / 32], pf16_t w, co
 #pragma unroll
         for (int k = 0; k < 15; ++k) w[k] = w[k + 1];
     }
+}
+
+template <int NT>
+__device__ __forceinline__ void pt_clear(float (&x)[NT][16]) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[d][i] = 0.0f;
+}
+template <int NT>
+__device__ __forceinline__ void pt_assign(pf16_t (&y)[NT], const float (&x)[NT][16]) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[d][i] = x[d][i];
 }
 
 // x . y of 32 rows of each: A operand rows r0 .. of x from memory (rows from len
@@ -570,9 +588,9 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     if (R.met) {
         // term by term, the maximum being known (of the rounded probabilities' sums alone)
         const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
-        R.l = R.l16 = 0.0f;
-#pragma unroll
-        for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
+        R.l = 0.0f;
+        float o[NT][16];
+        pt_clear(o);
 #pragma unroll 1
         for (int j0 = 0; j0 <= wlast; j0 += 32) {
             pf16_t p = pt_product<DT, D>(kb, a.k.st, j0, S.len, 0.0f, [&](int kk) { return R.q[kk]; });
@@ -582,9 +600,10 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
                 if (j0 + 8 * (i / 4) + 4 * (int)((threadIdx.x >> 5) & 1) + i % 4 > R.t) p[i] = 0.0f;
                 R.l += p[i];
             }
-            pt_add_terms<DT, D>(R.o, p, vb, a.v.st, j0, 0, min(R.t + 1, S.len));
+            pt_add_terms<DT, D>(o, p, vb, a.v.st, j0, 0, min(R.t + 1, S.len));
         }
         R.l16 = R.l;
+        pt_assign(R.o, o);
     }
 
     const int64_t at = S.start + W.t;
@@ -806,16 +825,17 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     }
     if (!W.live) return;
     if (R.met) {
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
+        float dq[D / 32][16];
+        pt_clear(dq);
 #pragma unroll 1
         for (int j0 = 0; j0 <= wlast; j0 += 32) {
             const pf16_t s = pt_product<DT, D>(kb, a.k.st, j0, S.len, 0.0f, [&](int kk) { return R.q[kk]; });
             pf16_t ds = pt_product<DT, D>(vb, a.v.st, j0, S.len, R.delta, [&](int kk) { return R.g[kk]; });
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] *= __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -R.lse2)) * up;
-            pt_add_terms<DT, D>(R.dq, ds, kb, a.k.st, j0, 0, min(R.t + 1, S.len));
+            pt_add_terms<DT, D>(dq, ds, kb, a.k.st, j0, 0, min(R.t + 1, S.len));
         }
+        pt_assign(R.dq, dq);
     }
     pt_store<DT, D>(const_cast<char *>(a.dq.p) + at * a.dq.st + W.h * a.dq.sh, R.dq, a.scale / up, W.mine);
 }
@@ -1011,27 +1031,36 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
         step(q1, g1, l1, d1);
     }
     if (R.met) {
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) R.dk[d] = R.dv[d] = pf16_t{};
+        // dk, then dv, each alone: both at once take registers that the loop above could not have
+        auto again = [&](pf16_t (&sum)[D / 32], auto keys) {
+            constexpr bool DK = decltype(keys)::value;
+            float acc[D / 32][16];
+            pt_clear(acc);
 #pragma unroll 1
-        for (int g = 0; g < a.G; ++g) {
-            const int64_t h = hk * a.G + g;
-            const char *qb = a.q.p + (int64_t)S.start * a.q.st + h * a.q.sh, *gb = a.g.p + (int64_t)S.start * a.g.st + h * a.g.sh;
+            for (int g = 0; g < a.G; ++g) {
+                const int64_t h = hk * a.G + g;
+                const char *qb = a.q.p + (int64_t)S.start * a.q.st + h * a.q.sh, *gb = a.g.p + (int64_t)S.start * a.g.st + h * a.g.sh;
 #pragma unroll 1
-            for (int j0 = w0 / 64 * 64 + 32 * upper; j0 < S.len; j0 += 64) {       // the rows that this half takes in every tile
-                if (j0 + 31 < w0) continue;
-                pf16_t s = pt_product<DT, D>(qb, a.q.st, j0, S.len, 0.0f, [&](int kk) { return KLDS ? AK.rows(kt, 0, kk) : R.k[KLDS ? 0 : kk]; });
-                pf16_t ds = pt_product<DT, D>(gb, a.g.st, j0, S.len, 0.0f, [&](int kk) { return R.v[kk]; });
+                for (int j0 = w0 / 64 * 64 + 32 * upper; j0 < S.len; j0 += 64) {       // the rows that this half takes in every tile
+                    if (j0 + 31 < w0) continue;
+                    const int64_t row = h * a.N + S.start + min(j0 + (lane & 31), S.len - 1);
+                    const float l = a.lse2[row], d = a.delta[row];
+                    pf16_t w = pt_product<DT, D>(qb, a.q.st, j0, S.len, 0.0f, [&](int kk) { return KLDS ? AK.rows(kt, 0, kk) : R.k[KLDS ? 0 : kk]; });
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int64_t row = h * a.N + S.start + min(j0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4, S.len - 1);
-                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - a.lse2[row]));
-                    ds[i] = s[i] * ((ds[i] + a.delta[row]) * up);
+                    for (int i = 0; i < 16; ++i)
+                        w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - __shfl(l, 8 * (i / 4) + 4 * (lane >> 5) + i % 4, 64)));
+                    if constexpr (DK) {
+                        const pf16_t dp = pt_product<DT, D>(gb, a.g.st, j0, S.len, 0.0f, [&](int kk) { return R.v[kk]; });
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] *= (dp[i] + __shfl(d, 8 * (i / 4) + 4 * (lane >> 5) + i % 4, 64)) * up;
+                    }
+                    pt_add_terms<DT, D>(acc, w, DK ? qb : gb, DK ? a.q.st : a.g.st, j0, R.s, S.len);
                 }
-                pt_add_terms<DT, D>(R.dv, s, gb, a.g.st, j0, R.s, S.len);
-                pt_add_terms<DT, D>(R.dk, ds, qb, a.q.st, j0, R.s, S.len);
             }
-        }
+            pt_assign(sum, acc);
+        };
+        again(R.dk, std::true_type());
+        again(R.dv, std::false_type());
     }
     // dk, then dv, of the upper half by way of the tiles' buffers, one a wave
     char *lds = kw == 0 ? q0 : kw == 1 ? q1 : kw == 2 ? g0 : g1;
