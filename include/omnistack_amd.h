@@ -495,9 +495,9 @@ int omni_prompt_attn(const void *q, const int64_t *q_strides, const void *k, con
  * inputs, dout the gradient of out; writes dq, dk, dv (dk and dv summed over the group's
  * query heads), zeros in rows behind the last sequence.  No atomics: the same
  * bits on every run.  workspace (16-byte aligned):
- * omni_prompt_attn_backward_workspace_size(N, Hq) bytes.
+ * omni_prompt_attn_backward_workspace_size(N, Hq, Hkv, head_dim, B) bytes.
  */
-size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq);
+size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq, int Hkv, int head_dim, int64_t B);
 int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
                               const void *v, const int64_t *v_strides, int dtype, int64_t N, int Hq, int Hkv,
                               int head_dim, const int32_t *cu_seqlens, int64_t B, float scale, int causal,

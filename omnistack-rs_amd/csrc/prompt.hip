@@ -42,12 +42,13 @@ struct PromptArgs {
     PromptHeads g, dq, dk, dv;           // backward: the output's gradient, and those of q, k and v
     float *lse;                          // (Hq, N), or NULL
     float *lse2, *delta;                 // backward, (Hq, N): lse log2 e, and -sum_d g o
+    float *parts;                        // backward, (heads of the group in parts, dk and dv, N, Hkv, D)
     float *peaks;                        // backward in f16: kPtPeaks largest squared norms of g's rows, then of v's
     const int32_t *cu;
     int64_t N;
     int B, Hq, Hkv, G;
     int causal, negate, fill;            // fill: rows of no sequence get zeros
-    int peak_rows;
+    int peak_rows, n_parts;
     float c, cs, scale;                  // |scale| log2(e), scale log2(e)
     float hide;                          // a hidden score: cs times it is -inf
 };
@@ -430,9 +431,10 @@ struct PtRow {
     bool met;                            // an infinity or NaN among hidden values
 };
 
-// LO: the probabilities' rounding errors, rounded in turn, are added as well.
+// LO: of the first tile, the probabilities' rounding errors, rounded in turn, are
+// added as well.
 template <int DT, int D, bool LO>
-__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len, bool masked) {
+__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len, bool masked, bool first) {
     constexpr int NT = PtRow<DT, D>::NT;
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
@@ -475,7 +477,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
         R.m = mn;
     }
     const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
-    uint32_t p[2][8], lo[LO ? 2 : 1][8];
+    uint32_t p[2][8];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         float x[16];
@@ -487,12 +489,19 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[b][i] = pt_pack<DT>(x[2 * i], x[2 * i + 1]);
-            if constexpr (LO) {
-                const float e0 = x[2 * i] - pt_value<DT>(p[b][i]), e1 = x[2 * i + 1] - pt_value<DT>(p[b][i] >> 16);
-                lo[b][i] = pt_pack<DT>(e0, e1);
-                sum16 = pt_add2<DT>(lo[b][i], sum16);
-            }
             sum16 = pt_add2<DT>(p[b][i], sum16);
+        }
+        if (LO && first) {
+            uint32_t lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                lo[i] = pt_pack<DT>(x[2 * i] - pt_value<DT>(p[b][i]), x[2 * i + 1] - pt_value<DT>(p[b][i] >> 16));
+                sum16 = pt_add2<DT>(lo[i], sum16);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int d = 0; d < NT; ++d) R.o[d] = pt_mfma<DT>(A.cols(V, 32 * b + 16 * k, d), pt_frag(lo + 4 * k), R.o[d]);
         }
         R.l16 += sum16;
         if (a.lse) {
@@ -511,9 +520,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
             const ps8_t pb = pt_frag(p[b] + 4 * k);
 #pragma unroll
             for (int d = 0; d < NT; ++d) {
-                const ps8_t v = A.cols(V, 32 * b + 16 * k, d);
-                R.o[d] = pt_mfma<DT>(v, pb, R.o[d]);
-                if constexpr (LO) R.o[d] = pt_mfma<DT>(v, pt_frag(lo[b] + 4 * k), R.o[d]);
+                R.o[d] = pt_mfma<DT>(A.cols(V, 32 * b + 16 * k, d), pb, R.o[d]);
             }
         }
     __builtin_amdgcn_s_setprio(0);
@@ -563,11 +570,10 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
 
     const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;   // keys that the block sees
     const int wlast = a.causal ? W.last : S.len - 1;                                  // the last that the wave sees
-    auto step = [&](const char *K, const char *V, int j0, auto even) {
+    auto step = [&](const char *K, const char *V, int j0) {
         if (!W.live || j0 > wlast) return;
         const bool masked = j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > W.first);
-        if (LO && decltype(even)::value && j0 == 0) pt_forward_tile<DT, D, LO>(a, A, R, K, V, j0, S.len, masked);
-        else pt_forward_tile<DT, D, false>(a, A, R, K, V, j0, S.len, masked);
+        pt_forward_tile<DT, D, LO>(a, A, R, K, V, j0, S.len, masked, j0 == 0);
     };
     for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
         pt_sync();                       // this tile is there, the other buffers are read
@@ -575,14 +581,14 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
             ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1, wave);
             cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1, wave);
         }
-        step(k0, v0, j0, std::true_type());
+        step(k0, v0, j0);
         if (j0 + kPtKeys >= kend) break;
         pt_sync();
         if (j0 + 2 * kPtKeys < kend) {
             ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0, wave);
             cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0, wave);
         }
-        step(k1, v1, j0 + kPtKeys, std::false_type());
+        step(k1, v1, j0 + kPtKeys);
     }
     if (!W.live) return;
     if (R.met) {
@@ -965,23 +971,26 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     const int hk = (int)(bid % a.Hkv);
     // the first keys are seen by the most rows
-    const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, 1, bid / a.Hkv, false);
+    const int64_t rest = bid / a.Hkv;
+    const int part = (int)(rest % a.n_parts), GP = a.G / a.n_parts, h0 = hk * a.G + part * GP;   // the query heads of this block
+    const PtSlot S = pt_slot<kPtKvKeys>(a.cu, a.B, a.N, 1, rest / a.n_parts, false);
     if (S.tile < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kw = wave & 3, upper = wave >> 2;
     const int key0 = S.tile * kPtKvKeys;
     if (S.none) {
+        if (part) return;
         pt_zero_rows<D, kPtKvKeys>(a.dk, S.start, key0, S.len, hk, 1);
         pt_zero_rows<D, kPtKvKeys>(a.dv, S.start, key0, S.len, hk, 1);
         return;
     }
     const int first = a.causal ? key0 / kPtQRows : 0, tiles = (S.len + kPtQRows - 1) / kPtQRows - first;
-    const int n = tiles * a.G;
+    const int n = tiles * GP;
     PtCopy<D, kPtQRows> cp;
     cp.init(kw);
     const PromptHeads &src = upper ? a.g : a.q;          // the lower waves copy q, the upper g
-    const char *sb = src.p + (int64_t)S.start * src.st + (int64_t)hk * a.G * src.sh;
-    const float *stat = (upper ? a.delta : a.lse2) + (int64_t)hk * a.G * a.N + S.start;
+    const char *sb = src.p + (int64_t)S.start * src.st + (int64_t)h0 * src.sh;
+    const float *stat = (upper ? a.delta : a.lse2) + (int64_t)h0 * a.N + S.start;
     int gi = 0, ji = first;              // head and tile that the next copy takes
     auto copy = [&](char *Q, char *G, float *L, float *Dl) {
         cp.issue(sb + gi * src.sh, src.st, ji * kPtQRows, S.len, upper ? G : Q, kw);
@@ -1037,8 +1046,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
             float acc[D / 32][16];
             pt_clear(acc);
 #pragma unroll 1
-            for (int g = 0; g < a.G; ++g) {
-                const int64_t h = hk * a.G + g;
+            for (int g = 0; g < GP; ++g) {
+                const int64_t h = h0 + g;
                 const char *qb = a.q.p + (int64_t)S.start * a.q.st + h * a.q.sh, *gb = a.g.p + (int64_t)S.start * a.g.st + h * a.g.sh;
 #pragma unroll 1
                 for (int j0 = w0 / 64 * 64 + 32 * upper; j0 < S.len; j0 += 64) {       // the rows that this half takes in every tile
@@ -1074,9 +1083,43 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
     if (upper || !live) return;
     pt_take(lds, R.dv);
     const bool mine = R.s < S.len;
-    pt_store<DT, D>(const_cast<char *>(a.dk.p) + (int64_t)(S.start + R.s) * a.dk.st + hk * a.dk.sh, R.dk, a.scale / scale, mine);
-    pt_store<DT, D>(const_cast<char *>(a.dv.p) + (int64_t)(S.start + R.s) * a.dv.st + hk * a.dv.sh, R.dv,
-                    DT == OMNI_F16 ? 6.103515625e-5f : 1.0f, mine);
+    const float fk = a.scale / scale, fv = DT == OMNI_F16 ? 6.103515625e-5f : 1.0f;
+    if (a.n_parts == 1) {
+        pt_store<DT, D>(const_cast<char *>(a.dk.p) + (int64_t)(S.start + R.s) * a.dk.st + hk * a.dk.sh, R.dk, fk, mine);
+        pt_store<DT, D>(const_cast<char *>(a.dv.p) + (int64_t)(S.start + R.s) * a.dv.st + hk * a.dv.sh, R.dv, fv, mine);
+    } else if (mine) {
+        float *p = a.parts + (((int64_t)part * 2 * a.N + S.start + R.s) * a.Hkv + hk) * D + 4 * (lane >> 5), *q = p + a.N * a.Hkv * D;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                *reinterpret_cast<float4 *>(p + 32 * d + 2 * i) = make_float4(R.dk[d][i] * fk, R.dk[d][i + 1] * fk, R.dk[d][i + 2] * fk, R.dk[d][i + 3] * fk);
+                *reinterpret_cast<float4 *>(q + 32 * d + 2 * i) = make_float4(R.dv[d][i] * fv, R.dv[d][i + 1] * fv, R.dv[d][i + 2] * fv, R.dv[d][i + 3] * fv);
+            }
+    }
+}
+
+// dk and dv of the parts, added in their order: a thread for eight dims.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_parts_kernel(PromptArgs a) {
+    const int64_t rows = min((int64_t)max(a.cu[a.B], 0), a.N), each = a.N * a.Hkv * D;
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    const int d = (int)(e % D), hk = (int)(e / D % a.Hkv);
+    const int64_t t = e / D / a.Hkv;
+    if (t >= rows) return;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        float x[8] = {};
+        for (int p = 0; p < a.n_parts; ++p) {
+            const float4 *src = reinterpret_cast<const float4 *>(a.parts + (2 * p + w) * each + e);
+            const float4 u = src[0], v = src[1];
+            x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
+            x[4] += v.x; x[5] += v.y; x[6] += v.z; x[7] += v.w;
+        }
+        const PromptHeads &o = w ? a.dv : a.dk;
+        *reinterpret_cast<uint4 *>(const_cast<char *>(o.p) + t * o.st + hk * o.sh + 2 * d) =
+            make_uint4(pt_pack<DT>(x[0], x[1]), pt_pack<DT>(x[2], x[3]), pt_pack<DT>(x[4], x[5]), pt_pack<DT>(x[6], x[7]));
+    }
 }
 
 // ── host ────────────────────────────────────────────────────────────────
@@ -1174,7 +1217,7 @@ template <int DT, int D>
 static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
     const char *who = "omni_prompt_attn_backward";
     dim3 rows, keys;
-    OMNI_CHECK_ARG(prompt_grid((a.N * a.G / kPtRows + a.B + 1) * a.Hkv, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv, keys),
+    OMNI_CHECK_ARG(prompt_grid((a.N * a.G / kPtRows + a.B + 1) * a.Hkv, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv * a.n_parts, keys),
                    "%s: grid too large", who);
     hipLaunchKernelGGL((prompt_delta_kernel<DT, D>), dim3(a.peak_rows), dim3(256), 0, st, a);
     OMNI_CHECK_LAUNCH(who);
@@ -1182,11 +1225,38 @@ static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
     OMNI_CHECK_LAUNCH(who);
     hipLaunchKernelGGL((prompt_dkv_kernel<DT, D>), keys, dim3(64 * kPtKvWaves), 0, st, a);
     OMNI_CHECK_LAUNCH(who);
+    if (a.n_parts > 1) {
+        // fewer than 2^24 rows of dk (prompt_parts)
+        hipLaunchKernelGGL((prompt_parts_kernel<DT, D>), dim3((unsigned)((a.N * a.Hkv * D / 8 + 255) / 256)), dim3(256), 0, st, a);
+        OMNI_CHECK_LAUNCH(who);
+    }
     return OMNI_OK;
 }
 
-extern "C" size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq) {
-    return N > 0 && Hq > 0 ? (size_t)N * (size_t)Hq * 8 + kPtPeaks * 8 : 0;
+// Parts that the query heads of a kv head are dealt to in the launch for dk and
+// dv, whose blocks each hold a CU: doubled while there are not two blocks for
+// each CU, since a first key's block runs through every row of every head.  Each
+// part writes its sums in fp32 and another launch adds them.  32 heads over 8 of
+// 128, causal, the whole gradient, one part against this rule against four
+// blocks a CU: 2048 tokens 371 / 260 / 260 us, 4096 710 / 590 / 615, nine
+// sequences of 20 to 3000 tokens 586 / 534 / 590, 8192 1835 / 1840 / 1870;
+// 4096 without a mask 935 / 965 / 990.
+static int prompt_parts(int64_t N, int64_t B, int Hq, int Hkv) {
+    const int G = Hq / Hkv;
+    const int64_t blocks = (N / kPtKvKeys + B) * Hkv;
+    int parts = 1;
+    while (G % (2 * parts) == 0 && blocks * parts < 2 * device_cus()) parts *= 2;
+    return parts;
+}
+
+static size_t prompt_stats_bytes(int64_t N, int Hq) {
+    return (((size_t)N * (size_t)Hq * 2 + 2 * kPtPeaks) * 4 + 15) / 16 * 16;
+}
+
+extern "C" size_t omni_prompt_attn_backward_workspace_size(int64_t N, int Hq, int Hkv, int head_dim, int64_t B) {
+    if (N <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || B < 0) return 0;
+    const int parts = prompt_parts(N, B, Hq, Hkv);
+    return prompt_stats_bytes(N, Hq) + (parts > 1 ? (size_t)parts * 2 * (size_t)N * (size_t)Hkv * (size_t)head_dim * 4 : 0);
 }
 
 extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
@@ -1211,7 +1281,7 @@ extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides
     OMNI_TRY(prompt_heads(who, "dk", dk, dk_strides, a.dk));
     OMNI_TRY(prompt_heads(who, "dv", dv, dv_strides, a.dv));
     OMNI_CHECK_ARG(cu_seqlens && lse, "%s: NULL cu_seqlens or lse", who);
-    const size_t need = omni_prompt_attn_backward_workspace_size(N, Hq);
+    const size_t need = omni_prompt_attn_backward_workspace_size(N, Hq, Hkv, head_dim, B);
     if (!workspace || workspace_bytes < need) {
         set_error("%s: workspace of %zu bytes needed", who, need);
         return OMNI_EWORKSPACE;
@@ -1221,6 +1291,8 @@ extern "C" int omni_prompt_attn_backward(const void *q, const int64_t *q_strides
     a.peaks = static_cast<float *>(workspace);
     a.lse2 = a.peaks + 2 * kPtPeaks;
     a.delta = a.lse2 + (size_t)N * Hq;
+    a.n_parts = prompt_parts(N, B, Hq, Hkv);
+    a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + prompt_stats_bytes(N, Hq));
     a.causal = causal != 0;
     a.peak_rows = (int)(N / 4 + 1 < kPtPeaks ? N / 4 + 1 : kPtPeaks);
     hipStream_t st = as_stream(stream);

@@ -89,7 +89,7 @@ SIGNATURES = {
                                             _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
     "omni_prompt_attn": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp, _c_i64,
                                   _c_f32, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "omni_prompt_attn_backward_workspace_size": (_c_sz, [_c_i64, _c_int]),
+    "omni_prompt_attn_backward_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int, _c_int, _c_i64]),
     "omni_prompt_attn_backward": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp,
                                            _c_i64, _c_f32, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                            _vp, _vp, _vp, _vp, _c_sz, _vp]),

@@ -94,7 +94,7 @@ class _PromptAttention(torch.autograd.Function):
         do = _rows(do)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=ctx.dev) for t in (q, k, v))
         L = _lib.lib()
-        ws_bytes = L.omni_prompt_attn_backward_workspace_size(N, Hq)
+        ws_bytes = L.omni_prompt_attn_backward_workspace_size(N, Hq, k.shape[1], D, cu.numel() - 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ctx.dev) if ws_bytes else None
         with _lib.on_device(ctx.dev):
             _lib.check(L.omni_prompt_attn_backward(

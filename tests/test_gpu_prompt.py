@@ -312,7 +312,10 @@ def test_native_refusals():
                     (dict(cu=None), "NULL")):
         assert call(**kw) == _lib.OMNI_EINVAL and msg in _lib.last_error(), (kw, _lib.last_error())
     assert call(N=0, q=None) == 0
-    assert L.omni_prompt_attn_backward_workspace_size(10, 4) == 10 * 4 * 8 + 4096
+    size = L.omni_prompt_attn_backward_workspace_size
+    assert size(10, 2, 2, 64, 1) == 10 * 2 * 8 + 4096            # the rows' statistics and the f16 peaks
+    assert size(10, 4, 1, 64, 1) in (10 * 4 * 8 + 4096, 10 * 4 * 8 + 4096 + 4 * 2 * 10 * 64 * 4)   # and parts of a group's heads
+    assert size(0, 4, 1, 64, 1) == 0 and size(10, 3, 2, 64, 1) == 0
     a = (4096, s)
     rc = L.omni_prompt_attn_backward(*a, *a, *a, 2, 5, 2, 1, 64, 4096, 1, 1.0, 1, *a, *a, 4096, *a, *a, *a, *a, 4096, 100, None)
     assert rc == _lib.OMNI_EWORKSPACE and "workspace" in _lib.last_error()
