@@ -434,17 +434,18 @@ __global__ __launch_bounds__(64 * kRpWaves) void rope_backward_kernel(RopeArgs a
     }
 }
 
-// Columns of the partial sums: 16 threads a column, 16 columns a block.
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float *partial, int rows, int D, int w_dtype, void *dwq, void *dwk) {
-    __shared__ float red[16][17];
+// Columns of the partial sums: 64 threads a column, 16 columns a block.
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float *partial, int rows, int D, int w_dtype, void *dwq, void *dwk) {
+    __shared__ float red[64][17];
     const int col = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
     float v = 0.0f;
-    for (int r = part; r < rows; r += 16) v += partial[(int64_t)r * 2 * D + col];
+#pragma unroll 8
+    for (int r = part; r < rows; r += 64) v += partial[(int64_t)r * 2 * D + col];
     red[part][threadIdx.x % 16] = v;
     __syncthreads();
     if (part) return;
 #pragma unroll
-    for (int p = 1; p < 16; ++p) v += red[p][threadIdx.x];
+    for (int p = 1; p < 64; ++p) v += red[p][threadIdx.x];
     void *out = col < D ? dwq : dwk;
     const int d = col < D ? col : col - D;
     if (w_dtype == OMNI_F32) static_cast<float *>(out)[d] = v;
@@ -626,7 +627,7 @@ extern "C" int omni_qk_norm_rope_backward(const void *q, const int64_t *q_stride
         OMNI_CHECK_LAUNCH(who);
     }
     if (norm) {
-        hipLaunchKernelGGL(rope_dw_kernel, dim3(2 * head_dim / 16), dim3(256), 0, st, static_cast<const float *>(workspace),
+        hipLaunchKernelGGL(rope_dw_kernel, dim3(2 * head_dim / 16), dim3(1024), 0, st, static_cast<const float *>(workspace),
                            blocks, head_dim, w_dtype, dq_weight, dk_weight);
         OMNI_CHECK_LAUNCH(who);
     }

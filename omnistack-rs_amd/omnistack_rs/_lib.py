@@ -6,7 +6,6 @@ are not on a HIP device.  There is no CPU fallback.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -165,15 +164,13 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_NO_SWITCH = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context in which `device` is current (a launch takes the current
-    device's code and properties); nothing to do where it already is."""
+def on_device(device: torch.device, fn, *args) -> int:
+    """fn(*args) with `device` current (a launch takes the current device's
+    code and properties)."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_SWITCH
-    return torch.cuda.device(device)
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 _LEAF_STREAM = "omnistack_rs.stream"
@@ -199,9 +196,7 @@ def hold_leaves(device: torch.device, *tensors: Optional[torch.Tensor]) -> list:
     return nodes
 
 
-def i64_array(*values: int) -> ctypes.Array:
-    """Host int64 array argument (strides)."""
-    return (ctypes.c_int64 * len(values))(*values)
+I64x2, I64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3      # host arrays of strides
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

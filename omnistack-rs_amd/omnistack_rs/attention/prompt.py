@@ -23,15 +23,18 @@ _HEAD_DIMS = (32, 64, 128)
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` as the kernels read it: the last dim contiguous, 16-byte steps, no
-    negative or huge token stride."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) < 1 << 24 and \
-            all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-        return t
+    huge token stride."""
+    if t.data_ptr() % 16 == 0 and t.stride(0) < 1 << 24:
+        if t.is_contiguous():
+            return t
+        if t.stride(-1) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
-    return _lib.i64_array(*(0 if n == 1 else s for n, s in zip(t.shape[:2], t.stride())))
+    s = t.stride()
+    return _lib.I64x2(0 if t.shape[0] == 1 else s[0], 0 if t.shape[1] == 1 else s[1])
 
 
 def _check(q, k, v, cu_seqlens, scale, validate):
@@ -50,7 +53,7 @@ def _check(q, k, v, cu_seqlens, scale, validate):
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not abs(scale) <= 3.0e38:
         raise ValueError(f"scale must be finite, got {scale}")
-    cu = torch.as_tensor(cu_seqlens)
+    cu = cu_seqlens if isinstance(cu_seqlens, torch.Tensor) else torch.as_tensor(cu_seqlens)
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"cu_seqlens must be int32 or int64 (n_sequences + 1,), got {cu.dtype} {tuple(cu.shape)}")
     if validate or not cu.is_cuda:
@@ -58,7 +61,9 @@ def _check(q, k, v, cu_seqlens, scale, validate):
         if int(host[0]) != 0 or bool((host[1:] < host[:-1]).any()) or int(host[-1]) > N:
             raise ValueError(f"cu_seqlens must rise from 0 to at most {N}")
     dev = _lib.require_device(q, k, v, cu if cu.is_cuda else None)
-    return dev, cu.to(device=dev, dtype=torch.int32).contiguous(), scale
+    if cu.dtype != torch.int32 or not cu.is_cuda or not cu.is_contiguous():
+        cu = cu.to(device=dev, dtype=torch.int32).contiguous()
+    return dev, cu, scale
 
 
 def _forward(q, k, v, cu, scale, causal, out, need_lse, dev, need_rest=False):
@@ -67,12 +72,13 @@ def _forward(q, k, v, cu, scale, causal, out, need_lse, dev, need_rest=False):
     o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
     lse = torch.empty(Hq, N, dtype=torch.float32, device=dev) if need_lse else None
     rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_rest else None
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().omni_prompt_attn(
-            _lib.ptr(qc), _strides(qc), _lib.ptr(kc), _strides(kc), _lib.ptr(vc), _strides(vc), _lib.dtype_code(q.dtype),
-            N, Hq, k.shape[1], D, _lib.ptr(cu), cu.numel() - 1, scale, int(causal), int(out is None),
-            _lib.ptr(o), _strides(o), _lib.ptr(lse), _lib.ptr(rest), _strides(rest) if need_rest else None,
-            _lib.stream_of(dev)))
+    rc = _lib.on_device(
+        dev, _lib.lib().omni_prompt_attn, qc.data_ptr(), _strides(qc), kc.data_ptr(), _strides(kc), vc.data_ptr(),
+        _strides(vc), _lib.dtype_code(q.dtype), N, Hq, k.shape[1], D, cu.data_ptr(), cu.numel() - 1, scale, int(causal),
+        int(out is None), o.data_ptr(), _strides(o), _lib.ptr(lse), _lib.ptr(rest), _strides(rest) if need_rest else None,
+        _lib.stream_of(dev))
+    if rc:
+        _lib.check(rc)
     return (o, lse, rest) if need_rest else (o, lse)
 
 
@@ -96,12 +102,12 @@ class _PromptAttention(torch.autograd.Function):
         L = _lib.lib()
         ws_bytes = L.omni_prompt_attn_backward_workspace_size(N, Hq, k.shape[1], D, cu.numel() - 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ctx.dev) if ws_bytes else None
-        with _lib.on_device(ctx.dev):
-            _lib.check(L.omni_prompt_attn_backward(
-                _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(v), _strides(v), _lib.dtype_code(q.dtype),
-                N, Hq, k.shape[1], D, _lib.ptr(cu), cu.numel() - 1, ctx.scale, int(ctx.causal),
-                _lib.ptr(o), _strides(o), _lib.ptr(rest), _strides(rest), _lib.ptr(lse), _lib.ptr(do), _strides(do), _lib.ptr(dq), _strides(dq),
-                _lib.ptr(dk), _strides(dk), _lib.ptr(dv), _strides(dv), _lib.ptr(ws), ws_bytes, _lib.stream_of(ctx.dev)))
+        _lib.check(_lib.on_device(
+            ctx.dev, L.omni_prompt_attn_backward, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
+            _strides(v), _lib.dtype_code(q.dtype), N, Hq, k.shape[1], D, cu.data_ptr(), cu.numel() - 1, ctx.scale,
+            int(ctx.causal), o.data_ptr(), _strides(o), rest.data_ptr(), _strides(rest), lse.data_ptr(),
+            do.data_ptr(), _strides(do), dq.data_ptr(), _strides(dq), dk.data_ptr(), _strides(dk), dv.data_ptr(),
+            _strides(dv), _lib.ptr(ws), ws_bytes, _lib.stream_of(ctx.dev)))
         return dq, dk, dv, None, None, None, None
 
 

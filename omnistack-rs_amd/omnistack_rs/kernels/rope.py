@@ -80,18 +80,21 @@ class RotaryEmbedding:
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """`t` as the kernels read it: the last dim contiguous, 16-byte steps."""
-    step = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % step == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        step = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % step == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
     """Element strides (batch, token, head) of (N, H, D) or (B, H, T, D)."""
-    s = [0 if n == 1 else st for n, st in zip(t.shape, t.stride())]
-    b, tok, h = (0, s[0], s[1]) if t.dim() == 3 else (s[0], s[2], s[1])
-    return _lib.i64_array(b, tok, h)
+    s = t.stride()
+    if 1 in t.shape:
+        s = tuple(0 if n == 1 else st for n, st in zip(t.shape, s))
+    return _lib.I64x3(0, s[0], s[1]) if len(s) == 3 else _lib.I64x3(s[0], s[2], s[1])
 
 
 def _check(q, k, positions, rotary, q_weight, k_weight, eps):
@@ -130,26 +133,32 @@ def _check(q, k, positions, rotary, q_weight, k_weight, eps):
     dev = _lib.require_device(q, k, positions, q_weight, k_weight)
     if dev != rotary.device:
         raise ValueError(f"rotary is on {rotary.device}, q on {dev}")
-    return dev, rows, pos if pos.dim() == 3 else pos[:, None]
+    return dev, rows, pos
 
 
 def _common(q, k, pos, rotary, wq, wk, eps, rows):
     """The arguments that both directions share, behind the tensors."""
+    ps = pos.stride()
     return (_lib.dtype_code(q.dtype), *rows, q.shape[1], k.shape[1], rotary.head_dim, _lib.ptr(pos),
-            int(pos.dtype == torch.int64), _lib.i64_array(*pos.stride()), _lib.ptr(rotary.turns),
+            int(pos.dtype == torch.int64), _lib.I64x3(ps[0], 0 if len(ps) == 2 else ps[1], ps[-1]), _lib.ptr(rotary.turns),
             _lib.ptr(rotary.pair_axes), rotary.rotary_dim, int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk),
             0 if wq is None else _lib.dtype_code(wq.dtype), float(eps))
 
 
 def _forward(q, k, pos, rotary, wq, wk, eps, rows, dev, out):
     qc, kc = _heads(q), _heads(k)
-    wq, wk = (None if w is None else _heads(w) for w in (wq, wk))
-    qo, ko = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().omni_qk_norm_rope(
-            _lib.ptr(qc), _strides(qc), _lib.ptr(kc), _strides(kc),
-            *_common(qc, kc, pos, rotary, wq, wk, eps, rows),
-            _lib.ptr(qo), _strides(qo), _lib.ptr(ko), _strides(ko), _lib.stream_of(dev)))
+    if wq is not None:
+        wq, wk = _heads(wq), _heads(wk)
+    if out is not None:
+        qo, ko = out
+    else:
+        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
+    rc = _lib.on_device(
+        dev, _lib.lib().omni_qk_norm_rope, qc.data_ptr(), _strides(qc), kc.data_ptr(), _strides(kc),
+        *_common(qc, kc, pos, rotary, wq, wk, eps, rows),
+        qo.data_ptr(), _strides(qo), ko.data_ptr(), _strides(ko), _lib.stream_of(dev))
+    if rc:
+        _lib.check(rc)
     return qo, ko
 
 
@@ -175,12 +184,11 @@ class _QKNormRope(torch.autograd.Function):
         L = _lib.lib()
         ws_bytes = L.omni_qk_norm_rope_backward_workspace_size(ctx.rotary.head_dim) if norm else 0
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        with _lib.on_device(dev):
-            _lib.check(L.omni_qk_norm_rope_backward(
-                _lib.ptr(q), _strides(q), _lib.ptr(k), _strides(k),
-                *_common(q, k, pos, ctx.rotary, wqc, wkc, ctx.eps, ctx.rows),
-                _lib.ptr(gq), _strides(gq), _lib.ptr(gk), _strides(gk), _lib.ptr(dq), _strides(dq), _lib.ptr(dk),
-                _strides(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_of(dev)))
+        _lib.check(_lib.on_device(
+            dev, L.omni_qk_norm_rope_backward, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
+            *_common(q, k, pos, ctx.rotary, wqc, wkc, ctx.eps, ctx.rows),
+            gq.data_ptr(), _strides(gq), gk.data_ptr(), _strides(gk), dq.data_ptr(), _strides(dq), dk.data_ptr(),
+            _strides(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_of(dev)))
         return dq, dk, None, None, dwq, dwk, None, None, None
 
 
