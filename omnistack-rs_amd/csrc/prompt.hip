@@ -401,6 +401,28 @@ struct PtQueries {
     }
 };
 
+// Sums of one wave to another by way of 128 D bytes of LDS, a KB for four registers of its lanes.
+template <int NT>
+__device__ __forceinline__ void pt_give(char *lds, const pf16_t (&x)[NT]) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16) =
+                make_float4(x[d][i], x[d][i + 1], x[d][i + 2], x[d][i + 3]);
+}
+template <int NT>
+__device__ __forceinline__ void pt_take(const char *lds, pf16_t (&x)[NT], float f = 1.0f) {
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 y = *reinterpret_cast<const float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16);
+            x[d][i] = fmaf(y.x, f, x[d][i]); x[d][i + 1] = fmaf(y.y, f, x[d][i + 1]);
+            x[d][i + 2] = fmaf(y.z, f, x[d][i + 2]); x[d][i + 3] = fmaf(y.w, f, x[d][i + 3]);
+        }
+}
+
 // ── forward ─────────────────────────────────────────────────────────────
 //
 // A wave holds 32 query rows as the B operand of S^T = K Q^T, so lane n and
@@ -431,10 +453,11 @@ struct PtRow {
     bool met;                            // an infinity or NaN among hidden values
 };
 
-// LO: of the first tile, the probabilities' rounding errors, rounded in turn, are
+// at: the tile's bytes in K and V (in the lane's offsets already).  LO: of the first tile, the probabilities' rounding errors, rounded in turn, are
 // added as well.
 template <int DT, int D, bool LO>
-__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K, const char *V, int j0, int len, bool masked, bool first) {
+__device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLane<D> &lane_at, PtRow<DT, D> &R, const char *K,
+                                                const char *V, int at, int j0, int len, bool masked, bool first) {
     constexpr int NT = PtRow<DT, D>::NT;
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
@@ -449,7 +472,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
         for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
     __builtin_amdgcn_s_setprio(0);
-    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(V, kPtKeys * 2 * D));
+    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(V + at, kPtKeys * 2 * D));
     if (masked) {
         // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
         const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -526,10 +549,13 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
     __builtin_amdgcn_s_setprio(0);
 }
 
-template <int DT, int D, bool LO>
-__global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(PromptArgs a) {
-    __shared__ __attribute__((aligned(16))) char k0[kPtKeys * 2 * D], k1[kPtKeys * 2 * D];
-    __shared__ __attribute__((aligned(16))) char v0[kPtKeys * 2 * D], v1[kPtKeys * 2 * D];
+// KS = 2: four more waves hold the same rows and take every second tile of keys;
+// the halves are joined through LDS at the end.
+template <int DT, int D, bool LO, int KS>
+__global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(PromptArgs a) {
+    constexpr int TILE = kPtKeys * 2 * D, STEP = KS * kPtKeys;
+    __shared__ __attribute__((aligned(16))) char k0[KS * TILE], k1[KS * TILE];
+    __shared__ __attribute__((aligned(16))) char v0[KS * TILE], v1[KS * TILE];
     constexpr int NT = D / 32;
     // kv heads vary fastest, so that with eight of them (or a multiple) a kv
     // head's blocks share an XCD and its L2
@@ -537,26 +563,32 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
     const int hk = (int)(bid % a.Hkv);
     const PtSlot S = pt_slot<kPtRows>(a.cu, a.B, a.N, a.G, bid / a.Hkv, true);
     if (S.tile < 0) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave = all & (kPtWaves - 1), upper = KS == 2 ? all / kPtWaves : 0;
     const int row0 = S.tile * kPtRows;
     if (S.none) {
         if (!a.fill) return;
         pt_zero_rows<D, kPtRows>(a.o, S.start, row0, S.len, hk * a.G, a.G);
-        for (int e = threadIdx.x; a.lse && e < kPtRows; e += 64 * kPtWaves) {
+        for (int e = threadIdx.x; a.lse && e < kPtRows; e += blockDim.x) {
             const int r = row0 + e, t = r / a.G;
             if (t < S.len) a.lse[(int64_t)(hk * a.G + r - t * a.G) * a.N + S.start + t] = -INFINITY;
         }
         return;
     }
     const char *kb = a.k.p + (int64_t)S.start * a.k.st + hk * a.k.sh, *vb = a.v.p + (int64_t)S.start * a.v.st + hk * a.v.sh;
-    PtCopy<D, kPtKeys> ck, cv;
-    ck.init(wave);
-    cv.init(wave);
-    ck.issue(kb, a.k.st, 0, S.len, k0, wave);
-    cv.issue(vb, a.v.st, 0, S.len, v0, wave);
+    const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;   // keys that the block sees
+    PtCopy<D, kPtKeys> cp;
+    cp.init(wave);
+    // this half's tile of the pair from key j on
+    auto copy = [&](int j, char *K, char *V) {
+        j += kPtKeys * upper;
+        if (j >= kend) return;
+        cp.issue(kb, a.k.st, j, S.len, K + TILE * upper, wave);
+        cp.issue(vb, a.v.st, j, S.len, V + TILE * upper, wave);
+    };
+    copy(0, k0, v0);
 
     PtLane<D> A;
-    A.init();
+    A.init(kPtKeys * upper);
     PtQueries W;
     W.init(a, S, hk, row0 + 32 * wave);
     PtRow<DT, D> R;
@@ -568,27 +600,44 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_forward_kernel(Prompt
 #pragma unroll
     for (int d = 0; d < NT; ++d) R.o[d] = pf16_t{};
 
-    const int kend = a.causal ? min((row0 + kPtRows - 1) / a.G + 1, S.len) : S.len;   // keys that the block sees
     const int wlast = a.causal ? W.last : S.len - 1;                                  // the last that the wave sees
     auto step = [&](const char *K, const char *V, int j0) {
+        j0 += kPtKeys * upper;
         if (!W.live || j0 > wlast) return;
         const bool masked = j0 + kPtKeys > S.len || (a.causal && j0 + kPtKeys - 1 > W.first);
-        pt_forward_tile<DT, D, LO>(a, A, R, K, V, j0, S.len, masked, j0 == 0);
+        pt_forward_tile<DT, D, LO>(a, A, R, K, V, TILE * upper, j0, S.len, masked, j0 == 0);
     };
-    for (int j0 = 0; j0 < kend; j0 += 2 * kPtKeys) {
+    for (int j0 = 0; j0 < kend; j0 += 2 * STEP) {
         pt_sync();                       // this tile is there, the other buffers are read
-        if (j0 + kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + kPtKeys, S.len, k1, wave);
-            cv.issue(vb, a.v.st, j0 + kPtKeys, S.len, v1, wave);
-        }
+        copy(j0 + STEP, k1, v1);
         step(k0, v0, j0);
-        if (j0 + kPtKeys >= kend) break;
+        if (j0 + STEP >= kend) break;
         pt_sync();
-        if (j0 + 2 * kPtKeys < kend) {
-            ck.issue(kb, a.k.st, j0 + 2 * kPtKeys, S.len, k0, wave);
-            cv.issue(vb, a.v.st, j0 + 2 * kPtKeys, S.len, v0, wave);
+        copy(j0 + 2 * STEP, k0, v0);
+        step(k1, v1, j0 + STEP);
+    }
+    if constexpr (KS == 2) {
+        char *lds = (wave & 2 ? k1 : k0) + (wave & 1) * TILE;
+        float4 *stat = reinterpret_cast<float4 *>(v0) + wave * 64 + (threadIdx.x & 63);
+        __syncthreads();
+        if (upper) {
+            pt_give(lds, R.o);
+            *stat = make_float4(R.m, R.l, R.l16, R.met ? 1.0f : 0.0f);
         }
-        step(k1, v1, j0 + kPtKeys);
+        __syncthreads();
+        if (upper) return;
+        const float4 u = *stat;
+        const float mn = fmaxf(R.m, u.x);
+        const float f = R.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(R.m - mn), fu = u.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(u.x - mn);
+        R.l = R.l * f + u.y * fu;
+        R.l16 = R.l16 * f + u.z * fu;
+        R.m = mn;
+        R.met = R.met || u.w != 0.0f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) R.o[d][i] *= f;
+        pt_take(lds, R.o, fu);
     }
     if (!W.live) return;
     if (R.met) {
@@ -940,27 +989,6 @@ __device__ __forceinline__ void pt_copy_stat(const float *base, int j0, int len,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(R, (PT_LDS void *)lds, 4, (uint32_t)min((int)(threadIdx.x & 63), left - 1) * 4u, 0, 0, 0);
 }
 
-// The upper half's sums to the lower half: lane's registers in LDS, a KB a register quad and wave.
-template <int NT>
-__device__ __forceinline__ void pt_give(char *lds, const pf16_t (&x)[NT]) {
-#pragma unroll
-    for (int d = 0; d < NT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16) =
-                make_float4(x[d][i], x[d][i + 1], x[d][i + 2], x[d][i + 3]);
-}
-template <int NT>
-__device__ __forceinline__ void pt_take(const char *lds, pf16_t (&x)[NT]) {
-#pragma unroll
-    for (int d = 0; d < NT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 y = *reinterpret_cast<const float4 *>(lds + (4 * d + i / 4) * 1024 + (threadIdx.x & 63) * 16);
-            x[d][i] += y.x; x[d][i + 1] += y.y; x[d][i + 2] += y.z; x[d][i + 3] += y.w;
-        }
-}
-
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptArgs a) {
     constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
@@ -1177,8 +1205,20 @@ using namespace omni;
 
 template <int DT, int D>
 static void prompt_launch_forward(const PromptArgs &a, dim3 grid, hipStream_t st) {
-    if (a.olo.p) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, true>), grid, dim3(64 * kPtWaves), 0, st, a);
-    else hipLaunchKernelGGL((prompt_forward_kernel<DT, D, false>), grid, dim3(64 * kPtWaves), 0, st, a);
+    // Where all blocks start at once and rows are long, the longest block is the
+    // launch's time: eight waves a block halve it.  Two waves of one block keep
+    // step on their SIMD, though, where those of two blocks fill each other's
+    // gaps, so that it pays up to two four-wave blocks a CU only, and not for
+    // short sequences.  Four waves against eight, causal, head_dim 128: 2048
+    // tokens, 32 heads over 8, 72 / 67 us, 16 heads 61 / 51, 8 heads over 1 59 /
+    // 50, 8192 tokens of those 204 / 171, 1024 tokens 42 / 39; 3000 tokens of 32
+    // heads 102 / 118, 16 sequences of 128 27 / 34; head_dim 32, 2048 tokens 40 / 36.
+    const bool split = a.N * a.Hq / kPtRows <= 2 * device_cus() && a.N >= (int64_t)1024 * a.B;
+    const dim3 one(64 * kPtWaves), two(2 * 64 * kPtWaves);
+    if (a.olo.p && split) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, true, 2>), grid, two, 0, st, a);
+    else if (a.olo.p) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, true, 1>), grid, one, 0, st, a);
+    else if (split) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, false, 2>), grid, two, 0, st, a);
+    else hipLaunchKernelGGL((prompt_forward_kernel<DT, D, false, 1>), grid, one, 0, st, a);
 }
 template <int DT>
 static void prompt_launch_forward(const PromptArgs &a, int D, dim3 grid, hipStream_t st) {

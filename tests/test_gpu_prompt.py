@@ -134,6 +134,10 @@ SHAPES = [
     ([1] * 200, 0, 2, 1, 32, "bf16", True),
     ([], 5, 2, 1, 64, "bf16", True),
     ([1030], 0, 2, 2, 128, "f16", False),
+    # long and few: the forward's waves split the keys
+    ([1100], 3, 4, 1, 64, "bf16", True),
+    ([1025, 1089], 0, 3, 1, 32, "f16", True),
+    ([1345], 0, 8, 2, 128, "bf16", True),
 ]
 
 
@@ -323,15 +327,15 @@ def test_native_refusals():
 
 @gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-@pytest.mark.parametrize("D,dtype,G", [(128, "bf16", 4), (64, "f16", 1), (32, "bf16", 3)])
-def test_infinities_and_nan_stay_with_who_sees_them(device, bad, D, dtype, G):
+@pytest.mark.parametrize("D,dtype,G,more", [(128, "bf16", 4, 0), (64, "f16", 1, 0), (32, "bf16", 3, 0), (64, "bf16", 2, 3000)])
+def test_infinities_and_nan_stay_with_who_sees_them(device, bad, D, dtype, G, more):
     """A token that holds an infinity or a NaN in q, k, v or the output's
     gradient: what does not see it is as if it held an ordinary number (the
     bars of two computations of one result), other sequences and heads are the
     same bits (f16: the scale of ds may be another power of two, within the
     bars); what sees a NaN is NaN."""
     from omnistack_rs.attention import prompt_attention
-    lengths, Hkv = [70, 230, 40], 2
+    lengths, Hkv = [70, 230, 40 + more], 2           # more: the forward's waves split the keys
     cu, N = _cu(lengths)
     base = [t.to(device) for t in _inputs(N, Hkv * G, Hkv, D, dtype, 60)]
     a, b = 70, 300                                   # the second sequence's tokens
