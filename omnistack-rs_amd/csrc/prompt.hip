@@ -88,6 +88,24 @@ __device__ __forceinline__ float pt_add2(uint32_t v, float c) {
     }
 }
 
+// x . y of eight values each, and c.
+template <int DT>
+__device__ __forceinline__ float pt_dot8(ps8_t x, ps8_t y, float c) {
+    const uint4 a = __builtin_bit_cast(uint4, x), b = __builtin_bit_cast(uint4, y);
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == OMNI_BF16) {
+            typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+            c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, u[i]), __builtin_bit_cast(b2, w[i]), c, false);
+        } else {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            c = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, u[i]), __builtin_bit_cast(h2, w[i]), c, false);
+        }
+    }
+    return c;
+}
+
 __device__ __forceinline__ ps8_t pt_frag(const uint32_t *p) {
     return __builtin_bit_cast(ps8_t, make_uint4(p[0], p[1], p[2], p[3]));
 }
@@ -675,9 +693,10 @@ __global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(P
 // delta_t = sum_d g_td o_td;  p_ts = exp(scale q_t . k_s - lse_t);
 //   dv_s = sum_t p_ts g_t,            ds_ts = p_ts (g_t . v_s - delta_t),
 //   dq_t = scale sum_s ds_ts k_s,     dk_s = scale sum_t ds_ts q_t,
-// dk and dv summed over the group's query heads.  Three launches without
-// atomics, so that results repeat bit for bit: delta; dq by blocks of query
-// rows; dk and dv by blocks of keys.  Scores and g . v are formed twice for it,
+// dk and dv summed over the group's query heads.  Two launches without atomics,
+// so that results repeat bit for bit: delta and dq by blocks of query rows; dk
+// and dv by blocks of keys (delta in a launch of its own, which reads what dq's
+// reads again, took 46 us of a gradient of 8192 tokens).  Scores and g . v are formed twice for it,
 // seven products instead of five.
 //
 // p and ds go to the matrix units in the inputs' 16 bits.  In f16, p is scaled
@@ -687,63 +706,38 @@ __global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(P
 constexpr int kPtPeaks = 512;
 constexpr float kPtF16P = 14.0f;
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
+// f16: largest squared norms of the rows of g and of v, a pair for each block.
+template <int D>
+__global__ __launch_bounds__(256) void prompt_peaks_kernel(PromptArgs a) {
     constexpr int LPH = D / 8, HPW = 64 / LPH;
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, sub = lane % LPH, grp = lane / LPH;
-    auto norm = [&](const uint4 x, const uint4 y) {          // sum over a head's lanes of x . y
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s = fmaf(pt_value<DT>(u[i]), pt_value<DT>(w[i]), s);
-            s = fmaf(pt_value<DT>(u[i] >> 16), pt_value<DT>(w[i] >> 16), s);
-        }
+    auto norm = [&](const PromptHeads &x, int64_t t, int h) {
+        const ps8_t v = *reinterpret_cast<const ps8_t *>(x.p + t * x.st + h * x.sh + sub * 16);
+        float s = pt_dot8<OMNI_F16>(v, v, 0.0f);
 #pragma unroll
         for (int m = LPH / 2; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
-        return s;
+        return s < INFINITY ? s : 0.0f;              // what is not finite has no say: its results are not either
     };
     float pg = 0.0f, pv = 0.0f;
     const int64_t rows = min((int64_t)max(a.cu[a.B], 0), a.N);   // what lies behind the last sequence counts for nothing
     for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < rows; t += (int64_t)gridDim.x * 4) {
-        for (int h0 = 0; h0 < a.Hq; h0 += HPW) {
-            const int h = min(h0 + grp, a.Hq - 1);
-            const uint4 g = *reinterpret_cast<const uint4 *>(a.g.p + t * a.g.st + h * a.g.sh + sub * 16);
-            const uint4 o = *reinterpret_cast<const uint4 *>(a.o.p + t * a.o.st + h * a.o.sh + sub * 16);
-            const uint4 lo = *reinterpret_cast<const uint4 *>(a.olo.p + t * a.olo.st + h * a.olo.sh + sub * 16);
-            const float d = norm(g, o) + norm(g, lo);
-            if (sub == 0 && h0 + grp < a.Hq) {
-                a.delta[(int64_t)h * a.N + t] = -d;
-                a.lse2[(int64_t)h * a.N + t] = a.lse[(int64_t)h * a.N + t] * 1.44269504f;
-            }
-            // what is not finite has no say: its results are not either
-            if constexpr (DT == OMNI_F16) { const float n = norm(g, g); pg = n > pg && n < INFINITY ? n : pg; }
-        }
-        if constexpr (DT == OMNI_F16)
-            for (int h0 = 0; h0 < a.Hkv; h0 += HPW) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(a.v.p + t * a.v.st + min(h0 + grp, a.Hkv - 1) * a.v.sh + sub * 16);
-                const float n = norm(v, v);
-                pv = n > pv && n < INFINITY ? n : pv;
-            }
+        for (int h = 0; h < a.Hq; h += HPW) pg = fmaxf(pg, norm(a.g, t, min(h + grp, a.Hq - 1)));
+        for (int h = 0; h < a.Hkv; h += HPW) pv = fmaxf(pv, norm(a.v, t, min(h + grp, a.Hkv - 1)));
     }
-    if constexpr (DT == OMNI_F16) {
-        __shared__ float peak[2][4];
+    __shared__ float peak[2][4];
 #pragma unroll
-        for (int m = 32; m >= LPH; m /= 2) {
-            const float x = __shfl_xor(pg, m, 64), y = __shfl_xor(pv, m, 64);
-            pg = fmaxf(pg, x);
-            pv = fmaxf(pv, y);
-        }
-        if (lane == 0) {
-            peak[0][wave] = pg;
-            peak[1][wave] = pv;
-        }
-        __syncthreads();
-        if (threadIdx.x < 2) {
-            float m = 0.0f;
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, peak[threadIdx.x][w]);
-            a.peaks[threadIdx.x * kPtPeaks + blockIdx.x] = m;
-        }
+    for (int m = 32; m >= LPH; m /= 2) {
+        pg = fmaxf(pg, __shfl_xor(pg, m, 64));
+        pv = fmaxf(pv, __shfl_xor(pv, m, 64));
+    }
+    if (lane == 0) {
+        peak[0][wave] = pg;
+        peak[1][wave] = pv;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float *p = peak[threadIdx.x];
+        a.peaks[threadIdx.x * kPtPeaks + blockIdx.x] = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
     }
 }
 
@@ -850,8 +844,24 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
     const int64_t at = S.start + W.t;
     pt_load_rows<D>(a.q.p + at * a.q.st + W.h * a.q.sh, R.q);
     pt_load_rows<D>(a.g.p + at * a.g.st + W.h * a.g.sh, R.g);
-    R.lse2 = a.lse2[(int64_t)W.h * a.N + at];
-    R.delta = a.delta[(int64_t)W.h * a.N + at];
+    {
+        // delta of the rows, for the launch after this one as well
+        ps8_t o[D / 16], rest[D / 16];
+        pt_load_rows<D>(a.o.p + at * a.o.st + W.h * a.o.sh, o);
+        pt_load_rows<D>(a.olo.p + at * a.olo.st + W.h * a.olo.sh, rest);
+        float d[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            d[0] = pt_dot8<DT>(R.g[kk], o[kk], d[0]);
+            d[1] = pt_dot8<DT>(R.g[kk], rest[kk], d[1]);
+        }
+        R.delta = -pt_sum_halves(d[0] + d[1]);
+        R.lse2 = a.lse[(int64_t)W.h * a.N + at] * 1.44269504f;
+        if (W.mine && (threadIdx.x & 32) == 0) {
+            a.delta[(int64_t)W.h * a.N + at] = R.delta;
+            a.lse2[(int64_t)W.h * a.N + at] = R.lse2;
+        }
+    }
     const float up = pt_ds_scale<DT>(a);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) R.dq[d] = pf16_t{};
@@ -1259,8 +1269,10 @@ static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
     dim3 rows, keys;
     OMNI_CHECK_ARG(prompt_grid((a.N * a.G / kPtRows + a.B + 1) * a.Hkv, rows) && prompt_grid((a.N / kPtKvKeys + a.B + 1) * a.Hkv * a.n_parts, keys),
                    "%s: grid too large", who);
-    hipLaunchKernelGGL((prompt_delta_kernel<DT, D>), dim3(a.peak_rows), dim3(256), 0, st, a);
-    OMNI_CHECK_LAUNCH(who);
+    if constexpr (DT == OMNI_F16) {
+        hipLaunchKernelGGL((prompt_peaks_kernel<D>), dim3(a.peak_rows), dim3(256), 0, st, a);
+        OMNI_CHECK_LAUNCH(who);
+    }
     hipLaunchKernelGGL((prompt_dq_kernel<DT, D>), rows, dim3(64 * kPtWaves), 0, st, a);
     OMNI_CHECK_LAUNCH(who);
     hipLaunchKernelGGL((prompt_dkv_kernel<DT, D>), keys, dim3(64 * kPtKvWaves), 0, st, a);
