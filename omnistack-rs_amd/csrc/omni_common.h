@@ -19,6 +19,12 @@ void set_error(const char *fmt, ...);
         }                                           \
     } while (0)
 
+#define OMNI_TRY(call)                   \
+    do {                                 \
+        const int rc_ = (call);          \
+        if (rc_ != OMNI_OK) return rc_;  \
+    } while (0)
+
 #define OMNI_CHECK_LAUNCH(what)                                              \
     do {                                                                     \
         hipError_t e_ = hipGetLastError();                                   \

@@ -286,8 +286,7 @@ __device__ __forceinline__ void pt_zero_rows(const PromptHeads &o, int start, in
 // multiplies their weight of 0 with it.  Tiles that hide some are therefore
 // looked through (a tenth of such a tile's time), and a wave that met an
 // infinity or a NaN there computes its result again, term by term and from
-// memory.  Tokens behind the sequence need no look: the copies put its last
-// token in their place, which all that could see them see.
+// memory.  (Tokens behind the sequence have its last token in their place.)
 template <int DT>
 __device__ __forceinline__ bool pt_all_finite(const char *tile, int bytes) {
     // an exponent of ones carries into the sign's place
@@ -490,7 +489,7 @@ __device__ __forceinline__ void pt_forward_tile(const PromptArgs &a, const PtLan
         for (int kk = 0; kk < D / 16; ++kk) s[b] = pt_mfma<DT>(A.rows(K, 32 * b, kk), R.q[kk], s[b]);
     }
     __builtin_amdgcn_s_setprio(0);
-    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(V + at, kPtKeys * 2 * D));
+    R.met = R.met || (masked && !pt_all_finite<DT>(V + at, kPtKeys * 2 * D));
     if (masked) {
         // the keys of register i of block b: j0 + 32 b + 8 (i / 4) + 4 half + i % 4
         const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
@@ -661,6 +660,7 @@ __global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(P
     if (R.met) {
         // term by term, the maximum being known (of the rounded probabilities' sums alone)
         const float off = (R.m == -INFINITY ? 0.0f : R.m) - (DT == OMNI_F16 ? kPtF16Up : 0.0f);
+        const int end = a.causal ? R.t + 1 : S.len;
         R.l = 0.0f;
         float o[NT][16];
         pt_clear(o);
@@ -670,10 +670,10 @@ __global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(P
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -off));
-                if (j0 + 8 * (i / 4) + 4 * (int)((threadIdx.x >> 5) & 1) + i % 4 > R.t) p[i] = 0.0f;
+                if (j0 + 8 * (i / 4) + 4 * (int)((threadIdx.x >> 5) & 1) + i % 4 >= end) p[i] = 0.0f;
                 R.l += p[i];
             }
-            pt_add_terms<DT, D>(o, p, vb, a.v.st, j0, 0, min(R.t + 1, S.len));
+            pt_add_terms<DT, D>(o, p, vb, a.v.st, j0, 0, end);
         }
         R.l16 = R.l;
         pt_assign(R.o, o);
@@ -775,7 +775,7 @@ __device__ __forceinline__ void pt_dq_tile(const PromptArgs &a, const PtLane<D> 
                                            bool masked, float up) {
     const PtLane<D> A = lane_at.fresh();
     const int half = (threadIdx.x >> 5) & 1;
-    R.met = R.met || (masked && a.causal && !pt_all_finite<DT>(K, kPtKeys * 2 * D));
+    R.met = R.met || (masked && !pt_all_finite<DT>(K, kPtKeys * 2 * D));
     const int seen = (a.causal ? min(R.t, len - 1) : len - 1) - j0 - 4 * half;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -898,7 +898,7 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
             pf16_t ds = pt_product<DT, D>(vb, a.v.st, j0, S.len, R.delta, [&](int kk) { return R.g[kk]; });
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] *= __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -R.lse2)) * up;
-            pt_add_terms<DT, D>(dq, ds, kb, a.k.st, j0, 0, min(R.t + 1, S.len));
+            pt_add_terms<DT, D>(dq, ds, kb, a.k.st, j0, 0, a.causal ? R.t + 1 : S.len);
         }
         pt_assign(R.dq, dq);
     }
@@ -939,7 +939,7 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D>
                                             const float *delta, int j0, int r0, int len, bool masked, float up) {
     constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
     const PtLane<D> A = lane_at.fresh(), AK = KLDS ? key_at.fresh() : A;
-    R.met = R.met || (masked && a.causal && !(pt_all_finite<DT>(Q + r0 * 2 * D, 64 * D) && pt_all_finite<DT>(G + r0 * 2 * D, 64 * D)));
+    R.met = R.met || (masked && !(pt_all_finite<DT>(Q + r0 * 2 * D, 64 * D) && pt_all_finite<DT>(G + r0 * 2 * D, 64 * D)));
     const int half = (threadIdx.x >> 5) & 1;
     pf16_t s = {}, dp;
 #pragma unroll
@@ -1088,8 +1088,8 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
                 const int64_t h = h0 + g;
                 const char *qb = a.q.p + (int64_t)S.start * a.q.st + h * a.q.sh, *gb = a.g.p + (int64_t)S.start * a.g.st + h * a.g.sh;
 #pragma unroll 1
-                for (int j0 = w0 / 64 * 64 + 32 * upper; j0 < S.len; j0 += 64) {       // the rows that this half takes in every tile
-                    if (j0 + 31 < w0) continue;
+                for (int j0 = (a.causal ? w0 / 64 * 64 : 0) + 32 * upper; j0 < S.len; j0 += 64) {   // the rows that this half takes in every tile
+                    if (a.causal && j0 + 31 < w0) continue;
                     const int64_t row = h * a.N + S.start + min(j0 + (lane & 31), S.len - 1);
                     const float l = a.lse2[row], d = a.delta[row];
                     pf16_t w = pt_product<DT, D>(qb, a.q.st, j0, S.len, 0.0f, [&](int kk) { return KLDS ? AK.rows(kt, 0, kk) : R.k[KLDS ? 0 : kk]; });
@@ -1101,7 +1101,7 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
 #pragma unroll
                         for (int i = 0; i < 16; ++i) w[i] *= (dp[i] + __shfl(d, 8 * (i / 4) + 4 * (lane >> 5) + i % 4, 64)) * up;
                     }
-                    pt_add_terms<DT, D>(acc, w, DK ? qb : gb, DK ? a.q.st : a.g.st, j0, R.s, S.len);
+                    pt_add_terms<DT, D>(acc, w, DK ? qb : gb, DK ? a.q.st : a.g.st, j0, a.causal ? R.s : 0, S.len);
                 }
             }
             pt_assign(sum, acc);
@@ -1206,12 +1206,6 @@ static bool prompt_grid(int64_t blocks, dim3 &grid) {
 }  // namespace omni
 
 using namespace omni;
-
-#define OMNI_TRY(call)                   \
-    do {                                 \
-        const int rc_ = (call);          \
-        if (rc_ != OMNI_OK) return rc_;  \
-    } while (0)
 
 template <int DT, int D>
 static void prompt_launch_forward(const PromptArgs &a, dim3 grid, hipStream_t st) {

@@ -547,12 +547,6 @@ static void rope_launch(const RopeArgs &a, int dtype, int D, int interleaved, bo
 
 using namespace omni;
 
-#define OMNI_TRY(call)                   \
-    do {                                 \
-        const int rc_ = (call);          \
-        if (rc_ != OMNI_OK) return rc_;  \
-    } while (0)
-
 extern "C" int omni_qk_norm_rope(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, int dtype,
                                  int64_t B, int64_t T, int Hq, int Hkv, int head_dim, const void *positions, int positions64,
                                  const int64_t *position_strides, const uint64_t *turns, const uint8_t *pair_axes,

@@ -144,4 +144,6 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         o, lse = _PromptAttention.apply(q, k, v, cu, scale, causal, dev)
         return (o, lse) if return_lse else o
     o, lse = _forward(q, k, v, cu, scale, causal, out, return_lse, dev)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)      # a graph that saved it must notice
     return (o, lse) if return_lse else o

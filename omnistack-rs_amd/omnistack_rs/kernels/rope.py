@@ -16,7 +16,6 @@ fractions of a turn.
 """
 from __future__ import annotations
 
-from fractions import Fraction
 from typing import Optional, Sequence
 
 import torch
@@ -25,7 +24,8 @@ from .. import _lib
 from .hadamard import HEAD_DIM
 
 _HEAD_DIMS = (32, 64, 128, 256)
-_PI = Fraction(31415926535897932384626433832795028841971, 10 ** 40)
+# 2^64 / 2 pi, times 2^64
+_TURNS = 54157620742477409023451113735280473968
 
 
 class RotaryEmbedding:
@@ -70,12 +70,17 @@ class RotaryEmbedding:
         if any(a < 0 or a > 255 for a in axes) or not 1 <= self.n_axes <= 256:
             raise ValueError("position axes must lie in [0, 255]")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, R, bool(interleaved)
-        # fractions of a turn per position, 64 bits, as the int64 with the same bits
-        turns = [round(Fraction(f) / (2 * _PI) * (1 << 64)) % (1 << 64) for f in freq]
-        dev = torch.device(device)
-        self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64).to(dev)
-        self.pair_axes = torch.tensor(axes, dtype=torch.uint8).to(dev)
-        self.device = self.turns.device
+        # fractions of a turn per position, 64 bits, as the int64 with the same
+        # bits, and behind them the axes' bytes: one upload
+        turns = []
+        for f in freq:
+            num, den = f.as_integer_ratio()
+            turns.append(((2 * num * _TURNS // (den << 64) + 1 >> 1) + (1 << 63)) % (1 << 64) - (1 << 63))
+        axis_bytes = bytes(axes) + bytes(-n % 8)
+        words = [int.from_bytes(axis_bytes[i:i + 8], "little", signed=True) for i in range(0, n, 8)]
+        both = torch.tensor(turns + words, dtype=torch.int64).to(device)
+        self.turns, self.pair_axes = both[:n], both[n:].view(torch.uint8)[:n]
+        self.device = both.device
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -223,7 +228,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     if grad:
         held = _lib.hold_leaves(dev, q, k, q_weight, k_weight)  # noqa: F841 (alive until the graph holds them)
         return _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev)
-    return _forward(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev, out)
+    res = _forward(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev, out)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)      # a graph that saved them must notice
+    return res
 
 
 def _span(t: torch.Tensor):

@@ -252,6 +252,72 @@ def test_layouts_and_out(device):
 
 
 @gpu
+def test_infinity_in_the_last_token_without_a_mask(device):
+    """Rows behind a sequence that does not fill its tile have no part in it:
+    an infinite value of the last token makes infinite outputs, not NaN, and an
+    infinite gradient an infinite dv."""
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([70])
+    q, k, v, do = (t.to(device) for t in _inputs(N, 2, 1, 64, "bf16", 47))
+    v[69, 0, 3] = float("inf")
+    o = prompt_attention(q, k, v, cu, causal=False)
+    assert bool((o[:, :, 3] == float("inf")).all()) and bool(torch.isfinite(o[:, :, :3]).all())
+    v[69, 0, 3] = 1.0
+    do[69, 1, 5] = float("-inf")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    dv = torch.autograd.grad(prompt_attention(*leaves, cu, causal=False), leaves, do)[2]
+    assert bool((dv[:, 0, 5] == float("-inf")).all()) and bool(torch.isfinite(dv[:, 0, 6:]).all())
+
+
+@gpu
+def test_far_offsets(device):
+    """Token strides of 2 MB: the last tokens lie past 2^32 bytes."""
+    from omnistack_rs.attention import prompt_attention
+    N, Hq, Hkv, D = 2200, 2, 1, 64
+    cu = torch.tensor([0, 100, 2100, N], dtype=torch.int32, device=device)
+    q, k, v, do = (t.to(device) for t in _inputs(N, Hq, Hkv, D, "bf16", 48))
+    want = prompt_attention(q, k, v, cu)
+    buf = torch.empty(N, 1 << 20, dtype=torch.bfloat16, device=device)
+    at = 0
+    far = []
+    for t in (q, k, v, do):
+        w = t.shape[1] * D
+        buf[:, at:at + w] = t.reshape(N, w)
+        far.append(buf[:, at:at + w].view(N, -1, D))
+        at += w
+    out = buf[:, at:at + Hq * D].view(N, Hq, D)
+    assert torch.equal(prompt_attention(*far[:3], cu, out=out), want)
+    near = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(prompt_attention(*near, cu), near, do)
+    leaves = [t.detach().requires_grad_() for t in far[:3]]
+    for a, b in zip(torch.autograd.grad(prompt_attention(*leaves, cu), leaves, far[3]), grads):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_many_short_sequences(device):
+    """5000 sequences of 0 to 3 tokens: more than one step of the search for a block's sequence."""
+    from omnistack_rs.attention import prompt_attention
+    lengths = torch.randint(0, 4, (5000,), generator=_data.gen(49)).tolist()
+    cu, N = _cu(lengths, 2)
+    q, k, v, do = (t.to(device) for t in _inputs(N, 2, 1, 32, "f16", 50))
+    seq = torch.repeat_interleave(torch.arange(5000), torch.tensor(lengths)).to(device)
+    n = N - 2
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = prompt_attention(*leaves, cu)
+    grads = torch.autograd.grad(o, leaves, do)
+    # the whole pack as one sequence of which a token sees its own sequence's alone
+    for h in range(2):
+        Q, K, V = q[:n, h].detach().double(), k[:n, 0].detach().double(), v[:n, 0].detach().double()
+        see = (seq[:, None] == seq[None]) & torch.ones(n, n, dtype=torch.bool, device=device).tril()
+        p = torch.softmax(torch.where(see, Q @ K.T / math.sqrt(32), -math.inf), -1)
+        err = (o[:n, h].double() - p @ V).abs()
+        assert bool((err <= 2.0 ** -11 * ((p @ V).abs() + 2 * (p @ V.abs())) + 2.0 ** -25).all())
+    assert bool((o[n:] == 0).all()) and all(bool((g[n:] == 0).all()) for g in grads)
+    assert all(bool(torch.isfinite(g).all()) for g in grads)
+
+
+@gpu
 def test_capture_and_other_stream(device):
     from omnistack_rs.attention import prompt_attention
     cu, N = _cu([90, 1, 200])

@@ -228,6 +228,25 @@ def test_in_place_and_out(device):
 
 
 @gpu
+def test_far_offsets_and_version(device):
+    """Token strides of 2 MB: the last tokens lie past 2^32 bytes.  Writing in
+    place is seen by a graph that saved the tensor."""
+    from omnistack_rs.kernels.rope import RotaryEmbedding, qk_norm_rope
+    N, Hq, Hkv, D = 2200, 4, 2, 64
+    q, k, gq, gk, wq, wk = (t.to(device) for t in _inputs(N, Hq, Hkv, D, "bf16", 16, "bf16"))
+    rot, pos = RotaryEmbedding(D, device=device), torch.arange(N, device=device)
+    want = qk_norm_rope(q, k, pos, rot, wq, wk)
+    buf = torch.empty(N, 1 << 20, dtype=torch.bfloat16, device=device)
+    qs, ks = buf[:, :Hq * D].view(N, Hq, D), buf[:, -Hkv * D:].view(N, Hkv, D)
+    qs.copy_(q)
+    ks.copy_(k)
+    assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(qs, ks, pos, rot, wq, wk), want))
+    before = qs._version
+    qk_norm_rope(qs, ks, pos, rot, wq, wk, out=(qs, ks))
+    assert torch.equal(qs, want[0]) and torch.equal(ks, want[1]) and qs._version > before
+
+
+@gpu
 def test_zero_rows_and_special_values(device):
     """No tokens give no outputs (and zero weight gradients); a row of zeros
     stays zero; NaN and infinity stay in their own head."""
