@@ -81,6 +81,7 @@ class RotaryEmbedding:
         both = torch.tensor(turns + words, dtype=torch.int64).to(device)
         self.turns, self.pair_axes = both[:n], both[n:].view(torch.uint8)[:n]
         self.device = both.device
+        self._args = (self.turns.data_ptr(), self.pair_axes.data_ptr(), R, int(self.interleaved))
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -103,51 +104,52 @@ def _strides(t: torch.Tensor):
 
 
 def _check(q, k, positions, rotary, q_weight, k_weight, eps):
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
-        raise ValueError(f"q and k must be (N, heads, head_dim) or (B, heads, T, head_dim), got {tuple(q.shape)} "
-                         f"and {tuple(k.shape)}")
+    """(device, (batch, tokens), positions as (axes, tokens) or (axes, batch, tokens))."""
+    qs, ks = q.shape, k.shape
+    packed = len(qs) == 3
+    if not (packed or len(qs) == 4) or len(ks) != len(qs):
+        raise ValueError(f"q and k must be (N, heads, head_dim) or (B, heads, T, head_dim), got {tuple(qs)} "
+                         f"and {tuple(ks)}")
     if not isinstance(rotary, RotaryEmbedding):
         raise TypeError("rotary must be a RotaryEmbedding")
     D = rotary.head_dim
-    rows = (1, q.shape[0]) if q.dim() == 3 else (q.shape[0], q.shape[2])
-    krows = (1, k.shape[0]) if k.dim() == 3 else (k.shape[0], k.shape[2])
-    if q.shape[-1] != D or k.shape[-1] != D or rows != krows or q.shape[1] < 1 or k.shape[1] < 1:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree but for their heads and have head_dim {D}")
+    rows, krows = ((1, qs[0]), (1, ks[0])) if packed else ((qs[0], qs[2]), (ks[0], ks[2]))
+    if qs[-1] != D or ks[-1] != D or rows != krows or qs[1] < 1 or ks[1] < 1:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} must agree but for their heads and have head_dim {D}")
     if q.dtype != k.dtype:
         raise ValueError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
-    unit = 8 if _lib.dtype_code(q.dtype) == 0 else 16
-    if rotary.rotary_dim % unit:
-        raise ValueError(f"rotary_dim must be a multiple of {unit} for {q.dtype}, got {rotary.rotary_dim}")
+    if rotary.rotary_dim % (8 if _lib.dtype_code(q.dtype) == 0 else 16):
+        raise ValueError(f"rotary_dim must be a multiple of {8 if q.dtype == torch.float32 else 16} for {q.dtype}, "
+                         f"got {rotary.rotary_dim}")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("q_weight and k_weight must be given together")
-    for w in (q_weight, k_weight):
-        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q_weight.dtype):
-            raise ValueError(f"q_weight and k_weight must be ({D},) of one dtype, got {w.dtype} {tuple(w.shape)}")
     if q_weight is not None:
         _lib.dtype_code(q_weight.dtype)
-        if not float(eps) >= 0.0:
+        for w in (q_weight, k_weight):
+            if w.dim() != 1 or w.shape[0] != D or w.dtype != q_weight.dtype:
+                raise ValueError(f"q_weight and k_weight must be ({D},) of one dtype, got {w.dtype} {tuple(w.shape)}")
+        if not eps >= 0.0:
             raise ValueError(f"eps must be >= 0, got {eps}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-    A = rotary.n_axes
-    want = (A, rows[1]) if q.dim() == 3 else (A, *rows)
-    try:
-        pos = positions.expand(want)
-    except RuntimeError:
-        raise ValueError(f"positions must broadcast to {want}, got {tuple(positions.shape)}") from None
+    want = (rotary.n_axes, rows[1]) if packed else (rotary.n_axes, *rows)
+    if positions.shape != want:
+        try:
+            positions = positions.expand(want)
+        except RuntimeError:
+            raise ValueError(f"positions must broadcast to {want}, got {tuple(positions.shape)}") from None
     dev = _lib.require_device(q, k, positions, q_weight, k_weight)
     if dev != rotary.device:
         raise ValueError(f"rotary is on {rotary.device}, q on {dev}")
-    return dev, rows, pos
+    return dev, rows, positions
 
 
 def _common(q, k, pos, rotary, wq, wk, eps, rows):
     """The arguments that both directions share, behind the tensors."""
     ps = pos.stride()
-    return (_lib.dtype_code(q.dtype), *rows, q.shape[1], k.shape[1], rotary.head_dim, _lib.ptr(pos),
-            int(pos.dtype == torch.int64), _lib.I64x3(ps[0], 0 if len(ps) == 2 else ps[1], ps[-1]), _lib.ptr(rotary.turns),
-            _lib.ptr(rotary.pair_axes), rotary.rotary_dim, int(rotary.interleaved), _lib.ptr(wq), _lib.ptr(wk),
-            0 if wq is None else _lib.dtype_code(wq.dtype), float(eps))
+    return (_lib.dtype_code(q.dtype), *rows, q.shape[1], k.shape[1], rotary.head_dim, pos.data_ptr(),
+            int(pos.dtype == torch.int64), _lib.I64x3(ps[0], 0 if len(ps) == 2 else ps[1], ps[-1]), *rotary._args,
+            _lib.ptr(wq), _lib.ptr(wk), 0 if wq is None else _lib.dtype_code(wq.dtype), eps)
 
 
 def _forward(q, k, pos, rotary, wq, wk, eps, rows, dev, out):
@@ -215,8 +217,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     for calls that need none.  Forward and backward can be captured in a HIP
     graph once no eager autograd graph of the same leaves is alive (refused
     otherwise)."""
+    eps = float(eps)
     dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
+        q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)))
     if out is not None:
         if grad:
             raise ValueError("out= takes no gradient: call it under torch.no_grad()")
@@ -227,8 +231,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
         _check_overlap(q, k, out)
     if grad:
         held = _lib.hold_leaves(dev, q, k, q_weight, k_weight)  # noqa: F841 (alive until the graph holds them)
-        return _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev)
-    res = _forward(q, k, pos, rotary, q_weight, k_weight, float(eps), rows, dev, out)
+        return _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, eps, rows, dev)
+    res = _forward(q, k, pos, rotary, q_weight, k_weight, eps, rows, dev, out)
     if out is not None:
         torch.autograd.graph.increment_version(out)      # a graph that saved them must notice
     return res
