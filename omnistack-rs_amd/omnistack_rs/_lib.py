@@ -176,24 +176,18 @@ def on_device(device: torch.device, fn, *args) -> int:
 _LEAF_STREAM = "omnistack_rs.stream"
 
 
-def hold_leaves(device: torch.device, *tensors: Optional[torch.Tensor]) -> list:
-    """Gradient nodes of the leaves among `tensors`, marked with the stream of
-    their first use; keep the list until the graph that uses them is built.
-    Under graph capture, a leaf whose node another stream made (an eager graph
-    of it is still alive) is refused: the backward pass would make the
-    captured stream wait for that one, which ends the process when the capture
-    closes."""
+def mark_leaves(device: torch.device, fn) -> None:
+    """Mark the gradient nodes of the leaves that autograd node `fn` reaches
+    first with the stream of their first use.  Under graph capture, a leaf
+    whose node another stream made (an eager graph of it is still alive) is
+    refused: the backward pass would make the captured stream wait for that
+    one, which ends the process when the capture closes."""
     stream = stream_of(device)
-    nodes = []
-    for t in tensors:
-        if t is None or not t.requires_grad or not t.is_leaf:
-            continue
-        node = torch.autograd.graph.get_gradient_edge(t).node
-        if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("graph capture with gradients: an autograd graph of the same leaves, built on another "
-                               "stream, is still alive; delete its outputs before capturing")
-        nodes.append(node)
-    return nodes
+    for node, _ in fn.next_functions:
+        if node is not None and hasattr(node, "variable"):
+            if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("graph capture with gradients: an autograd graph of the same leaves, built on "
+                                   "another stream, is still alive; delete its outputs before capturing")
 
 
 I64x2, I64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3      # host arrays of strides

@@ -140,8 +140,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or any(overlap(out, t) for t in (q, k, v)):
             raise ValueError("out must not overlap q, k or v, nor itself")
     if grad:
-        held = _lib.hold_leaves(dev, q, k, v)  # noqa: F841 (alive until the graph holds them)
         o, lse = _PromptAttention.apply(q, k, v, cu, scale, causal, dev)
+        _lib.mark_leaves(dev, o.grad_fn)
         return (o, lse) if return_lse else o
     o, lse = _forward(q, k, v, cu, scale, causal, out, return_lse, dev)
     if out is not None:

@@ -230,8 +230,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
                                  "their last dim contiguous and rows at 16-byte steps")
         _check_overlap(q, k, out)
     if grad:
-        held = _lib.hold_leaves(dev, q, k, q_weight, k_weight)  # noqa: F841 (alive until the graph holds them)
-        return _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, eps, rows, dev)
+        res = _QKNormRope.apply(q, k, pos, rotary, q_weight, k_weight, eps, rows, dev)
+        _lib.mark_leaves(dev, res[0].grad_fn)
+        return res
     res = _forward(q, k, pos, rotary, q_weight, k_weight, eps, rows, dev, out)
     if out is not None:
         torch.autograd.graph.increment_version(out)      # a graph that saved them must notice
