@@ -193,6 +193,11 @@ def mark_leaves(device: torch.device, fn) -> None:
 I64x2, I64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3      # host arrays of strides
 
 
+def empty_as(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and device (1.3 us of host time, torch.empty 2.3)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

@@ -27,7 +27,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     if t.data_ptr() % 16 == 0 and t.stride(0) < 1 << 24:
         if t.is_contiguous():
             return t
-        if t.stride(-1) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        a, b, c = t.stride()
+        if c == 1 and (a % 8 == 0 or t.shape[0] == 1) and (b % 8 == 0 or t.shape[1] == 1):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -69,9 +70,9 @@ def _check(q, k, v, cu_seqlens, scale, validate):
 def _forward(q, k, v, cu, scale, causal, out, need_lse, dev, need_rest=False):
     N, Hq, D = q.shape
     qc, kc, vc = _rows(q), _rows(k), _rows(v)
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    o = _lib.empty_as(q) if out is None else out
     lse = torch.empty(Hq, N, dtype=torch.float32, device=dev) if need_lse else None
-    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_rest else None
+    rest = _lib.empty_as(q) if need_rest else None
     rc = _lib.on_device(
         dev, _lib.lib().omni_prompt_attn, qc.data_ptr(), _strides(qc), kc.data_ptr(), _strides(kc), vc.data_ptr(),
         _strides(vc), _lib.dtype_code(q.dtype), N, Hq, k.shape[1], D, cu.data_ptr(), cu.numel() - 1, scale, int(causal),
@@ -98,7 +99,7 @@ class _PromptAttention(torch.autograd.Function):
         q, k, v, o, rest, lse, cu = ctx.saved_tensors
         N, Hq, D = q.shape
         do = _rows(do)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=ctx.dev) for t in (q, k, v))
+        dq, dk, dv = (_lib.empty_as(t) for t in (q, k, v))
         L = _lib.lib()
         ws_bytes = L.omni_prompt_attn_backward_workspace_size(N, Hq, k.shape[1], D, cu.numel() - 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ctx.dev) if ws_bytes else None

@@ -89,9 +89,14 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
             return t
-        step = 16 // t.element_size()
-        if t.stride(-1) == 1 and all(s % step == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-            return t
+        st = t.stride()
+        if st[-1] == 1:
+            step = 16 // t.element_size()
+            for s, n in zip(st[:-1], t.shape):
+                if s % step and n > 1:
+                    break
+            else:
+                return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -159,7 +164,7 @@ def _forward(q, k, pos, rotary, wq, wk, eps, rows, dev, out):
     if out is not None:
         qo, ko = out
     else:
-        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
+        qo, ko = _lib.empty_as(q), _lib.empty_as(k)
     rc = _lib.on_device(
         dev, _lib.lib().omni_qk_norm_rope, qc.data_ptr(), _strides(qc), kc.data_ptr(), _strides(kc),
         *_common(qc, kc, pos, rotary, wq, wk, eps, rows),
@@ -186,7 +191,7 @@ class _QKNormRope(torch.autograd.Function):
         gq, gk = _heads(gq), _heads(gk)
         q, k = _heads(q), _heads(k)
         wqc, wkc = (None if w is None else _heads(w) for w in (wq, wk))
-        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
+        dq, dk = _lib.empty_as(q), _lib.empty_as(k)
         dwq, dwk = (torch.empty_like(wqc), torch.empty_like(wkc)) if norm else (None, None)
         L = _lib.lib()
         ws_bytes = L.omni_qk_norm_rope_backward_workspace_size(ctx.rotary.head_dim) if norm else 0
