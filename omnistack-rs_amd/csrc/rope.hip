@@ -23,6 +23,11 @@
 // compute each of the token's angles once and pass them through LDS, and the
 // pair's other half comes from the lane D / 2 away, in the input's own 16 bits
 // and before the norm, whose factor both halves share.
+//
+// 32 + 8 heads of 128 in bf16: 65536 tokens 253 us, 5.3 TB/s, the rate of a copy
+// of as many bytes (1.34 GB; HBM moves just those); 4096 tokens 17 us; 64 tokens
+// 4.0 us, a chain of position, angles, LDS and one head.  Two heads' loads ahead
+// instead of one, or four times the waves for 4096 tokens: no difference.
 #include "omni_common.h"
 
 namespace omni {
@@ -385,7 +390,9 @@ __device__ __forceinline__ void rp_backward_heads(const RopeArgs &a, RpLane<DT, 
 
 // Weight gradients: a lane's sums over its tokens and heads, the wave's lanes
 // of one dim, the block's waves; a row of partial sums a block, summed by
-// rope_dw_kernel in their order (the same on every run).
+// rope_dw_kernel in their order (the same on every run).  8192 tokens of 32 + 8
+// heads of 128 in bf16: 48 us, 5.2 TB/s, and 4.0 us for the sums (20 with fewer
+// threads a column).
 template <int DT, int D, int PAIR>
 __global__ __launch_bounds__(64 * kRpWaves) void rope_backward_kernel(RopeArgs a) {
     using V = RpVec<DT>;
