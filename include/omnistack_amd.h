@@ -450,8 +450,9 @@ int omni_qk_norm_rope(const void *q, const int64_t *q_strides, const void *k, co
 
 /*
  * Its gradient: dq_out, dk_out are the gradients of the outputs; writes dq, dk
- * and, with weights, dq_weight and dk_weight (head_dim, w_dtype; summed over
- * tokens and heads in fp32, in the same order on every run).  q and k are the
+ * and, with weights, dq_weight and dk_weight (head_dim, w_dtype; summed in fp32
+ * within a block of tokens and in fp64 over the blocks, in the same order on
+ * every run).  q and k are the
  * forward's inputs, read only with weights.  workspace:
  * omni_qk_norm_rope_backward_workspace_size(head_dim) bytes with weights, none
  * without.

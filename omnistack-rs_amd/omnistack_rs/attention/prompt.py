@@ -101,7 +101,7 @@ class _PromptAttention(torch.autograd.Function):
         do = _rows(do)
         dq, dk, dv = (_lib.empty_as(t) for t in (q, k, v))
         L = _lib.lib()
-        ws_bytes = L.omni_prompt_attn_backward_workspace_size(N, Hq, k.shape[1], D, cu.numel() - 1)
+        ws_bytes = _lib.on_device(ctx.dev, L.omni_prompt_attn_backward_workspace_size, N, Hq, k.shape[1], D, cu.numel() - 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ctx.dev) if ws_bytes else None
         _lib.check(_lib.on_device(
             ctx.dev, L.omni_prompt_attn_backward, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
