@@ -125,11 +125,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     to t of its sequence.  Returns (N, n_heads, head_dim) in q's dtype, and
     with ``return_lse`` the rows' log of summed exponentials, float32
     (n_heads, N; it has no gradient).  Gradients for q, k and v; forward and
-    backward can be captured in a HIP graph once no eager autograd graph of the
-    same leaves is alive (refused otherwise).  Rows behind the last sequence are zeros (lse -inf); in
-    ``out``, a tensor to write into (no gradient then), they stay as they were.  ``validate``
-    checks cu_seqlens on the host (a device sync when it is on the device);
-    without it values that break the rules give rows of no meaning."""
+    backward can be captured in a HIP graph (``validate`` off, cu_seqlens on the
+    device) once no eager autograd graph of the same leaves is alive, which is
+    refused where these operators built it.  Rows behind the last sequence are
+    zeros (lse -inf); in ``out``, a tensor to write into (no gradient then), they
+    stay as they were.  ``validate`` checks cu_seqlens on the host (a device
+    sync when it is on the device); without it values that break the rules give
+    rows of no meaning."""
     dev, cu, scale = _check(q, k, v, cu_seqlens, scale, validate)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:

@@ -81,7 +81,6 @@ class RotaryEmbedding:
         both = torch.tensor(turns + words, dtype=torch.int64).to(device)
         self.turns, self.pair_axes = both[:n], both[n:].view(torch.uint8)[:n]
         self.device = both.device
-        self._args = (self.turns.data_ptr(), self.pair_axes.data_ptr(), R, int(self.interleaved))
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
@@ -153,7 +152,8 @@ def _common(q, k, pos, rotary, wq, wk, eps, rows):
     """The arguments that both directions share, behind the tensors."""
     ps = pos.stride()
     return (_lib.dtype_code(q.dtype), *rows, q.shape[1], k.shape[1], rotary.head_dim, pos.data_ptr(),
-            int(pos.dtype == torch.int64), _lib.I64x3(ps[0], 0 if len(ps) == 2 else ps[1], ps[-1]), *rotary._args,
+            int(pos.dtype == torch.int64), _lib.I64x3(ps[0], 0 if len(ps) == 2 else ps[1], ps[-1]),
+            rotary.turns.data_ptr(), rotary.pair_axes.data_ptr(), rotary.rotary_dim, int(rotary.interleaved),
             _lib.ptr(wq), _lib.ptr(wk), 0 if wq is None else _lib.dtype_code(wq.dtype), eps)
 
 
@@ -220,8 +220,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     contiguous, or ``out`` (two tensors of the inputs' shapes; the inputs
     themselves turn in place).  Gradients for q, k and the weights; ``out`` is
     for calls that need none.  Forward and backward can be captured in a HIP
-    graph once no eager autograd graph of the same leaves is alive (refused
-    otherwise)."""
+    graph once no eager autograd graph of the same leaves is alive, which is
+    refused where these operators built it."""
     eps = float(eps)
     dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (

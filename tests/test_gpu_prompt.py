@@ -6,8 +6,10 @@ u32 that of fp32.  Scores are fp32 sums of exact products: each is off by at
 most (D + 2) u32 |scale| sum |q||k| <= X, an absolute error in the exponent, so
 a probability is off by a factor within 1 +- (2 X + 2^-20) (its own error, the
 row sum's and the exponential's).  A probability is then rounded to the
-inputs' type, u p, before the product with v (row sums take the unrounded).
-So |o - o'| <= (u + 2 X + 2^-20) sum_s p |v| + u |o|.
+inputs' type, u p, before the product with v; row sums take the rounded, so
+that the weights' errors d_s, |d_s| <= u p, leave sum_s d_s (v - o), at most
+u sum_s p |v| + u |o|.
+So |o - o'| <= (u + 2 X + 2^-20) sum_s p |v| + 2 u |o|.
 Backward, with e = 2 X + 2^-20 + u for a rounded probability: dv is off by
 e sum p |g| + u |dv|.  dp - delta is an fp32 sum of D products, and delta comes
 from the rounded output: off by Y = (u + D u32) (|g| . |o| + sum_d |g||v|) + |g| . |o - o'|;
@@ -79,7 +81,7 @@ def _want(q, k, v, cu, causal, scale, do=None):
             O = p @ V
             o[a:b, h], lse[h, a:b] = O, l
             pmin = 2.0 ** -126 if q.dtype == torch.bfloat16 else 2.0 ** -31
-            ob[a:b, h] = u * O.abs() + e * (p @ V.abs()) + pmin * (see.double() @ V.abs())
+            ob[a:b, h] = 2 * u * O.abs() + e * (p @ V.abs()) + pmin * (see.double() @ V.abs())
             if do is None:
                 continue
             g = g64[a:b, h]

@@ -247,6 +247,22 @@ def test_far_offsets_and_version(device):
 
 
 @gpu
+def test_copied_rotary_embedding(device):
+    """A copy holds its own frequencies and reads no others."""
+    import copy
+
+    from omnistack_rs.kernels.rope import RotaryEmbedding, qk_norm_rope
+    q, k, *_ = (t.to(device) for t in _inputs(20, 4, 2, 64, "bf16", 51, "bf16"))
+    pos = torch.arange(20, device=device)
+    rot = RotaryEmbedding(64, device=device)
+    other = copy.deepcopy(rot)
+    want = qk_norm_rope(q, k, pos, rot)
+    rot.turns.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(qk_norm_rope(q, k, pos, other), want))
+    assert torch.equal(qk_norm_rope(q, k, pos, rot)[0], q)
+
+
+@gpu
 def test_zero_rows_and_special_values(device):
     """No tokens give no outputs (and zero weight gradients); a row of zeros
     stays zero; NaN and infinity stay in their own head."""
