@@ -254,6 +254,54 @@ def test_layouts_and_out(device):
 
 
 @gpu
+def test_broadcast_inputs_and_gradients(device):
+    """One kv head and one query row spread over many, an output gradient of
+    one value: the bits of their copies, and gradients summed over the spread."""
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([70, 140])
+    q, k, v, do = (t.to(device) for t in _inputs(N, 4, 1, 64, "bf16", 47))
+    cu, q, do = cu.to(device), q[:1], do[:1, :1, :1]
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    wide = [t.expand(N, h, 64) for t, h in zip(leaves, (4, 2, 2))]
+    o = prompt_attention(*wide, cu)
+    grads = torch.autograd.grad(o, wide, do.expand(N, 4, 64), retain_graph=True)
+    copies = [t.detach().contiguous().requires_grad_() for t in wide]
+    want = prompt_attention(*copies, cu)
+    assert torch.equal(o.detach(), want.detach())
+    ref = torch.autograd.grad(want, copies, do.expand(N, 4, 64).contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(grads, ref))
+    sums = torch.autograd.grad(o, leaves, do.expand(N, 4, 64))
+    for got, r, d in zip(sums, ref, (0, 1, 1)):
+        assert got.shape[d] == 1 and torch.equal(got, r.sum(d, keepdim=True))
+
+
+@gpu
+def test_two_streams_at_once(device):
+    """Passes on two streams, queued together, give what each gives alone."""
+    from omnistack_rs.attention import prompt_attention
+    cu, N = _cu([300, 1500])
+    cu = cu.to(device)
+    sets = [[t.to(device) for t in _inputs(N, 4, 2, 64, "f16", s)] for s in (48, 49)]
+
+    def step(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = prompt_attention(*leaves, cu, validate=False)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(step(*s))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@gpu
 def test_infinity_in_the_last_token_without_a_mask(device):
     """Rows behind a sequence that does not fill its tile have no part in it:
     an infinite value of the last token makes infinite outputs, not NaN, and an

@@ -247,6 +247,25 @@ def test_far_offsets_and_version(device):
 
 
 @gpu
+def test_broadcast_inputs_and_gradients(device):
+    """One key head spread over many and output gradients of one value: the bits of their copies."""
+    from omnistack_rs.kernels.rope import RotaryEmbedding, qk_norm_rope
+    N, D = 37, 64
+    q, k, _, _, wq, wk = (t.to(device) for t in _inputs(N, 4, 1, D, "bf16", 52, "f32"))
+    rot, pos, one = RotaryEmbedding(D, device=device), torch.arange(N, device=device), q[:1, :1, :1]
+    leaf = k.clone().requires_grad_()
+    args = [q.clone().requires_grad_(), leaf.expand(N, 3, D), wq.requires_grad_(), wk.requires_grad_()]
+    y = qk_norm_rope(*args[:2], pos, rot, *args[2:])
+    grads = torch.autograd.grad(y, args, (one.expand(N, 4, D), one.expand(N, 3, D)), retain_graph=True)
+    copies = [t.detach().contiguous().requires_grad_() for t in args]
+    want = qk_norm_rope(*copies[:2], pos, rot, *copies[2:])
+    ref = torch.autograd.grad(want, copies, (one.expand(N, 4, D).contiguous(), one.expand(N, 3, D).contiguous()))
+    assert all(torch.equal(a.detach(), b.detach()) for a, b in zip((*y, *grads), (*want, *ref)))
+    back, = torch.autograd.grad(y, [leaf], (one.expand(N, 4, D), one.expand(N, 3, D)))
+    assert torch.equal(back, ref[1].sum(1, keepdim=True))
+
+
+@gpu
 def test_copied_rotary_embedding(device):
     """A copy holds its own frequencies and reads no others."""
     import copy
