@@ -71,7 +71,11 @@ def _forward(q, k, v, cu, scale, causal, out, need_lse, dev, need_rest=False):
     N, Hq, D = q.shape
     qc, kc, vc = _rows(q), _rows(k), _rows(v)
     o = _lib.empty_as(q) if out is None else out
-    lse = torch.empty(Hq, N, dtype=torch.float32, device=dev) if need_lse else None
+    lse = None
+    if need_lse:                                     # the kernel leaves rows of no sequence as they were where out= does
+        lse = torch.empty(Hq, N, dtype=torch.float32, device=dev)
+        if out is not None:
+            lse.fill_(-math.inf)
     rest = _lib.empty_as(q) if need_rest else None
     rc = _lib.on_device(
         dev, _lib.lib().omni_prompt_attn, qc.data_ptr(), _strides(qc), kc.data_ptr(), _strides(kc), vc.data_ptr(),

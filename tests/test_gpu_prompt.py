@@ -245,6 +245,9 @@ def test_layouts_and_out(device):
     out = torch.full((N, Hq, D), 7.0, device=device, dtype=q.dtype)
     assert prompt_attention(q, k, v, cu, out=out) is out
     assert torch.equal(out[:200], want[:200]) and bool((out[200:] == 7).all())
+    torch.full((Hq, N), 3.0, device=device)          # what a fresh lse would hold
+    lse = prompt_attention(q, k, v, cu, out=out, return_lse=True)[1]
+    assert torch.equal(lse, prompt_attention(q, k, v, cu, return_lse=True)[1]) and bool((lse[:, 200:] == -math.inf).all())
     with pytest.raises(ValueError, match="overlap"):
         prompt_attention(q, k, v, cu, out=q)
     with pytest.raises(ValueError, match="gradient"):
