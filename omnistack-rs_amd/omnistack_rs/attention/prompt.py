@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ..kernels.rope import overlap
+from ..kernels.rope import folded, overlap
 
 _HEAD_DIMS = (32, 64, 128)
 
@@ -144,7 +144,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or _rows(out) is not out:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {tuple(q.shape)} on {dev}, its last dim contiguous "
                              "and rows at 16-byte steps")
-        if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())) or any(overlap(out, t) for t in (q, k, v)):
+        if folded(out) or any(overlap(out, t) for t in (q, k, v)):
             raise ValueError("out must not overlap q, k or v, nor itself")
     if grad:
         o, lse = _PromptAttention.apply(q, k, v, cu, scale, causal, dev)

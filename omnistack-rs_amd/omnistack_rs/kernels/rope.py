@@ -251,6 +251,16 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def folded(t: torch.Tensor) -> bool:
+    """Whether two elements of `t` may lie in one place."""
+    extent = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < extent:
+            return True
+        extent += s * (n - 1)
+    return False
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two (rows, heads, dim) tensors may share memory.  Slices of one
     buffer interleave (q and k of a fused projection): those are apart where a
@@ -274,8 +284,8 @@ def _check_overlap(q, k, out):
 
     qo, ko = out
     for o in out:
-        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
-            raise ValueError("out must not be a broadcast view")
+        if folded(o):
+            raise ValueError("out must not be a broadcast view, nor overlap itself otherwise")
     if overlap(qo, ko) or overlap(qo, k) or overlap(ko, q) or not (same(qo, q) or not overlap(qo, q)) or \
             not (same(ko, k) or not overlap(ko, k)):
         raise ValueError("out may be q and k themselves, but must not overlap them otherwise")

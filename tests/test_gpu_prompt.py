@@ -250,6 +250,8 @@ def test_layouts_and_out(device):
     assert torch.equal(lse, prompt_attention(q, k, v, cu, return_lse=True)[1]) and bool((lse[:, 200:] == -math.inf).all())
     with pytest.raises(ValueError, match="overlap"):
         prompt_attention(q, k, v, cu, out=q)
+    with pytest.raises(ValueError, match="nor itself"):
+        prompt_attention(q, k, v, cu, out=torch.empty((N + Hq) * D, device=device, dtype=q.dtype).as_strided((N, Hq, D), (D, D, 1)))
     with pytest.raises(ValueError, match="gradient"):
         prompt_attention(q.clone().requires_grad_(), k, v, cu, out=out)
     with pytest.raises(ValueError, match="rise"):

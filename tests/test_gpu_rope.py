@@ -223,6 +223,8 @@ def test_in_place_and_out(device):
     assert torch.equal(buf[:, (Hq + Hkv) * D:], tail)
     with pytest.raises(ValueError, match="overlap"):
         qk_norm_rope(q[1:], k[1:], pos[1:], rot, wq, wk, out=(q[:-1], torch.empty_like(k[1:])))
+    with pytest.raises(ValueError, match="overlap itself"):
+        qk_norm_rope(q, k, pos, rot, wq, wk, out=(torch.empty(N * D + Hq * D, device=device, dtype=q.dtype).as_strided((N, Hq, D), (D, D, 1)), k))
     with pytest.raises(ValueError, match="gradient"):
         qk_norm_rope(q, k, pos, rot, wq.clone().requires_grad_(), wk, out=(q, k))
 
@@ -373,6 +375,14 @@ def test_refusals_of_the_call():
             qk_norm_rope(*args, **kw)
     with pytest.raises(TypeError):
         qk_norm_rope(q, k, pos, None)
+
+
+def test_folded():
+    from omnistack_rs.kernels.rope import folded
+    x = torch.zeros(4, 6, 8)
+    assert not any(folded(t) for t in (x, x.transpose(0, 1), x[:, ::2], x[:1].transpose(0, 2), x[:0], torch.zeros(())))
+    assert folded(x[:1].expand(4, 6, 8)) and folded(x[:, :1].expand(4, 6, 8))
+    assert folded(x.view(-1).as_strided((4, 6, 8), (8, 8, 1))) and folded(x.view(-1).as_strided((4, 6, 8), (48, 4, 1)))
 
 
 def test_turns_are_the_frequencies():
