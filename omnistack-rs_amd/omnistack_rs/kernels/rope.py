@@ -16,6 +16,7 @@ fractions of a turn.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -262,19 +263,22 @@ def folded(t: torch.Tensor) -> bool:
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two (rows, heads, dim) tensors may share memory.  Slices of one
-    buffer interleave (q and k of a fused projection): those are apart where a
-    row's heads of each lie within rows of the same length, at columns of their
-    own."""
+    """Whether two (rows, heads, dim) or (batch, heads, rows, dim) tensors may
+    share memory.  Slices of one buffer interleave (q and k of a fused
+    projection): those are apart where all rows of both start a step's multiple
+    away from each other and the heads of each have columns of their own within
+    the step."""
     (a0, a1), (b0, b1) = _span(a), _span(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    if a.dim() != 3 or b.dim() != 3 or a.stride(0) != b.stride(0):
-        return True
-    row = a.stride(0) * a.element_size()
-    la, lb = (_span(t[:1])[1] - _span(t[:1])[0] for t in (a, b))
-    off = (b0 - a0) % row if row else 0
-    return off < la or off + lb > row
+    step = 0
+    for t in (a, b):
+        for d in range(t.dim() - 1):
+            if d != 1 and t.shape[d] > 1:             # rows and batches
+                step = math.gcd(step, t.stride(d) * t.element_size())
+    la, lb = (_span(t[:1] if t.dim() == 3 else t[:1, :, :1])[1] - t.data_ptr() for t in (a, b))
+    off = (b0 - a0) % step if step else 0
+    return off < la or off + lb > step
 
 
 def _check_overlap(q, k, out):

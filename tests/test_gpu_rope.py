@@ -221,6 +221,10 @@ def test_in_place_and_out(device):
     got = qk_norm_rope(qs, ks, pos, rot, wq, wk, out=(qs, ks))
     assert got[0] is qs and torch.equal(qs, want[0]) and torch.equal(ks, want[1])
     assert torch.equal(buf[:, (Hq + Hkv) * D:], tail)
+    buf = torch.cat([q.reshape(N, -1), k.reshape(N, -1)], 1)
+    qs, ks = (t.unflatten(0, (2, 25)).transpose(1, 2) for t in (buf[:, :Hq * D].view(N, Hq, D), buf[:, Hq * D:].view(N, Hkv, D)))
+    qk_norm_rope(qs, ks, pos.view(2, 25), rot, wq, wk, out=(qs, ks))       # (2, heads, 25, D)
+    assert all(torch.equal(t.transpose(1, 2).reshape(w.shape), w) for t, w in zip((qs, ks), want))
     with pytest.raises(ValueError, match="overlap"):
         qk_norm_rope(q[1:], k[1:], pos[1:], rot, wq, wk, out=(q[:-1], torch.empty_like(k[1:])))
     with pytest.raises(ValueError, match="overlap itself"):
@@ -383,6 +387,19 @@ def test_folded():
     assert not any(folded(t) for t in (x, x.transpose(0, 1), x[:, ::2], x[:1].transpose(0, 2), x[:0], torch.zeros(())))
     assert folded(x[:1].expand(4, 6, 8)) and folded(x[:, :1].expand(4, 6, 8))
     assert folded(x.view(-1).as_strided((4, 6, 8), (8, 8, 1))) and folded(x.view(-1).as_strided((4, 6, 8), (48, 4, 1)))
+
+
+def test_overlap():
+    from omnistack_rs.kernels.rope import overlap
+    D, row = 8, (3 + 2 + 2) * 8
+    buf = torch.zeros(10 * row)
+    q, k = buf.view(10, 7, D)[:, :3], buf.view(10, 7, D)[:, 3:5]
+    assert not overlap(q, k) and not overlap(k, q) and overlap(q, q) and overlap(q[1:], q[:-1]) and overlap(buf.view(10, 7, D)[:, 2:4], k)
+    q4, k4 = (t.unflatten(0, (2, 5)).transpose(1, 2) for t in (q, k))     # (2, heads, 5, D)
+    assert not overlap(q4, k4) and not overlap(k4, q4) and overlap(q4, q4) and overlap(q4[:1], q4) and overlap(q4, q4[:, 1:])
+    assert not overlap(q4[:1], k4[1:]) and not overlap(q[:1], k[:1]) and not overlap(q, torch.zeros(10, 3, D))
+    h = buf[:10 * 3 * D].view(3, 10, D).transpose(0, 1)                   # heads outermost: not told apart
+    assert overlap(h, h[:, 1:]) and not overlap(h[:, :1], h[:, 1:])
 
 
 def test_turns_are_the_frequencies():
