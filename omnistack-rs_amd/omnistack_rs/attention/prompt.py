@@ -139,7 +139,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     dev, cu, scale = _check(q, k, v, cu_seqlens, scale, validate)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:
-        if grad:
+        if grad or torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("out= takes no gradient: call it under torch.no_grad()")
         if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or _rows(out) is not out:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {tuple(q.shape)} on {dev}, its last dim contiguous "

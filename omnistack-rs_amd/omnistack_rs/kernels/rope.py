@@ -228,7 +228,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
         q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)))
     if out is not None:
-        if grad:
+        if grad or torch.is_grad_enabled() and any(t.requires_grad for t in out):
             raise ValueError("out= takes no gradient: call it under torch.no_grad()")
         for o, t in zip(out, (q, k)):
             if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or _heads(o) is not o:

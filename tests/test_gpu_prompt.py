@@ -254,6 +254,8 @@ def test_layouts_and_out(device):
         prompt_attention(q, k, v, cu, out=torch.empty((N + Hq) * D, device=device, dtype=q.dtype).as_strided((N, Hq, D), (D, D, 1)))
     with pytest.raises(ValueError, match="gradient"):
         prompt_attention(q.clone().requires_grad_(), k, v, cu, out=out)
+    with pytest.raises(ValueError, match="gradient"):
+        prompt_attention(q, k, v, cu, out=torch.empty_like(q, requires_grad=True))
     with pytest.raises(ValueError, match="rise"):
         prompt_attention(q, k, v, torch.tensor([0, 5, 4], device=device))
 

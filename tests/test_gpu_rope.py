@@ -231,6 +231,8 @@ def test_in_place_and_out(device):
         qk_norm_rope(q, k, pos, rot, wq, wk, out=(torch.empty(N * D + Hq * D, device=device, dtype=q.dtype).as_strided((N, Hq, D), (D, D, 1)), k))
     with pytest.raises(ValueError, match="gradient"):
         qk_norm_rope(q, k, pos, rot, wq.clone().requires_grad_(), wk, out=(q, k))
+    with pytest.raises(ValueError, match="gradient"):
+        qk_norm_rope(q, k, pos, rot, wq, wk, out=(torch.empty_like(q, requires_grad=True), torch.empty_like(k)))
 
 
 @gpu
