@@ -41,7 +41,7 @@ struct PromptArgs {
     PromptHeads q, k, v, o, olo;         // olo: what rounding took from o, for the gradient
     PromptHeads g, dq, dk, dv;           // backward: the output's gradient, and those of q, k and v
     float *lse;                          // (Hq, N), or NULL
-    float *lse2, *delta;                 // backward, (Hq, N): lse log2 e, and -sum_d g o
+    float *lse2, *delta;                 // backward, (Hq, N): lse log2 e (f16: less kPtF16P), and -sum_d g o
     float *parts;                        // backward, (heads of the group in parts, dk and dv, N, Hkv, D)
     float *peaks;                        // backward in f16: kPtPeaks largest squared norms of g's rows, then of v's
     const int32_t *cu;
@@ -875,7 +875,7 @@ __global__ __launch_bounds__(64 * kPtWaves, 2) void prompt_dq_kernel(PromptArgs 
         R.lse2 = a.lse[(int64_t)W.h * a.N + at] * 1.44269504f;
         if (W.mine && (threadIdx.x & 32) == 0) {
             a.delta[(int64_t)W.h * a.N + at] = R.delta;
-            a.lse2[(int64_t)W.h * a.N + at] = R.lse2;
+            a.lse2[(int64_t)W.h * a.N + at] = R.lse2 - (DT == OMNI_F16 ? kPtF16P : 0.0f);
         }
     }
     const float up = pt_ds_scale<DT>(a);
@@ -988,7 +988,7 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D>
         float p[4], ds[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - l[e]));
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], a.cs, -l[e]));
             ds[e] = p[e] * (DT == OMNI_F16 ? dp[i + e] * up : dp[i + e]);
         }
 #pragma unroll
@@ -1111,7 +1111,7 @@ __global__ __launch_bounds__(64 * kPtKvWaves, 2) void prompt_dkv_kernel(PromptAr
                     pf16_t w = pt_product<DT, D>(qb, a.q.st, j0, S.len, 0.0f, [&](int kk) { return KLDS ? AK.rows(kt, 0, kk) : R.k[KLDS ? 0 : kk]; });
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.cs, (DT == OMNI_F16 ? kPtF16P : 0.0f) - __shfl(l, 8 * (i / 4) + 4 * (lane >> 5) + i % 4, 64)));
+                        w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.cs, -__shfl(l, 8 * (i / 4) + 4 * (lane >> 5) + i % 4, 64)));
                     if constexpr (DK) {
                         const pf16_t dp = pt_product<DT, D>(gb, a.g.st, j0, S.len, 0.0f, [&](int kk) { return R.v[kk]; });
 #pragma unroll
