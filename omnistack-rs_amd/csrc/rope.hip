@@ -182,12 +182,14 @@ struct RpLane {
     float c[E], s[E];                    // of each dim; s carries the pair's sign (neighbours: by pair)
     float w[E], wp[E];                   // own and partner's weights
     int sub, grp, d0, partner;
+    bool turns;                          // its dims are among the first R
 
     __device__ __forceinline__ void place(const RopeArgs &a) {
         const int lane = threadIdx.x & 63;
         sub = lane % LPH;
         grp = lane / LPH;
         d0 = sub * E;
+        turns = PAIR == 0 || d0 < a.R;
         partner = lane;
         if constexpr (PAIR == 1) {
             const int half = a.R / 2;
@@ -218,9 +220,9 @@ struct RpLane {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (PAIR != 0 && d0 >= a.R) {
+        if (!turns) {                    // no pair: turn() leaves these dims
 #pragma unroll
-            for (int e = 0; e < E; ++e) { c[e] = 1.0f; s[e] = 0.0f; }
+            for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
         } else if constexpr (PAIR == 2) {
 #pragma unroll
             for (int e = 0; e < E / 2; ++e) { c[e] = cs[d0 / 2 + e]; s[e] = sn[d0 / 2 + e]; }
@@ -248,7 +250,8 @@ struct RpLane {
         }
         return o;
     }
-    // z rotated, z of the partner dims in zp (unused for neighbours)
+    // z rotated, z of the partner dims in zp (unused for neighbours).  Dims behind
+    // R are selected, not turned by nothing: an infinity times a sine of 0 is NaN.
     __device__ __forceinline__ void turn(const float (&z)[E], const float (&zp)[E], float (&y)[E]) const {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -258,6 +261,7 @@ struct RpLane {
             } else {
                 y[e] = fmaf(z[e], c[e], zp[e] * s[e]);
             }
+            if constexpr (PAIR != 0) y[e] = turns ? y[e] : z[e];
         }
     }
 };

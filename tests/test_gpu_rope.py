@@ -435,3 +435,55 @@ def test_native_refusals():
     rc = L.omni_qk_norm_rope_backward(4096, s, 4096, s, 0, 1, 2, 1, 1, 64, 4096, 0, s, 4096, 4096, 64, 0, 4096, 4096, 0, 1e-6,
                                       4096, s, 4096, s, 4096, s, 4096, s, 4096, 4096, None, 0, None)
     assert rc == _lib.OMNI_EWORKSPACE and "workspace" in _lib.last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize("R", [0, 32])
+def test_dims_behind_the_rotation_are_copies(device, dtype, pairs, R):
+    """Without a norm the dims behind rotary_dim keep their bits, infinities,
+    NaN and zeros' signs among them, and so do their gradients; the dims that
+    turn are those of ordinary neighbours."""
+    from omnistack_rs.kernels.rope import RotaryEmbedding, qk_norm_rope
+    N, D = 23, 64
+    q, k, gq, gk, _, _ = (t if t is None else t.to(device) for t in _inputs(N, 4, 2, D, dtype, 81))
+    rot = RotaryEmbedding(D, rotary_dim=R, interleaved=pairs != "halves", device=device)
+    pos = torch.arange(N, device=device) + 7
+    leaves = [q.clone().requires_grad_(), k.clone().requires_grad_()]
+    y = qk_norm_rope(*leaves, pos, rot)
+    clean = [t.detach() for t in (*y, *torch.autograd.grad(y, leaves, (gq, gk)))]
+    bad = [float("inf"), float("-inf"), float("nan"), -0.0]
+    for t in (q, k, gq, gk):
+        for i, x in enumerate(bad * 2):
+            t[i::5, i % 2, R + 3 * i + 1] = x
+    leaves = [q.clone().requires_grad_(), k.clone().requires_grad_()]
+    y = qk_norm_rope(*leaves, pos, rot)
+    got = [t.detach() for t in (*y, *torch.autograd.grad(y, leaves, (gq, gk)))]
+    bits = torch.int32 if dtype == "f32" else torch.int16
+    for g, c, x, name in zip(got, clean, (q, k, gq, gk), ("q", "k", "dq", "dk")):
+        assert torch.equal(g[..., :R].view(bits), c[..., :R].view(bits)), name
+        assert torch.equal(g[..., R:].contiguous().view(bits), x[..., R:].contiguous().view(bits)), name
+
+
+@gpu
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+def test_norm_with_an_infinity_behind_the_rotation(device, pairs):
+    """The head's factor is 0 then: its finite dims are zeros, and only the
+    infinite one is NaN."""
+    from omnistack_rs.kernels.rope import RotaryEmbedding, qk_norm_rope
+    N, D, R = 9, 64, 32
+    q, k, _, _, wq, wk = (t.to(device) for t in _inputs(N, 2, 1, D, "bf16", 82, "f32"))
+    rot, pos = RotaryEmbedding(D, rotary_dim=R, interleaved=pairs != "halves", device=device), torch.arange(N, device=device)
+    want = qk_norm_rope(q, k, pos, rot, wq, wk)
+    for at in (R, R + 5, D - 1):
+        x = q.clone()
+        x[4, 1, at] = float("inf")
+        got = qk_norm_rope(x, k, pos, rot, wq, wk)
+        assert torch.equal(got[1], want[1])
+        row = got[0][4, 1].clone()
+        assert bool(torch.isnan(row[at])), at
+        row[at] = 0
+        assert bool((row == 0).all()), at
+        got[0][4, 1] = want[0][4, 1]
+        assert torch.equal(got[0], want[0])
