@@ -945,8 +945,15 @@ struct PtGradKey {
     ps8_t k[KLDS ? 1 : D / 16], v[D / 16];
     pf16_t dk[NT], dv[NT];
     int s;
-    bool met;                            // an infinity or NaN among hidden rows
+    bool met;                            // an infinity or NaN among hidden rows, their statistics included
 };
+
+// Whether the row statistic's 32 values at `p` are finite.  A row may have none
+// (a NaN, or an infinite score) where q and g are ordinary, and the exponential
+// of a hidden score less a NaN is no 0.
+__device__ __forceinline__ bool pt_stat_finite(const float *p) {
+    return __builtin_amdgcn_ballot_w64((__float_as_uint(p[threadIdx.x & 31]) & 0x7f800000u) == 0x7f800000u) == 0;
+}
 
 // 32 rows from row j0 on, in the tiles from row r0 on.
 template <int DT, int D>
@@ -955,7 +962,8 @@ __device__ __forceinline__ void pt_dkv_tile(const PromptArgs &a, const PtLane<D>
                                             const float *delta, int j0, int r0, int len, bool masked, float up) {
     constexpr bool KLDS = PtGradKey<DT, D>::KLDS;
     const PtLane<D> A = lane_at.fresh(), AK = KLDS ? key_at.fresh() : A;
-    R.met = R.met || (masked && !(pt_all_finite<DT>(Q + r0 * 2 * D, 64 * D) && pt_all_finite<DT>(G + r0 * 2 * D, 64 * D)));
+    R.met = R.met || (masked && !(pt_all_finite<DT>(Q + r0 * 2 * D, 64 * D) && pt_all_finite<DT>(G + r0 * 2 * D, 64 * D) &&
+                                  pt_stat_finite(lse2)));
     const int half = (threadIdx.x >> 5) & 1;
     pf16_t s = {}, dp;
 #pragma unroll

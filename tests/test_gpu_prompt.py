@@ -502,3 +502,28 @@ def test_infinities_and_nan_stay_with_who_sees_them(device, bad, D, dtype, G, mo
                 assert ok, f"{name}: {err.max().item()}"
                 if math.isnan(bad) and rows.any() and not (which == 3 and i == 1):
                     assert bool(torch.isnan(g[a:b][rows]).any(-1).all()), f"{name}: NaN was lost"
+
+
+@gpu
+@pytest.mark.parametrize("D,dtype,G", [(128, "bf16", 1), (64, "f16", 2), (32, "bf16", 4)])
+@pytest.mark.parametrize("at", [5, 40])
+def test_rows_without_a_result_leave_the_keys_behind_them_alone(device, at, D, dtype, G):
+    """A key with an infinity makes six rows NaN and has no weight in the later
+    ones (their scores with it are -inf).  The gradients of the keys behind
+    those six rows, which these do not see, are those of the sequence without
+    that token."""
+    from omnistack_rs.attention import prompt_attention
+    n = 150
+    q, k, v, do = (t.to(device) for t in _inputs(n, 2 * G, 2, D, dtype, 71))
+    k[at, :, 3] = float("inf")
+    q[at:, :, 3] = -1.0
+    q[at:at + 6, :, 3] = 1.0
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = prompt_attention(*leaves, [0, n])
+    _, dk, dv = torch.autograd.grad(o, leaves, do)
+    rest = torch.cat([torch.arange(at), torch.arange(at + 1, n)]).to(device)
+    want = _want(q[rest], k[rest], v[rest], torch.tensor([0, n - 1]), True, 1 / math.sqrt(D), do[rest])
+    assert bool(torch.isnan(o[at:at + 6]).all()) and bool(torch.isnan(dv[at + 1:at + 6]).all())
+    for name, got in (("o", o.detach()), ("dk", dk), ("dv", dv)):
+        a, b = (t[at + 5:] for t in want[name])
+        _close(got[at + 6:], a, b, f"{name} behind the rows")
