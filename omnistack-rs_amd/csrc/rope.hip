@@ -222,7 +222,7 @@ struct RpLane {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (!turns) {                    // no pair: turn() leaves these dims
 #pragma unroll
-            for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
+            for (int e = 0; e < E; ++e) { c[e] = 1.0f; s[e] = 0.0f; }   // as zeros they cost 12 bytes of scratch
         } else if constexpr (PAIR == 2) {
 #pragma unroll
             for (int e = 0; e < E / 2; ++e) { c[e] = cs[d0 / 2 + e]; s[e] = sn[d0 / 2 + e]; }
