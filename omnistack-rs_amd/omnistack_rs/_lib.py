@@ -12,6 +12,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("OMNISTACK_AMD_LIB", os.path.join(_HERE, "_native", "libomnistack_amd.so"))
@@ -171,6 +172,16 @@ def on_device(device: torch.device, fn, *args) -> int:
         return fn(*args)
     with torch.cuda.device(device):
         return fn(*args)
+
+
+def refuse_tangents(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuse dual tensors: a kernel gives no tangent, and an output without one
+    would be a derivative of zero.  (Outside a dual level, the common case, one
+    comparison: the level is -1.)"""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no forward-mode derivative")
 
 
 _LEAF_STREAM = "omnistack_rs.stream"

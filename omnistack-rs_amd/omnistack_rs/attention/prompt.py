@@ -100,6 +100,7 @@ class _PromptAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, _):
+        _lib.refuse_tangents("prompt_attention's gradient", do)
         q, k, v, o, rest, lse, cu = ctx.saved_tensors
         N, Hq, D = q.shape
         do = _rows(do)
@@ -128,14 +129,16 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     on the host; lengths of zero are fine.  ``causal``: token t sees tokens up
     to t of its sequence.  Returns (N, n_heads, head_dim) in q's dtype, and
     with ``return_lse`` the rows' log of summed exponentials, float32
-    (n_heads, N; it has no gradient).  Gradients for q, k and v; forward and
-    backward can be captured in a HIP graph (``validate`` off, cu_seqlens on the
-    device) once no eager autograd graph of the same leaves is alive, which is
-    refused where these operators built it.  Rows behind the last sequence are
-    zeros (lse -inf); in ``out``, a tensor to write into (no gradient then), they
-    stay as they were.  ``validate`` checks cu_seqlens on the host (a device
+    (n_heads, N; it has no gradient).  Gradients for q, k and v, once and in
+    reverse mode (dual tensors are refused); forward and backward can be
+    captured in a HIP graph (``validate`` off, cu_seqlens on the device) once no
+    eager autograd graph of the same leaves is alive, which is refused where
+    these operators built it.  Rows behind the last sequence are zeros (lse
+    -inf); in ``out``, a tensor to write into (no gradient then), they stay as
+    they were.  ``validate`` checks cu_seqlens on the host (a device
     sync when it is on the device); without it values that break the rules give
     rows of no meaning."""
+    _lib.refuse_tangents("prompt_attention", q, k, v, out)
     dev, cu, scale = _check(q, k, v, cu_seqlens, scale, validate)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:

@@ -186,6 +186,7 @@ class _QKNormRope(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
+        _lib.refuse_tangents("qk_norm_rope's gradient", gq, gk)
         pos, *rest = ctx.saved_tensors
         q, k, wq, wk = rest if rest else (gq, gk, None, None)
         dev, norm = ctx.dev, bool(rest)
@@ -219,11 +220,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     for all axes.  ``q_weight`` / ``k_weight`` (head_dim,): the norms' weights;
     without them heads are rotated only.  Returns (q', k') in the inputs' dtype,
     contiguous, or ``out`` (two tensors of the inputs' shapes; the inputs
-    themselves turn in place).  Gradients for q, k and the weights; ``out`` is
-    for calls that need none.  Forward and backward can be captured in a HIP
-    graph once no eager autograd graph of the same leaves is alive, which is
-    refused where these operators built it."""
+    themselves turn in place).  Gradients for q, k and the weights, once and in
+    reverse mode (dual tensors are refused); ``out`` is for calls that need
+    none.  Forward and backward can be captured in a HIP graph once no eager
+    autograd graph of the same leaves is alive, which is refused where these
+    operators built it."""
     eps = float(eps)
+    _lib.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, *(() if out is None else out))
     dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
         q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)))

@@ -527,3 +527,28 @@ def test_rows_without_a_result_leave_the_keys_behind_them_alone(device, at, D, d
     for name, got in (("o", o.detach()), ("dk", dk), ("dv", dv)):
         a, b = (t[at + 5:] for t in want[name])
         _close(got[at + 6:], a, b, f"{name} behind the rows")
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor wants a derivative that the kernels do not form: refused
+    before any device work, with and without gradients."""
+    from torch.autograd import forward_ad
+    from omnistack_rs.attention import prompt_attention
+    from omnistack_rs.attention.prompt import _PromptAttention
+    q, k = torch.zeros(9, 4, 64, dtype=torch.bfloat16), torch.zeros(9, 2, 64, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        for i in range(3):
+            for grad in (False, True):
+                args = [q, k, k]
+                args[i] = forward_ad.make_dual(args[i].clone().requires_grad_(grad), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    prompt_attention(*args, [0, 9])
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    prompt_attention(*args, [0, 9])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            prompt_attention(q, k, k, [0, 9], out=forward_ad.make_dual(q.clone(), torch.ones_like(q)))
+        with pytest.raises(RuntimeError, match="HIP"):
+            prompt_attention(q, k, k, [0, 9])
+        dual = forward_ad.make_dual(q.clone(), torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="gradient has no forward-mode"):      # a tangent of the gradient
+            _PromptAttention.backward(None, dual, None)

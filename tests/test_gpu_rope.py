@@ -487,3 +487,33 @@ def test_norm_with_an_infinity_behind_the_rotation(device, pairs):
         assert bool((row == 0).all()), at
         got[0][4, 1] = want[0][4, 1]
         assert torch.equal(got[0], want[0])
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor wants a derivative that the kernels do not form: refused
+    before any device work, with and without gradients; the same numbers
+    without a tangent get as far as the device check."""
+    from torch.autograd import forward_ad
+    from omnistack_rs.kernels.rope import RotaryEmbedding, _QKNormRope, qk_norm_rope
+    rot, pos = RotaryEmbedding(64, device="cpu"), torch.arange(5)
+    q, k, w = torch.zeros(5, 4, 64), torch.zeros(5, 2, 64), torch.ones(64)
+    with forward_ad.dual_level():
+        for i in range(4):
+            for grad in (False, True):
+                args = [q, k, w, w]
+                args[i] = forward_ad.make_dual(args[i].clone().requires_grad_(grad), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    qk_norm_rope(*args[:2], pos, rot, *args[2:])
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    qk_norm_rope(*args[:2], pos, rot, *args[2:])
+        dual = forward_ad.make_dual(q.clone(), torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            qk_norm_rope(dual[1:], k[1:], pos[1:], rot)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            qk_norm_rope(q, k, pos, rot, out=(dual, k))
+        with pytest.raises(RuntimeError, match="HIP"):
+            qk_norm_rope(q, k, pos, rot, w, w)
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="HIP"):
+            qk_norm_rope(dual, k, pos, rot)
+        with pytest.raises(NotImplementedError, match="gradient has no forward-mode"):      # a tangent of the gradient
+            _QKNormRope.backward(None, dual, k)
