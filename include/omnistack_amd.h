@@ -479,7 +479,8 @@ int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const vo
  *   causal; kv head = hq / (Hq / Hkv).
  * Device pointers with host element strides {token, head}; the last dim is
  * contiguous, pointers and strides are multiples of 16 bytes, a token stride is
- * below 2^24 elements.  lse (Hq, N) f32 or NULL: log sum_s exp(scale q_t . k_s).
+ * below 2^24 elements, |scale| at most 2.3e38.  lse (Hq, N) f32 or NULL:
+ * log sum_s exp(scale q_t . k_s).
  * out_rest (as out) or NULL: what the rounding of out left, for the gradient.
  * Rows behind the last sequence: zeros (lse -inf) when fill_rest, else left as
  * they were.  cu_seqlens that break the rules give rows of no meaning, but

@@ -1204,7 +1204,8 @@ static int prompt_args(const char *who, int dtype, int64_t N, int Hq, int Hkv, i
     OMNI_CHECK_ARG(D == 32 || D == 64 || D == 128, "%s: head_dim must be 32, 64 or 128, got %d", who, D);
     OMNI_CHECK_ARG(N >= 0 && B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "%s: bad shape (Hq must be a multiple of Hkv)", who);
     OMNI_CHECK_ARG(N < (int64_t(1) << 31) && N * Hq < (int64_t(1) << 31) - 1024 && B < (int64_t(1) << 30), "%s: shape too large", who);
-    OMNI_CHECK_ARG(scale == scale && fabsf(scale) <= 3.0e38f, "%s: scale must be finite", who);
+    // times log2 e it stays finite
+    OMNI_CHECK_ARG(scale == scale && fabsf(scale) <= 2.3e38f, "%s: scale must be finite and at most 2.3e38 in size", who);
     a.N = N;
     a.B = (int)B;
     a.Hq = Hq;

@@ -52,8 +52,8 @@ def _check(q, k, v, cu_seqlens, scale, validate):
         raise ValueError(f"q, k and v must share float16 or bfloat16 (float32: reference_attn), got {q.dtype}, {k.dtype} "
                          f"and {v.dtype}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not abs(scale) <= 3.0e38:
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= 2.3e38:                     # the kernels multiply it by log2 e
+        raise ValueError(f"scale must be finite and at most 2.3e38 in size, got {scale}")
     cu = cu_seqlens if isinstance(cu_seqlens, torch.Tensor) else torch.as_tensor(cu_seqlens)
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"cu_seqlens must be int32 or int64 (n_sequences + 1,), got {cu.dtype} {tuple(cu.shape)}")

@@ -552,3 +552,22 @@ def test_forward_mode_is_refused():
         dual = forward_ad.make_dual(q.clone(), torch.ones_like(q))
         with pytest.raises(NotImplementedError, match="gradient has no forward-mode"):      # a tangent of the gradient
             _PromptAttention.backward(None, dual, None)
+
+
+def test_scales_that_leave_fp32_are_refused():
+    """The kernels multiply the scale by log2 e: 2.35e38 is the last that stays
+    finite there; the refusal starts at 2.3e38."""
+    import ctypes
+    from omnistack_rs import _lib
+    from omnistack_rs.attention import prompt_attention
+    q, k = torch.zeros(9, 4, 64, dtype=torch.bfloat16), torch.zeros(9, 2, 64, dtype=torch.bfloat16)
+    s = (ctypes.c_int64 * 2)(128, 64)
+    for x in (2.4e38, -2.4e38, 2.9e38):
+        with pytest.raises(ValueError, match="scale"):
+            prompt_attention(q, k, k, [0, 9], scale=x)
+        rc = _lib.lib().omni_prompt_attn(4096, s, 4096, s, 4096, s, 2, 0, 2, 1, 64, 4096, 1, x, 1, 1, 4096, s, None, None, None, None)
+        assert rc == _lib.OMNI_EINVAL and "scale" in _lib.last_error()
+    assert math.isfinite(torch.tensor(2.3e38 * 1.44269504, dtype=torch.float32).item())
+    with pytest.raises(RuntimeError, match="HIP"):
+        prompt_attention(q, k, k, [0, 9], scale=-2.3e38)
+    assert _lib.lib().omni_prompt_attn(4096, s, 4096, s, 4096, s, 2, 0, 2, 1, 64, 4096, 1, 2.29e38, 1, 1, 4096, s, None, None, None, None) == 0
