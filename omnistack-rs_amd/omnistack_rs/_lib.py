@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import weakref
 from typing import Optional
 
 import torch
@@ -185,20 +186,48 @@ def refuse_tangents(who: str, *tensors: Optional[torch.Tensor]) -> None:
 
 
 _LEAF_STREAM = "omnistack_rs.stream"
+_default_nodes = weakref.WeakSet()      # live gradient nodes of these operators that the default stream made
+
+
+def _leaf_nodes(nodes) -> set:
+    """The leaves' gradient nodes that autograd nodes `nodes` reach."""
+    leaves, seen, todo = set(), set(), list(nodes)
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        if hasattr(node, "variable"):
+            leaves.add(node)
+        else:
+            todo.extend(n for n, _ in node.next_functions)
+    return leaves
 
 
 def mark_leaves(device: torch.device, fn) -> None:
-    """Mark the gradient nodes of the leaves that autograd node `fn` reaches
-    first with the stream of their first use.  Under graph capture, a leaf
-    whose node another stream made (an eager graph of it is still alive) is
-    refused: the backward pass would make the captured stream wait for that
-    one, which ends the process when the capture closes."""
+    """Note the stream of autograd node `fn`, a call of an operator.  Under graph
+    capture, refuse it while an eager graph of the same leaves is alive: the
+    backward pass would make the capture wait for the stream that made the
+    leaves' gradient nodes, and where that is the default stream, closing the
+    capture ends the process.  Found are graphs through a node passed here on
+    the default stream, whatever lies between it and the leaves (only a capture
+    walks there), and, where a leaf feeds `fn` itself, the stream of its node's
+    first use if it is any other than the capture's."""
     stream = stream_of(device)
-    for node, _ in fn.next_functions:
-        if node is not None and hasattr(node, "variable"):
-            if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("graph capture with gradients: an autograd graph of the same leaves, built on "
-                                   "another stream, is still alive; delete its outputs before capturing")
+    if stream == 0:
+        _default_nodes.add(fn)
+        refuse = False
+    else:
+        refuse = _default_nodes and torch.cuda.is_current_stream_capturing() and \
+            not _leaf_nodes([fn]).isdisjoint(_leaf_nodes(_default_nodes))
+    if not refuse:
+        for node, _ in fn.next_functions:
+            if node is not None and hasattr(node, "variable"):
+                if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
+                    refuse = True
+    if refuse:
+        raise RuntimeError("graph capture with gradients: an autograd graph of the same leaves, built on "
+                           "another stream, is still alive; delete its outputs before capturing")
 
 
 I64x2, I64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3      # host arrays of strides

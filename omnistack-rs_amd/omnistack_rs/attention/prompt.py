@@ -132,10 +132,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (n_heads, N; it has no gradient).  Gradients for q, k and v, once and in
     reverse mode (dual tensors are refused); forward and backward can be
     captured in a HIP graph (``validate`` off, cu_seqlens on the device) once no
-    eager autograd graph of the same leaves is alive, which is refused where
-    these operators built it.  Rows behind the last sequence are zeros (lse
-    -inf); in ``out``, a tensor to write into (no gradient then), they stay as
-    they were.  ``validate`` checks cu_seqlens on the host (a device
+    eager autograd graph of the same leaves is alive: one through these
+    operators on the default stream is refused, as is one of leaves passed to
+    them directly.  Rows behind the last sequence are zeros (lse -inf); in
+    ``out``, a tensor to write into (no gradient then), they stay as they were.  ``validate`` checks cu_seqlens on the host (a device
     sync when it is on the device); without it values that break the rules give
     rows of no meaning."""
     _lib.refuse_tangents("prompt_attention", q, k, v, out)

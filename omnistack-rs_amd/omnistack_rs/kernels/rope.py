@@ -223,8 +223,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     themselves turn in place).  Gradients for q, k and the weights, once and in
     reverse mode (dual tensors are refused); ``out`` is for calls that need
     none.  Forward and backward can be captured in a HIP graph once no eager
-    autograd graph of the same leaves is alive, which is refused where these
-    operators built it."""
+    autograd graph of the same leaves is alive: one through these operators on
+    the default stream is refused, as is one of leaves passed to them directly."""
     eps = float(eps)
     _lib.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, *(() if out is None else out))
     dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
