@@ -571,3 +571,97 @@ def test_scales_that_leave_fp32_are_refused():
     with pytest.raises(RuntimeError, match="HIP"):
         prompt_attention(q, k, k, [0, 9], scale=-2.3e38)
     assert _lib.lib().omni_prompt_attn(4096, s, 4096, s, 4096, s, 2, 0, 2, 1, 64, 4096, 1, 2.29e38, 1, 1, 4096, s, None, None, None, None) == 0
+
+
+# What rounding the output left.  For a gradient the forward stores it, out_rest,
+# and takes the first 64 keys' probabilities as two 16-bit numbers each, p and
+# what rounding p left, off by u^2 p together.  With e2 = u^2 + 2 X + 2^-20 (the
+# probability's own errors, as at the top) weights that sum to one leave
+# e2 sum_s p |v - o|; two fp32 sums over at most 64 keys, two products each, leave
+# 128 u32 (sum_s p |v| + |o|); out_rest is rounded, u^2 |o| (f16: or half a
+# subnormal step, and the remainders of p half a step 2^-32 of the largest p).
+
+def _with_rest(q, k, v, lengths, scale, do):
+    """64-bit results of causal sequences of at most 64 tokens: o, dq, dk with
+    bars that grant delta what o + out_rest is off by and nothing for a rounded o;
+    and what o alone in place of o + out_rest does to dq and dk."""
+    u, D, G, f16 = torch.finfo(q.dtype).eps / 2, q.shape[2], q.shape[1] // k.shape[1], q.dtype == torch.float16
+    q64, k64, v64, g64 = (t.double() for t in (q, k, v, do))
+    res = {n: [torch.zeros_like(t) for _ in range(3)] for n, t in (("o", q64), ("dq", q64), ("dk", k64))}
+    sub = 2.0 ** -25 if f16 else 0.0
+    least = 2.0 ** -38 * 2 * g64.norm(dim=-1).max() * v64.norm(dim=-1).max() if f16 else 2.0 ** -126
+    a = 0
+    for n in lengths:
+        see = torch.ones(n, n, dtype=torch.bool, device=q.device).tril()
+        for h in range(q.shape[1]):
+            Q, K, V, g = q64[a:a + n, h], k64[a:a + n, h // G], v64[a:a + n, h // G], g64[a:a + n, h]
+            p = torch.softmax(torch.where(see, Q @ K.T * scale, -math.inf), -1)
+            X = ((D + 2) * U32 * abs(scale) * (Q.abs() @ K.abs().T) * see).amax(-1, keepdim=True)
+            O = p @ V
+            e2 = u * u + 2 * X + 2.0 ** -20
+            spread = (p[:, :, None] * (V[None] - O[:, None]).abs()).sum(1)
+            ob = e2 * spread + 128 * U32 * (p @ V.abs() + O.abs()) + u * u * O.abs() + sub
+            if f16:
+                ob = ob + 2.0 ** -32 * ((see.double() @ V.abs()) + see.sum(-1, keepdim=True) * O.abs())
+            dp, delta = g @ V.T, (g * O).sum(-1, keepdim=True)
+            Y = D * U32 * (g.abs() @ V.abs().T + (g.abs() * O.abs()).sum(-1, keepdim=True)) + (g.abs() * ob).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            dsb = p * Y + (2 * u + 2 * X + 2.0 ** -20) * ds.abs() + least * see
+            off = p * (g * (O.to(q.dtype).double() - O)).sum(-1, keepdim=True)       # of ds, from a rounded o
+            res["o"][0][a:a + n, h], res["o"][1][a:a + n, h] = O, ob
+            for name, hh, x, b, f in (("dq", h, ds @ K, dsb @ K.abs(), off @ K), ("dk", h // G, ds.T @ Q, dsb.T @ Q.abs(), off.T @ Q)):
+                for r, y in zip(res[name], (x * scale, b * abs(scale), f * scale)):
+                    r[a:a + n, hh] += y
+        a += n
+    for name in ("dq", "dk"):
+        res[name][1] += u * res[name][0].abs()
+    return res
+
+
+REST = [("bf16", 128, 4, 2), ("bf16", 64, 3, 1), ("f16", 32, 4, 4)]
+
+
+def _rest_inputs(D, dtype, Hq, Hkv, seed):
+    """v within half of 8, in sixteenths: dp - delta is a small difference of large terms."""
+    lengths = [64, 1, 17, 40, 2]
+    q, k, v, do = _inputs(sum(lengths), Hq, Hkv, D, dtype, seed, 0.25)
+    return lengths, q, k, (8 + (v.float().clamp(-2, 2) * 4).round() / 16).to(DT[dtype]), do
+
+
+@pytest.mark.parametrize("dtype,D,Hq,Hkv", REST)
+def test_the_rests_bars_would_notice(dtype, D, Hq, Hkv):
+    """A gradient from o alone, or with out_rest's sign turned (twice as far off), leaves the bars."""
+    lengths, q, k, v, do = _rest_inputs(D, dtype, Hq, Hkv, 91)
+    res = _with_rest(q, k, v, lengths, 1 / math.sqrt(D), do)
+    for name in ("dq", "dk"):
+        x, bar, off = res[name]
+        assert (off.abs() / bar).max() > 2, name
+    O, bar, _ = res["o"]
+    assert ((O.to(DT[dtype]).double() - O).abs() / bar).max() > 2
+    # probabilities without their remainders, on values around 0
+    q, k, v, _ = _inputs(64, Hq, Hkv, D, dtype, 92)
+    res = _with_rest(q, k, v, [64], 1 / math.sqrt(D), torch.zeros_like(q))
+    p = torch.exp(torch.where(torch.ones(64, 64).tril() > 0, q[:, 0].double() @ k[:, 0].double().T / math.sqrt(D), -math.inf))
+    p = (p / p.amax(-1, keepdim=True)).to(DT[dtype]).double()
+    o = (p / p.sum(-1, keepdim=True)) @ v[:, 0].double()
+    assert ((o - res["o"][0][:, 0]).abs() / res["o"][1][:, 0]).max() > 2
+
+
+@gpu
+@pytest.mark.parametrize("dtype,D,Hq,Hkv", REST)
+def test_out_and_its_rest(device, dtype, D, Hq, Hkv):
+    """out + out_rest is the 64-bit output, and delta is taken from both: dq and
+    dk of values that lie close together."""
+    from omnistack_rs.attention import prompt, prompt_attention
+    lengths, *near = _rest_inputs(D, dtype, Hq, Hkv, 91)
+    for which, (q, k, v, do) in (("near", near), ("around 0", _inputs(sum(lengths), Hq, Hkv, D, dtype, 92))):
+        q, k, v, do = (t.to(device) for t in (q, k, v, do))
+        cu = _cu(lengths)[0].to(device)
+        want = _with_rest(q, k, v, lengths, 1 / math.sqrt(D), do)
+        o, _, rest = prompt._forward(q, k, v, cu, 1 / math.sqrt(D), True, None, True, device, True)
+        assert bool((rest != 0).any())
+        _close(o.double() + rest.double(), *want["o"][:2], f"{which}: out and rest")
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        grads = torch.autograd.grad(prompt_attention(*leaves, cu), leaves, do)
+        _close(grads[0], *want["dq"][:2], f"{which}: dq")
+        _close(grads[1], *want["dk"][:2], f"{which}: dk")
