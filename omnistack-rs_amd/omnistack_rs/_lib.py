@@ -186,7 +186,11 @@ def refuse_tangents(who: str, *tensors: Optional[torch.Tensor]) -> None:
 
 
 _LEAF_STREAM = "omnistack_rs.stream"
-_default_nodes = weakref.WeakSet()      # live gradient nodes of these operators that the default stream made
+_default_nodes = set()      # weak references to the live gradient nodes of these operators that the default stream made
+
+
+def _of_leaf(node) -> bool:
+    return type(node).__name__ == "AccumulateGrad"
 
 
 def _leaf_nodes(nodes) -> set:
@@ -197,10 +201,13 @@ def _leaf_nodes(nodes) -> set:
         if node is None or node in seen:
             continue
         seen.add(node)
-        if hasattr(node, "variable"):
+        if _of_leaf(node):
             leaves.add(node)
-        else:
+            continue
+        try:
             todo.extend(n for n, _ in node.next_functions)
+        except RuntimeError:             # a function's context whose graph is gone
+            pass
     return leaves
 
 
@@ -215,14 +222,14 @@ def mark_leaves(device: torch.device, fn) -> None:
     first use if it is any other than the capture's."""
     stream = stream_of(device)
     if stream == 0:
-        _default_nodes.add(fn)
+        _default_nodes.add(weakref.ref(fn, _default_nodes.discard))
         refuse = False
     else:
         refuse = _default_nodes and torch.cuda.is_current_stream_capturing() and \
-            not _leaf_nodes([fn]).isdisjoint(_leaf_nodes(_default_nodes))
+            not _leaf_nodes([fn]).isdisjoint(_leaf_nodes(r() for r in list(_default_nodes)))
     if not refuse:
         for node, _ in fn.next_functions:
-            if node is not None and hasattr(node, "variable"):
+            if _of_leaf(node):
                 if node.metadata.setdefault(_LEAF_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing():
                     refuse = True
     if refuse:

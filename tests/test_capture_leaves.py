@@ -61,6 +61,12 @@ def test_the_eager_graph_counts_while_its_outputs_live(streams):
         streams(b.view(3, 2), a.detach(), stream=7, capturing=True)
     del x
     streams(b.view(3, 2), a.detach(), stream=7, capturing=True)
+    # a node's context may outlive its graph
+    out = streams(_behind(a), b * 1, stream=0, capturing=False)
+    context = out[0].grad_fn
+    del out
+    streams(_behind(a), b * 1, stream=7, capturing=True)
+    del context
     # a graph of another stream than the default one is joined by the engine
     side = streams(_behind(a), b * 1, stream=5, capturing=False)
     streams(_behind(a), b * 1, stream=7, capturing=True)
@@ -107,3 +113,28 @@ def test_capture_with_projections(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step())), f"replay {i}"
+
+
+def test_other_threads_may_build_graphs_meanwhile(streams):
+    """The walk takes a snapshot: graphs that other threads make and drop during it are no error."""
+    import threading
+    a, b = (torch.ones(6, requires_grad=True) for _ in range(2))
+    keep = [streams(_behind(a), b * 1, stream=0) for _ in range(200)]
+    stop = threading.Event()
+
+    def churn():
+        from omnistack_rs import _lib
+        while not stop.is_set():
+            out = _Op.apply(a * 1, b * 1)
+            _lib._default_nodes.add(_lib.weakref.ref(out[0].grad_fn, _lib._default_nodes.discard))
+
+    t = threading.Thread(target=churn)
+    t.start()
+    try:
+        for _ in range(20):
+            with pytest.raises(RuntimeError, match="still alive"):
+                streams(_behind(a), b * 1, stream=7, capturing=True)
+    finally:
+        stop.set()
+        t.join()
+    assert len(keep) == 200
