@@ -431,7 +431,8 @@ void omni_attn_paged_plan_destroy(omni_attn_paged_plan *plan);
  *   pair i of the first rotary_dim dims turned by positions[pair_axes[i]] * freq_i,
  * pairs being the halves (i, i + rotary_dim / 2) or, interleaved, neighbours
  * (2i, 2i + 1); dims behind rotary_dim keep z.  turns[i] (device, rotary_dim / 2)
- * = round(freq_i / 2 pi * 2^64) mod 2^64, the fraction of a turn per position;
+ * = round(freq_i / 2 pi * 2^64) mod 2^64, the fraction of a turn per position
+ * (its rounding costs |position| 2^-65 turns, 2e-7 radians at 2^40);
  * pair_axes[i] (device) names the pair's row of positions.
  * q, k, q_out, k_out: device pointers with host arrays of element strides
  * {batch, token, head}; the last dim is contiguous, pointers and strides are
@@ -480,7 +481,9 @@ int omni_qk_norm_rope_backward(const void *q, const int64_t *q_strides, const vo
  * Device pointers with host element strides {token, head}; the last dim is
  * contiguous, pointers and strides are multiples of 16 bytes, a token stride is
  * below 2^24 elements, |scale| at most 2.3e38.  lse (Hq, N) f32 or NULL:
- * log sum_s exp(scale q_t . k_s).
+ * log sum_s exp(scale q_t . k_s).  Scores are fp32: one of size X is off by about
+ * 2^-24 X, the gradient's probabilities by as much of themselves; past 2^23
+ * gradients have no meaning and outputs may not be finite.
  * out_rest (as out) or NULL: what the rounding of out left, for the gradient.
  * Rows behind the last sequence: zeros (lse -inf) when fill_rest, else left as
  * they were.  cu_seqlens that break the rules give rows of no meaning, but

@@ -459,16 +459,17 @@ __device__ __forceinline__ void pt_take(const char *lds, pf16_t (&x)[NT], float 
 // alone dq and dk were off by 1.5 to 2.8 times what rounding them costs
 // (sequences of 8 to 1024, scores of deviation 1 to 3), so by 1.4 to 1.5.
 //
-// Bound by the card's power, next to the matrix units: 32 heads over 8 of 128 in
-// bf16, one causal sequence of 32768 tokens 7.7 to 8.2 ms on different cards,
-// 1.07 to 1.14 PFLOP/s, where a large library product reaches 1.5; 8192 tokens
-// without a mask 985 us, 1.12 PFLOP/s, with the matrix units busy in half of the
-// cycles, vector instructions issuing in half, no LDS bank conflict and a clock
-// of 2.0 GHz.  The same call on zeros, which draw less, takes 857 us.  More
-// overlap did not pay: eight waves of which four always multiply while four take
-// exponentials, kept in turn by barriers, 1030 us; scores one tile ahead of the
-// products with V, 990.  64 rows a wave, which would halve the LDS reads, does
-// not fit the registers.
+// Bound by matrix and vector instructions that hardly overlap: 32 heads over 8 of
+// 128 in bf16, one causal sequence of 32768 tokens 7.7 to 8.2 ms on different
+// cards, 1.07 to 1.14 PFLOP/s, where a large library product reaches 1.5; 8192
+// tokens without a mask 970 to 990 us, 1.12 PFLOP/s, with the matrix units busy
+// in half of the cycles, vector instructions issuing in the other half (49.6 and
+// 48.5 %), no LDS bank conflict and a clock of 2.0 GHz.  Power is the lesser
+// part: the same call on zeros, which draw less, takes 857 us, still 1.28
+// PFLOP/s.  Two ways to more overlap did not pay: eight waves of which four
+// always multiply while four take exponentials, kept in turn by barriers, 1030
+// us; scores one tile ahead of the products with V, 990.  64 rows a wave, which
+// would halve the LDS reads, does not fit the registers of two waves a SIMD.
 
 template <int DT, int D>
 struct PtRow {
@@ -710,10 +711,11 @@ __global__ __launch_bounds__(64 * kPtWaves * KS, 2) void prompt_forward_kernel(P
 // reads again, took 46 us of a gradient of 8192 tokens).  Scores and g . v are formed twice for it,
 // seven products instead of five.
 //
-// 8192 tokens of 32 heads over 8 of 128 without a mask, bf16: dq 1.50 ms, 1.10
-// PFLOP/s of its three products, dk and dv 2.07 ms, 1.06 of theirs; matrix units
-// busy in 57 and 54 % of the cycles, clocks of 1.85 to 2.0 GHz, the forward that
-// keeps what a gradient needs 1.12 ms.
+// 8192 tokens of 32 heads over 8 of 128 without a mask, bf16: dq 1.40 to 1.50 ms,
+// 1.10 to 1.18 PFLOP/s of its three products, dk and dv 1.90 to 2.07 ms, 1.06 to
+// 1.16 of theirs; matrix units busy in 57 and 54 % of the cycles, clocks of 1.85
+// to 2.0 GHz, the forward that keeps what a gradient needs 1.05 to 1.12 ms.  All
+// three gradients are formed, also where only one is asked for.
 //
 // p and ds go to the matrix units in the inputs' 16 bits.  In f16, p is scaled
 // by 2^14 (p <= 1) and ds by the power of two that brings its bound, twice the
@@ -1238,10 +1240,13 @@ static void prompt_launch_forward(const PromptArgs &a, dim3 grid, hipStream_t st
     // launch's time: eight waves a block halve it.  Two waves of one block keep
     // step on their SIMD, though, where those of two blocks fill each other's
     // gaps, so that it pays up to two four-wave blocks a CU only, and not for
-    // short sequences.  Four waves against eight, causal, head_dim 128: 2048
-    // tokens, 32 heads over 8, 59 / 57 us, 16 heads 50 / 40, 8 heads over 1 47 /
-    // 37, 8192 tokens of those 195 / 163, 1024 tokens 28 / 24; 3000 tokens of 32
-    // heads 90 / 101, 16 sequences of 128 15 / 21; head_dim 32, 2048 tokens 27 / 23.
+    // short sequences.  Four waves against eight, causal, head_dim 128, 32 heads
+    // over 8: 1024 tokens 30 / 26 us, 1536 44 / 37, 1792 49 / 44, 2048 (two blocks
+    // a CU) 55 / 51, 2304 62 / 67, 2560 71 / 78, 3000 86 / 98; 8 heads over 1:
+    // 2048 46 / 36, 4096 88 / 66, 8192 (two blocks a CU) 189 / 147; 16 sequences of
+    // 128 15 / 21; head_dim 32, 2048 tokens 27 / 23.  Lengths are known here by
+    // their mean alone: 4096 tokens beside 30 single ones, 8 heads over 1, stay
+    // with four waves, 88 / 65.
     const bool split = a.N * a.Hq / kPtRows <= 2 * device_cus() && a.N >= (int64_t)1024 * a.B;
     const dim3 one(64 * kPtWaves), two(2 * 64 * kPtWaves);
     if (a.olo.p && split) hipLaunchKernelGGL((prompt_forward_kernel<DT, D, true, 2>), grid, two, 0, st, a);
@@ -1312,6 +1317,7 @@ static int prompt_launch_backward(const PromptArgs &a, hipStream_t st) {
 // blocks a CU: 2048 tokens 283 / 185 / 185 us, 4096 628 / 508 / 528, nine
 // sequences of 20 to 3000 tokens 498 / 451 / 499, 8192 1829 / 1832 / 1842;
 // 4096 without a mask 893 / 916 / 939.
+// Halves only: a group of 3, 5 or 7 heads stays whole, one of 6 is two parts.
 static int prompt_parts(int64_t N, int64_t B, int Hq, int Hkv) {
     const int G = Hq / Hkv;
     const int64_t blocks = (N / kPtKvKeys + B) * Hkv;

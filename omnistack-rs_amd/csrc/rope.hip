@@ -13,10 +13,11 @@
 // Angles: a frequency is held as a 64-bit fraction of a turn per position,
 // round(freq / 2 pi * 2^64), so that the low 64 bits of the integer product
 // with a position are the angle's fraction of a turn, the whole turns gone by
-// overflow and exact at any position (2^-65 turns per position; a table of
-// cosines would be 512 B a position at D = 128 and end at some length).  Its
-// top 32 bits give the quadrant and a remainder within pi / 4, where Taylor
-// polynomials of degree 9 and 10 err by less than 2e-9.
+// overflow.  The product is exact; the frequency's rounding costs |position|
+// 2^-65 turns, 2e-7 radians at 2^40, about what the fp32 cosine errs by, and 2e-4
+// at 2^50 (a table of cosines would be 512 B a position at D = 128 and end at
+// some length).  Its top 32 bits give the quadrant and a remainder within pi / 4,
+// where Taylor polynomials of degree 9 and 10 err by less than 2e-9.
 //
 // Bound by memory: 2 x 2 B an element.  A wave takes a token (or some of its
 // heads where tokens are few): a lane holds 16 B of a head, the wave's 64 lanes
@@ -505,7 +506,8 @@ static int rope_args(const char *who, int dtype, int64_t B, int64_t T, int Hq, i
     OMNI_CHECK_ARG(dtype_ok(dtype) && dtype_ok(w_dtype), "%s: bad dtype", who);
     OMNI_CHECK_ARG(D == 32 || D == 64 || D == 128 || D == 256, "%s: head_dim must be 32, 64, 128 or 256, got %d", who, D);
     OMNI_CHECK_ARG(B >= 0 && T >= 0 && Hq > 0 && Hkv > 0, "%s: bad shape", who);
-    // 2^24 heads a token and 2^40 tokens are far past any memory; their products stay below 2^63
+    // far past any memory.  A token is cut into parts only where tokens are fewer than 8 a CU
+    // (rope_split), so that units stay near 2^40
     OMNI_CHECK_ARG(Hq <= (1 << 24) && Hkv <= (1 << 24) && (T == 0 || B <= (int64_t(1) << 40) / T), "%s: shape too large", who);
     const int unit = dtype == OMNI_F32 ? 8 : 16;
     OMNI_CHECK_ARG(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % unit == 0,

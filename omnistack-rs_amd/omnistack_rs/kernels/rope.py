@@ -11,8 +11,10 @@ the end:
     (z_i, z_i') turned by positions[axis_i] * inv_freq_i
 
 over the pairs of the first ``rotary_dim`` dims; dims behind them keep z.
-Positions may be any integers, as far apart as 64 bits go: angles are exact
-fractions of a turn.
+Positions are integers of 32 or 64 bits.  An angle is an integer product, its
+whole turns gone by overflow; the frequency's rounding costs |position| 2^-65
+turns, 2e-7 radians at 2^40 (about what fp32 cosines err by), 2e-4 at 2^50 and
+0.2 at 2^60.
 """
 from __future__ import annotations
 
@@ -221,8 +223,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     without them heads are rotated only.  Returns (q', k') in the inputs' dtype,
     contiguous, or ``out`` (two tensors of the inputs' shapes; the inputs
     themselves turn in place).  Gradients for q, k and the weights, once and in
-    reverse mode (dual tensors are refused); ``out`` is for calls that need
-    none.  Forward and backward can be captured in a HIP graph once no eager
+    reverse mode (dual tensors are refused), all of them whichever are asked
+    for; ``out`` is for calls that need none.  Forward and backward can be captured in a HIP graph once no eager
     autograd graph of the same leaves is alive: one through these operators on
     the default stream is refused, as is one of leaves passed to them directly."""
     eps = float(eps)
