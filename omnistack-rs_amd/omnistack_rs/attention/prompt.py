@@ -123,25 +123,25 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """softmax(scale q k^T) v within each packed sequence.
 
     q (N, n_heads, head_dim), k and v (N, n_kv_heads, head_dim): float16 or
-    bfloat16, head_dim 32, 64 or 128, any strides (slices of a fused
-    projection are read in place).  ``cu_seqlens`` (n_sequences + 1,): where
-    each sequence starts and the last one ends, int32 or int64 on the device or
-    on the host; lengths of zero are fine.  ``causal``: token t sees tokens up
-    to t of its sequence.  Returns (N, n_heads, head_dim) in q's dtype, and
-    with ``return_lse`` the rows' log of summed exponentials, float32
-    (n_heads, N; it has no gradient).  Scores are fp32 numbers: one of size X is
-    off by about 2^-24 X, and the gradient's probabilities by as much of
-    themselves; past 2^23 gradients have no meaning and outputs may not be
-    finite.  Gradients for q, k and v, once and in reverse mode (dual
-    tensors are refused), all three whichever are asked for; forward and
-    backward can be captured in a HIP graph (``validate`` off, cu_seqlens on the device) once no
-    eager autograd graph of the same leaves is alive: one through these
-    operators on the default stream is refused, as is one of leaves passed to
-    them directly.  Rows behind the last sequence are zeros (lse -inf); in
-    ``out``, a tensor to write into (no gradient then), they stay as they were.  ``validate`` checks cu_seqlens on the host: a device
-    sync when it is on the device, some 25 us a call.  (On the host it is always
-    checked, and copied to the device.)  Without it values that break the rules
-    give rows of no meaning."""
+    bfloat16, head_dim 32, 64 or 128, any strides (slices of a fused projection
+    are read in place). ``cu_seqlens`` (n_sequences + 1,): where each sequence
+    starts and the last one ends, int32 or int64 on the device or on the host;
+    lengths of zero are fine. ``causal``: token t sees tokens up to t of its
+    sequence. Returns (N, n_heads, head_dim) in q's dtype, and with
+    ``return_lse`` the rows' log of summed exponentials, float32 (n_heads, N;
+    it has no gradient). Scores are fp32 numbers: one of size X is off by about
+    2^-24 X, and the gradient's probabilities by as much of themselves; past
+    2^23 gradients have no meaning and outputs may not be finite. Gradients for
+    q, k and v, once and in reverse mode (dual tensors are refused), all three
+    whichever are asked for; forward and backward can be captured in a HIP
+    graph (``validate`` off, cu_seqlens on the device) once no eager autograd
+    graph of the same leaves is alive: one through these operators on the
+    default stream is refused, as is one of leaves passed to them directly.
+    Rows behind the last sequence are zeros (lse -inf); in ``out``, a tensor to
+    write into (no gradient then), they stay as they were. ``validate`` checks
+    cu_seqlens on the host: a device sync when it is on the device, some 25 us
+    a call. (On the host it is always checked, and copied to the device.)
+    Without it values that break the rules give rows of no meaning."""
     _lib.refuse_tangents("prompt_attention", q, k, v, out)
     dev, cu, scale = _check(q, k, v, cu_seqlens, scale, validate)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)

@@ -214,19 +214,20 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
     """Norm (with weights) and position rotation of q and k, one launch.
 
     q (N, n_heads, head_dim) and k (N, n_kv_heads, head_dim), tokens packed, or
-    (B, heads, T, head_dim), the layout of the cache's encoder; float32, float16
-    or bfloat16, any strides (slices of a fused projection's output are read in
-    place; a last dim that is not contiguous, or rows off 16 bytes, are copied
-    first).  ``positions`` int32 or int64, broadcast to (n_axes, N) or
+    (B, heads, T, head_dim), the layout of the cache's encoder; float32,
+    float16 or bfloat16, any strides (slices of a fused projection's output are
+    read in place; a last dim that is not contiguous, or rows off 16 bytes, are
+    copied first). ``positions`` int32 or int64, broadcast to (n_axes, N) or
     (n_axes, B, T): one row for text, one per axis for images and video, or one
-    for all axes.  ``q_weight`` / ``k_weight`` (head_dim,): the norms' weights;
-    without them heads are rotated only.  Returns (q', k') in the inputs' dtype,
+    for all axes. ``q_weight`` / ``k_weight`` (head_dim,): the norms' weights;
+    without them heads are rotated only. Returns (q', k') in the inputs' dtype,
     contiguous, or ``out`` (two tensors of the inputs' shapes; the inputs
-    themselves turn in place).  Gradients for q, k and the weights, once and in
+    themselves turn in place). Gradients for q, k and the weights, once and in
     reverse mode (dual tensors are refused), all of them whichever are asked
-    for; ``out`` is for calls that need none.  Forward and backward can be captured in a HIP graph once no eager
-    autograd graph of the same leaves is alive: one through these operators on
-    the default stream is refused, as is one of leaves passed to them directly."""
+    for; ``out`` is for calls that need none. Forward and backward can be
+    captured in a HIP graph once no eager autograd graph of the same leaves is
+    alive: one through these operators on the default stream is refused, as is
+    one of leaves passed to them directly."""
     eps = float(eps)
     _lib.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, *(() if out is None else out))
     dev, rows, pos = _check(q, k, positions, rotary, q_weight, k_weight, eps)
