@@ -514,6 +514,110 @@ int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const voi
                               void *stream);
 
 /*
+ * Attention of drafted tokens over the paged cache (no counterpart in the
+ * reference): sequence b holds seq_lens[b] tokens, the last n_draft[b] of them
+ * (NULL: T) drafted and already in the cache; query token t of b is drafted
+ * token t.  It sees every token before the drafted ones and drafted token j
+ * where bit j of tree[b * tree_stride + t] is set (tree_stride 0: one tree for
+ * all).  q and out (B, Hq, T, 128) f16 or bf16, T 1 .. 64, 16-byte aligned,
+ * sign_flip 8-byte aligned; the pool, page table and codebooks as for
+ * omni_attn_paged, with up to 2^31 token rows (n_pages * Hkv * page_size).
+ * Products in fp16 with fp32 sums (f16 queries: two fp16 terms of q and of the
+ * centroids); a rotated row is not rounded to q's type.  Rows t >= n_draft[b]
+ * are zeros; a row that sees nothing, every row of a sequence whose lengths do
+ * not fit (0 <= n_draft <= T, n_draft <= length <= max_pages * page_size) or
+ * that reaches a page outside the pool is NaN.  workspace (16-byte aligned):
+ * omni_attn_tree_workspace_size(...) bytes.  The same bits on every run.
+ */
+size_t omni_attn_tree_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int64_t max_pages, int page_size,
+                                     int q_dtype);
+int omni_attn_tree(const void *q, int q_dtype, const uint8_t *k_nib, const uint8_t *k_qjl, const float *k_norms,
+                   const uint8_t *v_nib, int64_t n_pages, int page_size, const int32_t *page_table,
+                   int64_t max_pages, const int32_t *seq_lens, const int32_t *n_draft, const int64_t *tree,
+                   int64_t tree_stride, const float *codebooks, int per_head_codebook, const uint32_t *g_bits,
+                   int64_t B, int Hq, int Hkv, int64_t T, int head_dim, float scale, int with_qjl, int rotate_q,
+                   const int8_t *sign_flip, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Bounds of the blocks (pages) that hold tokens start[b] .. end[b] - 1 of
+ * sequence b (end NULL: start[b] + count): byte d of bounds (n_pages, Hkv, 128)
+ * is lo | hi << 4, the least and largest key code of dim d over the page's
+ * tokens before end[b].  Positions outside the table and pages outside the
+ * pool are passed over.
+ */
+int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t n_pages, int Hkv, int page_size,
+                      const int32_t *page_table, int64_t max_pages, const int32_t *start, const int32_t *end,
+                      int64_t count, int64_t B, void *stream);
+
+/*
+ * The blocks that each query reads: query t of sequence b sees the first
+ * seq_lens[b] - T + t + 1 tokens.  Of their blocks the first `first` and the
+ * last `recent` are taken, and those of the largest scores up to `top` in all
+ * (all of them where there are no more): whole numbers
+ *   sum_d Q+_d c[hi_d] - Q-_d c[lo_d],  Q+- = sum of max(+-q, 0) over the group's heads,
+ * Q and the head's centroids each times the power of two that brings their
+ * largest into [64, 128), rounded to whole numbers (127 at most); the lower
+ * block wins a tie, and a page outside the pool is taken first.  With codebooks
+ * that ascend this bounds the group's summed scores (without residual signs)
+ * from above.  blocks (B, Hkv, T, top) int32: ascending, -1 behind the last.
+ * q as for omni_attn_tree.  workspace (16-byte aligned):
+ * omni_block_select_workspace_size(...) bytes.
+ */
+size_t omni_block_select_workspace_size(int64_t B, int Hkv, int64_t T, int64_t max_pages, int top);
+int omni_block_select(const void *q, int q_dtype, const uint8_t *bounds, int64_t n_pages, int page_size,
+                      const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens, const float *codebooks,
+                      int per_head_codebook, int64_t B, int Hq, int Hkv, int64_t T, int head_dim, int top, int first,
+                      int recent, int rotate_q, const int8_t *sign_flip, int32_t *blocks, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/*
+ * Attention over selected blocks: query t of sequence b sees those of its
+ * first seq_lens[b] - T + t + 1 tokens that lie in blocks[b][kv head][t][0 ..
+ * top) (numbers outside the sequence's blocks are passed over; one named twice
+ * counts twice).  Everything else as omni_attn_tree.
+ */
+size_t omni_attn_blocks_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int top, int page_size, int q_dtype);
+int omni_attn_blocks(const void *q, int q_dtype, const uint8_t *k_nib, const uint8_t *k_qjl, const float *k_norms,
+                     const uint8_t *v_nib, int64_t n_pages, int page_size, const int32_t *page_table,
+                     int64_t max_pages, const int32_t *seq_lens, const int32_t *blocks, int top,
+                     const float *codebooks, int per_head_codebook, const uint32_t *g_bits, int64_t B, int Hq,
+                     int Hkv, int64_t T, int head_dim, float scale, int with_qjl, int rotate_q,
+                     const int8_t *sign_flip, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Prepared omni_attn_tree (bounds NULL) or omni_block_select followed by
+ * omni_attn_blocks (bounds given; one workspace for both, the larger of their
+ * sizes): the static arguments stored once, pointers kept and not copied.
+ * Each run has every argument check of the calls it makes.  Read-only once
+ * created; omni_attn_pages_plan_destroy frees it.
+ */
+typedef struct omni_attn_pages_plan omni_attn_pages_plan;
+int omni_attn_pages_plan_create(int q_dtype, const uint8_t *k_nib, const uint8_t *k_qjl, const float *k_norms,
+                                const uint8_t *v_nib, const uint8_t *bounds, int64_t n_pages, int page_size,
+                                int64_t max_pages, int32_t *blocks, int top, int first, int recent,
+                                const float *codebooks, int per_head_codebook, const uint32_t *g_bits, int64_t B,
+                                int Hq, int Hkv, int64_t T, float scale, int with_qjl, int rotate_q,
+                                const int8_t *sign_flip, void *out, void *workspace, size_t workspace_bytes,
+                                omni_attn_pages_plan **plan);
+int omni_attn_tree_plan_run(const omni_attn_pages_plan *plan, const void *q, const int32_t *page_table,
+                            const int32_t *seq_lens, const int64_t *tree, int64_t tree_stride,
+                            const int32_t *n_draft, void *stream);
+int omni_attn_blocks_plan_run(const omni_attn_pages_plan *plan, const void *q, const int32_t *page_table,
+                              const int32_t *seq_lens, void *stream);
+void omni_attn_pages_plan_destroy(omni_attn_pages_plan *plan);
+
+/*
+ * Accepted drafted tokens: for j < K, the cached token at position positions[b]
+ * + kept[b * K + j] (0 .. 63, others are passed over) moves to positions[b] + j,
+ * K's codes, signs and norm and V's codes; all are read before any is written.
+ * Positions outside the table and pages outside the pool are passed over.
+ * bounds (or NULL): brought up to date, of the tokens up to the last kept one.
+ */
+int omni_cache_keep(uint8_t *k_nib, uint8_t *k_qjl, float *k_norms, uint8_t *v_nib, uint8_t *bounds,
+                    int64_t n_pages, int Hkv, int page_size, const int32_t *page_table, int64_t max_pages,
+                    const int32_t *positions, const int32_t *kept, int64_t B, int K, void *stream);
+
+/*
  * Measurement helper with no counterpart in the reference: streams `bytes`
  * (a multiple of 16, 16-byte aligned device buffer) once with n_partials
  * blocks and writes one XOR fold per block to partials[0 .. n_partials),

@@ -25,6 +25,7 @@ LIB = os.path.join(OUT_DIR, "libomnistack_amd.so")
 
 ARCH = os.environ.get("OMNI_OFFLOAD_ARCH", "gfx950")
 SOURCES = ["host_api.cpp", "codec.hip", "attn.hip", "lora.hip", "calib.hip", "calib_inplace.hip", "dense.hip", "rope.hip", "prompt.hip",
+           "pages.hip", "blocks.hip",
            "probe.hip"]
 
 

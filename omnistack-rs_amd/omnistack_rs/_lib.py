@@ -94,6 +94,25 @@ SIGNATURES = {
     "omni_prompt_attn_backward": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp,
                                            _c_i64, _c_f32, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                            _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "omni_attn_tree_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int]),
+    "omni_attn_tree": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_int, _vp, _c_i64, _vp, _vp, _vp, _c_i64,
+                                _vp, _c_int, _vp, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_f32, _c_int, _c_int, _vp,
+                                _vp, _vp, _c_sz, _vp]),
+    "omni_block_bounds": (_c_int, [_vp, _vp, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "omni_block_select_workspace_size": (_c_sz, [_c_i64, _c_int, _c_i64, _c_i64, _c_int]),
+    "omni_block_select": (_c_int, [_vp, _c_int, _vp, _c_i64, _c_int, _vp, _c_i64, _vp, _vp, _c_int, _c_i64, _c_int,
+                                   _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_sz, _vp]),
+    "omni_attn_blocks_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_int]),
+    "omni_attn_blocks": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_int, _vp, _c_i64, _vp, _vp, _c_int,
+                                  _vp, _c_int, _vp, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_f32, _c_int, _c_int, _vp,
+                                  _vp, _vp, _c_sz, _vp]),
+    "omni_attn_pages_plan_create": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_int, _c_i64, _vp, _c_int, _c_int,
+                                             _c_int, _vp, _c_int, _vp, _c_i64, _c_int, _c_int, _c_i64, _c_f32, _c_int,
+                                             _c_int, _vp, _vp, _vp, _c_sz, ctypes.POINTER(_vp)]),
+    "omni_attn_tree_plan_run": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_i64, _vp, _vp]),
+    "omni_attn_blocks_plan_run": (_c_int, [_vp, _vp, _vp, _vp, _vp]),
+    "omni_attn_pages_plan_destroy": (None, [_vp]),
+    "omni_cache_keep": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp, _vp, _c_i64, _c_int, _vp]),
     "omni_hbm_read_probe": (_c_int, [_vp, _c_sz, _vp, _c_int, _vp]),
     "omni_attn_noalloc_scratch_bytes": (_c_sz, []),
     "omni_attn_noalloc": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_int, _vp,

@@ -39,10 +39,15 @@ class PagedKVCache:
     ``free(pages)`` returns them, ``write(pages, ...)`` copies a contiguous
     packed sequence (the encoder's output for one batch entry) into them,
     ``page_table(...)`` builds the int32 table ``paged_attention`` reads.
+    ``keep(...)`` moves accepted drafted tokens to the front of the drafted
+    ones.  With ``bounds``, ``k_bounds`` (n_pages, n_kv_heads, head_dim) uint8
+    holds each page's least key code of a dim in the low nibble and the largest
+    in the high one, which ``write``, ``append`` and ``keep`` follow
+    (``update_bounds`` after any other change).
     """
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 16, head_dim: int = HEAD_DIM,
-                 device="cuda"):
+                 device="cuda", bounds: bool = False):
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two in [16, 1024], got {page_size}")
         if n_pages < 1 or n_kv_heads < 1:
@@ -56,6 +61,7 @@ class PagedKVCache:
         self.k_qjl = torch.zeros(*shape, head_dim // 16, dtype=torch.uint8, device=dev)
         self.k_norms = torch.zeros(*shape, dtype=torch.float32, device=dev)
         self.v_nibbles = torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=dev)
+        self.k_bounds = torch.zeros(n_pages, n_kv_heads, head_dim, dtype=torch.uint8, device=dev) if bounds else None
         self._free = list(range(n_pages - 1, -1, -1))
 
     @property
@@ -106,6 +112,73 @@ class PagedKVCache:
         for pool, src in ((self.k_nibbles, k_nibbles), (self.k_qjl, k_qjl), (self.k_norms, k_norms),
                           (self.v_nibbles, v_nibbles)):
             pool[pg, :, slot] = src.to(device=self.device, dtype=pool.dtype).transpose(0, 1)
+        if self.k_bounds is not None and S:
+            where = torch.tensor([start, start + S], dtype=torch.int32, device=self.device)
+            self.update_bounds(self.page_table([pages]), where[:1], where[1:])
+
+    def update_bounds(self, page_table: torch.Tensor, start: torch.Tensor, end: torch.Tensor) -> None:
+        """``k_bounds`` of the pages that hold tokens start[b] .. end[b] - 1 of the
+        sequences in ``page_table``, from their tokens before end[b] (int32 on the
+        pool's device; positions outside the table and pages outside the pool are
+        passed over)."""
+        pt = self._check_rows(page_table, (("start", start), ("end", end)))
+        self._bounds(pt, start.contiguous(), end.contiguous(), 0)
+
+    def _check_rows(self, page_table, columns):
+        if page_table.dim() != 2 or page_table.shape[1] < 1 or page_table.dtype != torch.int32:
+            raise ValueError(f"page_table must be int32 (B, max_pages), got {page_table.dtype} {tuple(page_table.shape)}")
+        for name, t in columns:
+            if tuple(t.shape) != (page_table.shape[0],) or t.dtype != torch.int32:
+                raise ValueError(f"{name} must be int32 ({page_table.shape[0]},), got {t.dtype} {tuple(t.shape)}")
+        if any(t.device != self.device for t in (page_table, *(t for _, t in columns))):
+            raise ValueError(f"inputs must be on {self.device}")
+        return page_table.contiguous()
+
+    def _bounds(self, pt, start, end, count) -> None:
+        if self.k_bounds is None:
+            raise ValueError("this cache keeps no bounds: make it with PagedKVCache(..., bounds=True)")
+        _lib.require_device(self.k_nibbles)
+        _lib.check(_lib.on_device(
+            self.device, _lib.lib().omni_block_bounds, _lib.ptr(self.k_nibbles), _lib.ptr(self.k_bounds), self.n_pages,
+            self.n_kv_heads, self.page_size, _lib.ptr(pt), pt.shape[1], _lib.ptr(start), _lib.ptr(end), count, pt.shape[0],
+            _lib.stream_of(self.device)))
+
+    def keep(self, page_table: torch.Tensor, positions: torch.Tensor, kept: torch.Tensor, validate: bool = True) -> None:
+        """Accepted drafted tokens, to the front: the token at position
+        positions[b] + kept[b, j] of sequence b moves to positions[b] + j (int32
+        (B,) and (B, K), K <= 64; entries outside [0, 64) are passed over: pad
+        with -1).  All are read before any is written, so any order will do.  The
+        caller sets its sequence lengths to positions[b] + the number accepted.
+        Sequences must not share the pages concerned.  ``validate`` checks the
+        positions on the host (a device sync); without it tokens outside the
+        table or the pool are passed over."""
+        if kept.dim() != 2 or kept.shape[0] != page_table.shape[0] or kept.shape[1] > 64 or kept.dtype != torch.int32:
+            raise ValueError(f"kept must be int32 (B, K), K at most 64, got {kept.dtype} {tuple(kept.shape)}")
+        pt = self._check_rows(page_table, (("positions", positions),))
+        if kept.device != self.device:
+            raise ValueError(f"inputs must be on {self.device}")
+        _lib.require_device(self.k_nibbles)
+        B, K = kept.shape
+        if B == 0 or K == 0:
+            return
+        kc, pos = kept.contiguous(), positions.contiguous()
+        if validate:
+            kh, ph, ps = kc.cpu().to(torch.int64), pos.cpu().to(torch.int64), self.page_size
+            if bool((kh >= 64).any()):
+                raise ValueError("kept must lie below 64 (negative: none)")
+            far = torch.where(kh >= 0, torch.maximum(kh, torch.arange(K)[None, :]), 0).amax(1)
+            if bool(((ph < 0) | (ph + far >= pt.shape[1] * ps))[(kh >= 0).any(1)].any()):
+                raise ValueError(f"positions + kept must lie in [0, {pt.shape[1] * ps})")
+            ids, cols = pt.cpu().to(torch.int64), torch.arange(pt.shape[1])
+            touched = (cols[None, :] >= (ph // ps)[:, None]) & (cols[None, :] <= ((ph + far) // ps)[:, None])
+            bad = touched & (kh >= 0).any(1)[:, None] & ((ids < 0) | (ids >= self.n_pages))
+            if bool(bad.any()):
+                b, c = (int(x) for x in bad.nonzero()[0])
+                raise IndexError(f"page_table[{b}, {c}] = {int(ids[b, c])} lies outside the pool of {self.n_pages} pages")
+        _lib.check(_lib.on_device(
+            self.device, _lib.lib().omni_cache_keep, _lib.ptr(self.k_nibbles), _lib.ptr(self.k_qjl), _lib.ptr(self.k_norms),
+            _lib.ptr(self.v_nibbles), _lib.ptr(self.k_bounds), self.n_pages, self.n_kv_heads, self.page_size, _lib.ptr(pt),
+            pt.shape[1], _lib.ptr(pos), _lib.ptr(kc), B, K, _lib.stream_of(self.device)))
 
     def append(self, encoder, k: torch.Tensor, v: Optional[torch.Tensor], page_table: torch.Tensor,
                positions: torch.Tensor, validate: bool = True) -> None:
@@ -170,6 +243,8 @@ class PagedKVCache:
             _lib.ptr(encoder.cb), encoder.per_head, _lib.ptr(encoder.gb), _lib.ptr(encoder.tables),
             encoder.tables_bytes, _lib.ptr(pt), mp, _lib.ptr(pos), self.n_pages, ps, _lib.ptr(self.k_nibbles),
             _lib.ptr(self.k_qjl), _lib.ptr(self.k_norms), _lib.ptr(self.v_nibbles), _lib.stream_of(self.device)))
+        if self.k_bounds is not None:
+            self._bounds(pt, pos, None, T)
 
     def page_table(self, sequences: Sequence[Sequence[int]], max_pages: Optional[int] = None) -> torch.Tensor:
         """int32 (len(sequences), max_pages) table; unused entries are -1."""
@@ -184,14 +259,14 @@ class PagedKVCache:
     @classmethod
     def from_contiguous(cls, k_nibbles, k_qjl, k_norms, v_nibbles, page_size: int = 16,
                         seq_lens: Optional[Sequence[int]] = None, spare_pages: int = 0,
-                        generator: Optional[torch.Generator] = None):
+                        generator: Optional[torch.Generator] = None, bounds: bool = False):
         """Pages for a contiguous packed cache (B, n_kv_heads, S, ...): returns
         (cache, page_table, seq_lens).  Pages are assigned in a random order
         (``generator``), so no sequence's pages are contiguous or in order."""
         B, H, S, nb = k_nibbles.shape
         lens = [S] * B if seq_lens is None else [int(x) for x in seq_lens]
         need = sum((L + page_size - 1) // page_size for L in lens)
-        cache = cls(need + spare_pages, H, page_size, 2 * nb, device=k_nibbles.device)
+        cache = cls(need + spare_pages, H, page_size, 2 * nb, device=k_nibbles.device, bounds=bounds)
         order = torch.randperm(cache.n_pages, generator=generator).tolist()
         cache._free = list(reversed(order))
         seqs = []
