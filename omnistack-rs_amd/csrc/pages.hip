@@ -61,20 +61,27 @@ struct PageAttnArgs {
 
 constexpr int kPgTile = 32;
 constexpr int kPartRow = 128 + 4;            // floats of a split's row: O, then m and l
-constexpr int kLutBytes = 65536;             // [byte][256 B]: 64 columns of 4 B (HL: 32 of 8 B)
-constexpr int kSignOff = kLutBytes;          // [nibble][256 B]: 32 columns of four +-1.0 halves
-constexpr int kQimgOff = kSignOff + 4096;
+constexpr int kLutBytes = 65536;             // [byte][256 B]: 32 columns of 8 B
+constexpr int kQimgOff = kLutBytes;
+constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dword 3
 
-template <int NR, int NW, bool QJL, bool HL>
-struct PgLds {
-    static constexpr int kSteps = QJL ? 6 : 4;                               // B operands of a row group: q, then G q
-    static constexpr int kQimg = NR * kSteps * (HL ? 2 : 1) * 1024;
+// What a variant keeps where.  NR: groups of 16 query rows a block; HL: fp16
+// queries.
+template <int NR, bool QJL, bool HL>
+struct Pg {
+    static constexpr int NW = NR == 1 && !HL ? 12 : 8;                       // waves
+    static constexpr bool kQReg = NR <= 2;                                   // query operands in registers (else LDS)
+    static constexpr bool kAhead = NR <= 2;                                  // a wave forms the next tile's scores beside a tile's weights
+    static constexpr int kQSteps = HL ? 16 : 4;                              // B operands of a row group: q (HL: twice eight),
+    static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
+    static constexpr int kSteps = kQSteps + kGSteps;
+    static constexpr int kQimg = NR * kSteps * 1024;
     static constexpr int kCsc = kQimgOff + kQimg;                            // per row: score scale
-    static constexpr int kBad = kCsc + NR * 16 * 4;                          // per wave: met a page outside the pool
-    static constexpr int kUse = kBad + NW * 4;
-    static constexpr int kSlabs = NW * 16 * kPartRow * 4;                    // epilogue: the waves' O of one row group
-    static constexpr int kMl = kSlabs;                                       // then their m and l
-    static constexpr int kTotal = kUse > kMl + NW * 32 * 4 + NW * 4 ? kUse : kMl + NW * 32 * 4 + NW * 4;
+    static constexpr int kSees = kCsc + NR * 16 * 4;                         // per row: its tree mask
+    static constexpr int kUse = kSees + NR * 16 * 8;
+    static constexpr int kSlabs = NW * 16 * kPartRow * 4;                    // epilogue: the waves' O of one row group,
+    static constexpr int kMerge = kSlabs + NW * 32 * 4 + NW * 4;             // their m and l, a flag per wave
+    static constexpr int kLds = kUse > kMerge ? kUse : kMerge;
 };
 
 __device__ __forceinline__ uint32_t pg_pack(float x, float y) {
@@ -89,22 +96,17 @@ __device__ __forceinline__ half8_t pg_half8(uint32_t a, uint32_t b, uint32_t c, 
 __device__ __forceinline__ float4_t pg_mfma(half8_t a, half8_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ float pg_max(float a, float b) {           // as fmaxf, without quieting its operands first
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
+// The larger, or NaN if one is: single instructions (fmaxf quiets operands
+// first that the compiler cannot prove quiet, such as a matrix product's).
 __device__ __forceinline__ float pg_max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 // over lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float pg_max_groups(float m) {
     auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = pg_max(__uint_as_float(t[0]), __uint_as_float(t[1]));
+    m = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
     auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return pg_max(__uint_as_float(u[0]), __uint_as_float(u[1]));
+    return fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
 }
 __device__ __forceinline__ float pg_sum_groups(float v) {
     auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -123,17 +125,17 @@ struct PgList {
     bool bad;                    // a length that the table cannot hold, or more drafted tokens than there are
 };
 template <bool BLOCKS>
-__device__ __forceinline__ PgList pg_list(const PageAttnArgs &a, int64_t unit) {
+__device__ __forceinline__ PgList pg_list(const PageAttnArgs &a, uint32_t unit) {
     PgList l;
-    l.hk = (int)(unit % a.Hkv);
-    const int64_t bt = unit / a.Hkv;
-    l.b = BLOCKS ? bt / a.T : bt;
-    l.t = BLOCKS ? (int)(bt - l.b * a.T) : 0;
+    const uint32_t bt = unit / (uint32_t)a.Hkv;
+    l.hk = (int)(unit - bt * (uint32_t)a.Hkv);
+    l.b = BLOCKS ? bt / (uint32_t)a.T : bt;
+    l.t = BLOCKS ? (int)(bt - (uint32_t)l.b * (uint32_t)a.T) : 0;
     const int64_t len = a.seq_lens[l.b];
     l.bad = len < 0 || len > (a.max_pages << a.page_shift);
     if constexpr (BLOCKS) {
         l.nd = a.T;
-        l.seen = l.bad ? 0 : len - a.T + l.t + 1 > 0 ? len - a.T + l.t + 1 : 0;
+        l.seen = l.bad || len - a.T + l.t + 1 < 0 ? 0 : len - a.T + l.t + 1;
         l.base = 0;
         l.tiles = (((int64_t)a.top << (a.page_shift - 4)) + 1) >> 1;
     } else {
@@ -146,36 +148,38 @@ __device__ __forceinline__ PgList pg_list(const PageAttnArgs &a, int64_t unit) {
     return l;
 }
 // tiles of a split: even shares, so the splits of a short list are short
-__device__ __forceinline__ int64_t pg_share(int64_t tiles, int splits) { return (tiles + splits - 1) / splits; }
+__device__ __forceinline__ int64_t pg_share(int64_t tiles, int splits) {
+    return (int64_t)(((uint32_t)tiles + (uint32_t)splits - 1) / (uint32_t)splits);
+}
 
-struct PgTile {
-    uint4 k[2];        // code bytes 16 g .. + 15 of token n of half u
-    uint2 sg[2];       // its sign bytes
-    float4 nr[2];      // norms of tokens 4 g .. + 3
-    uint32_t v[8];     // code bytes 4 n .. + 3 of tokens 16 (i / 4) + 4 g + i % 4
-    int nv[2];         // tokens of each half that the list holds (wave-uniform)
+template <bool HL>
+struct PgKeys {
+    uint4 k[2];                  // code bytes 16 g .. + 15 of token n of half u
+    uint2 sg[2];                 // its sign bytes
+    float nr[2][HL ? 4 : 1];     // its norm; HL: the norms of tokens 4 g .. + 3
+};
+struct PgValues {
+    uint32_t v[8];               // code bytes 4 n .. + 3 of tokens 16 (i / 4) + 4 g + i % 4
 };
 
-template <int NR, int NW, bool QJL, bool HL, bool BLOCKS>
-__global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
-    using L = PgLds<NR, NW, QJL, HL>;
-    constexpr bool F16 = HL;
-    constexpr bool QREG = NR * (HL ? 2 : 1) <= 2;   // query operands in registers (else read from LDS in each tile)
-    __shared__ __attribute__((aligned(16))) unsigned char smem[L::kTotal];
+template <int NR, bool QJL, bool HL, bool BLOCKS>
+__global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(PageAttnArgs a) {
+    using L = Pg<NR, QJL, HL>;
+    constexpr int NW = L::NW;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[L::kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
 
     // block -> (unit, split, row chunk): the chunks of one (unit, split) eight
     // blocks apart, so that they run on one XCD and share its L2
-    const int64_t us_all = a.units * a.splits;
-    const int64_t grp = blockIdx.x / (8 * a.chunks);
-    const int rest = (int)(blockIdx.x - grp * 8 * a.chunks);
-    const int64_t us = grp * 8 + (rest & 7);
-    const int chunk = rest >> 3;
-    if (us >= us_all) return;
-    const int64_t unit = us / a.splits;
-    const int split = (int)(us - unit * a.splits);
+    const uint32_t grp = blockIdx.x / (8u * (uint32_t)a.chunks);
+    const uint32_t rest = blockIdx.x - grp * 8u * (uint32_t)a.chunks;
+    const uint32_t us = grp * 8u + (rest & 7u);
+    const int chunk = (int)(rest >> 3);
+    if (us >= (uint32_t)a.units * (uint32_t)a.splits) return;
+    const uint32_t unit = us / (uint32_t)a.splits;
+    const int split = (int)(us - unit * (uint32_t)a.splits);
     const PgList li = pg_list<BLOCKS>(a, unit);
     const int hk = li.hk;
     const int64_t share = pg_share(li.tiles, a.splits);
@@ -186,58 +190,112 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
     const int cnt = t_end - t_begin > wave ? (int)((t_end - t_begin - wave + NW - 1) / NW) : 0;
     uint32_t row0 = 0, row1 = 0, nvs = 0;
     bool page_bad = false;
-    auto fetch = [&](int first) {
-        uint32_t r[2], v[2];
+    int64_t slot_pos[2], slot_page[2];
+    int32_t slot_id[2];
+    auto fetch_slots = [&](int first) {                      // which tokens, and their page table entries
         const int64_t tile = t_begin + wave + (int64_t)NW * (first + lane);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int64_t half = 2 * tile + u;
-            int64_t pos = half << 4;                         // of its first token
-            int64_t page = half >> (a.page_shift - 4);
+            slot_pos[u] = half << 4;                         // of its first token
+            slot_page[u] = half >> (a.page_shift - 4);
             bool in = first + lane < cnt;
             if constexpr (BLOCKS) {
                 const int64_t nb = (li.seen + (1 << a.page_shift) - 1) >> a.page_shift;
-                in = in && page < a.top;
-                const int64_t blk = in ? a.blocks[((li.b * a.Hkv + hk) * a.T + li.t) * a.top + page] : -1;
-                in = in && blk >= 0 && blk < nb;
-                pos = (blk << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-                page = blk;
+                in = in && slot_page[u] < a.top;
+                const int64_t blk = in ? a.blocks[((li.b * a.Hkv + hk) * a.T + li.t) * a.top + slot_page[u]] : -1;
+                in = blk >= 0 && blk < nb;
+                slot_pos[u] = (blk << a.page_shift) + (slot_pos[u] & ((1 << a.page_shift) - 1));
+                slot_page[u] = blk;
             }
-            const int64_t left = in ? li.seen - pos : 0;
-            v[u] = left <= 0 ? 0u : left < 16 ? (uint32_t)left : 16u;
-            const int32_t id = v[u] ? a.page_table[li.b * a.max_pages + page] : 0;
-            const bool ok = id >= 0 && id < a.n_pages;
+            in = in && slot_pos[u] < li.seen;
+            if (!in) slot_pos[u] = li.seen;
+            slot_id[u] = in ? a.page_table[li.b * a.max_pages + slot_page[u]] : 0;
+        }
+    };
+    auto fetch_rows = [&]() {
+        uint32_t r[2], v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t left = li.seen - slot_pos[u];
+            v[u] = left < 16 ? (uint32_t)left : 16u;
+            const bool ok = slot_id[u] >= 0 && slot_id[u] < a.n_pages;
             page_bad = page_bad || !ok;
-            r[u] = (((uint32_t)(ok ? id : 0) * (uint32_t)a.Hkv + (uint32_t)hk) << a.page_shift) +
-                   (v[u] ? (uint32_t)(pos & ((1 << a.page_shift) - 1)) : 0u);
+            r[u] = (((uint32_t)(ok ? slot_id[u] : 0) * (uint32_t)a.Hkv + (uint32_t)hk) << a.page_shift) +
+                   (v[u] ? (uint32_t)(slot_pos[u] & ((1 << a.page_shift) - 1)) : 0u);
         }
         row0 = r[0];
         row1 = r[1];
         nvs = v[0] | (v[1] << 8);
     };
-    fetch(0);
-    auto load = [&](PgTile &R, int k) {
-        if ((k & 63) == 0 && k > 0) fetch(k);
-        const uint32_t r[2] = {(uint32_t)__builtin_amdgcn_readlane((int)row0, k & 63),
-                               (uint32_t)__builtin_amdgcn_readlane((int)row1, k & 63)};
-        const int v = __builtin_amdgcn_readlane((int)nvs, k & 63);
-        R.nv[0] = v & 255;
-        R.nv[1] = v >> 8;
+    auto rows_at = [&](int k, uint32_t (&r)[2], int &v) {
+        if ((k & 63) == 0 && k > 0) {
+            fetch_slots(k);
+            fetch_rows();
+        }
+        r[0] = (uint32_t)__builtin_amdgcn_readlane((int)row0, k & 63);
+        r[1] = (uint32_t)__builtin_amdgcn_readlane((int)row1, k & 63);
+        v = __builtin_amdgcn_readlane((int)nvs, k & 63);
+    };
+    // a half's 16 tokens of one array: the descriptor starts at its row, so a
+    // lane's offset is the same for every tile
+    auto half_of = [&](const void *base, uint32_t r, uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(reinterpret_cast<const char *>(base) + (uint64_t)r * bytes), (short)0,
+                                                 (int)(16 * bytes), kBufWord3);
+    };
+    auto load_k = [&](PgKeys<HL> &R, const uint32_t (&r)[2]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            R.k[u] = *reinterpret_cast<const uint4 *>(a.k_nib + (uint64_t)r[u] * 64 + (uint32_t)(64 * n + 16 * g));
-            if (QJL) {
-                R.sg[u] = *reinterpret_cast<const uint2 *>(a.k_qjl + (uint64_t)r[u] * 8 + (uint32_t)(8 * n));
-                R.nr[u] = *reinterpret_cast<const float4 *>(a.k_norms + (uint64_t)r[u] + (uint32_t)(4 * g));
+            R.k[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(half_of(a.k_nib, r[u], 64), 64 * n + 16 * g, 0, 0));
+            if constexpr (QJL) {
+                R.sg[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(half_of(a.k_qjl, r[u], 8), 8 * n, 0, 0));
+                if constexpr (HL) {
+                    const float4 f = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(half_of(a.k_norms, r[u], 4), 16 * g, 0, 0));
+                    R.nr[u][0] = f.x;
+                    R.nr[u][1] = f.y;
+                    R.nr[u][2] = f.z;
+                    R.nr[u][3] = f.w;
+                } else {
+                    R.nr[u][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(half_of(a.k_norms, r[u], 4), 4 * n, 0, 0));
+                }
             }
-            const uint8_t *vp = a.v_nib + (uint64_t)r[u] * 64;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                R.v[4 * u + i] = *reinterpret_cast<const uint32_t *>(vp + (uint32_t)(64 * (4 * g + i) + 4 * n));
         }
     };
-    PgTile R0, R1;
-    if (cnt > 0) load(R0, 0);
+    auto load_v = [&](PgValues &R, const uint32_t (&r)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const auto V = half_of(a.v_nib, r[u], 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) R.v[4 * u + i] = __builtin_amdgcn_raw_buffer_load_b32(V, 256 * g + 4 * n + 64 * i, 0, 0);
+        }
+    };
+    auto clamp = [&](int k) { return k < cnt ? k : cnt - 1; };     // past the end: the last tile again, from cache
+    auto load = [&](PgKeys<HL> &K, PgValues &V, int &v, int k) {
+        uint32_t r[2];
+        rows_at(clamp(k), r, v);
+        load_k(K, r);
+        load_v(V, r);
+    };
+    fetch_slots(0);
+
+    // ── the query rows of wave w < NR, on their way ───────────────────
+    const bool rows_mine = wave < NR;
+    const int q_rho = (chunk * NR + wave) * 16 + n;
+    uint4 q_raw[4];
+    uint2 q_flip[4];
+    uint32_t g_word[4];
+    if (rows_mine) {
+        const int rr = q_rho < a.rows ? q_rho : 0;
+        const int t = BLOCKS ? li.t : (int)((uint32_t)rr / (uint32_t)a.G);
+        const int hq = hk * a.G + (BLOCKS ? rr : rr - t * a.G);
+        const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + ((li.b * a.Hq + hq) * a.T + t) * 128 + 32 * g;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            q_raw[s] = reinterpret_cast<const uint4 *>(src)[s];
+            if (a.sign_flip) q_flip[s] = *reinterpret_cast<const uint2 *>(a.sign_flip + 32 * g + 8 * s);
+            if (QJL) g_word[s] = a.g_bits[((int64_t)hk * 64 + 16 * s + n) * 4 + g];
+        }
+    }
 
     // ── tables ────────────────────────────────────────────────────────
     const float *cbp = a.codebooks + (a.per_head ? hk * 16 : 0);
@@ -247,44 +305,41 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
     int cexp = 0;
     if (cmax > 0.0f && cmax < INFINITY) frexpf(cmax, &cexp);
     cexp = cexp < -100 ? -100 : cexp;
-    const float cmul = ldexpf(1.0f, 10 - cexp), cdiv = ldexpf(1.0f, cexp - 10);
+    // largest centroid in [2^(kc - 1), 2^kc): HL up to 2^10, for the remainders
+    // of small ones; else 1, for norms, which follow them, up to 65504 of it
+    constexpr int kc = HL ? 10 : 0;
+    const float cmul = ldexpf(1.0f, kc - cexp), cdiv = ldexpf(1.0f, cexp - kc);
     for (int m = tid; m < kLutBytes / 16; m += 64 * NW) {
         const int e = m >> 4;
         const float c0 = cbp[e & 15] * cmul, c1 = cbp[e >> 4] * cmul;
-        const uint32_t hi = pg_pack(c0, c1);
-        uint4 w = make_uint4(hi, hi, hi, hi);
-        if (HL) w.y = w.w = pg_pack(c0 - pg_h_lo(hi), c1 - pg_h_hi(hi));
-        *reinterpret_cast<uint4 *>(smem + 16 * m) = w;
-    }
-    if (QJL && tid < 512) {
-        const uint32_t v = (uint32_t)tid >> 5;
-        uint32_t w[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            w[k] = (((v >> (2 * k)) & 1) ? 0x3C00u : 0xBC00u) | ((((v >> (2 * k + 1)) & 1) ? 0x3C00u : 0xBC00u) << 16);
-        *reinterpret_cast<uint2 *>(smem + kSignOff + v * 256u + (tid & 31u) * 8u) = make_uint2(w[0], w[1]);
+        const uint32_t hi = pg_pack(c0, c1), lo = pg_pack(c0 - pg_h_lo(hi), c1 - pg_h_hi(hi));
+        *reinterpret_cast<uint4 *>(smem + 16 * m) = make_uint4(hi, lo, hi, lo);
     }
 
+    // ── the first tiles, on their way ─────────────────────────────────
+    fetch_rows();
+    PgKeys<HL> K0, K1;
+    PgValues V0, V1;
+    int nv0 = 0, nv1 = 0;                                   // tokens of each half that the list holds: low byte, next byte
+    if (cnt > 0) {
+        load(K0, V0, nv0, 0);
+        if constexpr (L::kAhead) load(K1, V1, nv1, 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
     // ── query rows: wave w < NR turns row group w into MFMA operands ──
-    uint4 *qimg = reinterpret_cast<uint4 *>(smem + kQimgOff);      // [rg][step][lane], HL: the remainders a plane on
-    constexpr int kPlane = NR * L::kSteps * 64;
+    uint4 *qimg = reinterpret_cast<uint4 *>(smem + kQimgOff) + (wave < NR ? wave : 0) * L::kSteps * 64 + lane;      // [rg][step][lane]
     float *csc_l = reinterpret_cast<float *>(smem + L::kCsc);
-    if (wave < NR) {
-        const int rho = (chunk * NR + wave) * 16 + n;
-        const bool ok = rho < a.rows;
-        const int rr = ok ? rho : 0;
-        const int t = BLOCKS ? li.t : rr / a.G;
-        const int hq = hk * a.G + (BLOCKS ? rr : rr - t * a.G);
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + ((li.b * a.Hq + hq) * a.T + t) * 128 + 32 * g;
+    if (rows_mine) {
+        const bool ok = q_rho < a.rows;
         float x[4][8];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const uint4 w4 = reinterpret_cast<const uint4 *>(src)[s];
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const uint32_t w[4] = {q_raw[s].x, q_raw[s].y, q_raw[s].z, q_raw[s].w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint16_t h = (uint16_t)((i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
-                x[s][i] = ok ? (F16 ? f16_to_f32(h) : bf16_to_f32(h)) : 0.0f;
+                x[s][i] = ok ? (HL ? f16_to_f32(h) : bf16_to_f32(h)) : 0.0f;
             }
         }
         if (a.rotate) {
@@ -292,13 +347,11 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
             // rounded to q's type in between
             if (a.sign_flip) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const uint2 f = *reinterpret_cast<const uint2 *>(a.sign_flip + 32 * g + 8 * s);
+                for (int s = 0; s < 4; ++s)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         x[s][i] = __uint_as_float(__float_as_uint(x[s][i]) ^
-                                                  (((i < 4 ? f.x >> (8 * i) : f.y >> (8 * i - 32)) & 0x80u) << 24));
-                }
+                                                  (((i < 4 ? q_flip[s].x >> (8 * i) : q_flip[s].y >> (8 * i - 32)) & 0x80u) << 24));
             }
 #pragma unroll
             for (int h = 1; h < 8; h <<= 1)
@@ -345,7 +398,8 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
         if (m > 0.0f && m < INFINITY) frexpf(m, &ex);
         ex = ex < -100 ? -100 : ex;
         const float sr = ldexpf(a.qscale < 0.0f ? -1.0f : 1.0f, 15 - ex);
-        if (g == 0) csc_l[16 * wave + n] = fabsf(a.qscale) * ldexpf(cdiv, ex - 15);
+        // at least FLT_MIN (scores are as good as 0 either way), so that a hidden score's -inf stays one
+        if (g == 0) csc_l[16 * wave + n] = fmaxf(fabsf(a.qscale) * ldexpf(cdiv, ex - 15), __FLT_MIN__);
         half8_t qh[4], ql[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -358,23 +412,29 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
             }
             qh[s] = pg_half8(hw[0], hw[1], hw[2], hw[3]);
             ql[s] = pg_half8(lw[0], lw[1], lw[2], lw[3]);
-            qimg[(wave * L::kSteps + s) * 64 + lane] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-            if (HL) qimg[kPlane + (wave * L::kSteps + s) * 64 + lane] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            if constexpr (HL) {
+                // two bytes of codes a step, centroid and remainder side by side: q, then its remainder, against both
+                qimg[64 * (2 * s)] = make_uint4(hw[0], hw[0], hw[1], hw[1]);
+                qimg[64 * (2 * s + 1)] = make_uint4(hw[2], hw[2], hw[3], hw[3]);
+                qimg[64 * (8 + 2 * s)] = make_uint4(lw[0], lw[0], lw[1], lw[1]);
+                qimg[64 * (8 + 2 * s + 1)] = make_uint4(lw[2], lw[2], lw[3], lw[3]);
+            } else {
+                qimg[64 * s] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            }
         }
         if (QJL) {
             // G q: projections 16 cb + 4 g + i of row n
             float p[4][4];
 #pragma unroll
             for (int cb = 0; cb < 4; ++cb) {
-                const uint32_t w = a.g_bits[((int64_t)hk * 64 + 16 * cb + n) * 4 + g];
                 float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     uint32_t e[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t two = (w >> (8 * s + 2 * j)) & 3u;
-                        e[j] = ((two & 1u) ? 0x3C00u : 0xBC00u) | ((two & 2u) ? 0x3C000000u : 0xBC000000u);
+                        const uint32_t not2 = ~g_word[cb] >> (8 * s + 2 * j);
+                        e[j] = 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
                     }
                     const half8_t ga = pg_half8(e[0], e[1], e[2], e[3]);
                     acc = pg_mfma(ga, qh[s], acc);
@@ -383,191 +443,269 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[cb][i] = acc[i] * a.alpha;
             }
+            // slots 2 j and 2 j + 1 of step s: projections 32 s + 4 g + j and 16 on, whose signs lie 16 bits apart
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 uint32_t hw[4], lw[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float v0 = p[2 * s + (j >> 1)][2 * (j & 1)], v1 = p[2 * s + (j >> 1)][2 * (j & 1) + 1];
-                    hw[j] = pg_pack(v0, v1);
-                    lw[j] = HL ? pg_pack(v0 - pg_h_lo(hw[j]), v1 - pg_h_hi(hw[j])) : 0u;
+                    hw[j] = pg_pack(p[2 * s][j], p[2 * s + 1][j]);
+                    lw[j] = HL ? pg_pack(p[2 * s][j] - pg_h_lo(hw[j]), p[2 * s + 1][j] - pg_h_hi(hw[j])) : 0u;
                 }
-                qimg[(wave * L::kSteps + 4 + s) * 64 + lane] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                if (HL) qimg[kPlane + (wave * L::kSteps + 4 + s) * 64 + lane] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                qimg[64 * (L::kQSteps + s)] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                if (HL) qimg[64 * (L::kQSteps + 2 + s)] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
             }
         }
+    }
+    uint64_t *sees_l = reinterpret_cast<uint64_t *>(smem + L::kSees);    // per row: the drafted tokens that it sees
+    if (!BLOCKS && tid < NR * 16) {
+        const int rho = chunk * NR * 16 + tid;
+        sees_l[tid] = rho < a.rows ? (uint64_t)a.tree[li.b * a.tree_stride + (uint32_t)rho / (uint32_t)a.G] : 0u;
     }
     __syncthreads();
 
     // ── main loop ─────────────────────────────────────────────────────
-    auto qop = [&](int rg, int s, int plane) {
-        return __builtin_bit_cast(half8_t, qimg[plane * kPlane + (rg * L::kSteps + s) * 64 + lane]);
-    };
-    half8_t qr[QREG ? NR : 1][L::kSteps][HL ? 2 : 1];
-    if constexpr (QREG) {
+    uint32_t q_off = kQimgOff + 16 * lane;
+    half8_t qr[L::kQReg ? NR : 1][L::kSteps];
+    if constexpr (L::kQReg) {
 #pragma unroll
         for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
-            for (int s = 0; s < L::kSteps; ++s)
-#pragma unroll
-                for (int p = 0; p < (HL ? 2 : 1); ++p) qr[rg][s][p] = qop(rg, s, p);
+            for (int s = 0; s < L::kSteps; ++s) qr[rg][s] = *reinterpret_cast<const half8_t *>(smem + q_off + (rg * L::kSteps + s) * 1024);
     }
-    auto q_at = [&](int rg, int s, int p) {
-        if constexpr (QREG) return qr[rg][s][p];
-        else return qop(rg, s, p);
+    auto q_at = [&](int rg, int s) {
+        if constexpr (L::kQReg) return qr[rg][s];
+        else return *reinterpret_cast<const half8_t *>(smem + q_off + (rg * L::kSteps + s) * 1024);
     };
     float csc[NR], m_run[NR], l_run[NR];
-    uint64_t sees[NR];
     float4_t oacc[NR][8];
 #pragma unroll
     for (int rg = 0; rg < NR; ++rg) {
         csc[rg] = csc_l[16 * rg + n];
         m_run[rg] = -__FLT_MAX__;        // finite: a tile without a visible key leaves exp2(-inf) = 0
         l_run[rg] = 0.0f;
-        sees[rg] = 0;
-        if constexpr (!BLOCKS) {
-            const int rho = (chunk * NR + rg) * 16 + n;
-            if (rho < a.rows) sees[rg] = (uint64_t)a.tree[li.b * a.tree_stride + rho / a.G];
-        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) oacc[rg][k] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const uint32_t laneoff = HL ? (lane & 31) * 8u : lane * 4u;
-    const uint32_t slane = kSignOff + (lane & 31) * 8u;
+    const uint32_t laneoff = (lane & 31) * 8u;
     const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
-    // table entry of byte k of w: (byte << 8) | the lane's column
+    // table address of byte k of w: (byte << 8) | the lane's column
     auto entry = [&](uint32_t w, int k) {
-        const uint32_t at = __builtin_amdgcn_perm(w, laneoff, 0x0C0C0000u | ((uint32_t)(4 + k) << 8));
-        if constexpr (HL) return *reinterpret_cast<const uint2 *>(smem + at);
-        else return make_uint2(*reinterpret_cast<const uint32_t *>(smem + at), 0u);
+        return smem + __builtin_amdgcn_perm(w, laneoff, 0x0C0C0000u | ((uint32_t)(4 + k) << 8));
     };
-    auto step = [&](const PgTile &R, int64_t tile) {
-        if (BLOCKS && R.nv[0] + R.nv[1] == 0) return;
-        float4_t acc[NR][2], qacc[NR][2];
+    // the fp16 centroids of a word's four bytes
+    auto four_bytes = [&](uint32_t w) {
+        uint32_t h[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int j = 0; j < 4; ++j) h[j] = *reinterpret_cast<const uint32_t *>(entry(w, j));
+        return pg_half8(h[0], h[1], h[2], h[3]);
+    };
+    // centroids and remainders of byte i of x and byte j of y
+    auto two_bytes = [&](uint32_t x, int i, uint32_t y, int j) {
+        const uint2 e0 = *reinterpret_cast<const uint2 *>(entry(x, i)), e1 = *reinterpret_cast<const uint2 *>(entry(y, j));
+        return pg_half8(e0.x, e0.y, e1.x, e1.y);
+    };
+    // scores of a tile, raw: lane (n, g) holds tokens 16 u + 4 g + i of row n
+    auto scores = [&](const PgKeys<HL> &R, float4_t (&acc)[NR][2]) {
+        if constexpr (!L::kQReg) asm volatile("" : "+v"(q_off));       // read again for each tile, not kept (and spilled)
 #pragma unroll
-            for (int rg = 0; rg < NR; ++rg) acc[rg][u] = qacc[rg][u] = float4_t{0.f, 0.f, 0.f, 0.f};
-            const uint32_t kw[4] = {R.k[u].x, R.k[u].y, R.k[u].z, R.k[u].w};
+        for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint2 e[4];
+            for (int u = 0; u < 2; ++u) acc[rg][u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] = entry(kw[s], k);
-                const half8_t ah = pg_half8(e[0].x, e[1].x, e[2].x, e[3].x);
-#pragma unroll
-                for (int rg = 0; rg < NR; ++rg) {
-                    acc[rg][u] = pg_mfma(ah, q_at(rg, s, 0), acc[rg][u]);
-                    if constexpr (HL) {
-                        acc[rg][u] = pg_mfma(ah, q_at(rg, s, 1), acc[rg][u]);
-                        acc[rg][u] = pg_mfma(pg_half8(e[0].y, e[1].y, e[2].y, e[3].y), q_at(rg, s, 0), acc[rg][u]);
-                    }
-                }
-            }
-            if constexpr (QJL) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint32_t w = s ? R.sg[u].y : R.sg[u].x;
-                    const uint2 e0 = *reinterpret_cast<const uint2 *>(smem + ((__builtin_amdgcn_ubfe(w, 4u * g, 4u) << 8) + slane));
-                    const uint2 e1 = *reinterpret_cast<const uint2 *>(smem + ((__builtin_amdgcn_ubfe(w, 16u + 4u * g, 4u) << 8) + slane));
-                    const half8_t sa = pg_half8(e0.x, e0.y, e1.x, e1.y);
-#pragma unroll
-                    for (int rg = 0; rg < NR; ++rg) {
-                        qacc[rg][u] = pg_mfma(sa, q_at(rg, 4 + s, 0), qacc[rg][u]);
-                        if constexpr (HL) qacc[rg][u] = pg_mfma(sa, q_at(rg, 4 + s, 1), qacc[rg][u]);
-                    }
-                }
-            }
-        }
-        float nr[8];
-        if constexpr (QJL) {
+        for (int s = 0; s < (HL ? 8 : 4); ++s) {
+            half8_t A[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                nr[4 * u] = R.nr[u].x * cmul;
-                nr[4 * u + 1] = R.nr[u].y * cmul;
-                nr[4 * u + 2] = R.nr[u].z * cmul;
-                nr[4 * u + 3] = R.nr[u].w * cmul;
+                const uint32_t kw[4] = {R.k[u].x, R.k[u].y, R.k[u].z, R.k[u].w};
+                if constexpr (HL) A[u] = two_bytes(kw[s >> 1], 2 * (s & 1), kw[s >> 1], 2 * (s & 1) + 1);
+                else A[u] = four_bytes(kw[s]);
+            }
+#pragma unroll
+            for (int rg = 0; rg < NR; ++rg)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    acc[rg][u] = pg_mfma(A[u], q_at(rg, s), acc[rg][u]);
+                    if constexpr (HL) acc[rg][u] = pg_mfma(A[u], q_at(rg, 8 + s), acc[rg][u]);
+                }
+        }
+        if constexpr (QJL) {
+            // the signs' part: the norm rides on the signs (fp16, 2^-12 of a
+            // small term), so that it adds to the same sums; HL: +-1, and sums
+            // of its own
+            float4_t qacc[HL ? NR : 1][2];
+            if constexpr (HL) {
+#pragma unroll
+                for (int rg = 0; rg < NR; ++rg) qacc[rg][0] = qacc[rg][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                half8_t A[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t nh = HL ? 0xBC00BC00u : pg_pack(-cmul * R.nr[u][0], -cmul * R.nr[u][0]);
+                    const uint32_t w = (s ? R.sg[u].y : R.sg[u].x) >> (4 * g);
+                    uint32_t e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = ((w << (15 - j)) & 0x80008000u) ^ nh;
+                    A[u] = pg_half8(e[0], e[1], e[2], e[3]);
+                }
+#pragma unroll
+                for (int rg = 0; rg < NR; ++rg)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if constexpr (HL) {
+                            qacc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), qacc[rg][u]);
+                            qacc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + 2 + s), qacc[rg][u]);
+                        } else {
+                            acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), acc[rg][u]);
+                        }
+                    }
+            }
+            if constexpr (HL) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float ni = R.nr[u][i] * cmul;
+#pragma unroll
+                        for (int rg = 0; rg < NR; ++rg) acc[rg][u][i] = __builtin_fmaf(ni, qacc[rg][u][i], acc[rg][u][i]);
+                    }
             }
         }
-        const bool full = R.nv[0] == 16 && R.nv[1] == 16 && (BLOCKS || (tile + 1) * kPgTile <= li.base);
-        half8_t pb[NR];
+    };
+    // Masks, and a row's running maximum raised where some lane's passes it by
+    // 2^8 (P stays within fp16).  m_run is the same in a row's four lane
+    // groups: each lane tests its own maximum, and the row's is formed only
+    // where one does.
+    auto settle = [&](float4_t (&acc)[NR][2], int64_t tile, int v) {
+        const int nv[2] = {v & 255, v >> 8};
+        if (!(v == 16 * 257 && (BLOCKS || (tile + 1) * kPgTile <= li.base))) {
 #pragma unroll
-        for (int rg = 0; rg < NR; ++rg) {
-            float sc[8];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = acc[rg][u][i];
-                    if constexpr (QJL) v = __builtin_fmaf(nr[4 * u + i], qacc[rg][u][i], v);
-                    sc[4 * u + i] = v * csc[rg];
-                }
-            if (!full) {
+            for (int rg = 0; rg < NR; ++rg) {
+                const uint64_t sees = BLOCKS ? 0u : sees_l[16 * rg + n];
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int tok = 4 * g + i;
-                        bool vis = tok < R.nv[u];
+                        bool vis = tok < nv[u];
                         if constexpr (!BLOCKS) {
                             const int64_t j = tile * kPgTile + 16 * u + tok - li.base;
-                            vis = vis && (j < 0 || ((sees[rg] >> (j & 63)) & 1u));
+                            vis = vis && (j < 0 || ((sees >> (j & 63)) & 1u));
                         }
-                        sc[4 * u + i] = vis ? sc[4 * u + i] : -INFINITY;
+                        acc[rg][u][i] = vis ? acc[rg][u][i] : -INFINITY;
                     }
             }
-            // m_run is the same in a row's four lane groups: each lane tests its
-            // own maximum, and the row's is formed only where some lane passes
-            // the old one by 2^8 (P stays within fp16)
-            float mt = pg_max3(pg_max3(sc[0], sc[1], sc[2]), pg_max3(sc[3], sc[4], sc[5]), pg_max(sc[6], sc[7]));
-            if (__builtin_amdgcn_ballot_w64(mt > m_run[rg] + 8.0f)) {
-                mt = pg_max_groups(mt);
-                const bool need = mt > m_run[rg] + 8.0f;
-                const float f = need ? __builtin_amdgcn_exp2f(m_run[rg] - mt) : 1.0f;
-                m_run[rg] = need ? mt : m_run[rg];
+        }
+        float mt[NR];
+        bool any = false;
+#pragma unroll
+        for (int rg = 0; rg < NR; ++rg) {
+            mt[rg] = pg_max3(pg_max3(acc[rg][0][0], acc[rg][0][1], acc[rg][0][2]), pg_max3(acc[rg][0][3], acc[rg][1][0], acc[rg][1][1]),
+                             __builtin_elementwise_maximum(acc[rg][1][2], acc[rg][1][3])) * csc[rg];
+            any = any || mt[rg] > m_run[rg] + 8.0f;
+        }
+        if (__builtin_amdgcn_ballot_w64(any)) {
+#pragma unroll
+            for (int rg = 0; rg < NR; ++rg) {
+                mt[rg] = pg_max_groups(mt[rg]);
+                const bool need = mt[rg] > m_run[rg] + 8.0f;
+                const float f = need ? __builtin_amdgcn_exp2f(m_run[rg] - mt[rg]) : 1.0f;
+                m_run[rg] = need ? mt[rg] : m_run[rg];
                 l_run[rg] *= f;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) oacc[rg][k] *= f;
             }
-            uint32_t p[4];
+        }
+    };
+    // P and its sums.  Exponents are formed from the raw scores: m_run's own
+    // rounding cancels between numerator and denominator.
+    auto weights = [&](const float4_t (&acc)[NR][2], half8_t (&pb)[NR][2]) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                p[k] = pg_pack(__builtin_amdgcn_exp2f(sc[2 * k] - m_run[rg]), __builtin_amdgcn_exp2f(sc[2 * k + 1] - m_run[rg]));
-                l_run[rg] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, p[k]), ones, l_run[rg], false);
+        for (int rg = 0; rg < NR; ++rg)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t p[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    p[k] = pg_pack(__builtin_amdgcn_exp2f(__builtin_fmaf(acc[rg][u][2 * k], csc[rg], -m_run[rg])),
+                                   __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rg][u][2 * k + 1], csc[rg], -m_run[rg])));
+                    l_run[rg] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, p[k]), ones, l_run[rg], false);
+                }
+                pb[rg][u] = pg_half8(p[0], p[0], p[1], p[1]);       // against centroids and remainders
             }
-            pb[rg] = pg_half8(p[0], p[1], p[2], p[3]);
-        }
-        uint32_t ev[4], od[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t va = R.v[2 * k], vb = R.v[2 * k + 1];
-            ev[k] = ((vb << 4) & 0xF0F0F0F0u) | (va & 0x0F0F0F0Fu);
-            od[k] = (vb & 0xF0F0F0F0u) | ((va >> 4) & 0x0F0F0F0Fu);
-        }
+    };
+    auto products = [&](const uint32_t (&ev)[4], const uint32_t (&od)[4], const half8_t (&pb)[NR][2]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {                       // dims 8 m + k
-            uint2 e[4];
+            const uint32_t (&w)[4] = k & 1 ? od : ev;
+            half8_t A[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = entry(k & 1 ? od[j] : ev[j], k >> 1);
-            const half8_t vh = pg_half8(e[0].x, e[1].x, e[2].x, e[3].x);
+            for (int u = 0; u < 2; ++u) A[u] = two_bytes(w[2 * u], k >> 1, w[2 * u + 1], k >> 1);
 #pragma unroll
-            for (int rg = 0; rg < NR; ++rg) {
-                oacc[rg][k] = pg_mfma(vh, pb[rg], oacc[rg][k]);
-                if constexpr (HL) oacc[rg][k] = pg_mfma(pg_half8(e[0].y, e[1].y, e[2].y, e[3].y), pb[rg], oacc[rg][k]);
-            }
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int rg = 0; rg < NR; ++rg) oacc[rg][k] = pg_mfma(A[u], pb[rg][u], oacc[rg][k]);
+        }
+    };
+    // two tokens' codes of one dim as one table byte: even dims, odd dims
+    auto pair_codes = [&](const PgValues &V, uint32_t (&ev)[4], uint32_t (&od)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t va = V.v[2 * j], vb = V.v[2 * j + 1];
+            ev[j] = ((vb << 4) & 0xF0F0F0F0u) | (va & 0x0F0F0F0Fu);
+            od[j] = (vb & 0xF0F0F0F0u) | ((va >> 4) & 0x0F0F0F0Fu);
         }
     };
     if (cnt > 0) {
         const int64_t t0 = t_begin + wave;
-        for (int k = 0;;) {
-            load(R1, k + 1 < cnt ? k + 1 : cnt - 1);        // past the end: the last tile again, from cache
-            __builtin_amdgcn_sched_barrier(0);
-            step(R0, t0 + (int64_t)NW * k);
-            if (++k >= cnt) break;
-            load(R0, k + 1 < cnt ? k + 1 : cnt - 1);
-            __builtin_amdgcn_sched_barrier(0);
-            step(R1, t0 + (int64_t)NW * k);
-            if (++k >= cnt) break;
+        uint32_t r[2];
+        int v;
+        half8_t pb[NR][2];
+        uint32_t ev[4], od[4];
+        if constexpr (L::kAhead) {
+            float4_t S0[NR][2], S1[NR][2];
+            // one tile, whose scores S are there: the next one's are formed
+            // beside its weights, the one after that is asked for
+            auto step = [&](float4_t (&S)[NR][2], float4_t (&next)[NR][2], PgKeys<HL> &K, const PgKeys<HL> &Knext, PgValues &V,
+                            int &nv, int k) {
+                rows_at(clamp(k + 2), r, v);
+                settle(S, t0 + (int64_t)NW * k, nv);
+                nv = v;
+                scores(Knext, next);
+                weights(S, pb);
+                pair_codes(V, ev, od);
+                load_k(K, r);
+                load_v(V, r);
+                products(ev, od, pb);
+            };
+            scores(K0, S0);
+            for (int k = 0;;) {
+                step(S0, S1, K0, K1, V0, nv0, k);
+                if (++k >= cnt) break;
+                step(S1, S0, K1, K0, V1, nv1, k);
+                if (++k >= cnt) break;
+            }
+        } else {
+            // waves in a matrix phase issue first: of a SIMD's two, one then
+            // works on its weights
+            for (int k = 0; k < cnt; ++k) {
+                float4_t S[NR][2];
+                rows_at(clamp(k + 1), r, v);
+                __builtin_amdgcn_s_setprio(1);
+                scores(K0, S);
+                __builtin_amdgcn_s_setprio(0);
+                load_k(K0, r);
+                settle(S, t0 + (int64_t)NW * k, nv0);
+                nv0 = v;
+                weights(S, pb);
+                pair_codes(V0, ev, od);
+                load_v(V0, r);
+                __builtin_amdgcn_s_setprio(1);
+                products(ev, od, pb);
+                __builtin_amdgcn_s_setprio(0);
+            }
         }
     }
 
@@ -576,7 +714,7 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
     const int64_t mine = t_end - t_begin;
     const int act = mine < 1 ? 1 : mine < NW ? (int)mine : NW;      // waves with tiles
     float *slab = reinterpret_cast<float *>(smem);
-    float *ml = reinterpret_cast<float *>(smem + L::kMl);          // [wave][16][2], then a flag per wave
+    float *ml = reinterpret_cast<float *>(smem + L::kSlabs);       // [wave][16][2], then a flag per wave
 #pragma unroll
     for (int rg = 0; rg < NR; ++rg) {
         __syncthreads();                                           // the tables (or the last row group's slabs) are done with
@@ -615,7 +753,7 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
                 nan += ml[NW * 32 + w];
             }
             if (nan != 0.0f) l = __builtin_nanf("");
-            const int t = BLOCKS ? li.t : rho / a.G;
+            const int t = BLOCKS ? li.t : (int)((uint32_t)rho / (uint32_t)a.G);
             if (a.splits == 1) {
                 const int hq = hk * a.G + (BLOCKS ? rho : rho - t * a.G);
                 const float s = cdiv / l;
@@ -624,12 +762,12 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (!BLOCKS && !li.bad && t >= li.nd) v[i] = 0.0f;
-                    h[i] = F16 ? f32_to_f16_rne(v[i]) : f32_to_bf16_rne(v[i]);
+                    h[i] = HL ? f32_to_f16_rne(v[i]) : f32_to_bf16_rne(v[i]);
                 }
                 *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + ((li.b * a.Hq + hq) * a.T + t) * 128 + d) =
                     make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
             } else {
-                float *p = a.ws + ((unit * a.splits + split) * a.rows + rho) * kPartRow;
+                float *p = a.ws + (((int64_t)unit * a.splits + split) * a.rows + rho) * kPartRow;
                 *reinterpret_cast<float4 *>(p + d) = make_float4(o.x * cdiv, o.y * cdiv, o.z * cdiv, o.w * cdiv);
                 if (d == 0) {
                     p[128] = m;
@@ -649,7 +787,7 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
     if (row >= a.units * a.rows) return;
     const int64_t unit = row / a.rows;
     const int rho = (int)(row - unit * a.rows);
-    const PgList li = pg_list<BLOCKS>(a, unit);
+    const PgList li = pg_list<BLOCKS>(a, (uint32_t)unit);
     const int64_t share = pg_share(li.tiles, a.splits);
     const int act = li.tiles < 1 ? 1 : (int)((li.tiles + share - 1) / share);
     const float *base = a.ws + (unit * a.splits * a.rows + rho) * kPartRow;
@@ -709,10 +847,10 @@ struct PagePlan {
 // tiles, `rows` query rows each.
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     PagePlan p;
-    p.nr = rows <= 16 ? 1 : 2;
+    p.nr = rows <= 16 || hl ? 1 : rows <= 32 ? 2 : 4;
     p.chunks = (rows + 16 * p.nr - 1) / (16 * p.nr);
     const int64_t cus = device_cus(), blocks = units * p.chunks;
-    const double tile = (p.nr == 1 ? 0.21 : 0.27) * (hl ? 1.6 : 1.0);
+    const double tile = (p.nr == 1 ? 0.21 : p.nr == 2 ? 0.25 : 0.35) * (hl ? 1.6 : 1.0);
     double best = 1e30;
     p.splits = 1;
     auto consider = [&](int64_t s) {
@@ -732,22 +870,19 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     return p;
 }
 
-template <int NR, int NW, bool QJL, bool HL, bool BLOCKS>
-static void page_launch(const PageAttnArgs &a, hipStream_t s) {
-    const int64_t us = (a.units * a.splits + 7) / 8 * 8;
-    hipLaunchKernelGGL((page_attn_kernel<NR, NW, QJL, HL, BLOCKS>), dim3((unsigned)(us * a.chunks)), dim3(64 * NW), 0, s, a);
+template <int NR, bool HL, bool BLOCKS>
+static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
+    const dim3 grid((unsigned)((a.units * a.splits + 7) / 8 * 8 * a.chunks));
+    if (qjl) hipLaunchKernelGGL((page_attn_kernel<NR, true, HL, BLOCKS>), grid, dim3(64 * Pg<NR, true, HL>::NW), 0, s, a);
+    else hipLaunchKernelGGL((page_attn_kernel<NR, false, HL, BLOCKS>), grid, dim3(64 * Pg<NR, false, HL>::NW), 0, s, a);
 }
 
 template <bool BLOCKS>
 static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, int nr, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (nr == 1) {
-        if (hl) qjl ? page_launch<1, 8, true, true, BLOCKS>(a, s) : page_launch<1, 8, false, true, BLOCKS>(a, s);
-        else qjl ? page_launch<1, 12, true, false, BLOCKS>(a, s) : page_launch<1, 12, false, false, BLOCKS>(a, s);
-    } else {
-        if (hl) qjl ? page_launch<2, 8, true, true, BLOCKS>(a, s) : page_launch<2, 8, false, true, BLOCKS>(a, s);
-        else qjl ? page_launch<2, 8, true, false, BLOCKS>(a, s) : page_launch<2, 8, false, false, BLOCKS>(a, s);
-    }
+    if (nr == 1) hl ? page_launch<1, true, BLOCKS>(a, qjl, s) : page_launch<1, false, BLOCKS>(a, qjl, s);
+    else if (nr == 2) page_launch<2, false, BLOCKS>(a, qjl, s);
+    else page_launch<4, false, BLOCKS>(a, qjl, s);
     OMNI_CHECK_LAUNCH("page_attn_kernel");
     if (a.splits > 1) {
         const unsigned blocks = (unsigned)((a.units * a.rows + 7) / 8);
