@@ -560,7 +560,7 @@ int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t n_pages, in
  * block wins a tie, and a page outside the pool is taken first.  With codebooks
  * that ascend this bounds the group's summed scores (without residual signs)
  * from above.  blocks (B, Hkv, T, top) int32: ascending, -1 behind the last.
- * q as for omni_attn_tree.  workspace (16-byte aligned):
+ * q and sign_flip as for omni_attn_tree.  workspace (16-byte aligned):
  * omni_block_select_workspace_size(...) bytes.
  */
 size_t omni_block_select_workspace_size(int64_t B, int Hkv, int64_t T, int64_t max_pages, int top);

@@ -105,11 +105,11 @@ struct SelectArgs {
     const int32_t *page_table, *seq_lens;
     const float *codebooks;
     const int8_t *sign_flip;
-    int32_t *scores;             // [(b T + t) Hkv + hk][max_pages]
+    int32_t *scores;             // [(b T + t) Hkv + hk][max_pages], as keys
     int32_t *blocks;             // (B, Hkv, T, top)
     int64_t max_pages, n_pages;
     int page_shift, per_head, Hq, Hkv, G, T, top, first, recent, rotate, f16;
-    int per_block;               // blocks scored by one thread block
+    int per_block, heads;        // block_score_kernel: blocks and kv heads of a thread block
 };
 
 // Blocks that query (b, t) sees; 0 where the length does not fit the table.
@@ -126,86 +126,215 @@ __device__ __forceinline__ double whole_scale(double most) {
 }
 __device__ __forceinline__ int whole(double x) { return (int)fmin(fmax(__builtin_rint(x), -127.0), 127.0); }
 
-// Four codes (one a byte) to four int8 centroids from the 16-byte table t.
-__device__ __forceinline__ uint32_t four_centroids(uint32_t codes, const uint32_t (&t)[4]) {
-    const uint32_t sel = codes & 0x07070707u;
+// Bits 0 .. 3 (NIBBLE 0) or 4 .. 7 of four bytes, codes, to four int8 centroids
+// from the 16-byte table t: both halves of the table by the low three bits, the
+// fourth choosing between them (byte selectors 12 and 13 give 0x00 and 0xff).
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t four_centroids(uint32_t x, const uint32_t (&t)[4]) {
+    const uint32_t sel = (NIBBLE ? x >> 4 : x) & 0x07070707u;
     const uint32_t low = __builtin_amdgcn_perm(t[1], t[0], sel), high = __builtin_amdgcn_perm(t[3], t[2], sel);
-    // selectors 12 and 13 give the bytes 0x00 and 0xff
-    const uint32_t up = __builtin_amdgcn_perm(0u, 0u, ((codes >> 3) & 0x01010101u) | 0x0C0C0C0Cu);
+    const uint32_t up = __builtin_amdgcn_perm(0u, 0u, ((x >> (NIBBLE ? 7 : 3)) & 0x01010101u) | 0x0C0C0C0Cu);
     return (low & ~up) | (high & up);
 }
 
+constexpr int kSelWaves = 8;
+
 struct ScoreLds {
-    double part[4][256];
-    double most[4];
-    int8_t q[256];               // Q+, then -Q-
-    int8_t cent[16];
+    double part[kSelWaves][256];
+    __attribute__((aligned(16))) int8_t q[256];      // Q+, then -Q-
+    __attribute__((aligned(16))) int8_t cent[16];
 };
 
-// Q+ and -Q- of query (b, t)'s heads hk G .. + G - 1 and the centroids, as
-// int8, by the block's 256 threads.
-__device__ __forceinline__ void whole_query(const SelectArgs &a, ScoreLds &sm, int64_t b, int t, int hk) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double qp[2] = {0.0, 0.0}, qn[2] = {0.0, 0.0};
-    for (int h = wave; h < a.G; h += 4) {
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + ((b * a.Hq + hk * a.G + h) * a.T + t) * 128;
-        const uint16_t u0 = src[lane], u1 = src[lane + 64];
-        double x = a.f16 ? f16_to_f32(u0) : bf16_to_f32(u0), y = a.f16 ? f16_to_f32(u1) : bf16_to_f32(u1);
-        if (a.rotate) {
-            if (a.sign_flip) {
-                x = a.sign_flip[lane] < 0 ? -x : x;
-                y = a.sign_flip[lane + 64] < 0 ? -y : y;
-            }
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const double px = __shfl_xor(x, m), py = __shfl_xor(y, m);
-                x = lane & m ? px - x : x + px;
-                y = lane & m ? py - y : y + py;
-            }
-            const double u = x, v = y;
-            x = u + v;
-            y = u - v;
-        }
-        qp[0] += fmax(x, 0.0);
-        qn[0] += fmin(x, 0.0);
-        qp[1] += fmax(y, 0.0);
-        qn[1] += fmin(y, 0.0);
-    }
-    sm.part[wave][lane] = qp[0];
-    sm.part[wave][lane + 64] = qp[1];
-    sm.part[wave][128 + lane] = qn[0];
-    sm.part[wave][192 + lane] = qn[1];
-    __syncthreads();
-    const double v = (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]);
-    double m = fabs(v);
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) m = fmax(m, __shfl_xor(m, k));
-    if (lane == 0) sm.most[wave] = m;
-    if (tid < 16) {
-        const float *c = a.codebooks + (a.per_head ? hk * 16 : 0);
-        double cm = 0.0;
-        for (int k = 0; k < 16; ++k) cm = fmax(cm, fabs((double)c[k]));
-        sm.cent[tid] = (int8_t)whole((double)c[tid] * whole_scale(cm));
-    }
-    __syncthreads();
-    m = fmax(fmax(sm.most[0], sm.most[1]), fmax(sm.most[2], sm.most[3]));
-    sm.q[tid] = (int8_t)whole(v * whole_scale(m));
-    __syncthreads();
+// x of lane c ^ m of a 16-lane row, m a power of two
+__device__ __forceinline__ uint32_t sel_row_xor(uint32_t v, int m, int c) {
+    if (m == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);             // quad_perm [1,0,3,2]
+    if (m == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);             // quad_perm [2,3,0,1]
+    if (m == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true);            // row_ror:8
+    const int up = __builtin_amdgcn_mov_dpp((int)v, 0x12C, 0xf, 0xf, true);                          // row_ror:12: lane c + 4
+    const int dn = __builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, true);                          // row_ror:4: lane c - 4
+    return (uint32_t)(c & 4 ? dn : up);
+}
+__device__ __forceinline__ double sel_row_xor(double x, int m, int c) {
+    const uint64_t v = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, ((uint64_t)sel_row_xor((uint32_t)(v >> 32), m, c) << 32) | sel_row_xor((uint32_t)v, m, c));
 }
 
-// Scores of the blocks between the first and the recent ones: eight lanes a
-// block, 16 dims each.  Bound by the read of the bounds (128 B a block and
-// head) where there are many, else by launch and the query's preparation.
-__global__ __launch_bounds__(256) void block_score_kernel(SelectArgs a) {
-    __shared__ ScoreLds sm;
-    const int hk = blockIdx.y;
-    const int64_t bt = blockIdx.z, b = bt / a.T;
-    const int t = (int)(bt - b * a.T);
-    const int64_t nb = seen_blocks(a, b, t);
-    const int64_t from = a.first + (int64_t)blockIdx.x * a.per_block, to = nb - a.recent;
-    if (nb <= a.top || from >= to) return;                       // block-uniform, before any barrier
-    whole_query(a, sm, b, t, hk);
+template <int HALF>
+__device__ __forceinline__ double sel_sum(double x) {           // over lanes l and l ^ 16 or l ^ 32
+    const uint64_t v = __builtin_bit_cast(uint64_t, x);
+    uint64_t p, r;
+    if constexpr (HALF == 16) {
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+        p = ((uint64_t)hi[0] << 32) | lo[0];
+        r = ((uint64_t)hi[1] << 32) | lo[1];
+    } else {
+        const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+        p = ((uint64_t)hi[0] << 32) | lo[0];
+        r = ((uint64_t)hi[1] << 32) | lo[1];
+    }
+    return __builtin_bit_cast(double, p) + __builtin_bit_cast(double, r);
+}
+
+// Q+ and -Q- of query (b, t)'s heads hk G .. + G - 1 and the centroids, as
+// int8: four heads a wave at a time, 16 lanes a head, eight dims a lane.  The
+// constructor asks for the loads of heads 4 `first` .. + 3.
+struct WholeQuery {
+    uint4 raw;
+    uint2 flip;
+    float cent;
+    __device__ __forceinline__ uint4 head(const SelectArgs &a, int64_t b, int t, int hk, int h, int c) const {
+        return *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
+                                                ((b * a.Hq + hk * a.G + (h < a.G ? h : 0)) * a.T + t) * 128 + 8 * c);
+    }
+    __device__ __forceinline__ WholeQuery(const SelectArgs &a, int64_t b, int t, int hk, int first) {
+        const int lane = threadIdx.x & 63, c = lane & 15;
+        raw = head(a, b, t, hk, 4 * first + (lane >> 4), c);
+        flip = make_uint2(0u, 0u);
+        if (a.sign_flip) flip = *reinterpret_cast<const uint2 *>(a.sign_flip + 8 * c);
+        cent = (a.codebooks + (a.per_head ? hk * 16 : 0))[c];
+    }
+    // the wave's sums over heads 4 first .. + 3, then every 4 `stride` on: dim 8 c + j of Q+ in place 16 j + c, of -Q- 128 on
+    __device__ __forceinline__ void sums(const SelectArgs &a, double *part, int64_t b, int t, int hk, int first, int stride) const {
+        const int lane = threadIdx.x & 63, c = lane & 15;
+        double qp[8], qn[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qp[j] = qn[j] = 0.0;
+        for (int h0 = 4 * first; h0 < a.G; h0 += 4 * stride) {
+            const int h = h0 + (lane >> 4);
+            const uint4 w4 = h0 == 4 * first ? raw : head(a, b, t, hk, h, c);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            double x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint16_t u = (uint16_t)((j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+                u ^= (uint16_t)(((j < 4 ? flip.x >> (8 * j) : flip.y >> (8 * j - 32)) & 0x80u) << 8);
+                x[j] = h < a.G ? (double)(a.f16 ? f16_to_f32(u) : bf16_to_f32(u)) : 0.0;
+            }
+            if (a.rotate) {
+#pragma unroll
+                for (int m = 1; m < 8; m <<= 1)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (!(j & m)) {
+                            const double u = x[j], l = x[j + m];
+                            x[j] = u + l;
+                            x[j + m] = u - l;
+                        }
+#pragma unroll
+                for (int m = 1; m < 16; m <<= 1) {
+                    const double sgn = c & m ? -1.0 : 1.0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = __builtin_fma(sgn, x[j], sel_row_xor(x[j], m, c));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                qp[j] += fmax(x[j], 0.0);
+                qn[j] += fmin(x[j], 0.0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            qp[j] = sel_sum<32>(sel_sum<16>(qp[j]));
+            qn[j] = sel_sum<32>(sel_sum<16>(qn[j]));
+            if (lane < 16) {
+                part[16 * j + c] = qp[j];
+                part[128 + 16 * j + c] = qn[j];
+            }
+        }
+    }
+    __device__ __forceinline__ int8_t centroid() const {          // lane l: of code l % 16
+        const int c = threadIdx.x & 15;
+        float cm = fabsf(cent);
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) cm = fmaxf(cm, __uint_as_float(sel_row_xor(__float_as_uint(cm), m, c)));
+        return (int8_t)whole((double)cent * whole_scale((double)cm));
+    }
+    // v[k]: place 64 k + lane of the summed sums; each wave finds the largest, and stores its places `mask` names
+    __device__ __forceinline__ static void store(const double (&v)[4], int8_t *q, uint32_t mask) {
+        const int lane = threadIdx.x & 63, c = lane & 15;
+        double m = fmax(fmax(fabs(v[0]), fabs(v[1])), fmax(fabs(v[2]), fabs(v[3])));
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) m = fmax(m, sel_row_xor(m, k, c));
+#pragma unroll
+        for (int k = 16; k < 64; k <<= 1) m = fmax(m, __shfl_xor(m, k));
+        const double scale = whole_scale(m);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int place = 64 * k + lane;
+            if ((mask >> k) & 1u) q[(place & 128) + 8 * c + ((place & 127) >> 4)] = (int8_t)whole(v[k] * scale);
+        }
+    }
+    // one kv head by the whole block
+    __device__ __forceinline__ void form(const SelectArgs &a, ScoreLds &sm, int64_t b, int t, int hk) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int groups = (a.G + 3) >> 2, waves = groups < kSelWaves ? groups : kSelWaves;
+        if (wave < waves) sums(a, sm.part[wave], b, t, hk, wave, kSelWaves);
+        const int8_t ci = centroid();
+        if (tid < 16) sm.cent[tid] = ci;
+        __syncthreads();
+        double v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = 0.0;
+            for (int w = 0; w < waves; ++w) v[k] += sm.part[w][64 * k + lane];
+        }
+        if (wave < 4) store(v, sm.q, 1u << wave);
+        __syncthreads();
+    }
+};
+
+// The score of the block whose bounds the eight lanes of `lane`'s group hold 16
+// dims each of, as an unsigned key that orders as it does.  A page outside the
+// pool is selected first, so that its rows come out NaN.
+__device__ __forceinline__ uint32_t block_key(const uint4 &w, int32_t id, int64_t n_pages, const uint32_t (&qp)[4],
+                                              const uint32_t (&qn)[4], const uint32_t (&tab)[4], int lane) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    int s = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        s = __builtin_amdgcn_sdot4((int)four_centroids<1>(x[j], tab), (int)qp[j], s, false);
+        s = __builtin_amdgcn_sdot4((int)four_centroids<0>(x[j], tab), (int)qn[j], s, false);
+    }
+#pragma unroll
+    for (int m = 1; m < 4; m <<= 1) s += (int)sel_row_xor((uint32_t)s, m, lane & 15);
+    s += __builtin_amdgcn_mov_dpp(s, 0x141, 0xf, 0xf, true);      // row_half_mirror: the other quad's sum
+    return id >= 0 && id < n_pages ? (uint32_t)s ^ 0x80000000u : 0xffffffffu;
+}
+
+// Scores of blocks from .. to - 1 by the block's eight waves, put(block, score
+// as an unsigned key that orders as it does): eight lanes a block, 16 dims
+// each; a wave has 64 blocks' bounds in flight.  Bound by the read of the
+// bounds (128 B a block and head) where there are many, else by the chain
+// query, page table, bounds.
+template <typename Put>
+__device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQuery &wq, ScoreLds &sm, int64_t b, int t, int hk, int from,
+                                             int to, Put &&put) {
+    constexpr int U = 8;                                          // loads in flight
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 7;
+    const int32_t *pt = a.page_table + b * a.max_pages;
+    int32_t id[U];
+    uint4 w[U];
+    auto ids = [&](int p0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = p0 + 8 * u + (lane >> 3);
+            id[u] = p < to ? pt[p] : 0;
+        }
+    };
+    auto bounds = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool ok = id[u] >= 0 && id[u] < a.n_pages;
+            w[u] = *reinterpret_cast<const uint4 *>(a.bounds + ((uint64_t)((uint32_t)(ok ? id[u] : 0) * (uint32_t)a.Hkv + (uint32_t)hk) * 128 + 16u * (uint32_t)c));
+        }
+    };
+    int p0 = from + 8 * U * wave;
+    ids(p0);
+    bounds();
+    wq.form(a, sm, b, t, hk);
     uint32_t qp[4], qn[4], tab[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -213,26 +342,18 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectArgs a) {
         qn[j] = reinterpret_cast<const uint32_t *>(sm.q)[32 + 4 * c + j];
         tab[j] = reinterpret_cast<const uint32_t *>(sm.cent)[j];
     }
-    const int64_t end = from + a.per_block < to ? from + a.per_block : to;
-    const int32_t *pt = a.page_table + b * a.max_pages;
-    int32_t *out = a.scores + (bt * a.Hkv + hk) * a.max_pages;
-    for (int64_t p0 = from + 8 * wave; p0 < end; p0 += 32) {
-        const int64_t p = p0 + (lane >> 3);
-        const int32_t id = p < end ? pt[p] : 0;
-        const bool ok = id >= 0 && id < a.n_pages;
-        const uint4 w4 = *reinterpret_cast<const uint4 *>(a.bounds + ((int64_t)(ok ? id : 0) * a.Hkv + hk) * 128 + 16 * c);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        int s = 0;
+    for (; p0 < to; p0 += 8 * U * kSelWaves) {
+        uint32_t s[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s = __builtin_amdgcn_sdot4((int)four_centroids((w[j] >> 4) & 0x0F0F0F0Fu, tab), (int)qp[j], s, false);
-            s = __builtin_amdgcn_sdot4((int)four_centroids(w[j] & 0x0F0F0F0Fu, tab), (int)qn[j], s, false);
+        for (int u = 0; u < U; ++u) s[u] = block_key(w[u], id[u], a.n_pages, qp, qn, tab, lane);
+        const int at = p0;
+        ids(p0 + 8 * U * kSelWaves);
+        if (p0 + 8 * U * kSelWaves < to) bounds();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = at + 8 * u + (lane >> 3);
+            if (c == 0 && p < to) put(p, s[u]);
         }
-        s += __shfl_xor(s, 1);
-        s += __shfl_xor(s, 2);
-        s += __shfl_xor(s, 4);
-        // a page outside the pool is selected first, so that its rows come out NaN
-        if (c == 0 && p < end) out[p] = ok ? s : 0x7fffffff;
     }
 }
 
@@ -241,38 +362,227 @@ __global__ __launch_bounds__(256) void block_score_kernel(SelectArgs a) {
 // One block per (b, t, hk): the score that the last of `need` blocks has, by
 // digits of eight bits from the top of the scores' range (a histogram in LDS
 // per digit), then the blocks above it and the first ones equal to it in
-// ascending order (a scan over the threads' consecutive shares).
-constexpr int kPickThreads = 512;
-constexpr int kPickLds = 12288;          // scores held in LDS; more are read again for every digit
+// ascending order.  SCORED: the
+// scores are there already, by block_score_kernel.
+constexpr int kPickLds = 16384;          // scores held in LDS; more are read again for every digit
 
-__global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectArgs a) {
+// The key (at most `range`) that the `need`-th largest has, and of the equal
+// ones how many are needed (in `need`).  each(shift, at, count) calls count(x)
+// for every key x whose bits from `shift` up are `at`.
+template <typename Each>
+__device__ __forceinline__ uint32_t find_digits(uint32_t range, uint32_t &need, uint32_t *hist, uint32_t *sh, Each &&each) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    int shift = range ? 32 - __builtin_clz(range) : 0;
+    uint32_t prefix = 0u;
+    while (shift > 0) {
+        const int low = shift > 8 ? shift - 8 : 0, width = shift - low;
+        if (tid < 256) hist[tid] = 0u;
+        __syncthreads();
+        each(shift, prefix, [&](uint32_t x) { atomicAdd(&hist[(x >> low) & ((1u << width) - 1u)], 1u); });
+        __syncthreads();
+        if (tid < 64) {
+            // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
+            const uint4 h4 = *reinterpret_cast<const uint4 *>(&hist[252 - 4 * lane]);
+            const uint32_t c[4] = {h4.w, h4.z, h4.y, h4.x};
+            const uint32_t sum = (c[0] + c[1]) + (c[2] + c[3]);
+            uint32_t incl = sum;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const uint32_t up = __shfl_up(incl, m);
+                incl += lane >= m ? up : 0u;
+            }
+            uint32_t above = incl - sum;
+            if (above < need && need <= incl) {                   // one lane
+                bool found = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (!found && need <= above + c[j]) {
+                        sh[0] = (prefix << width) | (uint32_t)(255 - 4 * lane - j);
+                        sh[1] = need - above;
+                        found = true;
+                    }
+                    above += c[j];
+                }
+            }
+        }
+        __syncthreads();                                         // hist may be cleared again
+        prefix = sh[0];
+        need = sh[1];
+        shift = low;
+    }
+    return prefix;
+}
+
+// The `need` largest of n <= R 512 keys (in LDS, from kmin to kmax), the first
+// of equal ones: their places, counted from `first`, ascending.  Thread tid
+// holds keys tid, tid + 512, ...
+template <int R>
+__device__ __forceinline__ void pick_held(uint32_t *keys, int n, uint32_t kmin, uint32_t kmax, uint32_t need, uint32_t *hist,
+                                          uint32_t *sh, int first, int32_t *out) {
+    constexpr int kThreads = 64 * kSelWaves;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t x[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) x[j] = j * kThreads + tid < n ? keys[j * kThreads + tid] - kmin : 0u;
+    const uint32_t prefix = find_digits(kmax - kmin, need, hist, sh, [&](int shift, uint32_t at, auto &&count) {
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            if (j * kThreads + tid < n && (shift >= 32 || x[j] >> shift == at)) count(x[j]);
+    });
+    // counts of either kind by 64 consecutive keys, (j, wave)
+    uint32_t *const cnt = keys;
+    __syncthreads();                                             // keys are read
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const bool in = j * kThreads + tid < n;
+        const uint64_t above = __builtin_amdgcn_ballot_w64(in && x[j] > prefix), equal = __builtin_amdgcn_ballot_w64(in && x[j] == prefix);
+        if (lane == 0) cnt[j * kSelWaves + wave] = (uint32_t)__popcll(above) | ((uint32_t)__popcll(equal) << 16);
+    }
+    __syncthreads();
+    // their exclusive sums, each wave for itself, two counts a lane (8192 of either kind at most: 16 bits hold them)
+    const bool some = 2 * lane < R * kSelWaves;
+    const uint2 two = *reinterpret_cast<const uint2 *>(&cnt[some ? 2 * lane : 0]);
+    const uint32_t both = some ? two.x + two.y : 0u;
+    uint32_t incl = both;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t up = __shfl_up(incl, m);
+        incl += lane >= m ? up : 0u;
+    }
+    const uint32_t first_of = incl - both;
+    const uint64_t before = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        if (j * kThreads >= n) break;                            // uniform
+        const bool in = j * kThreads + tid < n;
+        const uint64_t above = __builtin_amdgcn_ballot_w64(in && x[j] > prefix), equal = __builtin_amdgcn_ballot_w64(in && x[j] == prefix);
+        const int item = j * kSelWaves + wave;
+        const uint32_t base = (uint32_t)__builtin_amdgcn_readlane((int)first_of, item >> 1) +
+                              (item & 1 ? (uint32_t)__builtin_amdgcn_readlane((int)two.x, item >> 1) : 0u);
+        const uint32_t g = (base & 0xffffu) + (uint32_t)__popcll(above & before), e = (base >> 16) + (uint32_t)__popcll(equal & before);
+        if (((above >> lane) & 1u) || (((equal >> lane) & 1u) && e < need)) out[g + (e < need ? e : need)] = first + j * kThreads + tid;
+    }
+}
+
+// Scores where rows are fewer than CUs and long: the read of the bounds over
+// the whole chip, `heads` kv heads (a divisor of 8, or 8) of a share of one
+// query's blocks by a thread block, so that a wave's load is 8 / heads pages'
+// neighbouring bounds, a KB.
+__global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectArgs a) {
+    constexpr int U = 8;                                          // loads in flight
+    __shared__ __attribute__((aligned(16))) int8_t qs[8][256];
+    __shared__ __attribute__((aligned(16))) int8_t cs[8][16];
+    __shared__ double part[8][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 7;
+    const int64_t b = blockIdx.z;
+    const int sets = a.Hkv / a.heads, share = (int)(blockIdx.x / (unsigned)sets), h0 = ((int)blockIdx.x - share * sets) * a.heads;
+    const int t = blockIdx.y;
+    const int nb = (int)seen_blocks(a, b, t);
+    const int from = a.first + share * a.per_block, last = nb - a.recent;
+    if (nb <= a.top || from >= last) return;                     // block-uniform, before any barrier
+    const int to = from + a.per_block < last ? from + a.per_block : last;
+    const int32_t *pt = a.page_table + b * a.max_pages;
+    const int per = 8 / a.heads, mine = (lane >> 3) / a.heads, hk = h0 + (lane >> 3) - mine * a.heads;     // pages a load; this lane's
+    int32_t id[U];
+    uint4 w[U];
+    auto ids = [&](int p0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = p0 + per * u + mine;
+            id[u] = p < to ? pt[p] : 0;
+        }
+    };
+    auto bounds = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool ok = id[u] >= 0 && id[u] < a.n_pages;
+            w[u] = *reinterpret_cast<const uint4 *>(a.bounds + ((uint64_t)((uint32_t)(ok ? id[u] : 0) * (uint32_t)a.Hkv + (uint32_t)hk) * 128 + 16u * (uint32_t)c));
+        }
+    };
+    const int step = per * U * kSelWaves;
+    int p0 = from + per * U * wave;
+    ids(p0);
+    bounds();
+    if (wave < a.heads) {                                        // a wave forms a head's query by itself
+        const WholeQuery wq(a, b, t, h0 + wave, 0);
+        wq.sums(a, part[wave], b, t, h0 + wave, 0, 1);
+        const int8_t ci = wq.centroid();
+        if (lane < 16) cs[wave][lane] = ci;
+        double v[4];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<volatile double *>(&part[wave][64 * k + lane]);
+        WholeQuery::store(v, qs[wave], 15u);
+    }
+    __syncthreads();
+    uint32_t qp[4], qn[4], tab[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        qp[j] = reinterpret_cast<const uint32_t *>(qs[hk - h0])[4 * c + j];
+        qn[j] = reinterpret_cast<const uint32_t *>(qs[hk - h0])[32 + 4 * c + j];
+        tab[j] = reinterpret_cast<const uint32_t *>(cs[hk - h0])[j];
+    }
+    uint32_t *out = reinterpret_cast<uint32_t *>(a.scores) + ((b * a.T + t) * a.Hkv + hk) * a.max_pages;
+    for (; p0 < to; p0 += step) {
+        uint32_t s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = block_key(w[u], id[u], a.n_pages, qp, qn, tab, lane);
+        const int at = p0;
+        ids(p0 + step);
+        if (p0 + step < to) bounds();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = at + per * u + mine;
+            if (c == 0 && p < to) out[p] = s[u];
+        }
+    }
+}
+
+template <bool SCORED>
+__global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs a) {
+    constexpr int kThreads = 64 * kSelWaves;
     __shared__ uint32_t keys[kPickLds];
+    __shared__ ScoreLds sm;
     __shared__ uint32_t hist[256];
-    __shared__ uint32_t wred[2][kPickThreads / 64];
+    __shared__ uint32_t wred[2][kSelWaves];
     __shared__ uint32_t sh[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x;                              // (b T + t) Hkv + hk
-    const int64_t bt = row / a.Hkv, b = bt / a.T;
-    const int hk = (int)(row - bt * a.Hkv), t = (int)(bt - b * a.T);
+    const int hk = blockIdx.x, t = blockIdx.y;
+    const int64_t b = blockIdx.z, row = (b * a.T + t) * a.Hkv + hk;
+    const WholeQuery wq(a, b, t, hk, (int)(threadIdx.x >> 6));
     const int64_t nb = seen_blocks(a, b, t);
     int32_t *out = a.blocks + ((b * a.Hkv + hk) * a.T + t) * a.top;
     if (nb <= a.top) {
-        for (int i = tid; i < a.top; i += kPickThreads) out[i] = i < nb ? i : -1;
+        for (int i = tid; i < a.top; i += kThreads) out[i] = i < nb ? i : -1;
         return;
     }
-    for (int i = tid; i < a.first + a.recent; i += kPickThreads)
+    for (int i = tid; i < a.first + a.recent; i += kThreads)
         out[i < a.first ? i : a.top - a.recent + (i - a.first)] = (int32_t)(i < a.first ? i : nb - a.recent + (i - a.first));
     uint32_t need = (uint32_t)(a.top - a.first - a.recent);
     if (need == 0) return;                                       // uniform
     const int n = (int)(nb - a.first - a.recent);                // > need
-    const int32_t *src = a.scores + row * a.max_pages + a.first;
+    uint32_t *const src = reinterpret_cast<uint32_t *>(a.scores) + row * a.max_pages + a.first;
     const bool held = n <= kPickLds;
     uint32_t kmin = 0xffffffffu, kmax = 0u;
-    for (int i = tid; i < n; i += kPickThreads) {
-        const uint32_t k = (uint32_t)src[i] ^ 0x80000000u;
-        if (held) keys[i] = k;
-        kmin = k < kmin ? k : kmin;
-        kmax = k > kmax ? k : kmax;
+    if constexpr (SCORED) {
+        for (int i0 = tid; i0 < n; i0 += 8 * kThreads) {          // eight loads in flight
+            uint32_t k[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = src[i0 + j * kThreads < n ? i0 + j * kThreads : i0];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (held && i0 + j * kThreads < n) keys[i0 + j * kThreads] = k[j];
+                kmin = k[j] < kmin ? k[j] : kmin;
+                kmax = k[j] > kmax ? k[j] : kmax;
+            }
+        }
+    } else {
+        score_blocks(a, wq, sm, b, t, hk, a.first, (int)nb - a.recent, [&](int p, uint32_t k) {
+            if (held) keys[p - a.first] = k;
+            else src[p - a.first] = k;
+            kmin = k < kmin ? k : kmin;
+            kmax = k > kmax ? k : kmax;
+        });
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
@@ -284,91 +594,57 @@ __global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectArgs a) 
         wred[0][wave] = kmin;
         wred[1][wave] = kmax;
     }
-    __syncthreads();
+    __syncthreads();                                             // the keys too, in LDS or (block-wide) in memory
 #pragma unroll
-    for (int w = 0; w < kPickThreads / 64; ++w) {
+    for (int w = 0; w < kSelWaves; ++w) {
         kmin = wred[0][w] < kmin ? wred[0][w] : kmin;
         kmax = wred[1][w] > kmax ? wred[1][w] : kmax;
     }
-    auto key = [&](int i) { return (held ? keys[i] : (uint32_t)src[i] ^ 0x80000000u) - kmin; };
-    // `prefix`: the digits found so far, the key's bits from `shift` up
-    const uint32_t range = kmax - kmin;
-    int shift = range ? 32 - __builtin_clz(range) : 0;
-    uint32_t prefix = 0u;
-    while (shift > 0) {
-        const int low = shift > 8 ? shift - 8 : 0, width = shift - low;
-        __syncthreads();                                         // hist and sh of the last digit are read
-        if (tid < 256) hist[tid] = 0u;
-        __syncthreads();
-        for (int i = tid; i < n; i += kPickThreads) {
+    if (n <= 2 * kThreads) return pick_held<2>(keys, n, kmin, kmax, need, hist, sh, a.first, out + a.first);
+    if (n <= 16 * kThreads) return pick_held<16>(keys, n, kmin, kmax, need, hist, sh, a.first, out + a.first);
+    auto key = [&](int i) { return (held ? keys[i] : src[i]) - kmin; };
+    const uint32_t prefix = find_digits(kmax - kmin, need, hist, sh, [&](int shift, uint32_t at, auto &&count) {
+        for (int i = tid; i < n; i += kThreads) {
             const uint32_t x = key(i);
-            if (shift >= 32 || x >> shift == prefix) atomicAdd(&hist[(x >> low) & ((1u << width) - 1u)], 1u);
+            if (shift >= 32 || x >> shift == at) count(x);
         }
-        __syncthreads();
-        if (wave == 0) {
-            // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
-            uint32_t c[4], sum = 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                c[j] = hist[255 - 4 * lane - j];
-                sum += c[j];
-            }
-            uint32_t incl = sum;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const uint32_t up = __shfl_up(incl, m);
-                incl += lane >= m ? up : 0u;
-            }
-            uint32_t above = incl - sum;
-            if (above < need && need <= incl) {                   // one lane
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (above < need && need <= above + c[j]) {
-                        sh[0] = (prefix << width) | (uint32_t)(255 - 4 * lane - j);
-                        sh[1] = need - above;
-                        need = 0u;                                // found
-                    }
-                    above += c[j];
-                }
-            }
-        }
-        __syncthreads();
-        prefix = sh[0];
-        need = sh[1];
-        shift = low;
-    }
+    });
     // ── the blocks above `prefix`, and the first `need` equal to it ──
-    const int each = (n + kPickThreads - 1) / kPickThreads, i0 = tid * each, i1 = i0 + each < n ? i0 + each : n;
-    uint32_t gt = 0u, eq = 0u;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t x = key(i);
-        gt += x > prefix ? 1u : 0u;
-        eq += x == prefix ? 1u : 0u;
+    // each wave takes a share of consecutive blocks, 64 at a time: its count of
+    // either kind first, then the places
+    const int share = ((n + kSelWaves - 1) / kSelWaves + 63) & ~63, w0 = wave * share, w1 = w0 + share < n ? w0 + share : n;
+    auto kinds = [&](int i0, uint64_t &above, uint64_t &equal) {
+        const int i = i0 + lane;
+        const uint32_t x = i < w1 ? key(i) : 0u;
+        above = __builtin_amdgcn_ballot_w64(i < w1 && x > prefix);
+        equal = __builtin_amdgcn_ballot_w64(i < w1 && x == prefix);
+    };
+    uint32_t pg = 0u, pe = 0u;
+    for (int i0 = w0; i0 < w1; i0 += 64) {
+        uint64_t above, equal;
+        kinds(i0, above, equal);
+        pg += (uint32_t)__popcll(above);
+        pe += (uint32_t)__popcll(equal);
     }
-    uint32_t igt = gt, ieq = eq;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const uint32_t ug = __shfl_up(igt, m), ue = __shfl_up(ieq, m);
-        igt += lane >= m ? ug : 0u;
-        ieq += lane >= m ? ue : 0u;
+    __syncthreads();                                             // wred is read
+    if (lane == 0) {
+        wred[0][wave] = pg;
+        wred[1][wave] = pe;
     }
     __syncthreads();
-    if (lane == 63) {
-        wred[0][wave] = igt;
-        wred[1][wave] = ieq;
-    }
-    __syncthreads();
-    uint32_t pg = igt - gt, pe = ieq - eq;
+    pg = pe = 0u;
     for (int w = 0; w < wave; ++w) {
         pg += wred[0][w];
         pe += wred[1][w];
     }
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t x = key(i);
-        const bool take = x > prefix || (x == prefix && pe < need);
-        if (take) out[a.first + pg + (pe < need ? pe : need)] = a.first + i;
-        pg += x > prefix ? 1u : 0u;
-        pe += x == prefix ? 1u : 0u;
+    const uint64_t before = ((uint64_t)1 << lane) - 1;
+    for (int i0 = w0; i0 < w1; i0 += 64) {
+        uint64_t above, equal;
+        kinds(i0, above, equal);
+        const uint32_t g = pg + (uint32_t)__popcll(above & before), e = pe + (uint32_t)__popcll(equal & before);
+        if (((above >> lane) & 1u) || (((equal >> lane) & 1u) && e < need)) out[a.first + g + (e < need ? e : need)] = a.first + i0 + lane;
+        pg += (uint32_t)__popcll(above);
+        pe += (uint32_t)__popcll(equal);
     }
 }
 
@@ -477,19 +753,27 @@ extern "C" int omni_block_select(const void *q, int q_dtype, const uint8_t *boun
     }
     SelectArgs a{q, bounds, page_table, seq_lens, codebooks, rotate_q ? sign_flip : nullptr, (int32_t *)workspace, blocks,
                  max_pages, n_pages, shift, per_head_codebook, Hq, Hkv, Hq / Hkv, (int)T, top, first, recent, rotate_q,
-                 q_dtype == OMNI_F16, 0};
+                 q_dtype == OMNI_F16, 0, 1};
     const int64_t rows = B * T * Hkv;
-    if (ws) {
-        // shares of 64 blocks at least, four thread blocks a CU
-        int64_t per = (max_pages * rows + 4 * device_cus() - 1) / (4 * device_cus());
-        per = per < 64 ? 64 : per > (1 << 20) ? 1 << 20 : (per + 31) / 32 * 32;
+    // One launch where a row's blocks are few or the rows fill the chip; else
+    // the scores over the whole chip first.
+    const int64_t cus = device_cus();
+    a.heads = Hkv % 8 == 0 ? 8 : 8 % Hkv == 0 ? Hkv : 1;
+    if (ws && max_pages > 1024 && 2 * rows <= cus) {
+        // about two thread blocks a CU, whole rounds of their waves
+        const int64_t round = 8 / a.heads * 8 * kSelWaves;
+        int64_t per = max_pages * (rows / a.heads) / (2 * cus) / round * round;
+        per = per < round ? round : per;
         a.per_block = (int)per;
-        hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((max_pages + per - 1) / per), (unsigned)Hkv, (unsigned)(B * T)),
-                           dim3(256), 0, as_stream(stream), a);
+        const unsigned shares = (unsigned)((max_pages + per - 1) / per);
+        hipLaunchKernelGGL(block_score_kernel, dim3(shares * (unsigned)(Hkv / a.heads), (unsigned)T, (unsigned)B), dim3(64 * kSelWaves),
+                           0, as_stream(stream), a);
         OMNI_CHECK_LAUNCH("block_score_kernel");
+        hipLaunchKernelGGL(block_select_kernel<true>, dim3((unsigned)Hkv, (unsigned)T, (unsigned)B), dim3(64 * kSelWaves), 0, as_stream(stream), a);
+    } else {
+        hipLaunchKernelGGL(block_select_kernel<false>, dim3((unsigned)Hkv, (unsigned)T, (unsigned)B), dim3(64 * kSelWaves), 0, as_stream(stream), a);
     }
-    hipLaunchKernelGGL(block_pick_kernel, dim3((unsigned)rows), dim3(kPickThreads), 0, as_stream(stream), a);
-    OMNI_CHECK_LAUNCH("block_pick_kernel");
+    OMNI_CHECK_LAUNCH("block_select_kernel");
     return OMNI_OK;
 }
 

@@ -55,6 +55,7 @@ struct PageAttnArgs {
     const int32_t *blocks;       // blocks: (B, Hkv, T, top) block numbers, others are skipped
     int64_t max_pages, n_pages, tree_stride, units;
     int page_shift, per_head, Hq, Hkv, G, T, rows, chunks, splits, top, rotate;
+    uint64_t hkv_magic, t_magic, g_magic;        // pg_div by Hkv, T and G
     float qscale;                // scale log2 e
     float alpha, wht_scale;      // sqrt(2/pi) / 128, 1 / sqrt(128) as fp32
 };
@@ -67,21 +68,25 @@ constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dwor
 
 // What a variant keeps where.  NR: groups of 16 query rows a block; HL: fp16
 // queries.
-template <int NR, bool QJL, bool HL>
+template <int NR, bool QJL, bool HL, int WAVES>
 struct Pg {
-    static constexpr int NW = NR == 1 && !HL ? 12 : 8;                       // waves
+    static constexpr int NW = WAVES;
     static constexpr bool kQReg = NR <= 2;                                   // query operands in registers (else LDS)
-    static constexpr bool kAhead = NR <= 2;                                  // a wave forms the next tile's scores beside a tile's weights
+    static constexpr int PF = NR <= 2 ? 2 : 1;                               // tiles a wave holds
     static constexpr int kQSteps = HL ? 16 : 4;                              // B operands of a row group: q (HL: twice eight),
     static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
     static constexpr int kSteps = kQSteps + kGSteps;
     static constexpr int kQimg = NR * kSteps * 1024;
     static constexpr int kCsc = kQimgOff + kQimg;                            // per row: score scale
     static constexpr int kSees = kCsc + NR * 16 * 4;                         // per row: its tree mask
-    static constexpr int kUse = kSees + NR * 16 * 8;
-    static constexpr int kSlabs = NW * 16 * kPartRow * 4;                    // epilogue: the waves' O of one row group,
-    static constexpr int kMerge = kSlabs + NW * 32 * 4 + NW * 4;             // their m and l, a flag per wave
-    static constexpr int kLds = kUse > kMerge ? kUse : kMerge;
+    static constexpr int kM = kSees + NR * 16 * 8;                           // [row][wave]: running maxima, then sums
+    static constexpr int kFlags = kM + 2 * NR * 16 * NW * 4;                 // per wave: met a page outside the pool
+    static constexpr int kUse = kFlags + 16 * 4;
+    // the merge: the waves' O of MR row groups at a time, from 0 on (over the tables and the query rows)
+    static constexpr int MR = NR > 1 && NW <= 8 ? 2 : 1;
+    static constexpr int kSlabs = NW * MR * 16 * kPartRow * 4;
+    static constexpr int kMoved = kSlabs > kCsc ? kSlabs - kCsc : 0;         // what lies behind them moves up
+    static constexpr int kLds = kUse + kMoved;
 };
 
 __device__ __forceinline__ uint32_t pg_pack(float x, float y) {
@@ -95,6 +100,16 @@ __device__ __forceinline__ half8_t pg_half8(uint32_t a, uint32_t b, uint32_t c, 
 }
 __device__ __forceinline__ float4_t pg_mfma(half8_t a, half8_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// x of lane c ^ m of a 16-lane row, m a power of two
+__device__ __forceinline__ float pg_row_xor(float x, int m, int c) {
+    const int v = __float_as_int(x);
+    if (m == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true));            // quad_perm [1,0,3,2]
+    if (m == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true));            // quad_perm [2,3,0,1]
+    if (m == 8) return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true));           // row_ror:8
+    const int up = __builtin_amdgcn_mov_dpp(v, 0x12C, 0xf, 0xf, true);                               // row_ror:12: lane c + 4
+    const int dn = __builtin_amdgcn_mov_dpp(v, 0x124, 0xf, 0xf, true);                               // row_ror:4: lane c - 4
+    return __int_as_float(c & 4 ? dn : up);
 }
 // The larger, or NaN if one is: single instructions (fmaxf quiets operands
 // first that the compiler cannot prove quiet, such as a matrix product's).
@@ -115,6 +130,9 @@ __device__ __forceinline__ float pg_sum_groups(float v) {
     return __uint_as_float(u[0]) + __uint_as_float(u[1]);
 }
 
+// floor(x / d) as (x (floor(2^32 / d) + 1)) >> 32: exact for x d < 2^32
+__device__ __forceinline__ uint32_t pg_div(uint32_t x, uint64_t magic) { return (uint32_t)(((uint64_t)x * magic) >> 32); }
+
 // The list that a unit (b, t, hk) or (b, hk) reads: `seen` tokens of sequence
 // b, in tree calls the first `base` of them by every row.  Tiles are of the
 // list's slots: positions in a sequence, or `top` blocks one after another.
@@ -127,10 +145,14 @@ struct PgList {
 template <bool BLOCKS>
 __device__ __forceinline__ PgList pg_list(const PageAttnArgs &a, uint32_t unit) {
     PgList l;
-    const uint32_t bt = unit / (uint32_t)a.Hkv;
+    const uint32_t bt = pg_div(unit, a.hkv_magic);
     l.hk = (int)(unit - bt * (uint32_t)a.Hkv);
-    l.b = BLOCKS ? bt / (uint32_t)a.T : bt;
+    l.b = BLOCKS ? pg_div(bt, a.t_magic) : bt;
     l.t = BLOCKS ? (int)(bt - (uint32_t)l.b * (uint32_t)a.T) : 0;
+    return l;
+}
+template <bool BLOCKS>
+__device__ __forceinline__ void pg_length(const PageAttnArgs &a, PgList &l) {
     const int64_t len = a.seq_lens[l.b];
     l.bad = len < 0 || len > (a.max_pages << a.page_shift);
     if constexpr (BLOCKS) {
@@ -145,7 +167,6 @@ __device__ __forceinline__ PgList pg_list(const PageAttnArgs &a, uint32_t unit) 
         l.base = l.seen - l.nd;
         l.tiles = (l.seen + kPgTile - 1) / kPgTile;
     }
-    return l;
 }
 // tiles of a split: even shares, so the splits of a short list are short
 __device__ __forceinline__ int64_t pg_share(int64_t tiles, int splits) {
@@ -162,26 +183,50 @@ struct PgValues {
     uint32_t v[8];               // code bytes 4 n .. + 3 of tokens 16 (i / 4) + 4 g + i % 4
 };
 
-template <int NR, bool QJL, bool HL, bool BLOCKS>
-__global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(PageAttnArgs a) {
-    using L = Pg<NR, QJL, HL>;
-    constexpr int NW = L::NW;
+template <int NR, bool QJL, bool HL, bool BLOCKS, int NW>
+__global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
+    using L = Pg<NR, QJL, HL, NW>;
     __shared__ __attribute__((aligned(16))) unsigned char smem[L::kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
 
-    // block -> (unit, split, row chunk): the chunks of one (unit, split) eight
-    // blocks apart, so that they run on one XCD and share its L2
-    const uint32_t grp = blockIdx.x / (8u * (uint32_t)a.chunks);
-    const uint32_t rest = blockIdx.x - grp * 8u * (uint32_t)a.chunks;
-    const uint32_t us = grp * 8u + (rest & 7u);
-    const int chunk = (int)(rest >> 3);
-    if (us >= (uint32_t)a.units * (uint32_t)a.splits) return;
-    const uint32_t unit = us / (uint32_t)a.splits;
-    const int split = (int)(us - unit * (uint32_t)a.splits);
-    const PgList li = pg_list<BLOCKS>(a, unit);
+    // x: eight units, then row chunks; y: splits; z: groups of eight units.  The
+    // chunks of one (unit, split) are eight blocks apart: they run on one XCD
+    // and share its L2.
+    const uint32_t unit = blockIdx.z * 8u + (blockIdx.x & 7u);
+    const int chunk = (int)(blockIdx.x >> 3), split = (int)blockIdx.y;
+    if (unit >= (uint32_t)a.units) return;
+    PgList li = pg_list<BLOCKS>(a, unit);
     const int hk = li.hk;
+
+    // ── query rows, four a wave, on their way: 16 lanes a row, eight dims a lane ──
+    constexpr int kPasses = NR * 4 / NW + (NR * 4 % NW ? 1 : 0);
+    const int c = lane & 15;                                // dims 8 c .. + 7
+    uint4 q_raw[kPasses];
+    uint2 q_flip = make_uint2(0u, 0u);
+    bool q_ok[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int rl = 4 * (wave + i * NW) + g, rho = chunk * NR * 16 + rl;     // row of the block, of the unit
+        q_ok[i] = rl < NR * 16 && rho < a.rows;
+        const int rr = q_ok[i] ? rho : 0;
+        const int t = BLOCKS ? li.t : (int)pg_div((uint32_t)rr, a.g_magic);
+        const int hq = hk * a.G + (BLOCKS ? rr : rr - t * a.G);
+        q_raw[i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + ((li.b * a.Hq + hq) * a.T + t) * 128 + 8 * c);
+    }
+    if (a.sign_flip) q_flip = *reinterpret_cast<const uint2 *>(a.sign_flip + 8 * c);
+    // G rows 16 cb + n, word g, for the product of row group rg that this wave forms
+    constexpr int kGPasses = QJL ? kPasses : 0;
+    uint32_t g_word[QJL ? kPasses : 1];
+#pragma unroll
+    for (int i = 0; i < kGPasses; ++i) g_word[i] = a.g_bits[((int64_t)hk * 64 + 16 * ((wave + i * NW) & 3) + n) * 4 + g];
+    uint64_t sees_row = 0;
+    if (!BLOCKS && tid < NR * 16 && chunk * NR * 16 + tid < a.rows)
+        sees_row = (uint64_t)a.tree[li.b * a.tree_stride + pg_div((uint32_t)(chunk * NR * 16 + tid), a.g_magic)];
+    const float cent = (a.codebooks + (a.per_head ? hk * 16 : 0))[c];      // lane l: centroid l % 16
+
+    pg_length<BLOCKS>(a, li);
     const int64_t share = pg_share(li.tiles, a.splits);
     const int64_t t_begin = split * share, t_end = t_begin + share < li.tiles ? t_begin + share : li.tiles;
     if (split > 0 && t_begin >= li.tiles) return;           // the merge counts the splits that have tiles
@@ -278,30 +323,11 @@ __global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(P
     };
     fetch_slots(0);
 
-    // ── the query rows of wave w < NR, on their way ───────────────────
-    const bool rows_mine = wave < NR;
-    const int q_rho = (chunk * NR + wave) * 16 + n;
-    uint4 q_raw[4];
-    uint2 q_flip[4];
-    uint32_t g_word[4];
-    if (rows_mine) {
-        const int rr = q_rho < a.rows ? q_rho : 0;
-        const int t = BLOCKS ? li.t : (int)((uint32_t)rr / (uint32_t)a.G);
-        const int hq = hk * a.G + (BLOCKS ? rr : rr - t * a.G);
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + ((li.b * a.Hq + hq) * a.T + t) * 128 + 32 * g;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            q_raw[s] = reinterpret_cast<const uint4 *>(src)[s];
-            if (a.sign_flip) q_flip[s] = *reinterpret_cast<const uint2 *>(a.sign_flip + 32 * g + 8 * s);
-            if (QJL) g_word[s] = a.g_bits[((int64_t)hk * 64 + 16 * s + n) * 4 + g];
-        }
-    }
-
     // ── tables ────────────────────────────────────────────────────────
-    const float *cbp = a.codebooks + (a.per_head ? hk * 16 : 0);
-    float cmax = 0.0f;
+    float cmax = fabsf(cent);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) cmax = fmaxf(cmax, fabsf(cbp[k]));
+    for (int m = 1; m < 16; m <<= 1) cmax = fmaxf(cmax, pg_row_xor(cmax, m, c));
+    cmax = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(cmax)));
     int cexp = 0;
     if (cmax > 0.0f && cmax < INFINITY) frexpf(cmax, &cexp);
     cexp = cexp < -100 ? -100 : cexp;
@@ -309,11 +335,16 @@ __global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(P
     // of small ones; else 1, for norms, which follow them, up to 65504 of it
     constexpr int kc = HL ? 10 : 0;
     const float cmul = ldexpf(1.0f, kc - cexp), cdiv = ldexpf(1.0f, cexp - kc);
-    for (int m = tid; m < kLutBytes / 16; m += 64 * NW) {
-        const int e = m >> 4;
-        const float c0 = cbp[e & 15] * cmul, c1 = cbp[e >> 4] * cmul;
-        const uint32_t hi = pg_pack(c0, c1), lo = pg_pack(c0 - pg_h_lo(hi), c1 - pg_h_hi(hi));
-        *reinterpret_cast<uint4 *>(smem + 16 * m) = make_uint4(hi, lo, hi, lo);
+    {
+        const uint16_t h = f32_to_f16_rne(cent * cmul);
+        const uint32_t both = (uint32_t)h | ((uint32_t)f32_to_f16_rne(cent * cmul - f16_to_f32(h)) << 16);
+#pragma unroll
+        for (int i = 0; i < (4096 + 64 * NW - 1) / (64 * NW); ++i) {
+            const int m = tid + 64 * NW * i, e = m >> 4;           // 16 threads a byte
+            const uint32_t w0 = __shfl(both, e & 15), w1 = __shfl(both, (e >> 4) & 15);
+            const uint32_t hi = __builtin_amdgcn_perm(w1, w0, 0x05040100u), lo = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+            if (m < 4096) *reinterpret_cast<uint4 *>(smem + 16 * m) = make_uint4(hi, lo, hi, lo);
+        }
     }
 
     // ── the first tiles, on their way ─────────────────────────────────
@@ -323,146 +354,123 @@ __global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(P
     int nv0 = 0, nv1 = 0;                                   // tokens of each half that the list holds: low byte, next byte
     if (cnt > 0) {
         load(K0, V0, nv0, 0);
-        if constexpr (L::kAhead) load(K1, V1, nv1, 1);
+        if constexpr (L::PF == 2) load(K1, V1, nv1, 1);
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    // ── query rows: wave w < NR turns row group w into MFMA operands ──
-    uint4 *qimg = reinterpret_cast<uint4 *>(smem + kQimgOff) + (wave < NR ? wave : 0) * L::kSteps * 64 + lane;      // [rg][step][lane]
-    float *csc_l = reinterpret_cast<float *>(smem + L::kCsc);
-    if (rows_mine) {
-        const bool ok = q_rho < a.rows;
-        float x[4][8];
+    // ── query rows into MFMA operands ─────────────────────────────────
+    uint4 *qimg = reinterpret_cast<uint4 *>(smem + kQimgOff);      // [rg][step][lane]
+    float *csc_l = reinterpret_cast<float *>(smem + L::kMoved + L::kCsc);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint32_t w[4] = {q_raw[s].x, q_raw[s].y, q_raw[s].z, q_raw[s].w};
+    for (int i = 0; i < kPasses; ++i) {
+        const int rl = 4 * (wave + i * NW) + g, rg = rl >> 4;
+        if (4 * (wave + i * NW) >= NR * 16) break;                 // wave-uniform
+        float x[8];
+        {
+            const uint32_t w[4] = {q_raw[i].x, q_raw[i].y, q_raw[i].z, q_raw[i].w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint16_t h = (uint16_t)((i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
-                x[s][i] = ok ? (HL ? f16_to_f32(h) : bf16_to_f32(h)) : 0.0f;
+            for (int j = 0; j < 8; ++j) {
+                const uint16_t h = (uint16_t)((j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+                x[j] = q_ok[i] ? (HL ? f16_to_f32(h) : bf16_to_f32(h)) : 0.0f;
             }
         }
         if (a.rotate) {
-            // the normalized WHT in stage order h = 1 .. 64; the row is not
-            // rounded to q's type in between
+            // the normalized WHT in stage order h = 1 .. 64, not rounded to
+            // q's type in between
             if (a.sign_flip) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        x[s][i] = __uint_as_float(__float_as_uint(x[s][i]) ^
-                                                  (((i < 4 ? q_flip[s].x >> (8 * i) : q_flip[s].y >> (8 * i - 32)) & 0x80u) << 24));
+                for (int j = 0; j < 8; ++j)
+                    x[j] = __uint_as_float(__float_as_uint(x[j]) ^
+                                           (((j < 4 ? q_flip.x >> (8 * j) : q_flip.y >> (8 * j - 32)) & 0x80u) << 24));
             }
 #pragma unroll
             for (int h = 1; h < 8; h <<= 1)
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
+                for (int j = 0; j < 8; ++j)
+                    if (!(j & h)) {
+                        const float u = x[j], l = x[j + h];
+                        x[j] = u + l;
+                        x[j + h] = u - l;
+                    }
+            // stages 8 .. 64: lanes c ^ 1, 2, 4, 8 (an fma with +-1 rounds as the sum)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (!(i & h)) {
-                            const float u = x[s][i], l = x[s][i + h];
-                            x[s][i] = u + l;
-                            x[s][i + h] = u - l;
-                        }
+            for (int m = 1; m < 16; m <<= 1) {
+                const float sgn = c & m ? -1.0f : 1.0f;
 #pragma unroll
-            for (int h = 1; h < 4; h <<= 1)
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(sgn, x[j], pg_row_xor(x[j], m, c));
+            }
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    if (!(s & h))
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float u = x[s][i], l = x[s + h][i];
-                            x[s][i] = u + l;
-                            x[s + h][i] = u - l;
-                        }
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) xlane_pair_butterfly<16>(x[s][i], x[s][i + 1]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) xlane_pair_butterfly<32>(x[s][i], x[s][i + 1]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[s][i] *= a.wht_scale;
+            for (int j = 0; j < 8; ++j) x[j] *= a.wht_scale;
         }
-        float m = 0.0f;
+        float m = fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
+                        fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[s][i]));
-        m = pg_max_groups(m);
+        for (int k = 1; k < 16; k <<= 1) m = fmaxf(m, pg_row_xor(m, k, c));
         int ex = 0;
         if (m > 0.0f && m < INFINITY) frexpf(m, &ex);
         ex = ex < -100 ? -100 : ex;
         const float sr = ldexpf(a.qscale < 0.0f ? -1.0f : 1.0f, 15 - ex);
         // at least FLT_MIN (scores are as good as 0 either way), so that a hidden score's -inf stays one
-        if (g == 0) csc_l[16 * wave + n] = fmaxf(fabsf(a.qscale) * ldexpf(cdiv, ex - 15), __FLT_MIN__);
-        half8_t qh[4], ql[4];
+        if (c == 0) csc_l[rl] = fmaxf(fabsf(a.qscale) * ldexpf(cdiv, ex - 15), __FLT_MIN__);
+        uint32_t hw[4], lw[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            uint32_t hw[4], lw[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float v0 = x[s][2 * j] * sr, v1 = x[s][2 * j + 1] * sr;
-                hw[j] = pg_pack(v0, v1);
-                lw[j] = HL ? pg_pack(v0 - pg_h_lo(hw[j]), v1 - pg_h_hi(hw[j])) : 0u;
-            }
-            qh[s] = pg_half8(hw[0], hw[1], hw[2], hw[3]);
-            ql[s] = pg_half8(lw[0], lw[1], lw[2], lw[3]);
-            if constexpr (HL) {
-                // two bytes of codes a step, centroid and remainder side by side: q, then its remainder, against both
-                qimg[64 * (2 * s)] = make_uint4(hw[0], hw[0], hw[1], hw[1]);
-                qimg[64 * (2 * s + 1)] = make_uint4(hw[2], hw[2], hw[3], hw[3]);
-                qimg[64 * (8 + 2 * s)] = make_uint4(lw[0], lw[0], lw[1], lw[1]);
-                qimg[64 * (8 + 2 * s + 1)] = make_uint4(lw[2], lw[2], lw[3], lw[3]);
-            } else {
-                qimg[64 * s] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const float v0 = x[2 * j] * sr, v1 = x[2 * j + 1] * sr;
+            hw[j] = pg_pack(v0, v1);
+            lw[j] = HL ? pg_pack(v0 - pg_h_lo(hw[j]), v1 - pg_h_hi(hw[j])) : 0u;
         }
-        if (QJL) {
-            // G q: projections 16 cb + 4 g + i of row n
-            float p[4][4];
+        // dims 8 c .. + 7 are step c % 4 of lane (row, c / 4)
+        uint4 *dst = qimg + rg * L::kSteps * 64 + 16 * (c >> 2) + (rl & 15);
+        const int s = c & 3;
+        if constexpr (HL) {
+            // two bytes of codes a step, centroid and remainder side by side: q, then its remainder, against both
+            dst[64 * (2 * s)] = make_uint4(hw[0], hw[0], hw[1], hw[1]);
+            dst[64 * (2 * s + 1)] = make_uint4(hw[2], hw[2], hw[3], hw[3]);
+            dst[64 * (8 + 2 * s)] = make_uint4(lw[0], lw[0], lw[1], lw[1]);
+            dst[64 * (8 + 2 * s + 1)] = make_uint4(lw[2], lw[2], lw[3], lw[3]);
+        } else {
+            dst[64 * s] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+        }
+    }
+    uint64_t *sees_l = reinterpret_cast<uint64_t *>(smem + L::kMoved + L::kSees);    // per row: the drafted tokens that it sees
+    if (!BLOCKS && tid < NR * 16) sees_l[tid] = sees_row;
+    __syncthreads();
+    if constexpr (QJL) {
+        // G q: projections 16 cb + 4 g + i of row n of group rg, a wave for each (rg, cb)
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-                float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < kGPasses; ++i) {
+            const int item = wave + i * NW, rg = item >> 2, cb = item & 3;
+            if (item >= NR * 4) break;                             // wave-uniform
+            const uint4 *img = qimg + rg * L::kSteps * 64 + lane;
+            float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
+            // HL: steps of two bytes with each value twice: the halves of a pair take signs of their own, the second of a pair 0
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    uint32_t e[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t not2 = ~g_word[cb] >> (8 * s + 2 * j);
-                        e[j] = 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
-                    }
-                    const half8_t ga = pg_half8(e[0], e[1], e[2], e[3]);
-                    acc = pg_mfma(ga, qh[s], acc);
-                    if (HL) acc = pg_mfma(ga, ql[s], acc);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[cb][i] = acc[i] * a.alpha;
-            }
-            // slots 2 j and 2 j + 1 of step s: projections 32 s + 4 g + j and 16 on, whose signs lie 16 bits apart
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint32_t hw[4], lw[4];
+            for (int s = 0; s < L::kQSteps; ++s) {
+                uint32_t e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    hw[j] = pg_pack(p[2 * s][j], p[2 * s + 1][j]);
-                    lw[j] = HL ? pg_pack(p[2 * s][j] - pg_h_lo(hw[j]), p[2 * s + 1][j] - pg_h_hi(hw[j])) : 0u;
+                    if constexpr (HL) {
+                        const uint32_t not2 = ~g_word[i] >> (4 * (s & 7) + 2 * (j >> 1));
+                        e[j] = j & 1 ? 0u : 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
+                    } else {
+                        const uint32_t not2 = ~g_word[i] >> (8 * s + 2 * j);
+                        e[j] = 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
+                    }
                 }
-                qimg[64 * (L::kQSteps + s)] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                if (HL) qimg[64 * (L::kQSteps + 2 + s)] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                acc = pg_mfma(pg_half8(e[0], e[1], e[2], e[3]), __builtin_bit_cast(half8_t, img[64 * s]), acc);
+            }
+            // slots 2 j and 2 j + 1 of step s: projections 32 s + 4 g + j and 16 on, whose signs lie 16 bits apart
+            uint16_t *dst = reinterpret_cast<uint16_t *>(qimg + (rg * L::kSteps + L::kQSteps + (cb >> 1)) * 64 + lane) + (cb & 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = acc[j] * a.alpha;
+                const uint16_t h = f32_to_f16_rne(p);
+                dst[2 * j] = h;
+                if constexpr (HL) dst[2 * 64 * 8 + 2 * j] = f32_to_f16_rne(p - f16_to_f32(h));
             }
         }
+        __syncthreads();
     }
-    uint64_t *sees_l = reinterpret_cast<uint64_t *>(smem + L::kSees);    // per row: the drafted tokens that it sees
-    if (!BLOCKS && tid < NR * 16) {
-        const int rho = chunk * NR * 16 + tid;
-        sees_l[tid] = rho < a.rows ? (uint64_t)a.tree[li.b * a.tree_stride + (uint32_t)rho / (uint32_t)a.G] : 0u;
-    }
-    __syncthreads();
 
     // ── main loop ─────────────────────────────────────────────────────
     uint32_t q_off = kQimgOff + 16 * lane;
@@ -664,96 +672,129 @@ __global__ __launch_bounds__((64 * Pg<NR, QJL, HL>::NW)) void page_attn_kernel(P
         int v;
         half8_t pb[NR][2];
         uint32_t ev[4], od[4];
-        if constexpr (L::kAhead) {
-            float4_t S0[NR][2], S1[NR][2];
-            // one tile, whose scores S are there: the next one's are formed
-            // beside its weights, the one after that is asked for
-            auto step = [&](float4_t (&S)[NR][2], float4_t (&next)[NR][2], PgKeys<HL> &K, const PgKeys<HL> &Knext, PgValues &V,
-                            int &nv, int k) {
-                rows_at(clamp(k + 2), r, v);
-                settle(S, t0 + (int64_t)NW * k, nv);
-                nv = v;
-                scores(Knext, next);
-                weights(S, pb);
-                pair_codes(V, ev, od);
-                load_k(K, r);
-                load_v(V, r);
-                products(ev, od, pb);
-            };
-            scores(K0, S0);
+        // one tile; the one PF on is asked for as its registers come free.
+        // Waves in a matrix phase issue first: of a SIMD's, others then work
+        // on their weights.
+        auto step = [&](PgKeys<HL> &K, PgValues &V, int &nv, int k) {
+            float4_t S[NR][2];
+            rows_at(clamp(k + L::PF), r, v);
+            __builtin_amdgcn_s_setprio(1);
+            scores(K, S);
+            __builtin_amdgcn_s_setprio(0);
+            load_k(K, r);
+            settle(S, t0 + (int64_t)NW * k, nv);
+            nv = v;
+            weights(S, pb);
+            pair_codes(V, ev, od);
+            load_v(V, r);
+            __builtin_amdgcn_s_setprio(1);
+            products(ev, od, pb);
+            __builtin_amdgcn_s_setprio(0);
+        };
+        if constexpr (L::PF == 2) {
             for (int k = 0;;) {
-                step(S0, S1, K0, K1, V0, nv0, k);
+                step(K0, V0, nv0, k);
                 if (++k >= cnt) break;
-                step(S1, S0, K1, K0, V1, nv1, k);
+                step(K1, V1, nv1, k);
                 if (++k >= cnt) break;
             }
         } else {
-            // waves in a matrix phase issue first: of a SIMD's two, one then
-            // works on its weights
-            for (int k = 0; k < cnt; ++k) {
-                float4_t S[NR][2];
-                rows_at(clamp(k + 1), r, v);
-                __builtin_amdgcn_s_setprio(1);
-                scores(K0, S);
-                __builtin_amdgcn_s_setprio(0);
-                load_k(K0, r);
-                settle(S, t0 + (int64_t)NW * k, nv0);
-                nv0 = v;
-                weights(S, pb);
-                pair_codes(V0, ev, od);
-                load_v(V0, r);
-                __builtin_amdgcn_s_setprio(1);
-                products(ev, od, pb);
-                __builtin_amdgcn_s_setprio(0);
-            }
+            for (int k = 0; k < cnt; ++k) step(K0, V0, nv0, k);
         }
     }
 
-    // ── merge of the waves, a row group at a time ─────────────────────
+    // ── merge of the waves ────────────────────────────────────────────
+    // Every wave scales its O by 2^(m - the row's largest m) and adds up the
+    // row's sum; the slabs are then summed.
     const bool wave_bad = __builtin_amdgcn_ballot_w64(page_bad) != 0;
     const int64_t mine = t_end - t_begin;
     const int act = mine < 1 ? 1 : mine < NW ? (int)mine : NW;      // waves with tiles
     float *slab = reinterpret_cast<float *>(smem);
-    float *ml = reinterpret_cast<float *>(smem + L::kSlabs);       // [wave][16][2], then a flag per wave
+    float *m_l = reinterpret_cast<float *>(smem + L::kMoved + L::kM), *l_l = m_l + NR * 16 * NW;
+    float *flags = reinterpret_cast<float *>(smem + L::kMoved + L::kFlags);
 #pragma unroll
     for (int rg = 0; rg < NR; ++rg) {
-        __syncthreads();                                           // the tables (or the last row group's slabs) are done with
-        if ((chunk * NR + rg) * 16 >= a.rows) break;               // block-uniform
-        if (wave < act) {
-            const float l = pg_sum_groups(l_run[rg]);
-            if (g == 0) {
-                ml[(wave * 16 + n) * 2] = m_run[rg];
-                ml[(wave * 16 + n) * 2 + 1] = l;
-            }
-            if (lane == 0) ml[NW * 32 + wave] = wave_bad ? 1.0f : 0.0f;
-            float *dst = slab + (wave * 16 + n) * kPartRow;
+        const float l = pg_sum_groups(l_run[rg]);
+        if (g == 0) {
+            m_l[(rg * 16 + n) * NW + wave] = m_run[rg];
+            l_l[(rg * 16 + n) * NW + wave] = l;
+        }
+    }
+    if (lane == 0) flags[wave] = wave_bad ? 1.0f : 0.0f;
+    __syncthreads();                                               // and the tables are done with
+    float row_l[NR];
+    float nan = li.bad ? 1.0f : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float4 *d4 = reinterpret_cast<float4 *>(dst + 8 * (4 * g + i));
-                d4[0] = make_float4(oacc[rg][0][i], oacc[rg][1][i], oacc[rg][2][i], oacc[rg][3][i]);
-                d4[1] = make_float4(oacc[rg][4][i], oacc[rg][5][i], oacc[rg][6][i], oacc[rg][7][i]);
+    for (int w = 0; w < NW; w += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(flags + w);
+        nan += (f.x + f.y) + (f.z + f.w);
+    }
+#pragma unroll
+    for (int rg = 0; rg < NR; ++rg) {
+        float4 mw[NW / 4], lw[NW / 4];
+#pragma unroll
+        for (int w = 0; w < NW / 4; ++w) {
+            mw[w] = *reinterpret_cast<const float4 *>(m_l + (rg * 16 + n) * NW + 4 * w);
+            lw[w] = *reinterpret_cast<const float4 *>(l_l + (rg * 16 + n) * NW + 4 * w);
+        }
+        float m = -__FLT_MAX__;
+#pragma unroll
+        for (int w = 0; w < NW / 4; ++w) m = fmaxf(m, fmaxf(fmaxf(mw[w].x, mw[w].y), fmaxf(mw[w].z, mw[w].w)));
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW / 4; ++w) {
+            l = __builtin_fmaf(__builtin_amdgcn_exp2f(mw[w].x - m), lw[w].x, l);
+            l = __builtin_fmaf(__builtin_amdgcn_exp2f(mw[w].y - m), lw[w].y, l);
+            l = __builtin_fmaf(__builtin_amdgcn_exp2f(mw[w].z - m), lw[w].z, l);
+            l = __builtin_fmaf(__builtin_amdgcn_exp2f(mw[w].w - m), lw[w].w, l);
+        }
+        row_l[rg] = nan != 0.0f ? __builtin_nanf("") : l;
+        const float f = __builtin_amdgcn_exp2f(m_run[rg] - m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) oacc[rg][k] *= f;
+        m_run[rg] = m;
+    }
+    __syncthreads();                                               // m_l and l_l are read
+    if (wave == 0 && g == 0) {
+#pragma unroll
+        for (int rg = 0; rg < NR; ++rg) {
+            m_l[rg * 16 + n] = m_run[rg];
+            l_l[rg * 16 + n] = row_l[rg];
+        }
+    }
+#pragma unroll
+    for (int r0 = 0; r0 < NR; r0 += L::MR) {
+        if (r0) __syncthreads();                                   // the last slabs are read
+        if ((chunk * NR + r0) * 16 >= a.rows) break;               // block-uniform
+        if (wave < act) {
+#pragma unroll
+            for (int rg = r0; rg < r0 + L::MR; ++rg) {
+                float *dst = slab + ((wave * L::MR + rg - r0) * 16 + n) * kPartRow;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4 *d4 = reinterpret_cast<float4 *>(dst + 8 * (4 * g + i));
+                    d4[0] = make_float4(oacc[rg][0][i], oacc[rg][1][i], oacc[rg][2][i], oacc[rg][3][i]);
+                    d4[1] = make_float4(oacc[rg][4][i], oacc[rg][5][i], oacc[rg][6][i], oacc[rg][7][i]);
+                }
             }
         }
         __syncthreads();
-        for (int e = tid; e < 16 * 32; e += 64 * NW) {
+        for (int e = tid; e < L::MR * 16 * 32; e += 64 * NW) {
             const int r = e >> 5, d = 4 * (e & 31);
-            const int rho = (chunk * NR + rg) * 16 + r;
+            const int rho = (chunk * NR + r0) * 16 + r;
             if (rho >= a.rows) break;
-            float m = -__FLT_MAX__, l = 0.0f, nan = li.bad ? 1.0f : 0.0f;
-            for (int w = 0; w < act; ++w) m = fmaxf(m, ml[(w * 16 + r) * 2]);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < act; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + r) * 2] - m);
-                const float4 v = *reinterpret_cast<const float4 *>(slab + (w * 16 + r) * kPartRow + d);
-                l = __builtin_fmaf(f, ml[(w * 16 + r) * 2 + 1], l);
-                o.x = __builtin_fmaf(f, v.x, o.x);
-                o.y = __builtin_fmaf(f, v.y, o.y);
-                o.z = __builtin_fmaf(f, v.z, o.z);
-                o.w = __builtin_fmaf(f, v.w, o.w);
-                nan += ml[NW * 32 + w];
-            }
-            if (nan != 0.0f) l = __builtin_nanf("");
-            const int t = BLOCKS ? li.t : (int)((uint32_t)rho / (uint32_t)a.G);
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+                if (w < act) {                                     // uniform
+                    const float4 v = *reinterpret_cast<const float4 *>(slab + (w * L::MR * 16 + r) * kPartRow + d);
+                    o.x += v.x;
+                    o.y += v.y;
+                    o.z += v.z;
+                    o.w += v.w;
+                }
+            const float m = m_l[r0 * 16 + r], l = l_l[r0 * 16 + r];
+            const int t = BLOCKS ? li.t : (int)pg_div((uint32_t)rho, a.g_magic);
             if (a.splits == 1) {
                 const int hq = hk * a.G + (BLOCKS ? rho : rho - t * a.G);
                 const float s = cdiv / l;
@@ -787,7 +828,8 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
     if (row >= a.units * a.rows) return;
     const int64_t unit = row / a.rows;
     const int rho = (int)(row - unit * a.rows);
-    const PgList li = pg_list<BLOCKS>(a, (uint32_t)unit);
+    PgList li = pg_list<BLOCKS>(a, (uint32_t)unit);
+    pg_length<BLOCKS>(a, li);
     const int64_t share = pg_share(li.tiles, a.splits);
     const int act = li.tiles < 1 ? 1 : (int)((li.tiles + share - 1) / share);
     const float *base = a.ws + (unit * a.splits * a.rows + rho) * kPartRow;
@@ -822,7 +864,7 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
                 o.w = __builtin_fmaf(f, v[k].w, o.w);
             }
     }
-    const int t = BLOCKS ? li.t : rho / a.G;
+    const int t = BLOCKS ? li.t : (int)pg_div((uint32_t)rho, a.g_magic);
     const int hq = li.hk * a.G + (BLOCKS ? rho : rho - t * a.G);
     const float s = 1.0f / l;
     float v[4] = {o.x * s, o.y * s, o.z * s, o.w * s};
@@ -870,19 +912,20 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     return p;
 }
 
-template <int NR, bool HL, bool BLOCKS>
+template <int NR, bool HL, bool BLOCKS, int NW>
 static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
-    const dim3 grid((unsigned)((a.units * a.splits + 7) / 8 * 8 * a.chunks));
-    if (qjl) hipLaunchKernelGGL((page_attn_kernel<NR, true, HL, BLOCKS>), grid, dim3(64 * Pg<NR, true, HL>::NW), 0, s, a);
-    else hipLaunchKernelGGL((page_attn_kernel<NR, false, HL, BLOCKS>), grid, dim3(64 * Pg<NR, false, HL>::NW), 0, s, a);
+    const dim3 grid(8u * (unsigned)a.chunks, (unsigned)a.splits, (unsigned)((a.units + 7) / 8));
+    if (qjl) hipLaunchKernelGGL((page_attn_kernel<NR, true, HL, BLOCKS, NW>), grid, dim3(64 * NW), 0, s, a);
+    else hipLaunchKernelGGL((page_attn_kernel<NR, false, HL, BLOCKS, NW>), grid, dim3(64 * NW), 0, s, a);
 }
 
 template <bool BLOCKS>
-static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, int nr, hipStream_t s) {
+static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (nr == 1) hl ? page_launch<1, true, BLOCKS>(a, qjl, s) : page_launch<1, false, BLOCKS>(a, qjl, s);
-    else if (nr == 2) page_launch<2, false, BLOCKS>(a, qjl, s);
-    else page_launch<4, false, BLOCKS>(a, qjl, s);
+    if (hl) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
+    else if (p.nr == 1) page_launch<1, false, BLOCKS, 12>(a, qjl, s);
+    else if (p.nr == 2) page_launch<2, false, BLOCKS, 8>(a, qjl, s);
+    else page_launch<4, false, BLOCKS, 8>(a, qjl, s);
     OMNI_CHECK_LAUNCH("page_attn_kernel");
     if (a.splits > 1) {
         const unsigned blocks = (unsigned)((a.units * a.rows + 7) / 8);
@@ -892,6 +935,8 @@ static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, int nr, hipStream_t 
     }
     return OMNI_OK;
 }
+
+static uint64_t magic(int64_t d) { return (uint64_t(1) << 32) / (uint64_t)d + 1; }
 
 // The pool's geometry: page_size a power of two, every token row of the pool
 // (page, head, slot) numbered below 2^31, positions in 32 bits.
@@ -915,7 +960,7 @@ static int page_check(const char *who, const void *q, int q_dtype, const void *k
     OMNI_CHECK_ARG(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: need B >= 0 and n_heads a multiple of n_kv_heads", who);
     OMNI_CHECK_ARG(T >= 1 && T <= 64, "%s: 1 to 64 query tokens, got %lld", who, (long long)T);
     OMNI_CHECK_ARG(Hq / Hkv <= 1024, "%s: at most 1024 query heads per kv head", who);
-    OMNI_CHECK_ARG(B <= (int64_t(1) << 22) / Hkv / T, "%s: batch too large", who);
+    OMNI_CHECK_ARG(Hkv <= 4096 && B <= (int64_t(1) << 19) / Hkv / T, "%s: at most 4096 kv heads and B * T * n_kv_heads at most 2^19", who);
     OMNI_CHECK_ARG(fabsf(scale) <= 2.3e38f, "%s: scale must be finite and at most 2.3e38 in size", who);
     if (B == 0) return OMNI_OK;
     OMNI_CHECK_ARG(q && k_nib && v_nib && codebooks && out, "%s: NULL pointer", who);
@@ -954,9 +999,9 @@ extern "C" int omni_attn_tree(const void *q, int q_dtype, const uint8_t *k_nib, 
     }
     PageAttnArgs a{q, out, (float *)workspace, k_nib, k_qjl, v_nib, k_norms, codebooks, g_bits, rotate_q ? sign_flip : nullptr,
                    page_table, seq_lens, n_draft, tree, nullptr, max_pages, n_pages, tree_stride, B * Hkv, shift,
-                   per_head_codebook, Hq, Hkv, G, (int)T, (int)T * G, p.chunks, p.splits, 0, rotate_q,
+                   per_head_codebook, Hq, Hkv, G, (int)T, (int)T * G, p.chunks, p.splits, 0, rotate_q, magic(Hkv), magic(T), magic(G),
                    (float)((double)scale * 1.4426950408889634), (float)(sqrt(2.0 / M_PI) / 128.0), inv_sqrt_dim_f32(128)};
-    return page_run<false>(a, q_dtype, with_qjl != 0, p.nr, as_stream(stream));
+    return page_run<false>(a, q_dtype, with_qjl != 0, p, as_stream(stream));
 }
 
 extern "C" size_t omni_attn_blocks_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int top, int page_size, int q_dtype) {
@@ -985,9 +1030,9 @@ extern "C" int omni_attn_blocks(const void *q, int q_dtype, const uint8_t *k_nib
     }
     PageAttnArgs a{q, out, (float *)workspace, k_nib, k_qjl, v_nib, k_norms, codebooks, g_bits, rotate_q ? sign_flip : nullptr,
                    page_table, seq_lens, nullptr, nullptr, blocks, max_pages, n_pages, 0, B * T * Hkv, shift,
-                   per_head_codebook, Hq, Hkv, G, (int)T, G, p.chunks, p.splits, top, rotate_q,
+                   per_head_codebook, Hq, Hkv, G, (int)T, G, p.chunks, p.splits, top, rotate_q, magic(Hkv), magic(T), magic(G),
                    (float)((double)scale * 1.4426950408889634), (float)(sqrt(2.0 / M_PI) / 128.0), inv_sqrt_dim_f32(128)};
-    return page_run<true>(a, q_dtype, with_qjl != 0, p.nr, as_stream(stream));
+    return page_run<true>(a, q_dtype, with_qjl != 0, p, as_stream(stream));
 }
 
 // ── prepared calls (PagedTreeAttention, PagedBlockAttention) ────────────

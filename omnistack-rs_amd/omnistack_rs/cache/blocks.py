@@ -65,7 +65,7 @@ def select_blocks(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor
     if validate:
         _ascend(cb)
     qc = aligned(q)
-    sf = _lib.sign_flip_i8(sign_flip, D, dev) if (rotate_q and sign_flip is not None) else None
+    sf = aligned(_lib.sign_flip_i8(sign_flip, D, dev), 8) if (rotate_q and sign_flip is not None) else None
     blocks = torch.empty(B, cache.n_kv_heads, T, top, dtype=torch.int32, device=dev)
     L = _lib.lib()
     ws_bytes = L.omni_block_select_workspace_size(B, cache.n_kv_heads, T, pt.shape[1], top)
