@@ -83,7 +83,7 @@ struct Pg {
     static constexpr int kFlags = kM + 2 * NR * 16 * NW * 4;                 // per wave: met a page outside the pool
     static constexpr int kUse = kFlags + 16 * 4;
     // the merge: the waves' O of MR row groups at a time, from 0 on (over the tables and the query rows)
-    static constexpr int MR = NR > 1 && NW <= 8 ? 2 : 1;
+    static constexpr int MR = NR % 2 == 0 && NW <= 8 ? 2 : 1;
     static constexpr int kSlabs = NW * MR * 16 * kPartRow * 4;
     static constexpr int kMoved = kSlabs > kCsc ? kSlabs - kCsc : 0;         // what lies behind them moves up
     static constexpr int kLds = kUse + kMoved;
@@ -888,26 +888,29 @@ struct PagePlan {
 // Row groups per block and splits of a call: `units` lists of at most `tiles`
 // tiles, `rows` query rows each.
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
-    PagePlan p;
-    p.nr = rows <= 16 || hl ? 1 : rows <= 32 ? 2 : 4;
-    p.chunks = (rows + 16 * p.nr - 1) / (16 * p.nr);
-    const int64_t cus = device_cus(), blocks = units * p.chunks;
-    const double tile = (p.nr == 1 ? 0.21 : p.nr == 2 ? 0.25 : 0.35) * (hl ? 1.6 : 1.0);
+    // us: a block's fixed part, and per tile by its row groups
+    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.21, 0.30, 0.37, 0.45}, kTileHl = 0.36;
+    const int64_t cus = device_cus();
+    PagePlan p{1, 1, 1, 0};
     double best = 1e30;
-    p.splits = 1;
-    auto consider = [&](int64_t s) {
-        if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
-        const double t = (double)((blocks * s + cus - 1) / cus) * (5.0 + tile * (double)((tiles + s - 1) / s)) +
-                         (s > 1 ? 3.0 + 0.03 * (double)s : 0.0);
-        if (t < best) {
-            best = t;
-            p.splits = (int)s;
-        }
-    };
-    consider(1);
-    if (blocks > 0)
+    for (int nr = 1; nr <= (hl ? 1 : 4); ++nr) {
+        const int chunks = (rows + 16 * nr - 1) / (16 * nr);
+        const int64_t blocks = units * chunks;
+        auto consider = [&](int64_t s) {
+            if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
+            const double t = (double)((blocks * s + cus - 1) / cus) * (kFixed + (hl ? kTileHl : kTile[nr]) * (double)((tiles + s - 1) / s)) +
+                             (s > 1 ? 3.0 + 0.03 * (double)s + (double)units * (double)s * rows * kPartRow * 4e-6 * 2 / 3.5 : 0.0);
+            if (t < best) {
+                best = t;
+                p.nr = nr;
+                p.chunks = chunks;
+                p.splits = (int)s;
+            }
+        };
+        consider(1);
         for (int r = 1; r <= 4; ++r)
             for (int k = 0; k < 3; ++k) consider(r * cus / (blocks << k));
+    }
     p.ws = p.splits > 1 ? (size_t)units * p.splits * rows * kPartRow * 4 : 0;
     return p;
 }
@@ -925,6 +928,7 @@ static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, h
     if (hl) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
     else if (p.nr == 1) page_launch<1, false, BLOCKS, 12>(a, qjl, s);
     else if (p.nr == 2) page_launch<2, false, BLOCKS, 8>(a, qjl, s);
+    else if (p.nr == 3) page_launch<3, false, BLOCKS, 8>(a, qjl, s);
     else page_launch<4, false, BLOCKS, 8>(a, qjl, s);
     OMNI_CHECK_LAUNCH("page_attn_kernel");
     if (a.splits > 1) {
