@@ -71,9 +71,9 @@ constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dwor
 template <int NR, bool QJL, bool HL, int WAVES>
 struct Pg {
     static constexpr int NW = WAVES;
-    static constexpr bool kQReg = NR <= 2;                                   // query operands in registers (else LDS)
-    static constexpr int PF = NR <= 2 ? 2 : 1;                               // tiles a wave holds
-    static constexpr int kQSteps = HL ? 16 : 4;                              // B operands of a row group: q (HL: twice eight),
+    static constexpr int kQKept = NR > 2 ? 0 : HL && NR == 2 ? 8 : 99;                                   // query operands in registers (else LDS)
+    static constexpr int PF = NR <= (HL ? 1 : 2) ? 2 : 1;                               // tiles a wave holds
+    static constexpr int kQSteps = HL ? 8 : 4;                               // B operands of a row group: q (HL: twice four),
     static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
     static constexpr int kSteps = kQSteps + kGSteps;
     static constexpr int kQimg = NR * kSteps * 1024;
@@ -422,15 +422,8 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
         // dims 8 c .. + 7 are step c % 4 of lane (row, c / 4)
         uint4 *dst = qimg + rg * L::kSteps * 64 + 16 * (c >> 2) + (rl & 15);
         const int s = c & 3;
-        if constexpr (HL) {
-            // two bytes of codes a step, centroid and remainder side by side: q, then its remainder, against both
-            dst[64 * (2 * s)] = make_uint4(hw[0], hw[0], hw[1], hw[1]);
-            dst[64 * (2 * s + 1)] = make_uint4(hw[2], hw[2], hw[3], hw[3]);
-            dst[64 * (8 + 2 * s)] = make_uint4(lw[0], lw[0], lw[1], lw[1]);
-            dst[64 * (8 + 2 * s + 1)] = make_uint4(lw[2], lw[2], lw[3], lw[3]);
-        } else {
-            dst[64 * s] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-        }
+        dst[64 * s] = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+        if constexpr (HL) dst[64 * (4 + s)] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
     }
     uint64_t *sees_l = reinterpret_cast<uint64_t *>(smem + L::kMoved + L::kSees);    // per row: the drafted tokens that it sees
     if (!BLOCKS && tid < NR * 16) sees_l[tid] = sees_row;
@@ -443,19 +436,13 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
             if (item >= NR * 4) break;                             // wave-uniform
             const uint4 *img = qimg + rg * L::kSteps * 64 + lane;
             float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
-            // HL: steps of two bytes with each value twice: the halves of a pair take signs of their own, the second of a pair 0
 #pragma unroll
             for (int s = 0; s < L::kQSteps; ++s) {
                 uint32_t e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if constexpr (HL) {
-                        const uint32_t not2 = ~g_word[i] >> (4 * (s & 7) + 2 * (j >> 1));
-                        e[j] = j & 1 ? 0u : 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
-                    } else {
-                        const uint32_t not2 = ~g_word[i] >> (8 * s + 2 * j);
-                        e[j] = 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
-                    }
+                    const uint32_t not2 = ~g_word[i] >> (8 * (s & 3) + 2 * j);
+                    e[j] = 0x3C003C00u | ((not2 & 1u) << 15) | ((not2 & 2u) << 30);
                 }
                 acc = pg_mfma(pg_half8(e[0], e[1], e[2], e[3]), __builtin_bit_cast(half8_t, img[64 * s]), acc);
             }
@@ -474,15 +461,16 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
 
     // ── main loop ─────────────────────────────────────────────────────
     uint32_t q_off = kQimgOff + 16 * lane;
-    half8_t qr[L::kQReg ? NR : 1][L::kSteps];
-    if constexpr (L::kQReg) {
+    constexpr int kKept = L::kQKept < L::kSteps ? L::kQKept : L::kSteps;
+    half8_t qr[NR][kKept + 1];
+    {
 #pragma unroll
         for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
-            for (int s = 0; s < L::kSteps; ++s) qr[rg][s] = *reinterpret_cast<const half8_t *>(smem + q_off + (rg * L::kSteps + s) * 1024);
+            for (int s = 0; s < kKept; ++s) qr[rg][s] = *reinterpret_cast<const half8_t *>(smem + q_off + (rg * L::kSteps + s) * 1024);
     }
     auto q_at = [&](int rg, int s) {
-        if constexpr (L::kQReg) return qr[rg][s];
+        if (s < kKept) return qr[rg][s];
         else return *reinterpret_cast<const half8_t *>(smem + q_off + (rg * L::kSteps + s) * 1024);
     };
     float csc[NR], m_run[NR], l_run[NR];
@@ -508,6 +496,14 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
         for (int j = 0; j < 4; ++j) h[j] = *reinterpret_cast<const uint32_t *>(entry(w, j));
         return pg_half8(h[0], h[1], h[2], h[3]);
     };
+    // HL: and their remainders
+    auto four_pairs = [&](uint32_t w, half8_t &hi, half8_t &lo) {
+        uint2 e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = *reinterpret_cast<const uint2 *>(entry(w, j));
+        hi = pg_half8(e[0].x, e[1].x, e[2].x, e[3].x);
+        lo = pg_half8(e[0].y, e[1].y, e[2].y, e[3].y);
+    };
     // centroids and remainders of byte i of x and byte j of y
     auto two_bytes = [&](uint32_t x, int i, uint32_t y, int j) {
         const uint2 e0 = *reinterpret_cast<const uint2 *>(entry(x, i)), e1 = *reinterpret_cast<const uint2 *>(entry(y, j));
@@ -515,37 +511,14 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
     };
     // scores of a tile, raw: lane (n, g) holds tokens 16 u + 4 g + i of row n
     auto scores = [&](const PgKeys<HL> &R, float4_t (&acc)[NR][2]) {
-        if constexpr (!L::kQReg) asm volatile("" : "+v"(q_off));       // read again for each tile, not kept (and spilled)
+        if constexpr (kKept < L::kSteps) asm volatile("" : "+v"(q_off));       // read again for each tile, not kept (and spilled)
 #pragma unroll
         for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
             for (int u = 0; u < 2; ++u) acc[rg][u] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < (HL ? 8 : 4); ++s) {
-            half8_t A[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t kw[4] = {R.k[u].x, R.k[u].y, R.k[u].z, R.k[u].w};
-                if constexpr (HL) A[u] = two_bytes(kw[s >> 1], 2 * (s & 1), kw[s >> 1], 2 * (s & 1) + 1);
-                else A[u] = four_bytes(kw[s]);
-            }
-#pragma unroll
-            for (int rg = 0; rg < NR; ++rg)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    acc[rg][u] = pg_mfma(A[u], q_at(rg, s), acc[rg][u]);
-                    if constexpr (HL) acc[rg][u] = pg_mfma(A[u], q_at(rg, 8 + s), acc[rg][u]);
-                }
-        }
         if constexpr (QJL) {
-            // the signs' part: the norm rides on the signs (fp16, 2^-12 of a
-            // small term), so that it adds to the same sums; HL: +-1, and sums
-            // of its own
-            float4_t qacc[HL ? NR : 1][2];
-            if constexpr (HL) {
-#pragma unroll
-                for (int rg = 0; rg < NR; ++rg) qacc[rg][0] = qacc[rg][1] = float4_t{0.f, 0.f, 0.f, 0.f};
-            }
+            // the signs' part.  The norm rides on the signs (fp16, 2^-12 of a
+            // small term); HL: +-1, and the sums times the norms
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 half8_t A[2];
@@ -562,12 +535,8 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
                 for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        if constexpr (HL) {
-                            qacc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), qacc[rg][u]);
-                            qacc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + 2 + s), qacc[rg][u]);
-                        } else {
-                            acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), acc[rg][u]);
-                        }
+                        acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), acc[rg][u]);
+                        if constexpr (HL) acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + 2 + s), acc[rg][u]);
                     }
             }
             if constexpr (HL) {
@@ -577,9 +546,29 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
                     for (int i = 0; i < 4; ++i) {
                         const float ni = R.nr[u][i] * cmul;
 #pragma unroll
-                        for (int rg = 0; rg < NR; ++rg) acc[rg][u][i] = __builtin_fmaf(ni, qacc[rg][u][i], acc[rg][u][i]);
+                        for (int rg = 0; rg < NR; ++rg) acc[rg][u][i] *= ni;
                     }
             }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            half8_t A[2], Al[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t kw[4] = {R.k[u].x, R.k[u].y, R.k[u].z, R.k[u].w};
+                if constexpr (HL) four_pairs(kw[s], A[u], Al[u]);
+                else A[u] = four_bytes(kw[s]);
+            }
+#pragma unroll
+            for (int rg = 0; rg < NR; ++rg)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    acc[rg][u] = pg_mfma(A[u], q_at(rg, s), acc[rg][u]);
+                    if constexpr (HL) {                     // without remainder times remainder, 2^-24 of it
+                        acc[rg][u] = pg_mfma(A[u], q_at(rg, 4 + s), acc[rg][u]);
+                        acc[rg][u] = pg_mfma(Al[u], q_at(rg, s), acc[rg][u]);
+                    }
+                }
         }
     };
     // Masks, and a row's running maximum raised where some lane's passes it by
@@ -889,16 +878,16 @@ struct PagePlan {
 // tiles, `rows` query rows each.
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     // us: a block's fixed part, and per tile by its row groups
-    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.21, 0.30, 0.37, 0.45}, kTileHl = 0.36;
+    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.21, 0.30, 0.37, 0.45}, kTileHl[5] = {0.0, 0.30, 0.37, 0.55, 0.70};
     const int64_t cus = device_cus();
     PagePlan p{1, 1, 1, 0};
     double best = 1e30;
-    for (int nr = 1; nr <= (hl ? 1 : 4); ++nr) {
+    for (int nr = 1; nr <= 4; ++nr) {
         const int chunks = (rows + 16 * nr - 1) / (16 * nr);
         const int64_t blocks = units * chunks;
         auto consider = [&](int64_t s) {
             if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
-            const double t = (double)((blocks * s + cus - 1) / cus) * (kFixed + (hl ? kTileHl : kTile[nr]) * (double)((tiles + s - 1) / s)) +
+            const double t = (double)((blocks * s + cus - 1) / cus) * (kFixed + (hl ? kTileHl[nr] : kTile[nr]) * (double)((tiles + s - 1) / s)) +
                              (s > 1 ? 3.0 + 0.03 * (double)s + (double)units * (double)s * rows * kPartRow * 4e-6 * 2 / 3.5 : 0.0);
             if (t < best) {
                 best = t;
@@ -925,7 +914,10 @@ static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
 template <bool BLOCKS>
 static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (hl) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
+    if (hl && p.nr == 1) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
+    else if (hl && p.nr == 2) page_launch<2, true, BLOCKS, 8>(a, qjl, s);
+    else if (hl && p.nr == 3) page_launch<3, true, BLOCKS, 8>(a, qjl, s);
+    else if (hl) page_launch<4, true, BLOCKS, 8>(a, qjl, s);
     else if (p.nr == 1) page_launch<1, false, BLOCKS, 12>(a, qjl, s);
     else if (p.nr == 2) page_launch<2, false, BLOCKS, 8>(a, qjl, s);
     else if (p.nr == 3) page_launch<3, false, BLOCKS, 8>(a, qjl, s);
