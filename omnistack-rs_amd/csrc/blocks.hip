@@ -127,14 +127,13 @@ __device__ __forceinline__ double whole_scale(double most) {
 __device__ __forceinline__ int whole(double x) { return (int)fmin(fmax(__builtin_rint(x), -127.0), 127.0); }
 
 // Bits 0 .. 3 (NIBBLE 0) or 4 .. 7 of four bytes, codes, to four int8 centroids
-// from the 16-byte table t: both halves of the table by the low three bits, the
-// fourth choosing between them (byte selectors 12 and 13 give 0x00 and 0xff).
+// from the 16-byte table t: both halves of the table by the low three bits,
+// then byte k of either by the fourth.
 template <int NIBBLE>
 __device__ __forceinline__ uint32_t four_centroids(uint32_t x, const uint32_t (&t)[4]) {
     const uint32_t sel = (NIBBLE ? x >> 4 : x) & 0x07070707u;
     const uint32_t low = __builtin_amdgcn_perm(t[1], t[0], sel), high = __builtin_amdgcn_perm(t[3], t[2], sel);
-    const uint32_t up = __builtin_amdgcn_perm(0u, 0u, ((x >> (NIBBLE ? 7 : 3)) & 0x01010101u) | 0x0C0C0C0Cu);
-    return (low & ~up) | (high & up);
+    return __builtin_amdgcn_perm(high, low, ((x >> (NIBBLE ? 5 : 1)) & 0x04040404u) | 0x03020100u);
 }
 
 constexpr int kSelWaves = 8;
@@ -469,7 +468,7 @@ __device__ __forceinline__ void pick_held(uint32_t *keys, int n, uint32_t kmin, 
 // query's blocks by a thread block, so that a wave's load is 8 / heads pages'
 // neighbouring bounds, a KB.
 __global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectArgs a) {
-    constexpr int U = 8;                                          // loads in flight
+    constexpr int U = 4;                                          // loads in flight
     __shared__ __attribute__((aligned(16))) int8_t qs[8][256];
     __shared__ __attribute__((aligned(16))) int8_t cs[8][16];
     __shared__ double part[8][256];
@@ -761,7 +760,7 @@ extern "C" int omni_block_select(const void *q, int q_dtype, const uint8_t *boun
     a.heads = Hkv % 8 == 0 ? 8 : 8 % Hkv == 0 ? Hkv : 1;
     if (ws && max_pages > 1024 && 2 * rows <= cus) {
         // about two thread blocks a CU, whole rounds of their waves
-        const int64_t round = 8 / a.heads * 8 * kSelWaves;
+        const int64_t round = 8 / a.heads * 4 * kSelWaves;
         int64_t per = max_pages * (rows / a.heads) / (2 * cus) / round * round;
         per = per < round ? round : per;
         a.per_block = (int)per;
