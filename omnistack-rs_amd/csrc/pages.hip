@@ -72,7 +72,6 @@ template <int NR, bool QJL, bool HL, int WAVES>
 struct Pg {
     static constexpr int NW = WAVES;
     static constexpr int kQKept = NR > 2 ? 0 : HL && NR == 2 ? 8 : 99;                                   // query operands in registers (else LDS)
-    static constexpr int PF = NR <= (HL ? 1 : 2) ? 2 : 1;                               // tiles a wave holds
     static constexpr int kQSteps = HL ? 8 : 4;                               // B operands of a row group: q (HL: twice four),
     static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
     static constexpr int kSteps = kQSteps + kGSteps;
@@ -315,12 +314,6 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
         }
     };
     auto clamp = [&](int k) { return k < cnt ? k : cnt - 1; };     // past the end: the last tile again, from cache
-    auto load = [&](PgKeys<HL> &K, PgValues &V, int &v, int k) {
-        uint32_t r[2];
-        rows_at(clamp(k), r, v);
-        load_k(K, r);
-        load_v(V, r);
-    };
     fetch_slots(0);
 
     // ── tables ────────────────────────────────────────────────────────
@@ -349,12 +342,14 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
 
     // ── the first tiles, on their way ─────────────────────────────────
     fetch_rows();
-    PgKeys<HL> K0, K1;
-    PgValues V0, V1;
-    int nv0 = 0, nv1 = 0;                                   // tokens of each half that the list holds: low byte, next byte
+    PgKeys<HL> K;
+    PgValues V;
+    int nv = 0;                                   // tokens of each half that the list holds: low byte, next byte
     if (cnt > 0) {
-        load(K0, V0, nv0, 0);
-        if constexpr (L::PF == 2) load(K1, V1, nv1, 1);
+        uint32_t r[2];
+        rows_at(0, r, nv);
+        load_k(K, r);
+        load_v(V, r);
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -658,37 +653,27 @@ __global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
     if (cnt > 0) {
         const int64_t t0 = t_begin + wave;
         uint32_t r[2];
-        int v;
         half8_t pb[NR][2];
         uint32_t ev[4], od[4];
-        // one tile; the one PF on is asked for as its registers come free.
-        // Waves in a matrix phase issue first: of a SIMD's, others then work
-        // on their weights.
-        auto step = [&](PgKeys<HL> &K, PgValues &V, int &nv, int k) {
+        // The next tile is asked for as its registers come free.  Waves in a
+        // matrix phase issue first: of a SIMD's, others then work on their
+        // weights.
+        for (int k = 0; k < cnt; ++k) {
             float4_t S[NR][2];
-            rows_at(clamp(k + L::PF), r, v);
+            int next;
+            rows_at(clamp(k + 1), r, next);
             __builtin_amdgcn_s_setprio(1);
             scores(K, S);
             __builtin_amdgcn_s_setprio(0);
             load_k(K, r);
             settle(S, t0 + (int64_t)NW * k, nv);
-            nv = v;
+            nv = next;
             weights(S, pb);
             pair_codes(V, ev, od);
             load_v(V, r);
             __builtin_amdgcn_s_setprio(1);
             products(ev, od, pb);
             __builtin_amdgcn_s_setprio(0);
-        };
-        if constexpr (L::PF == 2) {
-            for (int k = 0;;) {
-                step(K0, V0, nv0, k);
-                if (++k >= cnt) break;
-                step(K1, V1, nv1, k);
-                if (++k >= cnt) break;
-            }
-        } else {
-            for (int k = 0; k < cnt; ++k) step(K0, V0, nv0, k);
         }
     }
 
@@ -871,6 +856,7 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
 
 struct PagePlan {
     int nr, chunks, splits;
+    bool wide;                   // one row group: twelve waves
     size_t ws;
 };
 
@@ -878,9 +864,9 @@ struct PagePlan {
 // tiles, `rows` query rows each.
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     // us: a block's fixed part, and per tile by its row groups
-    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.21, 0.30, 0.37, 0.45}, kTileHl[5] = {0.0, 0.30, 0.37, 0.55, 0.70};
+    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.18, 0.27, 0.36, 0.46}, kTileHl[5] = {0.0, 0.27, 0.36, 0.53, 0.70};
     const int64_t cus = device_cus();
-    PagePlan p{1, 1, 1, 0};
+    PagePlan p{1, 1, 1, false, 0};
     double best = 1e30;
     for (int nr = 1; nr <= 4; ++nr) {
         const int chunks = (rows + 16 * nr - 1) / (16 * nr);
@@ -900,6 +886,7 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
         for (int r = 1; r <= 4; ++r)
             for (int k = 0; k < 3; ++k) consider(r * cus / (blocks << k));
     }
+    p.wide = tiles / p.splits >= 64;
     p.ws = p.splits > 1 ? (size_t)units * p.splits * rows * kPartRow * 4 : 0;
     return p;
 }
@@ -914,11 +901,14 @@ static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
 template <bool BLOCKS>
 static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (hl && p.nr == 1) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
+    if (p.nr == 1 && p.wide) {
+        if (hl) page_launch<1, true, BLOCKS, 12>(a, qjl, s);
+        else page_launch<1, false, BLOCKS, 12>(a, qjl, s);
+    } else if (hl && p.nr == 1) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
     else if (hl && p.nr == 2) page_launch<2, true, BLOCKS, 8>(a, qjl, s);
     else if (hl && p.nr == 3) page_launch<3, true, BLOCKS, 8>(a, qjl, s);
     else if (hl) page_launch<4, true, BLOCKS, 8>(a, qjl, s);
-    else if (p.nr == 1) page_launch<1, false, BLOCKS, 12>(a, qjl, s);
+    else if (p.nr == 1) page_launch<1, false, BLOCKS, 8>(a, qjl, s);
     else if (p.nr == 2) page_launch<2, false, BLOCKS, 8>(a, qjl, s);
     else if (p.nr == 3) page_launch<3, false, BLOCKS, 8>(a, qjl, s);
     else page_launch<4, false, BLOCKS, 8>(a, qjl, s);
