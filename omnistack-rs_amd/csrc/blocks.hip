@@ -723,8 +723,13 @@ extern "C" int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t 
     return OMNI_OK;
 }
 
+// One launch where a row's blocks are few or the rows fill the chip; else the
+// scores over the whole chip first.
+static bool score_first(int64_t rows, int64_t max_pages) { return max_pages > 1024 && 2 * rows <= device_cus(); }
+
 extern "C" size_t omni_block_select_workspace_size(int64_t B, int Hkv, int64_t T, int64_t max_pages, int top) {
-    if (B <= 0 || Hkv <= 0 || T <= 0 || max_pages <= top) return 0;
+    if (B <= 0 || B > 65535 || Hkv <= 0 || Hkv > 65535 || T <= 0 || T > 64 || max_pages <= top || max_pages > (1 << 26)) return 0;
+    if (max_pages <= kPickLds && !score_first(B * Hkv * T, max_pages)) return 0;      // a row's scores stay in LDS
     return (size_t)B * Hkv * T * max_pages * 4;
 }
 
@@ -754,11 +759,9 @@ extern "C" int omni_block_select(const void *q, int q_dtype, const uint8_t *boun
                  max_pages, n_pages, shift, per_head_codebook, Hq, Hkv, Hq / Hkv, (int)T, top, first, recent, rotate_q,
                  q_dtype == OMNI_F16, 0, 1};
     const int64_t rows = B * T * Hkv;
-    // One launch where a row's blocks are few or the rows fill the chip; else
-    // the scores over the whole chip first.
     const int64_t cus = device_cus();
     a.heads = Hkv % 8 == 0 ? 8 : 8 % Hkv == 0 ? Hkv : 1;
-    if (ws && max_pages > 1024 && 2 * rows <= cus) {
+    if (max_pages > top && score_first(rows, max_pages)) {
         // about two thread blocks a CU, whole rounds of their waves
         const int64_t round = 8 / a.heads * 4 * kSelWaves;
         int64_t per = max_pages * (rows / a.heads) / (2 * cus) / round * round;

@@ -922,6 +922,16 @@ static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, h
     return OMNI_OK;
 }
 
+// (b, t, kv head): eight times the 65535 groups that a grid's z holds; times
+// 4096 kv heads or 64 tokens below 2^32, for pg_div
+constexpr int64_t kMostUnits = 524280;
+
+// What a workspace size may be asked of; a call checks the rest.
+static bool page_sizes(int64_t B, int Hq, int Hkv, int64_t T, int64_t pages, int page_size) {
+    return B > 0 && Hkv > 0 && Hkv <= 4096 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 1024 && T > 0 && T <= 64 &&
+           B <= kMostUnits / Hkv / T && page_size >= 16 && pages > 0 && pages <= (int64_t(1) << 30) / page_size;
+}
+
 static uint64_t magic(int64_t d) { return (uint64_t(1) << 32) / (uint64_t)d + 1; }
 
 // The pool's geometry: page_size a power of two, every token row of the pool
@@ -946,7 +956,8 @@ static int page_check(const char *who, const void *q, int q_dtype, const void *k
     OMNI_CHECK_ARG(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: need B >= 0 and n_heads a multiple of n_kv_heads", who);
     OMNI_CHECK_ARG(T >= 1 && T <= 64, "%s: 1 to 64 query tokens, got %lld", who, (long long)T);
     OMNI_CHECK_ARG(Hq / Hkv <= 1024, "%s: at most 1024 query heads per kv head", who);
-    OMNI_CHECK_ARG(Hkv <= 4096 && B <= (int64_t(1) << 19) / Hkv / T, "%s: at most 4096 kv heads and B * T * n_kv_heads at most 2^19", who);
+    OMNI_CHECK_ARG(Hkv <= 4096 && B <= kMostUnits / Hkv / T, "%s: at most 4096 kv heads and B * T * n_kv_heads at most %lld", who,
+                   (long long)kMostUnits);
     OMNI_CHECK_ARG(fabsf(scale) <= 2.3e38f, "%s: scale must be finite and at most 2.3e38 in size", who);
     if (B == 0) return OMNI_OK;
     OMNI_CHECK_ARG(q && k_nib && v_nib && codebooks && out, "%s: NULL pointer", who);
@@ -960,7 +971,7 @@ using namespace omni;
 
 extern "C" size_t omni_attn_tree_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int64_t max_pages, int page_size,
                                                 int q_dtype) {
-    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || T <= 0 || T > 64 || max_pages <= 0 || page_size < 16) return 0;
+    if (!page_sizes(B, Hq, Hkv, T, max_pages, page_size)) return 0;
     return page_plan(B * Hkv, (int)T * (Hq / Hkv), (max_pages * page_size + kPgTile - 1) / kPgTile, q_dtype == OMNI_F16).ws;
 }
 
@@ -991,7 +1002,7 @@ extern "C" int omni_attn_tree(const void *q, int q_dtype, const uint8_t *k_nib, 
 }
 
 extern "C" size_t omni_attn_blocks_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int top, int page_size, int q_dtype) {
-    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || T <= 0 || T > 64 || top <= 0 || page_size < 16) return 0;
+    if (!page_sizes(B, Hq, Hkv, T, top, page_size)) return 0;
     return page_plan(B * T * Hkv, Hq / Hkv, ((int64_t)top * page_size + kPgTile - 1) / kPgTile, q_dtype == OMNI_F16).ws;
 }
 

@@ -68,7 +68,7 @@ def select_blocks(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor
     sf = aligned(_lib.sign_flip_i8(sign_flip, D, dev), 8) if (rotate_q and sign_flip is not None) else None
     blocks = torch.empty(B, cache.n_kv_heads, T, top, dtype=torch.int32, device=dev)
     L = _lib.lib()
-    ws_bytes = L.omni_block_select_workspace_size(B, cache.n_kv_heads, T, pt.shape[1], top)
+    ws_bytes = _lib.on_device(dev, L.omni_block_select_workspace_size, B, cache.n_kv_heads, T, pt.shape[1], top)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.check(_lib.on_device(
         dev, L.omni_block_select, _lib.ptr(qc), _lib.dtype_code(q.dtype), _lib.ptr(cache.k_bounds), cache.n_pages,
@@ -141,7 +141,8 @@ class PagedBlockAttention(_Prepared):
         _ascend(self.cb)
         self.blocks = torch.empty(self.B, cache.n_kv_heads, self.T, top, dtype=torch.int32, device=self.device)
         L = _lib.lib()
-        select = L.omni_block_select_workspace_size(self.B, cache.n_kv_heads, self.T, self.max_pages, top)
+        select = _lib.on_device(self.device, L.omni_block_select_workspace_size, self.B, cache.n_kv_heads, self.T,
+                                self.max_pages, top)
         attend = _lib.on_device(self.device, L.omni_attn_blocks_workspace_size, self.B, self.Hq, cache.n_kv_heads, self.T, top,
                                 cache.page_size, _lib.dtype_code(q_dtype))
         self._make_plan(max(select, attend), cache.k_bounds, self.blocks, top, first, recent)

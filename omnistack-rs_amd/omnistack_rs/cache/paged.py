@@ -159,9 +159,11 @@ class PagedKVCache:
             raise ValueError(f"inputs must be on {self.device}")
         _lib.require_device(self.k_nibbles)
         B, K = kept.shape
+        kc, pos = kept.contiguous(), positions.contiguous()
+        if K == 0 and self.k_bounds is not None:         # the page of the last token that stays
+            self._bounds(pt, (pos - 1).clamp_min(0), pos, 0)
         if B == 0 or K == 0:
             return
-        kc, pos = kept.contiguous(), positions.contiguous()
         if validate:
             kh, ph, ps = kc.cpu().to(torch.int64), pos.cpu().to(torch.int64), self.page_size
             if bool((kh >= 64).any()):
