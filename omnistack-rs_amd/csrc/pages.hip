@@ -71,7 +71,10 @@ constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dwor
 template <int NR, bool QJL, bool HL, int WAVES>
 struct Pg {
     static constexpr int NW = WAVES;
-    static constexpr int kQKept = NR > 2 ? 0 : HL && NR == 2 ? 8 : 99;                                   // query operands in registers (else LDS)
+    // two blocks a CU (128 registers a lane) or one
+    static constexpr bool kPair = NR == 1 && NW == 8;
+    // steps whose B operands stay in registers; the others are read from LDS for every tile
+    static constexpr int kQKept = NR > 2 || kPair ? 0 : HL && NR == 2 ? 8 : 99;
     static constexpr int kQSteps = HL ? 8 : 4;                               // B operands of a row group: q (HL: twice four),
     static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
     static constexpr int kSteps = kQSteps + kGSteps;
@@ -86,6 +89,7 @@ struct Pg {
     static constexpr int kSlabs = NW * MR * 16 * kPartRow * 4;
     static constexpr int kMoved = kSlabs > kCsc ? kSlabs - kCsc : 0;         // what lies behind them moves up
     static constexpr int kLds = kUse + kMoved;
+    static_assert(kLds <= (kPair ? 81920 : 163840), "LDS of a CU");
 };
 
 __device__ __forceinline__ uint32_t pg_pack(float x, float y) {
@@ -183,7 +187,7 @@ struct PgValues {
 };
 
 template <int NR, bool QJL, bool HL, bool BLOCKS, int NW>
-__global__ __launch_bounds__(64 * NW) void page_attn_kernel(PageAttnArgs a) {
+__global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4)) void page_attn_kernel(PageAttnArgs a) {
     using L = Pg<NR, QJL, HL, NW>;
     __shared__ __attribute__((aligned(16))) unsigned char smem[L::kLds];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -856,15 +860,24 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
 
 struct PagePlan {
     int nr, chunks, splits;
-    bool wide;                   // one row group: twelve waves
+    bool wide;                   // one row group: twelve waves, one block a CU
     size_t ws;
 };
 
-// Row groups per block and splits of a call: `units` lists of at most `tiles`
-// tiles, `rows` query rows each.
+// Row groups per block and splits of a call, the cheapest by this estimate:
+// `units` lists of at most `tiles` tiles, `rows` query rows each.  More rows a
+// block share its table and the looked-up operands; fewer leave less of the
+// last block empty and fill more CUs.  Measured, lists of 8192 tokens: 64 rows
+// in fp16 187 us as one block each, 295 as four; lists of 20,011 tokens with
+// 264 rows 179 us as six blocks of 48, 205 as five of 64.  One row group: twelve
+// waves where every block has a CU to itself and a long list (256 lists of
+// 8192 tokens 51 us, eight waves 59), else eight, two blocks a CU, so that one's
+// prologue runs beside the other's tiles (768 lists of 75 to 2917 tokens in
+// fp16 55 us, twelve waves 59; 312 selections of 768 tokens 17, 21 with one
+// block a CU; 256 lists of 1024 tokens 13 either way, twelve waves 14).
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     // us: a block's fixed part, and per tile by its row groups
-    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.18, 0.27, 0.36, 0.46}, kTileHl[5] = {0.0, 0.27, 0.36, 0.53, 0.70};
+    constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.18, 0.27, 0.36, 0.46}, kTileHl[5] = {0.0, 0.24, 0.36, 0.53, 0.70};
     const int64_t cus = device_cus();
     PagePlan p{1, 1, 1, false, 0};
     double best = 1e30;
@@ -873,7 +886,9 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
         const int64_t blocks = units * chunks;
         auto consider = [&](int64_t s) {
             if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
-            const double t = (double)((blocks * s + cus - 1) / cus) * (kFixed + (hl ? kTileHl[nr] : kTile[nr]) * (double)((tiles + s - 1) / s)) +
+            const int64_t all = blocks * s, at_once = nr == 1 && all > cus ? 2 : 1;
+            const double tile = (hl ? kTileHl : kTile)[nr] * (at_once == 2 ? 2.1 : 1.0);
+            const double t = (double)((all + at_once * cus - 1) / (at_once * cus)) * (kFixed + tile * (double)((tiles + s - 1) / s)) +
                              (s > 1 ? 3.0 + 0.03 * (double)s + (double)units * (double)s * rows * kPartRow * 4e-6 * 2 / 3.5 : 0.0);
             if (t < best) {
                 best = t;
@@ -886,7 +901,7 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
         for (int r = 1; r <= 4; ++r)
             for (int k = 0; k < 3; ++k) consider(r * cus / (blocks << k));
     }
-    p.wide = tiles / p.splits >= 64;
+    p.wide = p.nr == 1 && units * p.chunks * p.splits <= cus && tiles / p.splits >= 64;
     p.ws = p.splits > 1 ? (size_t)units * p.splits * rows * kPartRow * 4 : 0;
     return p;
 }
@@ -901,7 +916,7 @@ static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
 template <bool BLOCKS>
 static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (p.nr == 1 && p.wide) {
+    if (p.wide) {
         if (hl) page_launch<1, true, BLOCKS, 12>(a, qjl, s);
         else page_launch<1, false, BLOCKS, 12>(a, qjl, s);
     } else if (hl && p.nr == 1) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
