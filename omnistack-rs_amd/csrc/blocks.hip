@@ -40,7 +40,8 @@ struct BoundsArgs {
 // and keeps nibble minima and maxima in 16-bit lanes.  The page's first tokens
 // up to `end` count, whatever start is, so what a page says does not depend on
 // how it was filled.  Bound by latency where a decode step touches a page per
-// sequence, else by the read of the codes.
+// sequence (5.8 us), else by the read of the codes (8 x 131072 tokens, 537 MB:
+// 174 us, 3.1 TB/s; a prompt pays it once).
 __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsArgs a) {
     typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
     const int64_t b = blockIdx.y;
@@ -305,9 +306,10 @@ __device__ __forceinline__ uint32_t block_key(const uint4 &w, int32_t id, int64_
 
 // Scores of blocks from .. to - 1 by the block's eight waves, put(block, score
 // as an unsigned key that orders as it does): eight lanes a block, 16 dims
-// each; a wave has 64 blocks' bounds in flight.  Bound by the read of the
-// bounds (128 B a block and head) where there are many, else by the chain
-// query, page table, bounds.
+// each; a wave has 64 blocks' bounds in flight.  Bound by the chain of query,
+// page table, bounds and digits: 32 x 8 rows of 512 blocks 10.7 us, choice
+// included (16.8 MB of bounds: 3 us at a copy's rate; a launch for the scores
+// and one for the choice 20).
 template <typename Put>
 __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQuery &wq, ScoreLds &sm, int64_t b, int t, int hk, int from,
                                              int to, Put &&put) {
@@ -361,8 +363,9 @@ __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQue
 // One block per (b, t, hk): the score that the last of `need` blocks has, by
 // digits of eight bits from the top of the scores' range (a histogram in LDS
 // per digit), then the blocks above it and the first ones equal to it in
-// ascending order.  SCORED: the
-// scores are there already, by block_score_kernel.
+// ascending order.  SCORED: the scores are there already, by
+// block_score_kernel; 64 rows of 8192 blocks 11.8 us, three digits of which
+// each takes a pass over the keys in registers and three barriers.
 constexpr int kPickLds = 16384;          // scores held in LDS; more are read again for every digit
 
 // The key (at most `range`) that the `need`-th largest has, and of the equal
@@ -466,7 +469,10 @@ __device__ __forceinline__ void pick_held(uint32_t *keys, int n, uint32_t kmin, 
 // Scores where rows are fewer than CUs and long: the read of the bounds over
 // the whole chip, `heads` kv heads (a divisor of 8, or 8) of a share of one
 // query's blocks by a thread block, so that a wave's load is 8 / heads pages'
-// neighbouring bounds, a KB.
+// neighbouring bounds, a KB.  8 x 8 rows of 8192 blocks (67 MB): 21 us, 3.2
+// TB/s: 5 us of query, then some 90 vector instructions for eight bounds.
+// Measured: two thread blocks a CU 21, one 24, four (two rounds) 27 us; eight
+// loads in flight, which spill at two blocks, 22.
 __global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectArgs a) {
     constexpr int U = 4;                                          // loads in flight
     __shared__ __attribute__((aligned(16))) int8_t qs[8][256];
@@ -723,8 +729,9 @@ extern "C" int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t 
     return OMNI_OK;
 }
 
-// One launch where a row's blocks are few or the rows fill the chip; else the
-// scores over the whole chip first.
+// One launch where a row's blocks are few or the rows fill the chip (32 x 8
+// rows of 512 blocks 10.7 us, 20 in two); else the scores over the whole chip
+// first (8 x 8 rows of 8192 blocks 33 us, 44 with one kv head a thread block).
 static bool score_first(int64_t rows, int64_t max_pages) { return max_pages > 1024 && 2 * rows <= device_cus(); }
 
 extern "C" size_t omni_block_select_workspace_size(int64_t B, int Hkv, int64_t T, int64_t max_pages, int top) {

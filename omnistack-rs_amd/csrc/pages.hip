@@ -11,24 +11,37 @@
 // of one or more query tokens); its waves take the tiles in turn, each with
 // its own running maximum and sum, and are merged at the end.  All products on
 // v_mfma_f32_16x16x32_f16, tokens on M for the scores and dims on M for P V:
-//   K pass    A = centroids of 16 tokens, looked up a code byte at a time in
-//             an LDS table (64 KB: a private column per lane, so a byte and the
-//             lane make the address with one v_perm and no bank is met twice);
-//             B = the query rows.  Lane (n, g) reads bytes 16 g .. + 15 of
-//             token n, so k-slot i of step s is dim 32 g + 8 s + i on both sides.
-//   QJL pass  A = the signs as +-1, B = sqrt(2/pi)/128 G q as it leaves the
-//             product G q (projections 16 cb + 4 g + i in lane (n, g)): the
-//             sign nibbles are picked in that order.
-//   P V       A = centroids again, two tokens' codes of one dim interleaved
-//             into one table byte; B = P as it leaves the scores.
+//   table     64 KB of LDS, a row of 256 bytes for every code byte: in 32
+//             columns its two centroids in fp16 and their remainders, 8 bytes.
+//             A lane reads its own column, so a byte and the lane make the
+//             address with one v_perm, and 32 lanes meet no bank twice.
+//   K pass    A = centroids of 16 tokens (fp16 calls: and remainders); B = the
+//             query rows.  Lane (n, g) reads bytes 16 g .. + 15 of token n, so
+//             k-slot i of step s is dim 32 g + 8 s + i on both sides.
+//   QJL pass  A = the signs, made from the sign words by shift, mask and xor
+//             (with the norm in bf16 calls, as 1 in fp16 ones); B =
+//             sqrt(2/pi)/128 G q, in the order of the sign bits that a lane
+//             takes: projections 32 s + 4 g + j and 16 on.
+//   P V       A = centroids and remainders side by side, two tokens' codes of
+//             one dim interleaved into one table byte; B = P, each value twice.
 // Numbers: q rows times a power of two (largest in [2^14, 2^15)) and the head's
-// centroids times one (largest in [2^9, 2^10)) are rounded to fp16.  bf16
-// queries that the call does not rotate lose nothing; rotated ones and the
-// centroids 2^-12 of themselves, P another 2^-12 (the same rounded P in
-// numerator and denominator): below the 2^-9 of the bf16 output.  fp16 queries
-// (HL) keep a second fp16 term of q and of the centroids in both products (22
-// bits), which leaves P's 2^-12 against the output's 2^-12.  Scores, maxima,
-// sums and accumulators are fp32.
+// centroids times one are rounded to fp16.  bf16 queries that the call does not
+// rotate lose nothing; rotated ones, K's centroids, norms and G q lose 2^-12 of
+// themselves, P another 2^-12 (the same rounded P in numerator and
+// denominator): below the 2^-9 of the bf16 output.  V's centroids keep a
+// second fp16 term in either type: their roundings do not average out over a
+// long list as P's do.  fp16 queries (HL) keep a second term of q, of G q and of K's
+// centroids too (22 bits), which leaves P's 2^-12 against the output's 2^-12.
+// Scores, maxima, sums and accumulators are fp32.
+//
+// What bounds it: many rows, the matrix and the vector units in turn (32
+// sequences of 8192 tokens and 16 drafted, 64 rows a list: 125 us, 686 TFLOP/s
+// of the 1200 that a large product reaches; matrix units busy in 43 % of the
+// cycles, vector instructions issuing in 49 %, 256 registers hold a SIMD at
+// two waves).  Few rows, the cache's read and the vector work per tile (16 rows
+// 51 us, 294 MB at 5.8 TB/s; a plain read reaches 7.1).  Short lists, a block's chain of dependent accesses, 7 to 8 us:
+// lengths, page ids, tiles and q one after another, the table (0.7 us), G q,
+// and the waves' merge (1.5 us).
 #include <math.h>
 
 #include <new>
@@ -62,7 +75,7 @@ struct PageAttnArgs {
 
 constexpr int kPgTile = 32;
 constexpr int kPartRow = 128 + 4;            // floats of a split's row: O, then m and l
-constexpr int kLutBytes = 65536;             // [byte][256 B]: 32 columns of 8 B
+constexpr int kLutBytes = 65536;             // the table
 constexpr int kQimgOff = kLutBytes;
 constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dword 3
 
@@ -659,9 +672,10 @@ __global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4))
         uint32_t r[2];
         half8_t pb[NR][2];
         uint32_t ev[4], od[4];
-        // The next tile is asked for as its registers come free.  Waves in a
-        // matrix phase issue first: of a SIMD's, others then work on their
-        // weights.
+        // The next tile is asked for as its registers come free (two tiles
+        // ahead: 54 instead of 51 us at 16 rows).  Waves in a matrix phase
+        // issue first: of a SIMD's, others then work on their weights (without:
+        // 56 instead of 54 us, 127 instead of 125 at 64 rows).
         for (int k = 0; k < cnt; ++k) {
             float4_t S[NR][2];
             int next;
@@ -798,7 +812,8 @@ __global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4))
 }
 
 // The splits' (m, l, O) of one row: 32 lanes, four dims each, eight splits'
-// loads in flight.
+// loads in flight (2 x 8 lists of 256 rows in four splits 5.7 us, 64 lists of
+// four rows in four 4.6: a launch and two round trips).
 template <bool F16, bool BLOCKS>
 __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
