@@ -26,8 +26,8 @@
 //             one dim interleaved into one table byte; B = P, each value twice.
 // Numbers: q rows times a power of two (largest in [2^14, 2^15)) and the head's
 // centroids times one are rounded to fp16.  bf16 queries that the call does not
-// rotate lose nothing; rotated ones, K's centroids, norms and G q lose 2^-12 of
-// themselves, P another 2^-12 (the same rounded P in numerator and
+// rotate lose nothing; rotated ones, K's centroids (less what is common to them,
+// see `fit`), norms and G q lose 2^-12 of themselves, P another 2^-12 (the same rounded P in numerator and
 // denominator): below the 2^-9 of the bf16 output.  V's centroids keep a
 // second fp16 term in either type: their roundings do not average out over a
 // long list as P's do.  fp16 queries (HL) keep a second term of q, of G q and of K's
@@ -370,6 +370,27 @@ __global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4))
     }
     __builtin_amdgcn_sched_barrier(0);
 
+    // The part of the centroids' rounding that is common to keys: where a row
+    // leans on a key along itself, its score is off by sum f c (h - c) / sum f c^2
+    // of itself, f the codes' frequencies; the score scale takes that back.  A
+    // calibrated codebook's codes come about as often as 1 / spacing^2 (points
+    // lie as density^(1/3)).  Score error of such rows 1e-4 to 3e-4 without,
+    // 2e-5 to 6e-5 with it; other codebooks: a weighted mean of the roundings.
+    float fit = 1.0f;
+    if constexpr (!HL) {
+        const float x = cent * cmul;
+        const float up = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x101, 0xf, 0xf, true));      // row_shl:1: lane c + 1
+        const float dn = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x111, 0xf, 0xf, true));      // row_shr:1: lane c - 1
+        const float gap = c == 0 ? up - x : c == 15 ? x - dn : 0.5f * (up - dn), w = __builtin_amdgcn_rcpf(gap * gap + 0x1p-20f);
+        float over = w * x * (f16_to_f32(f32_to_f16_rne(x)) - x), of = w * x * x;
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) {
+            over += pg_row_xor(over, m, c);
+            of += pg_row_xor(of, m, c);
+        }
+        fit = of > 0.0f ? 1.0f - over / of : 1.0f;
+    }
+
     // ── query rows into MFMA operands ─────────────────────────────────
     uint4 *qimg = reinterpret_cast<uint4 *>(smem + kQimgOff);      // [rg][step][lane]
     float *csc_l = reinterpret_cast<float *>(smem + L::kMoved + L::kCsc);
@@ -423,7 +444,7 @@ __global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4))
         ex = ex < -100 ? -100 : ex;
         const float sr = ldexpf(a.qscale < 0.0f ? -1.0f : 1.0f, 15 - ex);
         // at least FLT_MIN (scores are as good as 0 either way), so that a hidden score's -inf stays one
-        if (c == 0) csc_l[rl] = fmaxf(fabsf(a.qscale) * ldexpf(cdiv, ex - 15), __FLT_MIN__);
+        if (c == 0) csc_l[rl] = fmaxf(fabsf(a.qscale) * fit * ldexpf(cdiv, ex - 15), __FLT_MIN__);
         uint32_t hw[4], lw[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
