@@ -527,7 +527,8 @@ int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const voi
  * are zeros; a row that sees nothing, every row of a sequence whose lengths do
  * not fit (0 <= n_draft <= T, n_draft <= length <= max_pages * page_size) or
  * that reaches a page outside the pool is NaN.  workspace (16-byte aligned):
- * omni_attn_tree_workspace_size(...) bytes.  The same bits on every run.
+ * omni_attn_tree_workspace_size(...) bytes.  The same bits on every run.  At
+ * most 4096 kv heads of 1024 query heads each, B * T * Hkv at most 524280.
  */
 size_t omni_attn_tree_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int64_t max_pages, int page_size,
                                      int q_dtype);
@@ -542,7 +543,7 @@ int omni_attn_tree(const void *q, int q_dtype, const uint8_t *k_nib, const uint8
  * Bounds of the blocks (pages) that hold tokens start[b] .. end[b] - 1 of
  * sequence b (end NULL: start[b] + count): byte d of bounds (n_pages, Hkv, 128)
  * is lo | hi << 4, the least and largest key code of dim d over the page's
- * tokens before end[b].  Positions outside the table and pages outside the
+ * tokens before end[b].  B at most 65535.  Positions outside the table and pages outside the
  * pool are passed over.
  */
 int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t n_pages, int Hkv, int page_size,
@@ -561,7 +562,7 @@ int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t n_pages, in
  * that ascend this bounds the group's summed scores (without residual signs)
  * from above.  blocks (B, Hkv, T, top) int32: ascending, -1 behind the last.
  * q and sign_flip as for omni_attn_tree.  workspace (16-byte aligned):
- * omni_block_select_workspace_size(...) bytes.
+ * omni_block_select_workspace_size(...) bytes.  B * T at most 65535.
  */
 size_t omni_block_select_workspace_size(int64_t B, int Hkv, int64_t T, int64_t max_pages, int top);
 int omni_block_select(const void *q, int q_dtype, const uint8_t *bounds, int64_t n_pages, int page_size,
