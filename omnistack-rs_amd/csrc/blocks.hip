@@ -306,14 +306,14 @@ __device__ __forceinline__ uint32_t block_key(const uint4 &w, int32_t id, int64_
 
 // Scores of blocks from .. to - 1 by the block's eight waves, put(block, score
 // as an unsigned key that orders as it does): eight lanes a block, 16 dims
-// each; a wave has 64 blocks' bounds in flight.  Bound by the chain of query,
+// each; a wave has 32 blocks' bounds in flight (64 spill at two blocks a CU).  Bound by the chain of query,
 // page table, bounds and digits: 32 x 8 rows of 512 blocks 10.7 us, choice
 // included (16.8 MB of bounds: 3 us at a copy's rate; a launch for the scores
 // and one for the choice 20).
 template <typename Put>
 __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQuery &wq, ScoreLds &sm, int64_t b, int t, int hk, int from,
                                              int to, Put &&put) {
-    constexpr int U = 8;                                          // loads in flight
+    constexpr int U = 4;                                          // loads in flight
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 7;
     const int32_t *pt = a.page_table + b * a.max_pages;
     int32_t id[U];
@@ -366,7 +366,7 @@ __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQue
 // ascending order.  SCORED: the scores are there already, by
 // block_score_kernel; 64 rows of 8192 blocks 11.8 us, three digits of which
 // each takes a pass over the keys in registers and three barriers.
-constexpr int kPickLds = 16384;          // scores held in LDS; more are read again for every digit
+constexpr int kPickLds = 14336;          // scores held in LDS (two blocks a CU); more are read again for every digit
 
 // The key (at most `range`) that the `need`-th largest has, and of the equal
 // ones how many are needed (in `need`).  each(shift, at, count) calls count(x)
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectAr
 }
 
 template <bool SCORED>
-__global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs a) {
+__global__ __launch_bounds__(64 * kSelWaves, 4) void block_select_kernel(SelectArgs a) {
     constexpr int kThreads = 64 * kSelWaves;
     __shared__ uint32_t keys[kPickLds];
     __shared__ ScoreLds sm;

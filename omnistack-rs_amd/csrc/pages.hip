@@ -80,14 +80,12 @@ constexpr int kQimgOff = kLutBytes;
 constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dword 3
 
 // What a variant keeps where.  NR: groups of 16 query rows a block; HL: fp16
-// queries.
-template <int NR, bool QJL, bool HL, int WAVES>
+// queries; PAIR: two blocks a CU (128 registers a lane), else one.
+template <int NR, bool QJL, bool HL, int WAVES, bool PAIR>
 struct Pg {
     static constexpr int NW = WAVES;
-    // two blocks a CU (128 registers a lane) or one
-    static constexpr bool kPair = NR == 1 && NW == 8;
     // steps whose B operands stay in registers; the others are read from LDS for every tile
-    static constexpr int kQKept = NR > 2 || kPair ? 0 : HL && NR == 2 ? 8 : 99;
+    static constexpr int kQKept = NR > 2 || PAIR ? 0 : HL && NR == 2 ? 8 : 99;
     static constexpr int kQSteps = HL ? 8 : 4;                               // B operands of a row group: q (HL: twice four),
     static constexpr int kGSteps = QJL ? (HL ? 4 : 2) : 0;                   // then G q (HL: twice two)
     static constexpr int kSteps = kQSteps + kGSteps;
@@ -98,11 +96,11 @@ struct Pg {
     static constexpr int kFlags = kM + 2 * NR * 16 * NW * 4;                 // per wave: met a page outside the pool
     static constexpr int kUse = kFlags + 16 * 4;
     // the merge: the waves' O of MR row groups at a time, from 0 on (over the tables and the query rows)
-    static constexpr int MR = NR % 2 == 0 && NW <= 8 ? 2 : 1;
+    static constexpr int MR = NR % 2 == 0 && NW <= 8 && !PAIR ? 2 : 1;
     static constexpr int kSlabs = NW * MR * 16 * kPartRow * 4;
     static constexpr int kMoved = kSlabs > kCsc ? kSlabs - kCsc : 0;         // what lies behind them moves up
     static constexpr int kLds = kUse + kMoved;
-    static_assert(kLds <= (kPair ? 81920 : 163840), "LDS of a CU");
+    static_assert(kLds <= (PAIR ? 81920 : 163840), "LDS of a CU");
 };
 
 __device__ __forceinline__ uint32_t pg_pack(float x, float y) {
@@ -199,9 +197,9 @@ struct PgValues {
     uint32_t v[8];               // code bytes 4 n .. + 3 of tokens 16 (i / 4) + 4 g + i % 4
 };
 
-template <int NR, bool QJL, bool HL, bool BLOCKS, int NW>
-__global__ __launch_bounds__(64 * NW, (Pg<NR, QJL, HL, NW>::kPair ? 4 : NW / 4)) void page_attn_kernel(PageAttnArgs a) {
-    using L = Pg<NR, QJL, HL, NW>;
+template <int NR, bool QJL, bool HL, bool BLOCKS, int NW, bool PAIR>
+__global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel(PageAttnArgs a) {
+    using L = Pg<NR, QJL, HL, NW, PAIR>;
     __shared__ __attribute__((aligned(16))) unsigned char smem[L::kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -897,6 +895,7 @@ __global__ __launch_bounds__(256) void page_merge_kernel(PageAttnArgs a) {
 struct PagePlan {
     int nr, chunks, splits;
     bool wide;                   // one row group: twelve waves, one block a CU
+    bool pair;                   // two row groups: two blocks a CU
     size_t ws;
 };
 
@@ -910,27 +909,33 @@ struct PagePlan {
 // 8192 tokens 51 us, eight waves 59), else eight, two blocks a CU, so that one's
 // prologue runs beside the other's tiles (768 lists of 75 to 2917 tokens in
 // fp16 55 us, twelve waves 59; 312 selections of 768 tokens 17, 21 with one
-// block a CU; 256 lists of 1024 tokens 13 either way, twelve waves 14).
+// block a CU; 256 lists of 1024 tokens 13 either way, twelve waves 14).  Two
+// row groups spill at two blocks a CU (28 registers of a bf16 call): that pays
+// up to six tiles a list only (512 lists of 58 tokens 15 us, 18 with one; 256
+// lists of 8192 tokens 147 and 75).
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     // us: a block's fixed part, and per tile by its row groups
     constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.18, 0.27, 0.36, 0.46}, kTileHl[5] = {0.0, 0.24, 0.36, 0.53, 0.70};
     const int64_t cus = device_cus();
-    PagePlan p{1, 1, 1, false, 0};
+    PagePlan p{1, 1, 1, false, false, 0};
     double best = 1e30;
     for (int nr = 1; nr <= 4; ++nr) {
         const int chunks = (rows + 16 * nr - 1) / (16 * nr);
         const int64_t blocks = units * chunks;
         auto consider = [&](int64_t s) {
             if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
-            const int64_t all = blocks * s, at_once = nr == 1 && all > cus ? 2 : 1;
-            const double tile = (hl ? kTileHl : kTile)[nr] * (at_once == 2 ? 2.1 : 1.0);
-            const double t = (double)((all + at_once * cus - 1) / (at_once * cus)) * (kFixed + tile * (double)((tiles + s - 1) / s)) +
+            const int64_t all = blocks * s, n = (tiles + s - 1) / s;
+            const bool spills = nr == 2 && !hl && all > cus && n <= 6;
+            const int64_t at_once = (nr == 1 && all > cus) || spills ? 2 : 1;
+            const double tile = spills ? 1.0 : (hl ? kTileHl : kTile)[nr] * (at_once == 2 ? 2.1 : 1.0);
+            const double t = (double)((all + at_once * cus - 1) / (at_once * cus)) * ((spills ? 12.0 : kFixed) + tile * (double)n) +
                              (s > 1 ? 3.0 + 0.03 * (double)s + (double)units * (double)s * rows * kPartRow * 4e-6 * 2 / 3.5 : 0.0);
             if (t < best) {
                 best = t;
                 p.nr = nr;
                 p.chunks = chunks;
                 p.splits = (int)s;
+                p.pair = spills;
             }
         };
         consider(1);
@@ -942,27 +947,30 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     return p;
 }
 
-template <int NR, bool HL, bool BLOCKS, int NW>
+template <int NR, bool HL, bool BLOCKS, int NW, bool PAIR>
 static void page_launch(const PageAttnArgs &a, bool qjl, hipStream_t s) {
     const dim3 grid(8u * (unsigned)a.chunks, (unsigned)a.splits, (unsigned)((a.units + 7) / 8));
-    if (qjl) hipLaunchKernelGGL((page_attn_kernel<NR, true, HL, BLOCKS, NW>), grid, dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((page_attn_kernel<NR, false, HL, BLOCKS, NW>), grid, dim3(64 * NW), 0, s, a);
+    if (qjl) hipLaunchKernelGGL((page_attn_kernel<NR, true, HL, BLOCKS, NW, PAIR>), grid, dim3(64 * NW), 0, s, a);
+    else hipLaunchKernelGGL((page_attn_kernel<NR, false, HL, BLOCKS, NW, PAIR>), grid, dim3(64 * NW), 0, s, a);
+}
+
+template <bool HL, bool BLOCKS>
+static void page_launch(const PageAttnArgs &a, bool qjl, const PagePlan &p, hipStream_t s) {
+    if constexpr (!HL) {
+        if (p.pair) return page_launch<2, false, BLOCKS, 8, true>(a, qjl, s);
+    }
+    if (p.wide) page_launch<1, HL, BLOCKS, 12, false>(a, qjl, s);
+    else if (p.nr == 1) page_launch<1, HL, BLOCKS, 8, true>(a, qjl, s);
+    else if (p.nr == 2) page_launch<2, HL, BLOCKS, 8, false>(a, qjl, s);
+    else if (p.nr == 3) page_launch<3, HL, BLOCKS, 8, false>(a, qjl, s);
+    else page_launch<4, HL, BLOCKS, 8, false>(a, qjl, s);
 }
 
 template <bool BLOCKS>
 static int page_run(PageAttnArgs &a, int q_dtype, bool qjl, const PagePlan &p, hipStream_t s) {
     const bool hl = q_dtype == OMNI_F16;
-    if (p.wide) {
-        if (hl) page_launch<1, true, BLOCKS, 12>(a, qjl, s);
-        else page_launch<1, false, BLOCKS, 12>(a, qjl, s);
-    } else if (hl && p.nr == 1) page_launch<1, true, BLOCKS, 8>(a, qjl, s);
-    else if (hl && p.nr == 2) page_launch<2, true, BLOCKS, 8>(a, qjl, s);
-    else if (hl && p.nr == 3) page_launch<3, true, BLOCKS, 8>(a, qjl, s);
-    else if (hl) page_launch<4, true, BLOCKS, 8>(a, qjl, s);
-    else if (p.nr == 1) page_launch<1, false, BLOCKS, 8>(a, qjl, s);
-    else if (p.nr == 2) page_launch<2, false, BLOCKS, 8>(a, qjl, s);
-    else if (p.nr == 3) page_launch<3, false, BLOCKS, 8>(a, qjl, s);
-    else page_launch<4, false, BLOCKS, 8>(a, qjl, s);
+    if (hl) page_launch<true, BLOCKS>(a, qjl, p, s);
+    else page_launch<false, BLOCKS>(a, qjl, p, s);
     OMNI_CHECK_LAUNCH("page_attn_kernel");
     if (a.splits > 1) {
         const unsigned blocks = (unsigned)((a.units * a.rows + 7) / 8);

@@ -57,6 +57,29 @@ def test_rows_of_a_block(device, G, T, qjl, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("qjl", [True, False])
+@pytest.mark.parametrize("G,T,most", [(4, 8, 192), (3, 7, 60), (17, 1, 33), (1, 3, 500)])
+def test_more_short_lists_than_compute_units(device, G, T, most, qjl, dtype):
+    """600 lists of up to six tiles, 3 to 32 rows each, some of their sequences without drafted tokens or with fewer."""
+    from omnistack_rs.cache import paged_tree_attention, tree_masks
+    B, H, uid = 75, 8, 4
+    lens = [T + (b * 37) % (most - T + 1) for b in range(B)]
+    parts, cb = P.packed(B, H, max(lens), seed=371), P.codebooks(H)
+    q, tree = _q(B, G * H, T, 372, dtype), tree_masks(P.random_parents(B, T, 373))
+    cache, pt, lt = P.paged(device, parts, 16, lens)
+    got = paged_tree_attention(q.to(device), cache, pt, lt, cb.to(device), tree.to(device), user_id=uid, with_qjl=qjl)
+    want, bound = _tree_want(q, parts, cb, uid, lens, tree, qjl)
+    P.close(got, want, bound)
+    drafts = torch.tensor([(b * 3) % (T + 1) for b in range(B)], dtype=torch.int32, device=device)
+    some = paged_tree_attention(q.to(device), cache, pt, lt, cb.to(device), tree.to(device), user_id=uid, with_qjl=qjl,
+                                n_draft=drafts)
+    for b, n in enumerate(drafts.tolist()):
+        assert (some[b, :, n:] == 0).all() and torch.isfinite(some[b, :, :n]).all()
+        if n == T:
+            assert torch.equal(some[b], got[b])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("B,H,G,T,L", [(32, 8, 1, 4, 2200), (2, 8, 4, 16, 4111), (2, 4, 4, 8, 5000), (1, 3, 8, 6, 7001)])
 def test_long_lists(device, B, H, G, T, L, dtype):
     """More than 64 tiles a block, whole or in merged splits; centroids off center, which long sums of V would show."""
@@ -73,7 +96,7 @@ def test_long_lists(device, B, H, G, T, L, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("B,H,G,T,page,top", [(16, 4, 20, 4, 16, 5), (16, 4, 40, 4, 32, 3), (16, 4, 64, 4, 16, 4), (16, 8, 2, 2, 64, 40),
-                                              (1, 2, 4, 1, 128, 30)])
+                                              (1, 2, 4, 1, 128, 30), (20, 4, 24, 4, 32, 5), (35, 8, 3, 1, 16, 7)])
 def test_selected_blocks_rows(device, B, H, G, T, page, top, dtype):
     """Many heads a group, long selections, a selection in merged splits."""
     from omnistack_rs.cache import paged_block_attention

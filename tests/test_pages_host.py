@@ -91,8 +91,8 @@ def test_workspaces(L):
     need = L.omni_block_select_workspace_size(1, 2, 1, 4000, 4)
     assert need == 2 * 4000 * 4 and _select(L, mp=4000, ws=1, wsb=need - 1) == _lib.OMNI_EWORKSPACE
     assert L.omni_block_select_workspace_size(1, 2, 1, 1024, 4) == 0
-    assert L.omni_block_select_workspace_size(64, 8, 1, 16384, 4) == 0                  # rows fill the chip: scores in LDS
-    assert L.omni_block_select_workspace_size(64, 8, 1, 16385, 4) == 64 * 8 * 16385 * 4
+    assert L.omni_block_select_workspace_size(64, 8, 1, 14336, 4) == 0                  # rows fill the chip: scores in LDS
+    assert L.omni_block_select_workspace_size(64, 8, 1, 14337, 4) == 64 * 8 * 14337 * 4
     for args in ((0, 4, 2, 3, 40, 16, 2), (1, 5, 2, 3, 40, 16, 2), (1, 4, 2, 65, 40, 16, 2), (1, 4, 0, 3, 40, 16, 2),
                  (1 << 40, 4, 2, 3, 40, 16, 2), (1, 1 << 30, 1, 64, 40, 16, 2), (1, 4, 2, 3, 1 << 60, 16, 2), (1, 4, 2, 3, 40, 0, 2)):
         assert L.omni_attn_tree_workspace_size(*args) == 0
