@@ -306,10 +306,11 @@ __device__ __forceinline__ uint32_t block_key(const uint4 &w, int32_t id, int64_
 
 // Scores of blocks from .. to - 1 by the block's eight waves, put(block, score
 // as an unsigned key that orders as it does): eight lanes a block, 16 dims
-// each; a wave has 32 blocks' bounds in flight (64 spill at two blocks a CU).  Bound by the chain of query,
-// page table, bounds and digits: 32 x 8 rows of 512 blocks 10.7 us, choice
-// included (16.8 MB of bounds: 3 us at a copy's rate; a launch for the scores
-// and one for the choice 20).
+// each; a wave has 32 blocks' bounds in flight (64 spill at two thread blocks a
+// CU).  Bound by the chain of query, page table, bounds and digits: 32 x 8 rows
+// of 512 blocks 10.7 us, choice included (16.8 MB of bounds: 3 us at a copy's
+// rate; a launch for the scores and one for the choice 20); 312 rows of up to
+// 939 blocks 16 us, 18 with one thread block a CU.
 template <typename Put>
 __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQuery &wq, ScoreLds &sm, int64_t b, int t, int hk, int from,
                                              int to, Put &&put) {

@@ -39,9 +39,9 @@
 // of the 1200 that a large product reaches; matrix units busy in 43 % of the
 // cycles, vector instructions issuing in 49 %, 256 registers hold a SIMD at
 // two waves).  Few rows, the cache's read and the vector work per tile (16 rows
-// 51 us, 294 MB at 5.8 TB/s; a plain read reaches 7.1).  Short lists, a block's chain of dependent accesses, 7 to 8 us:
-// lengths, page ids, tiles and q one after another, the table (0.7 us), G q,
-// and the waves' merge (1.5 us).
+// 51 us, 294 MB at 5.8 TB/s; a plain read reaches 7.1).  Short lists, a block's
+// chain of dependent accesses, 7 to 8 us: lengths, page ids, tiles and q one
+// after another, the table (0.7 us), G q, and the waves' merge (1.5 us).
 #include <math.h>
 
 #include <new>
