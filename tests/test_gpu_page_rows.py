@@ -253,3 +253,33 @@ def test_keep_of_nothing_narrows_the_bounds(device):
     cache.append(enc, draft, draft, pt, at)
     cache.keep(pt, at, torch.full((B, 4), -1, dtype=torch.int32, device=device))
     assert torch.equal(cache.k_bounds[pt[:, :2].long()], before)
+
+
+@pytest.mark.parametrize("B,H,G,T,L", [(1, 1, 1024, 2, 45), (2, 4096, 1, 1, 20), (1, 1, 200, 64, 70)])
+def test_largest_groups_and_heads(device, B, H, G, T, L):
+    """1024 query heads a kv head, 4096 kv heads, 12,800 rows a list."""
+    from omnistack_rs.cache import PagedBlockAttention, paged_tree_attention, tree_masks
+    lens = [L - 3 * b for b in range(B)]
+    parts, cb = P.packed(B, H, L, seed=381), P.codebooks(H)
+    q, tree = _q(B, G * H, T, 382, torch.bfloat16), tree_masks(P.random_parents(B, T, 383))
+    cache, pt, lt = P.paged(device, parts, 16, lens, bounds=True)
+    got = paged_tree_attention(q.to(device), cache, pt, lt, cb.to(device), tree.to(device), user_id=2, with_qjl=False)
+    want, bound = _tree_want(q, parts, cb, 2, lens, tree, False)
+    P.close(got, want, bound)
+    # all of a sequence's blocks, for its last token: a chain's last row
+    att = PagedBlockAttention(cache, cb.to(device), G * H, B, pt.shape[1], pt.shape[1], user_id=2, with_qjl=False)
+    last = q[:, :, -1:].contiguous()
+    w, e = _tree_want(last, parts, cb, 2, lens, torch.ones(B, 1, dtype=torch.int64), False)
+    P.close(att.run(last.to(device), pt, lt), w, e)
+
+
+def test_no_sequences(device):
+    from omnistack_rs.cache import PagedBlockAttention, PagedTreeAttention
+    parts, cb = P.packed(1, 2, 20, seed=391), P.codebooks(2).to(device)
+    cache, pt, lt = P.paged(device, parts, 16, bounds=True)
+    q = torch.empty(0, 8, 3, 128, dtype=torch.bfloat16, device=device)
+    pt0, lt0, tree = pt[:0].contiguous(), lt[:0].contiguous(), torch.ones(3, dtype=torch.int64, device=device)
+    assert PagedTreeAttention(cache, cb, 8, 0, pt.shape[1], 3).run(q, pt0, lt0, tree).shape == (0, 8, 3, 128)
+    assert PagedBlockAttention(cache, cb, 8, 0, pt.shape[1], 2, 3).run(q, pt0, lt0).shape == (0, 8, 3, 128)
+    cache.keep(pt0, lt0, torch.empty(0, 3, dtype=torch.int32, device=device))
+    cache.update_bounds(pt0, lt0, lt0)
