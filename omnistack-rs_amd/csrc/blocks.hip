@@ -140,7 +140,7 @@ __device__ __forceinline__ uint32_t four_centroids(uint32_t x, const uint32_t (&
 constexpr int kSelWaves = 8;
 
 struct ScoreLds {
-    double part[kSelWaves][256];
+    __attribute__((aligned(16))) double part[kSelWaves][256];
     __attribute__((aligned(16))) int8_t q[256];      // Q+, then -Q-
     __attribute__((aligned(16))) int8_t cent[16];
 };
@@ -159,91 +159,81 @@ __device__ __forceinline__ double sel_row_xor(double x, int m, int c) {
     return __builtin_bit_cast(double, ((uint64_t)sel_row_xor((uint32_t)(v >> 32), m, c) << 32) | sel_row_xor((uint32_t)v, m, c));
 }
 
+// A stage of the Hadamard sums over lanes l and l ^ HALF: the sum in the lower
+// one, lower less upper in the other.
 template <int HALF>
-__device__ __forceinline__ double sel_sum(double x) {           // over lanes l and l ^ 16 or l ^ 32
+__device__ __forceinline__ double sel_stage(double x, int lane) {
     const uint64_t v = __builtin_bit_cast(uint64_t, x);
-    uint64_t p, r;
+    uint64_t lower, upper;
     if constexpr (HALF == 16) {
         const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
         const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
-        p = ((uint64_t)hi[0] << 32) | lo[0];
-        r = ((uint64_t)hi[1] << 32) | lo[1];
+        lower = ((uint64_t)hi[0] << 32) | lo[0];
+        upper = ((uint64_t)hi[1] << 32) | lo[1];
     } else {
         const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
         const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
-        p = ((uint64_t)hi[0] << 32) | lo[0];
-        r = ((uint64_t)hi[1] << 32) | lo[1];
+        lower = ((uint64_t)hi[0] << 32) | lo[0];
+        upper = ((uint64_t)hi[1] << 32) | lo[1];
     }
-    return __builtin_bit_cast(double, p) + __builtin_bit_cast(double, r);
+    return __builtin_fma(lane & HALF ? -1.0 : 1.0, __builtin_bit_cast(double, upper), __builtin_bit_cast(double, lower));
 }
 
 // Q+ and -Q- of query (b, t)'s heads hk G .. + G - 1 and the centroids, as
-// int8: four heads a wave at a time, 16 lanes a head, eight dims a lane.  The
-// constructor asks for the loads of heads 4 `first` .. + 3.
+// int8: a head a wave at a time, two dims a lane.  The constructor asks for the
+// loads of head `first`.
 struct WholeQuery {
-    uint4 raw;
-    uint2 flip;
+    uint32_t raw, flip;
     float cent;
-    __device__ __forceinline__ uint4 head(const SelectArgs &a, int64_t b, int t, int hk, int h, int c) const {
-        return *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
-                                                ((b * a.Hq + hk * a.G + (h < a.G ? h : 0)) * a.T + t) * 128 + 8 * c);
+    __device__ __forceinline__ uint32_t head(const SelectArgs &a, int64_t b, int t, int hk, int h) const {
+        return *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(a.q) +
+                                                   ((b * a.Hq + hk * a.G + (h < a.G ? h : 0)) * a.T + t) * 128 + 2 * (threadIdx.x & 63));
     }
     __device__ __forceinline__ WholeQuery(const SelectArgs &a, int64_t b, int t, int hk, int first) {
-        const int lane = threadIdx.x & 63, c = lane & 15;
-        raw = head(a, b, t, hk, 4 * first + (lane >> 4), c);
-        flip = make_uint2(0u, 0u);
-        if (a.sign_flip) flip = *reinterpret_cast<const uint2 *>(a.sign_flip + 8 * c);
-        cent = (a.codebooks + (a.per_head ? hk * 16 : 0))[c];
+        const int lane = threadIdx.x & 63;
+        raw = head(a, b, t, hk, first);
+        flip = 0u;
+        if (a.sign_flip) flip = *reinterpret_cast<const uint16_t *>(a.sign_flip + 2 * lane);
+        cent = (a.codebooks + (a.per_head ? hk * 16 : 0))[lane & 15];
     }
-    // the wave's sums over heads 4 first .. + 3, then every 4 `stride` on: dim 8 c + j of Q+ in place 16 j + c, of -Q- 128 on
+    // the wave's sums over heads first, first + stride, ..., N at a time (their
+    // chains side by side): Q+, then -Q-
+    template <int N>
     __device__ __forceinline__ void sums(const SelectArgs &a, double *part, int64_t b, int t, int hk, int first, int stride) const {
         const int lane = threadIdx.x & 63, c = lane & 15;
-        double qp[8], qn[8];
+        double qp[2] = {0.0, 0.0}, qn[2] = {0.0, 0.0};
+        for (int h0 = first; h0 < a.G; h0 += N * stride) {
+            double x[2 * N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qp[j] = qn[j] = 0.0;
-        for (int h0 = 4 * first; h0 < a.G; h0 += 4 * stride) {
-            const int h = h0 + (lane >> 4);
-            const uint4 w4 = h0 == 4 * first ? raw : head(a, b, t, hk, h, c);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            double x[8];
+            for (int k = 0; k < N; ++k) {
+                const int h = h0 + k * stride;
+                const uint32_t w = h == first ? raw : head(a, b, t, hk, h);
+                const uint16_t u[2] = {(uint16_t)((w & 0xffffu) ^ ((flip & 0x80u) << 8)), (uint16_t)((w >> 16) ^ (flip & 0x8000u))};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint16_t u = (uint16_t)((j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
-                u ^= (uint16_t)(((j < 4 ? flip.x >> (8 * j) : flip.y >> (8 * j - 32)) & 0x80u) << 8);
-                x[j] = h < a.G ? (double)(a.f16 ? f16_to_f32(u) : bf16_to_f32(u)) : 0.0;
+                for (int j = 0; j < 2; ++j) x[2 * k + j] = h < a.G ? (double)(a.f16 ? f16_to_f32(u[j]) : bf16_to_f32(u[j])) : 0.0;
             }
             if (a.rotate) {
 #pragma unroll
-                for (int m = 1; m < 8; m <<= 1)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (!(j & m)) {
-                            const double u = x[j], l = x[j + m];
-                            x[j] = u + l;
-                            x[j + m] = u - l;
-                        }
-#pragma unroll
-                for (int m = 1; m < 16; m <<= 1) {
-                    const double sgn = c & m ? -1.0 : 1.0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = __builtin_fma(sgn, x[j], sel_row_xor(x[j], m, c));
+                for (int k = 0; k < N; ++k) {
+                    const double sum = x[2 * k] + x[2 * k + 1], less = x[2 * k] - x[2 * k + 1];
+                    x[2 * k] = sum;
+                    x[2 * k + 1] = less;
                 }
+#pragma unroll
+                for (int m = 1; m < 16; m <<= 1)
+#pragma unroll
+                    for (int j = 0; j < 2 * N; ++j) x[j] = __builtin_fma(c & m ? -1.0 : 1.0, x[j], sel_row_xor(x[j], m, c));
+#pragma unroll
+                for (int j = 0; j < 2 * N; ++j) x[j] = sel_stage<32>(sel_stage<16>(x[j], lane), lane);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                qp[j] += fmax(x[j], 0.0);
-                qn[j] += fmin(x[j], 0.0);
+            for (int j = 0; j < 2 * N; ++j) {
+                qp[j & 1] += fmax(x[j], 0.0);
+                qn[j & 1] += fmin(x[j], 0.0);
             }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            qp[j] = sel_sum<32>(sel_sum<16>(qp[j]));
-            qn[j] = sel_sum<32>(sel_sum<16>(qn[j]));
-            if (lane < 16) {
-                part[16 * j + c] = qp[j];
-                part[128 + 16 * j + c] = qn[j];
-            }
-        }
+        *reinterpret_cast<double2 *>(part + 2 * lane) = make_double2(qp[0], qp[1]);
+        *reinterpret_cast<double2 *>(part + 128 + 2 * lane) = make_double2(qn[0], qn[1]);
     }
     __device__ __forceinline__ int8_t centroid() const {          // lane l: of code l % 16
         const int c = threadIdx.x & 15;
@@ -252,7 +242,7 @@ struct WholeQuery {
         for (int m = 1; m < 16; m <<= 1) cm = fmaxf(cm, __uint_as_float(sel_row_xor(__float_as_uint(cm), m, c)));
         return (int8_t)whole((double)cent * whole_scale((double)cm));
     }
-    // v[k]: place 64 k + lane of the summed sums; each wave finds the largest, and stores its places `mask` names
+    // v[k]: place 64 k + lane of the summed sums; each wave finds the largest, and stores the places that `mask` names
     __device__ __forceinline__ static void store(const double (&v)[4], int8_t *q, uint32_t mask) {
         const int lane = threadIdx.x & 63, c = lane & 15;
         double m = fmax(fmax(fabs(v[0]), fabs(v[1])), fmax(fabs(v[2]), fabs(v[3])));
@@ -262,16 +252,14 @@ struct WholeQuery {
         for (int k = 16; k < 64; k <<= 1) m = fmax(m, __shfl_xor(m, k));
         const double scale = whole_scale(m);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int place = 64 * k + lane;
-            if ((mask >> k) & 1u) q[(place & 128) + 8 * c + ((place & 127) >> 4)] = (int8_t)whole(v[k] * scale);
-        }
+        for (int k = 0; k < 4; ++k)
+            if ((mask >> k) & 1u) q[64 * k + lane] = (int8_t)whole(v[k] * scale);
     }
     // one kv head by the whole block
     __device__ __forceinline__ void form(const SelectArgs &a, ScoreLds &sm, int64_t b, int t, int hk) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-        const int groups = (a.G + 3) >> 2, waves = groups < kSelWaves ? groups : kSelWaves;
-        if (wave < waves) sums(a, sm.part[wave], b, t, hk, wave, kSelWaves);
+        const int waves = a.G < kSelWaves ? a.G : kSelWaves;
+        if (wave < waves) sums<1>(a, sm.part[wave], b, t, hk, wave, kSelWaves);
         const int8_t ci = centroid();
         if (tid < 16) sm.cent[tid] = ci;
         __syncthreads();
@@ -310,7 +298,7 @@ __device__ __forceinline__ uint32_t block_key(const uint4 &w, int32_t id, int64_
 // CU).  Bound by the chain of query, page table, bounds and digits: 32 x 8 rows
 // of 512 blocks 10.7 us, choice included (16.8 MB of bounds: 3 us at a copy's
 // rate; a launch for the scores and one for the choice 20); 312 rows of up to
-// 939 blocks 16 us, 18 with one thread block a CU.
+// 939 blocks 15.4 us, 18 with one thread block a CU.
 template <typename Put>
 __device__ __forceinline__ void score_blocks(const SelectArgs &a, const WholeQuery &wq, ScoreLds &sm, int64_t b, int t, int hk, int from,
                                              int to, Put &&put) {
@@ -470,15 +458,16 @@ __device__ __forceinline__ void pick_held(uint32_t *keys, int n, uint32_t kmin, 
 // Scores where rows are fewer than CUs and long: the read of the bounds over
 // the whole chip, `heads` kv heads (a divisor of 8, or 8) of a share of one
 // query's blocks by a thread block, so that a wave's load is 8 / heads pages'
-// neighbouring bounds, a KB.  8 x 8 rows of 8192 blocks (67 MB): 21 us, 3.2
+// neighbouring bounds, a KB.  8 x 8 rows of 8192 blocks (67 MB): 22 us, 3.0
 // TB/s: 5 us of query, then some 90 vector instructions for eight bounds.
 // Measured: two thread blocks a CU 21, one 24, four (two rounds) 27 us; eight
-// loads in flight, which spill at two blocks, 22.
+// loads in flight, which spill at two blocks, 22; query heads one after another
+// instead of four side by side 27.
 __global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectArgs a) {
     constexpr int U = 4;                                          // loads in flight
     __shared__ __attribute__((aligned(16))) int8_t qs[8][256];
     __shared__ __attribute__((aligned(16))) int8_t cs[8][16];
-    __shared__ double part[8][256];
+    __shared__ __attribute__((aligned(16))) double part[8][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 7;
     const int64_t b = blockIdx.z;
     const int sets = a.Hkv / a.heads, share = (int)(blockIdx.x / (unsigned)sets), h0 = ((int)blockIdx.x - share * sets) * a.heads;
@@ -511,7 +500,7 @@ __global__ __launch_bounds__(64 * kSelWaves, 4) void block_score_kernel(SelectAr
     bounds();
     if (wave < a.heads) {                                        // a wave forms a head's query by itself
         const WholeQuery wq(a, b, t, h0 + wave, 0);
-        wq.sums(a, part[wave], b, t, h0 + wave, 0, 1);
+        wq.sums<4>(a, part[wave], b, t, h0 + wave, 0, 1);
         const int8_t ci = wq.centroid();
         if (lane < 16) cs[wave][lane] = ci;
         double v[4];
