@@ -695,9 +695,11 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
         // ahead: 54 instead of 51 us at 16 rows).  Waves in a matrix phase
         // issue first: of a SIMD's, others then work on their weights (without:
         // 56 instead of 54 us, 127 instead of 125 at 64 rows).
-        for (int k = 0; k < cnt; ++k) {
+        // As a function of its operands: written out in the loop, 64 rows spill
+        // and 48 and 64 take 2 to 5 % longer.
+        int next;
+        auto step = [&](PgKeys<HL> &K, PgValues &V, int &nv, int k) {
             float4_t S[NR][2];
-            int next;
             rows_at(clamp(k + 1), r, next);
             __builtin_amdgcn_s_setprio(1);
             scores(K, S);
@@ -711,7 +713,8 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
             __builtin_amdgcn_s_setprio(1);
             products(ev, od, pb);
             __builtin_amdgcn_s_setprio(0);
-        }
+        };
+        for (int k = 0; k < cnt; ++k) step(K, V, nv, k);
     }
 
     // ── merge of the waves ────────────────────────────────────────────
