@@ -523,12 +523,14 @@ int omni_prompt_attn_backward(const void *q, const int64_t *q_strides, const voi
  * sign_flip 8-byte aligned; the pool, page table and codebooks as for
  * omni_attn_paged, with up to 2^31 token rows (n_pages * Hkv * page_size).
  * Products in fp16 with fp32 sums (f16 queries: two fp16 terms of q and of the
- * centroids); a rotated row is not rounded to q's type.  Rows t >= n_draft[b]
- * are zeros; a row that sees nothing, every row of a sequence whose lengths do
- * not fit (0 <= n_draft <= T, n_draft <= length <= max_pages * page_size) or
- * that reaches a page outside the pool is NaN.  workspace (16-byte aligned):
- * omni_attn_tree_workspace_size(...) bytes.  The same bits on every run.  At
- * most 4096 kv heads of 1024 query heads each, B * T * Hkv at most 524280.
+ * centroids); a rotated row is not rounded to q's type.  Scores are fp32: one of
+ * size X is off by about 2^-24 X, and past 2^24 outputs may not be finite.  Rows
+ * t >= n_draft[b] are zeros; a row that sees nothing, every row of a sequence
+ * whose lengths do not fit (0 <= n_draft <= T, n_draft <= length <= max_pages *
+ * page_size) or that reaches a page outside the pool is NaN.  workspace (16-byte
+ * aligned): omni_attn_tree_workspace_size(...) bytes.  The same bits on every
+ * run.  At most 4096 kv heads of 1024 query heads each, B * T * Hkv at most
+ * 524280.
  */
 size_t omni_attn_tree_workspace_size(int64_t B, int Hq, int Hkv, int64_t T, int64_t max_pages, int page_size,
                                      int q_dtype);

@@ -9,7 +9,7 @@
 // One block takes one list (a sequence, or the blocks of one query) of one kv
 // head, a split of its 32-token tiles, and 16 NR query rows (the group's heads
 // of one or more query tokens); its waves take the tiles in turn, each with
-// its own running maximum and sum, and are merged at the end.  All products on
+// its own running reference and sum, and are merged at the end.  All products on
 // v_mfma_f32_16x16x32_f16, tokens on M for the scores and dims on M for P V:
 //   table     64 KB of LDS, a row of 256 bytes for every code byte: in 32
 //             columns its two centroids in fp16 and their remainders, 8 bytes.
@@ -27,12 +27,12 @@
 // Numbers: q rows times a power of two (largest in [2^14, 2^15)) and the head's
 // centroids times one are rounded to fp16.  bf16 queries that the call does not
 // rotate lose nothing; rotated ones, K's centroids (less what is common to them,
-// see `fit`), norms and G q lose 2^-12 of themselves, P another 2^-12 (the same rounded P in numerator and
-// denominator): below the 2^-9 of the bf16 output.  V's centroids keep a
+// see `fit`), norms and G q lose 2^-12 of themselves, P another 2^-12 down to 2^-22 of the largest (the same
+// rounded P in numerator and denominator): below the 2^-9 of the bf16 output.  V's centroids keep a
 // second fp16 term in either type: their roundings do not average out over a
 // long list as P's do.  fp16 queries (HL) keep a second term of q, of G q and of K's
 // centroids too (22 bits), which leaves P's 2^-12 against the output's 2^-12.
-// Scores, maxima, sums and accumulators are fp32.
+// Scores, references, sums and accumulators are fp32.
 //
 // What bounds it: many rows, the matrix and the vector units in turn (32
 // sequences of 8192 tokens and 16 drafted, 64 rows a list: 125 us, 686 TFLOP/s
@@ -78,6 +78,7 @@ constexpr int kPartRow = 128 + 4;            // floats of a split's row: O, then
 constexpr int kLutBytes = 65536;             // the table
 constexpr int kQimgOff = kLutBytes;
 constexpr int kBufWord3 = 0x00020000;        // raw buffer, gfx9 descriptor dword 3
+constexpr float kLag = 13.0f, kBelow = 8.0f; // of the softmax's reference, base 2: see `settle`
 
 // What a variant keeps where.  NR: groups of 16 query rows a block; HL: fp16
 // queries; PAIR: two blocks a CU (128 registers a lane), else one.
@@ -92,7 +93,7 @@ struct Pg {
     static constexpr int kQimg = NR * kSteps * 1024;
     static constexpr int kCsc = kQimgOff + kQimg;                            // per row: score scale
     static constexpr int kSees = kCsc + NR * 16 * 4;                         // per row: its tree mask
-    static constexpr int kM = kSees + NR * 16 * 8;                           // [row][wave]: running maxima, then sums
+    static constexpr int kM = kSees + NR * 16 * 8;                           // [row][wave]: references, then sums
     static constexpr int kFlags = kM + 2 * NR * 16 * NW * 4;                 // per wave: met a page outside the pool
     static constexpr int kUse = kFlags + 16 * 4;
     // the merge: the waves' O of MR row groups at a time, from 0 on (over the tables and the query rows)
@@ -602,10 +603,14 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
                 }
         }
     };
-    // Masks, and a row's running maximum raised where some lane's passes it by
-    // 2^8 (P stays within fp16).  m_run is the same in a row's four lane
-    // groups: each lane tests its own maximum, and the row's is formed only
-    // where one does.
+    // Masks, and a row's reference m_run raised where some lane's maximum passes
+    // it by 2^13, to 2^8 below that maximum: P reaches 2^13 (2^15 with the
+    // roundings of scores below 2^25, base 2), near fp16's 65504, so that it
+    // loses the weights below 2^-33 of the largest and rounds those below 2^-22
+    // of it as subnormals.  (With the maximum itself as the reference, weights
+    // below 2^-25 were lost: 16384 of them a wave beside one key, 2.5 half steps
+    // of an fp16 output.)  m_run is the same in a row's four lane groups: each
+    // lane tests its own maximum, and the row's is formed only where one does.
     auto settle = [&](float4_t (&acc)[NR][2], int64_t tile, int v) {
         const int nv[2] = {v & 255, v >> 8};
         if (!(v == 16 * 257 && (BLOCKS || (tile + 1) * kPgTile <= li.base))) {
@@ -632,15 +637,15 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
         for (int rg = 0; rg < NR; ++rg) {
             mt[rg] = pg_max3(pg_max3(acc[rg][0][0], acc[rg][0][1], acc[rg][0][2]), pg_max3(acc[rg][0][3], acc[rg][1][0], acc[rg][1][1]),
                              __builtin_elementwise_maximum(acc[rg][1][2], acc[rg][1][3])) * csc[rg];
-            any = any || mt[rg] > m_run[rg] + 8.0f;
+            any = any || mt[rg] > m_run[rg] + kLag;
         }
         if (__builtin_amdgcn_ballot_w64(any)) {
 #pragma unroll
             for (int rg = 0; rg < NR; ++rg) {
                 mt[rg] = pg_max_groups(mt[rg]);
-                const bool need = mt[rg] > m_run[rg] + 8.0f;
-                const float f = need ? __builtin_amdgcn_exp2f(m_run[rg] - mt[rg]) : 1.0f;
-                m_run[rg] = need ? mt[rg] : m_run[rg];
+                const float to = mt[rg] > m_run[rg] + kLag ? mt[rg] - kBelow : m_run[rg];
+                const float f = __builtin_amdgcn_exp2f(m_run[rg] - to);
+                m_run[rg] = to;
                 l_run[rg] *= f;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) oacc[rg][k] *= f;

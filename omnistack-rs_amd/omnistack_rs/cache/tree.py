@@ -118,7 +118,8 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch
     all sequences; ``tree_masks`` makes it from parents) is set, itself included
     only if its own bit is.  Rows t >= n_draft[b] are zeros; a row that sees
     nothing is NaN.  ``rotate_q`` applies the signed Hadamard rotation of the
-    cache to q, not rounded to q's dtype in between.  With ``validate`` lengths,
+    cache to q, not rounded to q's dtype in between.  Scores are fp32 and meant
+    for sizes far below 2^24; past it outputs may not be finite.  With ``validate`` lengths,
     page ids and draft counts that do not fit raise (device-to-host copies);
     without it the rows of such sequences are NaN.  No gradient."""
     _lib.refuse_tangents("paged_tree_attention", q)

@@ -1,0 +1,81 @@
+"""The attention over drafted tokens' trees and selected blocks where its
+arithmetic could go wrong: one key far above a long tail, large scores, large
+norms, sums that nearly cancel.  Results are known in closed form; each
+tolerance is derived beside its use."""
+import math
+
+import pytest
+import torch
+
+from tests import _pages as P
+
+pytestmark = pytest.mark.gpu
+
+CB = P.codebooks(1)[0] / P.codebooks(1)[0, -1] * 2.7326            # N(0, 1)'s levels, ascending
+
+
+def _pool(device, kc, vc, page, kr=None):
+    """One head's tokens (codes kc, vc: (S, 128)) as a pool of one sequence."""
+    kn, vn = (c[None, None, :, 0::2] | (c[None, None, :, 1::2] << 4) for c in (kc, vc))
+    S = kc.shape[0]
+    kq = torch.full((1, 1, S, 8), 0xFF, dtype=torch.uint8)
+    kr = torch.zeros(1, 1, S) if kr is None else kr.view(1, 1, S)
+    return P.paged(device, (kn, kq, kr, vn), page)
+
+
+def _same(n, code):
+    return torch.full((n, 128), code, dtype=torch.uint8)
+
+
+def test_a_tail_far_below_one_key(device):
+    """One key and 131071 others, each 2^-25.1 of it: together 3.6e-3.  More than
+    four lists a compute unit, so that none is split: a wave's eighth of the tail
+    is held against the key itself."""
+    from omnistack_rs.cache import paged_tree_attention
+    S, B = 131072, 1100
+    kc, vc = _same(S, 8), _same(S, 0)
+    kc[0], vc[0] = 15, 15
+    cache, pt, lt = _pool(device, kc, vc, 1024)
+    a = 25.1 * math.log(2) * math.sqrt(128) / (128 * float(CB[15] - CB[8]))
+    q = torch.full((B, 1, 1, 128), a, dtype=torch.float16)
+    got = paged_tree_attention(q.to(device), cache, pt.expand(B, -1).contiguous(), lt.expand(B).contiguous(), CB.to(device),
+                               torch.ones(1, dtype=torch.int64, device=device), with_qjl=False, validate=False).double().cpu()
+    gap = float(q[0, 0, 0, 0]) * 128 * (float(CB[15]) - float(CB[8])) / math.sqrt(128)
+    assert 25.0 < gap / math.log(2) < 25.2
+    w = (S - 1) * math.exp(-gap)
+    want = float(CB[15]) * (1 - w) / (1 + w)
+    # the output's half step; of the tail's weights the rounding of P, 2^-25 of 2^-18 or more, and of their scores, 2^-16
+    # of 19; V's 22 bits
+    off = 2.0 ** -11 * want + 2 * w * float(CB[15]) * (2.0 ** -7 + 2.0 ** -11) + 2.0 ** -20
+    assert float((got - want).abs().max()) <= off
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6, 1.5e7])
+def test_large_scores(device, size, dtype):
+    """The key of the largest score takes all, however large, of either sign, alone
+    or among others; 64 rows whose scores' roundings differ."""
+    from omnistack_rs.cache import paged_tree_attention
+    S, T = 300, 64
+    g = torch.Generator().manual_seed(5)
+    kc, vc = _same(S, 8), torch.randint(0, 16, (S, 128), generator=g, dtype=torch.uint8)
+    kc[77], kc[78] = 15, 0
+    cache, pt, lt = _pool(device, kc, vc, 16)
+    top = 128 * float(CB[15])
+    q = ((0.7 + 0.3 * torch.rand(1, 1, T, 1, generator=g)) * torch.tensor([1.0, -1.0]).repeat(32)[None, None, :, None])
+    q = q.expand(1, 1, T, 128).to(dtype).contiguous()
+    none = torch.zeros(T, dtype=torch.int64, device=device)        # the cached tokens alone
+    for n, first in ((S, 0), (1, 77), (1, 78)):                    # all; each of the two alone
+        if n == S:
+            c, table, lens = cache, pt, lt
+        else:
+            c, table, lens = _pool(device, kc[first:first + 1], vc[first:first + 1], 16)
+        # T drafted tokens that nobody sees behind them
+        more = torch.full((1, table.shape[1] + 4), int(table[0, 0]), dtype=torch.int32, device=device)
+        more[0, :table.shape[1]] = table[0]
+        got = paged_tree_attention(q.to(device), c, more, lens + T, CB.to(device), none, scale=size / top, with_qjl=False)
+        for t in range(T):
+            v = CB[vc[(77 if t % 2 == 0 else 78) if n == S else first].long()].double()
+            # the output's half step, V's 22 bits; other keys: exp(-0.6 * 100) and less
+            err = (got[0, 0, t].double().cpu() - v).abs()
+            assert bool((err <= torch.finfo(dtype).eps / 2 * v.abs() + 2.0 ** -20).all()), (n, first, t)
