@@ -341,7 +341,8 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
     if (cmax > 0.0f && cmax < INFINITY) frexpf(cmax, &cexp);
     cexp = cexp < -100 ? -100 : cexp;
     // largest centroid in [2^(kc - 1), 2^kc): HL up to 2^10, for the remainders
-    // of small ones; else 1, for norms, which follow them, up to 65504 of it
+    // of small ones; else 1, for norms, which follow them: up to 65504 of it in
+    // the fast way
     constexpr int kc = HL ? 10 : 0;
     const float cmul = ldexpf(1.0f, kc - cexp), cdiv = ldexpf(1.0f, cexp - kc);
     {
@@ -548,6 +549,25 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
         for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
             for (int u = 0; u < 2; ++u) acc[rg][u] = float4_t{0.f, 0.f, 0.f, 0.f};
+        // the norms as fp16 holds them: one beyond its range by a power of two
+        // less, which its token's sums are multiplied by (a tile without such a
+        // norm, and every other token, keeps its bits).  Two tests a tile: 2 to
+        // 3 % of a call with 64 rows, 1 % of others.
+        float nrm[2] = {0.0f, 0.0f};
+        uint64_t large = 0;
+        auto beyond = [&](int u) {
+            const float x = cmul * R.nr[u][0];
+            return fabsf(x) > 65504.0f ? __builtin_amdgcn_frexp_expf(x) - 15 : 0;
+        };
+        if constexpr (QJL && !HL) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) nrm[u] = -cmul * R.nr[u][0];
+            large = __builtin_amdgcn_ballot_w64(fmaxf(fabsf(nrm[0]), fabsf(nrm[1])) > 65504.0f);
+            if (large) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) nrm[u] = __builtin_amdgcn_ldexpf(nrm[u], -beyond(u));
+            }
+        }
         if constexpr (QJL) {
             // the signs' part.  The norm rides on the signs (fp16, 2^-12 of a
             // small term); HL: +-1, and the sums times the norms
@@ -556,7 +576,7 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
                 half8_t A[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const uint32_t nh = HL ? 0xBC00BC00u : pg_pack(-cmul * R.nr[u][0], -cmul * R.nr[u][0]);
+                    const uint32_t nh = HL ? 0xBC00BC00u : pg_pack(nrm[u], nrm[u]);
                     const uint32_t w = (s ? R.sg[u].y : R.sg[u].x) >> (4 * g);
                     uint32_t e[4];
 #pragma unroll
@@ -570,6 +590,20 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
                         acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), acc[rg][u]);
                         if constexpr (HL) acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + 2 + s), acc[rg][u]);
                     }
+            }
+            if constexpr (!HL) {
+                if (large) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int e = beyond(u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int ei = __shfl(e, 4 * g + i);
+#pragma unroll
+                            for (int rg = 0; rg < NR; ++rg) acc[rg][u][i] = __builtin_amdgcn_ldexpf(acc[rg][u][i], ei);
+                        }
+                    }
+                }
             }
             if constexpr (HL) {
 #pragma unroll

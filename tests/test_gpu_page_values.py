@@ -79,3 +79,37 @@ def test_large_scores(device, size, dtype):
             # the output's half step, V's 22 bits; other keys: exp(-0.6 * 100) and less
             err = (got[0, 0, t].double().cpu() - v).abs()
             assert bool((err <= torch.finfo(dtype).eps / 2 * v.abs() + 2.0 ** -20).all()), (n, first, t)
+
+
+@pytest.mark.parametrize("B,T,G", [(1, 2, 4), (1, 8, 4), (1, 12, 4), (1, 16, 4), (160, 8, 4), (3, 1, 40)])
+@pytest.mark.parametrize("size", [4.0 * 65500, 4.0 * 65510, 1e7, 1e15, 1e30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_norms(device, size, dtype, B, T, G):
+    """Residual norms around and far beyond 65504 of the power of two above the largest centroid (4), some tokens of a tile
+    with one and some without, scores of a size that keeps every token's weight."""
+    from omnistack_rs.cache import paged_block_attention, paged_tree_attention
+    H, S, uid, page = 2, 45, 3, 16
+    parts, cb = list(P.packed(1, H, S, seed=401)), CB.repeat(H, 1)
+    for s, part in ((3, 1.0), (17, 0.5), (20, 0.9), (39, 0.25)):
+        parts[2][:, :, s] = size * part
+    cache, pt, lt = P.paged(device, parts, page)
+    pt, lt = pt.expand(B, -1).contiguous(), lt.expand(B).contiguous()
+    q = torch.randn(1, G * H, T, 128, generator=torch.Generator().manual_seed(402)).to(dtype)
+    scale = 4.0 / size
+    k, v = P.keys_values(*parts, cb, uid)
+    args = (q.expand(B, -1, -1, -1).contiguous().to(device), cache, pt, lt, cb.to(device))
+    kw = dict(user_id=uid, scale=scale)
+    # the last T tokens as drafted ones, each seeing itself and those before it; then all blocks
+    vis = torch.ones(T, S, dtype=torch.bool).tril(S - T)
+    tree = torch.tensor([(1 << (t + 1)) - 1 for t in range(T)], dtype=torch.int64, device=device)
+    tried = paged_tree_attention(*args, tree, **kw)
+    blocks = torch.arange(pt.shape[1], dtype=torch.int32, device=device).expand(B, H, T, -1).contiguous()
+    for got in (tried, paged_block_attention(*args, blocks, **kw)):
+        assert torch.equal(got, got[:1].expand_as(got))
+        most = 0.0
+        for h in range(G * H):
+            want, bound = P.attend(q[0, h].double(), k[0, h // G], v[0, h // G], vis, scale, dtype, False)
+            P.close(got[0, h], want, bound, f"head {h}")
+            s = torch.where(vis, q[0, h].double() @ k[0, h // G].T * scale, -math.inf).softmax(-1)
+            most = max(most, float(s[:, [3, 17, 20]].amax()))
+        assert most > 0.05                               # the weights of these tokens are no small part
