@@ -43,7 +43,9 @@ class PagedKVCache:
     ones.  With ``bounds``, ``k_bounds`` (n_pages, n_kv_heads, head_dim) uint8
     holds each page's least key code of a dim in the low nibble and the largest
     in the high one, which ``write``, ``append`` and ``keep`` follow
-    (``update_bounds`` after any other change).
+    (``update_bounds`` after any other change).  Bounds are of a page's tokens
+    up to the sequence's end: ``append`` and ``keep`` end it behind the last
+    token that they place, ``write`` there too or where its ``length`` says.
     """
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 16, head_dim: int = HEAD_DIM,
@@ -91,17 +93,24 @@ class PagedKVCache:
         self._free.extend(reversed(pages))
 
     def write(self, pages: Sequence[int], k_nibbles: torch.Tensor, k_qjl: torch.Tensor, k_norms: torch.Tensor,
-              v_nibbles: torch.Tensor, start: int = 0) -> None:
+              v_nibbles: torch.Tensor, start: int = 0, length: Optional[int] = None) -> None:
         """Copy one packed sequence, (n_kv_heads, S, ...) as ``encode_kv``
-        returns per batch entry, into ``pages`` from token ``start`` on."""
+        returns per batch entry, into ``pages`` from token ``start`` on.
+        ``length`` is the sequence's length afterwards (default start + S): give
+        it where the pages hold tokens behind these, as when the front of a
+        sequence is written again or its pieces come out of order, or the bounds
+        of a pool that keeps them would leave those tokens out."""
         H, ps = self.n_kv_heads, self.page_size
         if k_nibbles.dim() != 3 or k_nibbles.shape[0] != H:
             raise ValueError(f"k_nibbles must be ({H}, S, {self.head_dim // 2}), got {tuple(k_nibbles.shape)}")
         S = k_nibbles.shape[1]
         if start < 0:
             raise ValueError(f"start must be >= 0, got {start}")
-        if self.pages_for(start + S) > len(pages):
-            raise ValueError(f"{len(pages)} pages hold {len(pages) * ps} tokens, {start + S} needed")
+        end = start + S if length is None else int(length)
+        if end < start + S:
+            raise ValueError(f"length must be at least start + S = {start + S}, got {end}")
+        if self.pages_for(end) > len(pages):
+            raise ValueError(f"{len(pages)} pages hold {len(pages) * ps} tokens, {end} needed")
         # page ids are checked here: an index outside the pool inside the
         # device-side copy below would be a device assertion, not an error
         if any(not 0 <= int(p) < self.n_pages for p in pages):
@@ -113,7 +122,8 @@ class PagedKVCache:
                           (self.v_nibbles, v_nibbles)):
             pool[pg, :, slot] = src.to(device=self.device, dtype=pool.dtype).transpose(0, 1)
         if self.k_bounds is not None and S:
-            where = torch.tensor([start, start + S], dtype=torch.int32, device=self.device)
+            end = min(end, self.pages_for(start + S) * ps)             # of the pages written to
+            where = torch.tensor([start, end], dtype=torch.int32, device=self.device)
             self.update_bounds(self.page_table([pages]), where[:1], where[1:])
 
     def update_bounds(self, page_table: torch.Tensor, start: torch.Tensor, end: torch.Tensor) -> None:

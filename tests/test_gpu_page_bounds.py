@@ -1,0 +1,54 @@
+"""The bounds of the pages' key codes where tokens are written out of order, moved
+and dropped, and in tables of every width."""
+import pytest
+import torch
+
+from tests import _pages as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _want(cache, page, n):
+    """The bounds of a page's first n tokens, from the pool's codes."""
+    c = P.codes(cache.k_nibbles[page, :, :n].cpu())
+    return c.amin(1) | (c.amax(1) << 4)
+
+
+def _put(cache, pages, parts, a, b, **kw):
+    cache.write(pages, *(t[0, :, a:b] for t in parts), start=a, **kw)
+
+
+def test_writes_before_a_sequence_s_end(device):
+    """The front of a sequence written again, and pieces out of order, with the sequence's length: every token counts."""
+    from omnistack_rs.cache import PagedKVCache
+    H, ps, S = 3, 16, 45
+    parts = P.packed(1, H, S, seed=501)
+    cache = PagedKVCache(5, H, ps, device=device, bounds=True)
+    pages = cache.allocate(S)
+    lens = (16, 16, 13)
+
+    def check():
+        for p, n in zip(pages, lens):
+            assert torch.equal(cache.k_bounds[p].cpu().long(), _want(cache, p, n)), p
+
+    _put(cache, pages, parts, 0, S)
+    check()
+    narrow = list(P.packed(1, H, S, seed=502))
+    narrow[0] = torch.full_like(narrow[0], 0x88)                       # a code in the middle: later tokens alone reach further
+    _put(cache, pages, narrow, 0, 4, length=S)
+    check()
+    assert not torch.equal(cache.k_bounds[pages[0]].cpu().long(), _want(cache, pages[0], 4))
+    _put(cache, pages, narrow, 33, 36, length=S)
+    check()
+    cache.k_nibbles.zero_()
+    cache.k_bounds.zero_()
+    for a, b in ((40, 45), (20, 37), (8, 20), (37, 40), (0, 8)):       # each piece once, in no order
+        _put(cache, pages, parts, a, b, length=S)
+    check()
+    _put(cache, pages, parts, 0, 20)                                   # no length: the sequence ends here
+    assert torch.equal(cache.k_bounds[pages[1]].cpu().long(), _want(cache, pages[1], 4))
+    for kw in (dict(length=19), dict(length=49), dict(length=-1)):
+        before = cache.k_nibbles.clone()
+        with pytest.raises(ValueError):
+            _put(cache, pages, narrow, 0, 20, **kw)
+        assert torch.equal(cache.k_nibbles, before)
