@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsArgs a) {
         // up to the last kept token; the page of the token before them, which
         // the dropped ones may have widened, also where none is kept
         e = s;
-        for (int j = 0; j < a.count; ++j) e = a.kept[b * a.count + j] >= 0 ? s + j + 1 : e;
+        for (int j = 0; j < a.count; ++j) e = (uint32_t)a.kept[b * a.count + j] < 64u ? s + j + 1 : e;
         --s;
     }
     s = s < 0 ? 0 : s;                           // rows outside the table are not written by an append either

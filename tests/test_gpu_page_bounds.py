@@ -52,3 +52,24 @@ def test_writes_before_a_sequence_s_end(device):
         with pytest.raises(ValueError):
             _put(cache, pages, narrow, 0, 20, **kw)
         assert torch.equal(cache.k_nibbles, before)
+
+
+def test_kept_numbers_outside_the_tree(device):
+    """Entries that keep() passes over, 64 and above among them, put no token into the bounds."""
+    from omnistack_rs.cache import PagedKVCache
+    H, ps, L = 3, 16, 10
+    parts = P.packed(2, H, L + 5, seed=511)
+    caches = []
+    for last in (70, -1, 64, 1 << 30, -(1 << 31)):
+        cache = PagedKVCache(4, H, ps, device=device, bounds=True)
+        pages = [cache.allocate(L + 5) for _ in range(2)]
+        for b in range(2):
+            cache.write(pages[b], *(t[b] for t in parts))
+        kept = torch.tensor([[3, last, -1], [last, last, last]], dtype=torch.int32, device=device)
+        cache.keep(cache.page_table(pages), torch.full((2,), L, dtype=torch.int32, device=device), kept, validate=False)
+        for b, n in ((0, L + 1), (1, L)):
+            assert torch.equal(cache.k_bounds[pages[b][0]].cpu().long(), _want(cache, pages[b][0], n)), (last, b)
+        caches.append(cache)
+    for c in caches[1:]:
+        for name in ("k_nibbles", "k_qjl", "k_norms", "v_nibbles", "k_bounds"):
+            assert torch.equal(getattr(c, name), getattr(caches[0], name)), name
