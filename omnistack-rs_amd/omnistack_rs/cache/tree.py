@@ -201,6 +201,7 @@ class _Prepared:
 
     def _check_run(self, q, page_table, seq_lens):
         """Host-only checks (no device work, safe under graph capture)."""
+        _lib.refuse_tangents(type(self).__name__, q)
         if q.shape != self._shape or q.dtype != self.q_dtype or not q.is_contiguous() or q.data_ptr() % 16:
             raise ValueError(f"q must be a contiguous {self.q_dtype} tensor of shape {self._shape} at a multiple of 16 bytes")
         if page_table.shape != self._pt_shape or page_table.dtype != torch.int32 or not page_table.is_contiguous():

@@ -113,3 +113,25 @@ def test_large_norms(device, size, dtype, B, T, G):
             s = torch.where(vis, q[0, h].double() @ k[0, h // G].T * scale, -math.inf).softmax(-1)
             most = max(most, float(s[:, [3, 17, 20]].amax()))
         assert most > 0.05                               # the weights of these tokens are no small part
+
+
+def test_dual_tensors_are_refused(device):
+    """A tangent would be dropped in silence: the eager and the prepared calls raise."""
+    from torch.autograd import forward_ad
+    from omnistack_rs.cache import (PagedBlockAttention, PagedTreeAttention, paged_block_attention, paged_tree_attention,
+                                    select_blocks)
+    parts, cb = P.packed(2, 2, 40, seed=411), P.codebooks(2).to(device)
+    cache, pt, lt = P.paged(device, parts, 16, bounds=True)
+    q = torch.randn(2, 8, 1, 128, generator=torch.Generator().manual_seed(412)).to(torch.bfloat16).to(device)
+    tree = torch.ones(1, dtype=torch.int64, device=device)
+    tr, bl = PagedTreeAttention(cache, cb, 8, 2, pt.shape[1]), PagedBlockAttention(cache, cb, 8, 2, pt.shape[1], 2)
+    blocks = select_blocks(q, cache, pt, lt, cb, 2)
+    ref = [tr.run(q, pt, lt, tree).clone(), bl.run(q, pt, lt).clone()]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: paged_tree_attention(dual, cache, pt, lt, cb, tree),
+                     lambda: paged_block_attention(dual, cache, pt, lt, cb, blocks), lambda: tr.run(dual, pt, lt, tree),
+                     lambda: bl.run(dual, pt, lt)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(tr.run(q, pt, lt, tree), ref[0]) and torch.equal(bl.run(q, pt, lt), ref[1])
