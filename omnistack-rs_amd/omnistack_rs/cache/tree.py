@@ -86,12 +86,16 @@ def check_q(q: torch.Tensor, cache: PagedKVCache) -> None:
         raise ValueError(f"1 to {MAX_DRAFT} query tokens, got {q.shape[2]}")
 
 
+def as_int32(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous int32; what int32 does not hold stays out of every range (lengths, page ids and counts are not negative)."""
+    return (t.clamp(-1, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(dtype=torch.int32).contiguous()
+
+
 def check_tables(cache, page_table, seq_lens, B, dev, validate):
     """Page table and lengths as contiguous int32, checked on the host where asked."""
     if page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] < 1:
         raise ValueError(f"page_table must be ({B}, max_pages), got {tuple(page_table.shape)}")
-    pt = page_table.to(dtype=torch.int32).contiguous()
-    lens = seq_lens.to(dtype=torch.int32).reshape(-1).contiguous()
+    pt, lens = as_int32(page_table), as_int32(seq_lens.reshape(-1))
     if lens.numel() != B:
         raise ValueError(f"seq_lens must have {B} entries, got {lens.numel()}")
     if validate and B:
@@ -135,7 +139,7 @@ def paged_tree_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch
     if n_draft is not None:
         if n_draft.numel() != B:
             raise ValueError(f"n_draft must have {B} entries, got {n_draft.numel()}")
-        nd = n_draft.to(dtype=torch.int32).reshape(-1).contiguous()
+        nd = as_int32(n_draft.reshape(-1))
     if validate and B:
         n = torch.full((B,), T) if nd is None else nd.cpu().to(torch.int64)
         if bool(((n < 0) | (n > T) | (n > lens.cpu())).any()):

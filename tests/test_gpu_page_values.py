@@ -135,3 +135,32 @@ def test_dual_tensors_are_refused(device):
             with pytest.raises(NotImplementedError):
                 call()
         assert torch.equal(tr.run(q, pt, lt, tree), ref[0]) and torch.equal(bl.run(q, pt, lt), ref[1])
+
+
+def test_64_bit_numbers_do_not_wrap(device):
+    """Lengths, page ids and draft counts of int64 beyond int32, whose low words alone would fit."""
+    from omnistack_rs.cache import paged_block_attention, paged_tree_attention, select_blocks
+    parts, cb = P.packed(2, 2, 40, seed=421), P.codebooks(2).to(device)
+    cache, pt, lt = P.paged(device, parts, 16, bounds=True)
+    q = torch.randn(2, 8, 2, 128, generator=torch.Generator().manual_seed(422)).to(torch.bfloat16).to(device)
+    tree = torch.tensor([1, 3], dtype=torch.int64, device=device)
+    nd = torch.tensor([2, 1], device=device)
+    blocks = select_blocks(q, cache, pt, lt, cb, 2)
+    ref = paged_tree_attention(q, cache, pt, lt, cb, tree, n_draft=nd)
+    assert torch.equal(paged_tree_attention(q, cache, pt.long(), lt.long(), cb, tree, n_draft=nd.int()), ref)
+    for far in (1 << 32, -(1 << 32), 1 << 62):
+        for i in range(3):
+            a = [pt.long(), lt.long(), nd.clone()]
+            a[i].view(-1)[0] += far
+            kw = dict(n_draft=a[2])
+            with pytest.raises((ValueError, IndexError)):
+                paged_tree_attention(q, cache, a[0], a[1], cb, tree, **kw)
+            got = paged_tree_attention(q, cache, a[0], a[1], cb, tree, validate=False, **kw)
+            assert torch.isnan(got[0]).all() and torch.equal(got[1], ref[1])
+            if i < 2:
+                with pytest.raises((ValueError, IndexError)):
+                    select_blocks(q, cache, a[0], a[1], cb, 2)
+                with pytest.raises((ValueError, IndexError)):
+                    paged_block_attention(q, cache, a[0], a[1], cb, blocks)
+                got = paged_block_attention(q, cache, a[0], a[1], cb, blocks, validate=False)
+                assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
