@@ -86,8 +86,8 @@ def paged_block_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torc
     T + t + 1`` tokens that lie in ``blocks[b, kv head, t]`` (int32, as
     ``select_blocks`` gives them, in any order; numbers outside the query's
     blocks are passed over).  Returns q's shape and dtype; a query that sees
-    nothing is NaN.  ``validate`` also refuses a block named twice for one
-    query, which would count twice.  No gradient."""
+    nothing is NaN.  ``validate`` also refuses one of its blocks named twice for
+    a query, which would count twice.  No gradient."""
     _lib.refuse_tangents("paged_block_attention", q)
     check_q(q, cache)
     B, Hq, T, D = q.shape
@@ -100,7 +100,9 @@ def paged_block_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torc
     bl = blocks.contiguous()
     if validate and B:
         s = bl.cpu().sort(-1)[0]
-        if bool(((s[..., 1:] == s[..., :-1]) & (s[..., 1:] >= 0)).any()):
+        seen = (lens.cpu().to(torch.int64)[:, None] - T + 1 + torch.arange(T)).clamp_min(0)
+        n = ((seen + cache.page_size - 1) // cache.page_size)[:, None, :, None]          # blocks of each query
+        if bool(((s[..., 1:] == s[..., :-1]) & (s[..., 1:] >= 0) & (s[..., 1:] < n)).any()):
             raise ValueError("blocks names a block twice for one query")
     scale = check_scale(scale, D)
     cb, per_head = _prep_codebooks(codebooks, H, dev)

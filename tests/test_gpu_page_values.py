@@ -164,3 +164,32 @@ def test_64_bit_numbers_do_not_wrap(device):
                     paged_block_attention(q, cache, a[0], a[1], cb, blocks)
                 got = paged_block_attention(q, cache, a[0], a[1], cb, blocks, validate=False)
                 assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
+
+
+def test_numbers_passed_over_may_repeat(device):
+    """Any padding behind a query's blocks, the same number twice among it; one of its own blocks twice is refused."""
+    from omnistack_rs.cache import paged_block_attention
+    lens, T = [40, 70], 2
+    parts, cb = P.packed(2, 2, 70, seed=431), P.codebooks(2).to(device)
+    cache, pt, lt = P.paged(device, parts, 16, lens)
+    q = torch.randn(2, 8, T, 128, generator=torch.Generator().manual_seed(432)).to(torch.bfloat16).to(device)
+    blocks = torch.tensor([0, 2, -1, -1], dtype=torch.int32, device=device).expand(2, 2, T, 4).contiguous()
+    ref = paged_block_attention(q, cache, pt, lt, cb, blocks)
+    for pad in (-5, 3, 4, 5, 1 << 30):
+        other = blocks.clone()
+        other[0, :, :, 2:] = pad if pad != 5 else 3                    # sequence 0 has blocks 0 to 2
+        other[1, :, :, 2:] = pad if pad > 4 else -3                    # sequence 1 has blocks 0 to 4
+        assert torch.equal(paged_block_attention(q, cache, pt, lt, cb, other), ref), pad
+    # block 1 of sequence 0 is the last that query 0 of 17 tokens does not see
+    short = torch.tensor([17, 70], dtype=torch.int32, device=device)
+    twice = torch.tensor([0, 1, 1, -1], dtype=torch.int32, device=device).expand(2, 2, T, 4).contiguous()
+    twice[1], twice[0, :, 1, 2] = blocks[1], -1
+    once = torch.where(twice == 1, -1, twice)
+    once[0, :, 1, 1] = 1
+    got = paged_block_attention(q, cache, pt, short, cb, twice)
+    assert torch.equal(got, paged_block_attention(q, cache, pt, short, cb, once))
+    for b, t, n in ((0, 0, 0), (0, 1, 2), (1, 0, 4), (1, 1, 4)):
+        bad = blocks.clone()
+        bad[b, 1, t] = torch.tensor([n, -1, n, 9], dtype=torch.int32)
+        with pytest.raises(ValueError):
+            paged_block_attention(q, cache, pt, lt, cb, bad)
