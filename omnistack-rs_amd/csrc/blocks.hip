@@ -32,6 +32,7 @@ struct BoundsArgs {
     const int32_t *page_table, *start, *end;     // end NULL: start + count
     const int32_t *kept;                         // with it, count of them: the tokens that a move of drafted tokens leaves
     int64_t max_pages, n_pages, count;
+    int64_t page0;                               // pages of each sequence that earlier launches took
     int Hkv, page_shift;
 };
 
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsArgs a) {
     s = s < 0 ? 0 : s;                           // rows outside the table are not written by an append either
     e = e > cap ? cap : e;
     if (s >= e) return;
-    const int64_t pi = (s >> a.page_shift) + blockIdx.x;
+    const int64_t pi = (s >> a.page_shift) + a.page0 + blockIdx.x;
     if (pi << a.page_shift >= e) return;
     const int32_t id = a.page_table[b * a.max_pages + pi];
     if (id < 0 || id >= a.n_pages) return;
@@ -710,12 +711,18 @@ extern "C" int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t 
     OMNI_CHECK_ARG(B >= 0 && B <= 65535 && count >= 0, "omni_block_bounds: need 0 <= B <= 65535 and count >= 0");
     if (B == 0 || (end == nullptr && count == 0)) return OMNI_OK;
     OMNI_CHECK_ARG(k_nib && bounds && page_table && start, "omni_block_bounds: NULL pointer");
-    // pages that `count` tokens can touch (any number of tokens: the whole table)
+    // pages that `count` tokens can touch (2^32 reach any table's end from any start)
+    if (count > (int64_t(1) << 32)) count = int64_t(1) << 32;
     int64_t pages = end ? max_pages : (count + page_size - 2) / page_size + 1;
     if (pages > max_pages) pages = max_pages;
-    const BoundsArgs a{k_nib, bounds, page_table, start, end, nullptr, max_pages, n_pages, count, Hkv, shift};
-    hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)pages, (unsigned)B), dim3(256), 0, as_stream(stream), a);
-    OMNI_CHECK_LAUNCH("block_bounds_kernel");
+    BoundsArgs a{k_nib, bounds, page_table, start, end, nullptr, max_pages, n_pages, count, 0, Hkv, shift};
+    // a grid of 2^32 threads and more would be cut to its low 32 bits without an error
+    constexpr int64_t kMost = 1 << 20;
+    for (; a.page0 < pages; a.page0 += kMost) {
+        const int64_t n = pages - a.page0 < kMost ? pages - a.page0 : kMost;
+        hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)n, (unsigned)B), dim3(256), 0, as_stream(stream), a);
+        OMNI_CHECK_LAUNCH("block_bounds_kernel");
+    }
     return OMNI_OK;
 }
 
@@ -790,7 +797,7 @@ extern "C" int omni_cache_keep(uint8_t *k_nib, uint8_t *k_qjl, float *k_norms, u
     if (bounds) {
         int64_t pages = (K + 1 + page_size - 2) / page_size + 1;      // K tokens and the one before them
         if (pages > max_pages) pages = max_pages;
-        const BoundsArgs ba{k_nib, bounds, page_table, positions, nullptr, kept, max_pages, n_pages, K, Hkv, shift};
+        const BoundsArgs ba{k_nib, bounds, page_table, positions, nullptr, kept, max_pages, n_pages, K, 0, Hkv, shift};
         hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)pages, (unsigned)B), dim3(256), 0, as_stream(stream), ba);
         OMNI_CHECK_LAUNCH("block_bounds_kernel");
     }

@@ -73,3 +73,39 @@ def test_kept_numbers_outside_the_tree(device):
     for c in caches[1:]:
         for name in ("k_nibbles", "k_qjl", "k_norms", "v_nibbles", "k_bounds"):
             assert torch.equal(getattr(c, name), getattr(caches[0], name)), name
+
+
+def test_tables_of_more_pages_than_a_grid_holds(device):
+    """A sequence over 2^24 pages, most of them outside the pool; any count of tokens."""
+    from omnistack_rs import _lib
+    from omnistack_rs.cache import PagedKVCache
+    H, ps, n = 2, 16, (1 << 24) + 40
+    cache = PagedKVCache(6, H, ps, device=device, bounds=True)
+    cache.k_nibbles.random_(0, 256, generator=torch.Generator(device=device).manual_seed(521))
+    table = torch.full((1, n), -1, dtype=torch.int32, device=device)
+    where = {1: 0, 2: 1 << 20, 3: (1 << 24) - 1, 4: (1 << 24) + 3}            # page: its place
+    for page, i in where.items():
+        table[0, i] = page
+    end = where[4] * ps + 5
+    ends = torch.tensor([end], dtype=torch.int32, device=device)
+
+    def check():
+        for page in range(6):
+            want = _want(cache, page, 5 if page == 4 else ps) if page in where else torch.zeros(H, 128).long()
+            assert torch.equal(cache.k_bounds[page].cpu().long(), want), page
+
+    cache.update_bounds(table, torch.zeros_like(ends), ends)
+    check()
+    L = _lib.lib()
+    for start, count in ((0, end), (-9, end + 9)):
+        cache.k_bounds.zero_()
+        cache._bounds(table, torch.tensor([start], dtype=torch.int32, device=device), None, count)
+        check()
+    # counts far past the table's end: every page whole
+    for count in (1 << 31, (1 << 62) + 3, (1 << 63) - 1):
+        cache.k_bounds.zero_()
+        starts = torch.tensor([0], dtype=torch.int32, device=device)
+        assert L.omni_block_bounds(cache.k_nibbles.data_ptr(), cache.k_bounds.data_ptr(), 6, H, ps, table.data_ptr(), n,
+                                   starts.data_ptr(), None, count, 1, _lib.stream_of(device)) == 0
+        assert torch.equal(cache.k_bounds[4].cpu().long(), _want(cache, 4, ps)) and torch.equal(
+            cache.k_bounds[1].cpu().long(), _want(cache, 1, ps))
