@@ -561,8 +561,9 @@ int omni_block_bounds(const uint8_t *k_nib, uint8_t *bounds, int64_t n_pages, in
  * Q and the head's centroids each times the power of two that brings their
  * largest into [64, 128), rounded to whole numbers (127 at most); the lower
  * block wins a tie, and a page outside the pool is taken first.  With codebooks
- * that ascend this bounds the group's summed scores (without residual signs)
- * from above.  blocks (B, Hkv, T, top) int32: ascending, -1 behind the last.
+ * that ascend this is an upper bound of the group's summed scores (without
+ * residual signs) up to those roundings, which can leave it below the bound
+ * too.  blocks (B, Hkv, T, top) int32: ascending, -1 behind the last.
  * q and sign_flip as for omni_attn_tree.  workspace (16-byte aligned):
  * omni_block_select_workspace_size(...) bytes.  B * T at most 65535.
  */

@@ -10,12 +10,17 @@
 //   sum_h max_{lo <= code <= hi} q_h . c  =  sum_d Q+_d c[hi_d] - Q-_d c[lo_d],
 //   Q+ = sum_h max(q_h, 0),  Q- = sum_h max(-q_h, 0)
 // an upper bound of the group's summed scores q . c[code] (the residual signs
-// are left out), in whole numbers: Q and the head's centroids are each
+// are left out), here in whole numbers: Q and the head's centroids are each
 // multiplied by the power of two that brings their largest into [64, 128) and
-// rounded to int8.  A sum of 256 products of int8 lies below 2^22, so it does
-// not depend on its order; equal scores are equal, and the lower block wins.
-// Q+ and Q- are summed in fp64, where sums of 16-bit values are exact (the
-// rotation's too: its factor 1/sqrt(128) does not change the order).
+// rounded to the nearest int8 (127 at most), so that a score lies above or below
+// the bound by what those roundings sum up to.  A sum of 256 products of int8
+// lies below 2^22, so it does not depend on its order; equal scores are equal,
+// and the lower block wins.  Q+ and Q- are summed in fp64 (rotated rows without
+// the factor 1/sqrt(128), which does not change the order): exact for f16 (40
+// bits a value, 47 a rotated one) of up to 1024 heads, 64 rotated, and for bf16
+// (8 bits a value) where the exponents that meet in a sum span up to 45 bits
+// less those that its number of terms adds; past that a sum is off by 2^-53 of
+// itself, which can move a rounding to int8 at a tie only.
 #include <math.h>
 
 #include "omni_common.h"

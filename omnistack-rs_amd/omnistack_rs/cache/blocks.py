@@ -50,9 +50,10 @@ def select_blocks(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor
     Query token t of sequence b sees the first ``seq_lens[b] - T + t + 1``
     tokens.  Of their blocks the first ``first`` and the last ``recent`` are
     taken, then those of the largest scores; the lower block wins a tie.  The
-    score bounds sum_h q_h . c[code] over the kv head's query heads from above
-    (scores are of one sign: a negative scale wants -q here), q and codebooks
-    rounded to int8 by powers of two; residual signs take no part.  Arguments
+    score is the upper bound of sum_h q_h . c[code] over the kv head's query
+    heads (scores are of one sign: a negative scale wants -q here) with the sums
+    of q and the codebooks rounded to int8 by powers of two, so it can lie below
+    the bound by what that rounds away; residual signs take no part.  Arguments
     as for ``paged_tree_attention``; ``validate`` also checks that the codebooks
     ascend."""
     check_q(q, cache)

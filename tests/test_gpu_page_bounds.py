@@ -1,5 +1,7 @@
 """The bounds of the pages' key codes where tokens are written out of order, moved
 and dropped, and in tables of every width."""
+import math
+
 import pytest
 import torch
 
@@ -109,3 +111,52 @@ def test_tables_of_more_pages_than_a_grid_holds(device):
                                    starts.data_ptr(), None, count, 1, _lib.stream_of(device)) == 0
         assert torch.equal(cache.k_bounds[4].cpu().long(), _want(cache, 4, ps)) and torch.equal(
             cache.k_bounds[1].cpu().long(), _want(cache, 1, ps))
+
+
+def _scaled(x):
+    """x by the power of two that brings its largest into [64, 128), and rounded to whole numbers."""
+    x = x * 2.0 ** (7 - math.frexp(float(x.abs().max()))[1])
+    return x, torch.round(x).clamp(-127, 127)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G", [1, 4])
+def test_selected_blocks_bound_the_others_keys(device, G, dtype):
+    """No key of a block that was passed over scores above the bound of one that was taken, by more than the whole numbers'
+    rounding: of this query and codebook, the sum over dims of the largest difference that any code makes, for both."""
+    from omnistack_rs.cache import select_blocks
+    H, ps, n, top, first, recent = 2, 16, 700, 60, 2, 3
+    g = torch.Generator().manual_seed(531)
+    cb = P.codebooks(H)
+    q = (torch.randn(1, H, 1, 1, 128, generator=g) + 0.2 * torch.randn(1, H, G, 1, 128, generator=g)).reshape(1, H * G, 1, 128).to(dtype)
+    Q = q.double().view(H, G, 128)
+    # in every page one token follows the query's signs in some dims, none to all, the rest keep to the codes around zero
+    kc = torch.randint(6, 10, (H, n, ps, 128), generator=g)
+    with_q = torch.rand(H, n, 128, generator=g) < torch.rand(1, n, 1, generator=g)
+    best = torch.where(Q.sum(1) > 0, 15, 0)[:, None].expand(H, n, 128)
+    at = torch.randint(0, ps, (n,), generator=g)
+    kc[:, torch.arange(n), at] = torch.where(with_q, best, kc[:, torch.arange(n), at])
+    kc = kc.view(1, H, n * ps, 128).to(torch.uint8)
+    parts = P.packed(1, H, n * ps, seed=532)
+    kn = kc[..., 0::2] | (kc[..., 1::2] << 4)
+    cache, pt, lt = P.paged(device, (kn, *parts[1:]), ps, bounds=True)
+    got = select_blocks(q.to(device), cache, pt, lt, cb.to(device), top, first=first, recent=recent).cpu()[0, :, 0].long()
+    told_apart = 0
+    for h in range(H):
+        c = cb[h].double()
+        parts_q = torch.stack((Q[h].clamp_min(0).sum(0), (-Q[h]).clamp_min(0).sum(0)))
+        (sq, wq), (sc, wc) = _scaled(parts_q), _scaled(c)
+        slack = float((sq[..., None] * sc - wq[..., None] * wc).abs().amax(-1).sum())
+        unit = float((sq.sum() / parts_q.sum()) * (sc.abs().sum() / c.abs().sum()))          # the powers of two
+        codes = kc[0, h].view(n, ps, 128).long()
+        own = (c[codes] @ Q[h].sum(0)).amax(1) * unit                                       # a page's best key
+        bound = (c[codes.amax(1)] @ parts_q[0] - c[codes.amin(1)] @ parts_q[1]) * unit
+        assert bool((own <= bound + 1e-6).all())
+        taken = torch.zeros(n, dtype=torch.bool)
+        taken[got[h]] = True
+        assert int(taken.sum()) == top and taken[:first].all() and taken[n - recent:].all()
+        inner = torch.arange(n).ge(first) & torch.arange(n).lt(n - recent)
+        least = float(bound[taken & inner].min())
+        assert float(own[~taken].max()) <= least + 2 * slack
+        told_apart += int((own[inner].max() > bound[inner] + 2 * slack).sum())
+    assert told_apart > n // 2                                # most pages, if taken, would have failed
