@@ -193,3 +193,53 @@ def test_numbers_passed_over_may_repeat(device):
         bad[b, 1, t] = torch.tensor([n, -1, n, 9], dtype=torch.int32)
         with pytest.raises(ValueError):
             paged_block_attention(q, cache, pt, lt, cb, bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G,T", [(1, 1), (4, 8), (4, 12), (4, 16)])
+def test_values_that_cancel(device, G, T, dtype):
+    """Equal weights over values whose fp16 roundings are all that is left of them: the second term of V's centroids."""
+    from omnistack_rs.cache import paged_block_attention, paged_tree_attention
+    S, rest = 80, 0.49 * 2.0 ** -9                                     # less than half a step of fp16 at 2.5
+    cb = torch.linspace(-2.0, 2.0, 16)
+    cb[0], cb[15] = -2.5 + rest, 2.5 + rest
+    vc = _same(S, 0)
+    vc[1::2] = 15
+    cache, pt, lt = _pool(device, _same(S, 3), vc, 16)
+    q = torch.zeros(1, G, T, 128, dtype=dtype, device=device)
+    none = torch.zeros(T, dtype=torch.int64, device=device)
+    more = torch.cat((pt, pt[:, :4]), 1).contiguous()                  # drafted tokens that nobody sees
+    trees = paged_tree_attention(q, cache, more, lt + T, cb.to(device), none, with_qjl=False)
+    blocks = torch.arange(pt.shape[1], dtype=torch.int32, device=device).expand(1, 1, 1, -1).contiguous()
+    picked = paged_block_attention(q[:, :, :1], cache, pt, lt, cb.to(device), blocks, with_qjl=False)
+    want = (float(cb[0]) + float(cb[15])) / 2
+    # the output's half step; 22 bits of a centroid in [2, 4); fp32 sums of 80 such terms
+    off = torch.finfo(dtype).eps / 2 * want + 2.0 ** -20 + 80 * 2.0 ** -24 * 2.5
+    assert off < want / 16
+    for got in (trees, picked):
+        assert float((got.double() - want).abs().max()) <= off
+
+
+def test_roundings_common_to_a_codebook(device):
+    """Centroids that fp16 rounds by the same share of themselves, one key against as much weight in others far below it:
+    bf16 calls take the share back from the scores."""
+    from omnistack_rs.cache import paged_tree_attention
+    e = 0.45 * 2.0 ** -10                                              # below half a step of fp16 at a power of two
+    half = 2.0 ** torch.arange(-6, 2).double() * (1 + e)
+    cb = torch.cat((-half.flip(0), half)).float()
+    q = torch.full((1, 1, 1, 128), 0.49, dtype=torch.bfloat16)
+    gap = float(q[0, 0, 0, 0]) * 128 * (float(cb[15]) - float(cb[8])) / math.sqrt(128)
+    n = round(math.exp(gap))
+    assert 3e4 < n < 1e5
+    kc, vc = _same(n + 1, 8), _same(n + 1, 0)
+    kc[0], vc[0] = 15, 15
+    cache, pt, lt = _pool(device, kc, vc, 256)
+    got = paged_tree_attention(q.to(device), cache, pt, lt, cb.to(device), torch.ones(1, dtype=torch.int64, device=device),
+                               with_qjl=False, validate=False).double().cpu()
+    w = n * math.exp(-gap)
+    want = float(cb[15]) * (1 - w) / (1 + w)
+    # a share x of the others' weight moves the result by x / 2 of a value: of P's rounding 2^-12, of the scores' fp32 sums
+    # 2^-16 of 11; the output's half step and V's 22 bits.  The centroids' rounding would be 11 e = 4.8e-3.
+    off = float(cb[15]) * (2.0 ** -12 + 11 * 2.0 ** -16) / 2 + 2.0 ** -8 * abs(want) + 2.0 ** -20
+    assert off < float(cb[15]) * gap * e / 8
+    assert float((got - want).abs().max()) <= off
