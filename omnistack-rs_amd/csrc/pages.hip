@@ -543,29 +543,21 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
         return pg_half8(e0.x, e0.y, e1.x, e1.y);
     };
     // scores of a tile, raw: lane (n, g) holds tokens 16 u + 4 g + i of row n
-    auto scores = [&](const PgKeys<HL> &R, float4_t (&acc)[NR][2]) {
+    auto scores = [&](const PgKeys<HL> &R, float4_t (&acc)[NR][2], uint64_t &large) {
         if constexpr (kKept < L::kSteps) asm volatile("" : "+v"(q_off));       // read again for each tile, not kept (and spilled)
 #pragma unroll
         for (int rg = 0; rg < NR; ++rg)
 #pragma unroll
             for (int u = 0; u < 2; ++u) acc[rg][u] = float4_t{0.f, 0.f, 0.f, 0.f};
-        // the norms as fp16 holds them: one beyond its range by a power of two
-        // less, which its token's sums are multiplied by (a tile without such a
-        // norm, and every other token, keeps its bits).  Two tests a tile: 2 to
-        // 3 % of a call with 64 rows, 1 % of others.
+        // norms beyond fp16 count as 0 here, and in `large_signs`
         float nrm[2] = {0.0f, 0.0f};
-        uint64_t large = 0;
-        auto beyond = [&](int u) {
-            const float x = cmul * R.nr[u][0];
-            return fabsf(x) > 65504.0f ? __builtin_amdgcn_frexp_expf(x) - 15 : 0;
-        };
         if constexpr (QJL && !HL) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) nrm[u] = -cmul * R.nr[u][0];
-            large = __builtin_amdgcn_ballot_w64(fmaxf(fabsf(nrm[0]), fabsf(nrm[1])) > 65504.0f);
-            if (large) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) nrm[u] = __builtin_amdgcn_ldexpf(nrm[u], -beyond(u));
+            for (int u = 0; u < 2; ++u) {
+                const float x = -cmul * R.nr[u][0];
+                const bool over = fabsf(x) > 65504.0f;
+                large |= __builtin_amdgcn_ballot_w64(over);
+                nrm[u] = over ? 0.0f : x;
             }
         }
         if constexpr (QJL) {
@@ -590,20 +582,6 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
                         acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + s), acc[rg][u]);
                         if constexpr (HL) acc[rg][u] = pg_mfma(A[u], q_at(rg, L::kQSteps + 2 + s), acc[rg][u]);
                     }
-            }
-            if constexpr (!HL) {
-                if (large) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int e = beyond(u);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int ei = __shfl(e, 4 * g + i);
-#pragma unroll
-                            for (int rg = 0; rg < NR; ++rg) acc[rg][u][i] = __builtin_amdgcn_ldexpf(acc[rg][u][i], ei);
-                        }
-                    }
-                }
             }
             if constexpr (HL) {
 #pragma unroll
@@ -635,6 +613,42 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
                         acc[rg][u] = pg_mfma(Al[u], q_at(rg, s), acc[rg][u]);
                     }
                 }
+        }
+    };
+    // bf16 calls: the signs' part of tokens whose norm lies beyond 65504 of the
+    // table's unit, the norm less a power of two in fp16 and the sums times that;
+    // the other tokens of the tile add 0 and keep their bits.  From memory again,
+    // so that nothing waits in registers for what a calibrated cache does not
+    // hold (two comparisons a tile: 64 rows 1 to 4 %, 32 rows at two blocks a CU
+    // 2 to 3 %, others up to 1 %; with both ways inside `scores` 48 rows 7 %).
+    auto large_signs = [&](const uint32_t (&r)[2], float4_t (&acc)[NR][2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint2 sg = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(half_of(a.k_qjl, r[u], 8), 8 * n, 0, 0));
+            const float x = -cmul * __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(half_of(a.k_norms, r[u], 4), 4 * n, 0, 0));
+            const bool over = fabsf(x) > 65504.0f;
+            const int e = over ? __builtin_amdgcn_frexp_expf(x) - 15 : 0;
+            const float m = over ? __builtin_amdgcn_ldexpf(x, -e) : 0.0f;
+            const uint32_t nh = pg_pack(m, m);
+            half8_t A[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t w = (s ? sg.y : sg.x) >> (4 * g);
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = ((w << (15 - j)) & 0x80008000u) ^ nh;
+                A[s] = pg_half8(h[0], h[1], h[2], h[3]);
+            }
+            int ei[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ei[i] = __shfl(e, 4 * g + i);
+#pragma unroll
+            for (int rg = 0; rg < NR; ++rg) {
+                float4_t t = pg_mfma(A[0], q_at(rg, L::kQSteps), float4_t{0.f, 0.f, 0.f, 0.f});
+                t = pg_mfma(A[1], q_at(rg, L::kQSteps + 1), t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[rg][u][i] += __builtin_amdgcn_ldexpf(t[i], ei[i]);
+            }
         }
     };
     // Masks, and a row's reference m_run raised where some lane's maximum passes
@@ -728,6 +742,8 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
     if (cnt > 0) {
         const int64_t t0 = t_begin + wave;
         uint32_t r[2];
+        int next;
+        rows_at(0, r, next);                     // of the tile at hand (kept from above, two row groups spill more)
         half8_t pb[NR][2];
         uint32_t ev[4], od[4];
         // The next tile is asked for as its registers come free (two tiles
@@ -735,15 +751,19 @@ __global__ __launch_bounds__(64 * NW, (PAIR ? 4 : NW / 4)) void page_attn_kernel
         // issue first: of a SIMD's, others then work on their weights (without:
         // 56 instead of 54 us, 127 instead of 125 at 64 rows).
         // As a function of its operands: written out in the loop, 64 rows spill
-        // and 48 and 64 take 2 to 5 % longer.
-        int next;
+        // more (now 3 to 5 registers with signs) and 48 and 64 take 2 to 5 % longer.
         auto step = [&](PgKeys<HL> &K, PgValues &V, int &nv, int k) {
             float4_t S[NR][2];
+            const uint32_t now[2] = {r[0], r[1]};
+            uint64_t large = 0;
             rows_at(clamp(k + 1), r, next);
             __builtin_amdgcn_s_setprio(1);
-            scores(K, S);
+            scores(K, S, large);
             __builtin_amdgcn_s_setprio(0);
             load_k(K, r);
+            if constexpr (QJL && !HL) {
+                if (large) large_signs(now, S);
+            }
             settle(S, t0 + (int64_t)NW * k, nv);
             nv = next;
             weights(S, pb);
@@ -952,9 +972,10 @@ struct PagePlan {
 // prologue runs beside the other's tiles (768 lists of 75 to 2917 tokens in
 // fp16 55 us, twelve waves 59; 312 selections of 768 tokens 17, 21 with one
 // block a CU; 256 lists of 1024 tokens 13 either way, twelve waves 14).  Two
-// row groups spill at two blocks a CU (28 registers of a bf16 call): that pays
-// up to six tiles a list only (512 lists of 58 tokens 15 us, 18 with one; 256
-// lists of 8192 tokens 147 and 75).
+// row groups spill at two blocks a CU (57 registers of a bf16 call with signs, 22
+// without): that pays up to four tiles a list (512 lists in tables of 80, 112,
+// 144 and 176 tokens 15.8, 17.5, 19.5 and 22.0 us, with one block a CU 17.9,
+// 18.3, 18.4 and 19.7).
 static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
     // us: a block's fixed part, and per tile by its row groups
     constexpr double kFixed = 8.0, kTile[5] = {0.0, 0.18, 0.27, 0.36, 0.46}, kTileHl[5] = {0.0, 0.24, 0.36, 0.53, 0.70};
@@ -967,7 +988,7 @@ static PagePlan page_plan(int64_t units, int rows, int64_t tiles, bool hl) {
         auto consider = [&](int64_t s) {
             if (s < 1 || s > 256 || (s > 1 && tiles / s < 8)) return;
             const int64_t all = blocks * s, n = (tiles + s - 1) / s;
-            const bool spills = nr == 2 && !hl && all > cus && n <= 6;
+            const bool spills = nr == 2 && !hl && all > cus && n <= 4;
             const int64_t at_once = (nr == 1 && all > cus) || spills ? 2 : 1;
             const double tile = spills ? 1.0 : (hl ? kTileHl : kTile)[nr] * (at_once == 2 ? 2.1 : 1.0);
             const double t = (double)((all + at_once * cus - 1) / (at_once * cus)) * ((spills ? 12.0 : kFixed) + tile * (double)n) +
