@@ -46,8 +46,9 @@ struct BoundsArgs {
 // and keeps nibble minima and maxima in 16-bit lanes.  The page's first tokens
 // up to `end` count, whatever start is, so what a page says does not depend on
 // how it was filled.  Bound by latency where a decode step touches a page per
-// sequence (5.8 us), else by the read of the codes (8 x 131072 tokens, 537 MB:
-// 174 us, 3.1 TB/s; a prompt pays it once).
+// sequence (4 to 6 us), else by 4-byte loads and 16 lane moves per KB of codes
+// (8 x 131072 tokens, 537 MB: 153 to 174 us, 3.1 to 3.5 TB/s, 104 us at a copy's
+// rate); wider loads have not been tried.
 __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsArgs a) {
     typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
     const int64_t b = blockIdx.y;
@@ -661,7 +662,8 @@ struct KeepArgs {
 
 // One block per (head, sequence): token positions + kept[j] goes to positions
 // + j.  All rows are read before any is written, so the order of `kept` does
-// not matter.  Four threads a token, 16 code bytes of K and V each.
+// not matter.  Four threads a token, 16 code bytes of K and V each.  Bound by
+// latency: 4 to 64 tokens of 8 to 64 sequences 3.2 us, then the bounds' launch.
 __global__ __launch_bounds__(256) void cache_keep_kernel(KeepArgs a) {
     const int hk = blockIdx.x;
     const int64_t b = blockIdx.y;

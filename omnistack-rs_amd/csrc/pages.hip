@@ -27,21 +27,23 @@
 // Numbers: q rows times a power of two (largest in [2^14, 2^15)) and the head's
 // centroids times one are rounded to fp16.  bf16 queries that the call does not
 // rotate lose nothing; rotated ones, K's centroids (less what is common to them,
-// see `fit`), norms and G q lose 2^-12 of themselves, P another 2^-12 down to 2^-22 of the largest (the same
-// rounded P in numerator and denominator): below the 2^-9 of the bf16 output.  V's centroids keep a
-// second fp16 term in either type: their roundings do not average out over a
-// long list as P's do.  fp16 queries (HL) keep a second term of q, of G q and of K's
-// centroids too (22 bits), which leaves P's 2^-12 against the output's 2^-12.
+// see `fit`), norms and G q lose 2^-12 of themselves, P another 2^-12 down to
+// 2^-22 of the largest (the same rounded P in numerator and denominator): below
+// the 2^-9 of the bf16 output.  V's centroids keep a second fp16 term in either
+// type: their roundings do not average out over a long list as P's do.  fp16
+// queries (HL) keep a second term of q, of G q and of K's centroids too (22
+// bits), which leaves P's 2^-12 against the output's 2^-12.
 // Scores, references, sums and accumulators are fp32.
 //
 // What bounds it: many rows, the matrix and the vector units in turn (32
-// sequences of 8192 tokens and 16 drafted, 64 rows a list: 125 us, 686 TFLOP/s
-// of the 1200 that a large product reaches; matrix units busy in 43 % of the
-// cycles, vector instructions issuing in 49 %, 256 registers hold a SIMD at
-// two waves).  Few rows, the cache's read and the vector work per tile (16 rows
-// 51 us, 294 MB at 5.8 TB/s; a plain read reaches 7.1).  Short lists, a block's
-// chain of dependent accesses, 7 to 8 us: lengths, page ids, tiles and q one
-// after another, the table (0.7 us), G q, and the waves' merge (1.5 us).
+// sequences of 8192 tokens and 16 drafted, 64 rows a list: 124 us, 690 TFLOP/s
+// of the 1200 to 1550 that large products reach by their layout; matrix units
+// busy in 42 % of the cycles, vector instructions issuing in 45 %, 256 registers
+// hold a SIMD at two waves).  Few rows, the cache's read and the vector work per
+// tile (16 rows 52 us, 294 MB at 5.7 TB/s; a plain read reaches 7.1).  Short
+// lists, a block's chain of dependent accesses, 7 to 8 us: lengths, page ids,
+// tiles and q one after another, the table (0.7 us), G q, and the waves' merge
+// (1.5 us).
 #include <math.h>
 
 #include <new>

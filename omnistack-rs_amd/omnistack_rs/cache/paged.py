@@ -130,7 +130,8 @@ class PagedKVCache:
         """``k_bounds`` of the pages that hold tokens start[b] .. end[b] - 1 of the
         sequences in ``page_table``, from their tokens before end[b] (int32 on the
         pool's device; positions outside the table and pages outside the pool are
-        passed over)."""
+        passed over).  A page of several of the sequences (a shared prefix) must
+        hold as many tokens in each."""
         pt = self._check_rows(page_table, (("start", start), ("end", end)))
         self._bounds(pt, start.contiguous(), end.contiguous(), 0)
 

@@ -28,7 +28,9 @@ def tree_masks(parents: torch.Tensor) -> torch.Tensor:
     """The ``tree`` of ``paged_tree_attention`` from parents: integers (T,) or
     (B, T), ``parents[t]`` < t the drafted token that t follows, negative where
     it follows the last cached token.  int64 of the same shape; bit j of entry t
-    is set for t itself and every token on its way up."""
+    is set for t itself and every token on its way up.  Made on the host (a copy
+    and a wait where parents are on the device, not for graph capture): keep the
+    masks of a tree that is used again."""
     if parents.dim() not in (1, 2) or parents.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"parents must be int32 or int64 (T,) or (B, T), got {parents.dtype} {tuple(parents.shape)}")
     T = parents.shape[-1]
