@@ -160,3 +160,56 @@ def test_selected_blocks_bound_the_others_keys(device, G, dtype):
         assert float(own[~taken].max()) <= least + 2 * slack
         told_apart += int((own[inner].max() > bound[inner] + 2 * slack).sum())
     assert told_apart > n // 2                                # most pages, if taken, would have failed
+
+
+def test_a_drafting_step_captured(device):
+    """Append, tree attention, keep and the attention over selected blocks as one graph, replayed over a growing cache, against
+    the same step run eagerly on a cache of its own."""
+    from omnistack_rs.cache import PagedBlockAttention, PagedKVCache, PagedTreeAttention, tree_masks
+    from omnistack_rs.kernels.quantize import PackedKVEncoder
+    B, Hq, H, T, ps, top, uid = 3, 8, 2, 6, 16, 5, 7
+    cb = P.codebooks(H).to(device)
+    enc = PackedKVEncoder(cb, H, user_id=uid, dtype=torch.bfloat16, device=device)
+    g = torch.Generator().manual_seed(541)
+    tree = tree_masks(torch.tensor([-1, 0, 0, 1, 2, 3])).to(device)
+    first = torch.randn(B, H, 90, 128, generator=g).to(torch.bfloat16).to(device)
+    sides = []
+    for _ in range(2):
+        cache = PagedKVCache(60, H, ps, device=device, bounds=True)
+        pt = cache.page_table([cache.allocate(300) for _ in range(B)])
+        cache.append(enc, first, first, pt, torch.zeros(B, dtype=torch.int32, device=device))
+        att = PagedTreeAttention(cache, cb, Hq, B, pt.shape[1], T, user_id=uid)
+        sparse = PagedBlockAttention(cache, cb, Hq, B, pt.shape[1], top, user_id=uid)
+        sides.append((cache, pt, att, sparse))
+    k, v = (torch.zeros(B, H, T, 128, dtype=torch.bfloat16, device=device) for _ in range(2))
+    q, q1 = (torch.zeros(B, Hq, t, 128, dtype=torch.bfloat16, device=device) for t in (T, 1))
+    kept = torch.full((B, 4), -1, dtype=torch.int32, device=device)
+    lens = [torch.tensor([90, 80, 33], dtype=torch.int32, device=device) for _ in range(2)]
+
+    def step(i):
+        cache, pt, att, sparse = sides[i]
+        cache.append(enc, k, v, pt, lens[i], validate=False)
+        o = att.run(q, pt, lens[i] + T, tree)
+        cache.keep(pt, lens[i], kept, validate=False)
+        lens[i] += (kept >= 0).sum(1, dtype=torch.int32)
+        return o, sparse.run(q1, pt, lens[i])
+
+    step(1)                                                       # nothing kept: the lengths stay
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(1)
+    for i, paths in enumerate(([[0, 1, 3], [0], []], [[], [0, 2, 4], [0, 1, 3, 5]], [[0, 2], [0, 1], [0]], [[0], [], [0, 1]])):
+        for t in (k, v, q, q1):
+            t.copy_(torch.randn(t.shape, generator=g))
+        kept.fill_(-1)
+        for b, p in enumerate(paths):
+            kept[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
+        want = [t.clone() for t in step(0)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(lens[0], lens[1]) and all(torch.equal(a, b) for a, b in zip(outs, want)), i
+        assert torch.equal(sides[0][3].blocks, sides[1][3].blocks)
+        for name in ("k_nibbles", "k_qjl", "k_norms", "v_nibbles", "k_bounds"):
+            a, b = (getattr(s[0], name)[s[1].long()] for s in sides)
+            assert torch.equal(a, b), (i, name)
+        torch.zeros(1 << 20, device=device).sum().item()
